@@ -30,7 +30,7 @@ HIP_FLAGS = [
     "-mllvm", "-amdgpu-mfma-vgpr-form",
     "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
 ]
-SOURCES = ["kernels.hip", "api.hip"]
+SOURCES = ["kernels.hip", "cache_ops.hip", "logit_ops.hip", "api.hip"]
 
 
 def _run(cmd, cwd=None):

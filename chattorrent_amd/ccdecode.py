@@ -6,6 +6,7 @@ ABI. There is no CPU fallback: if the HIP library is missing, loading fails.
 """
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -28,7 +29,8 @@ EXPORTS = [
     "cc_slot_pages", "cc_free_pages", "cc_fill_random_kv", "cc_read_kv", "cc_write_kv", "cc_read_pages",
     "cc_stats_get", "cc_op_matmul_q8", "cc_op_store_kv", "cc_op_round_f16", "cc_op_topk", "cc_op_rmsnorm",
     "cc_op_attend", "cc_profile", "cc_profile_read", "cc_read_logits", "cc_mtp_draft", "cc_topk_noalloc",
-    "cc_decode_steps",
+    "cc_decode_steps", "cc_cache_of", "cc_bounds_bytes", "cc_kv_append", "cc_kv_bounds", "cc_attend_workspace",
+    "cc_attend_pages", "cc_logits_adjust", "cc_sample_workspace", "cc_sample",
 ]
 
 
@@ -61,19 +63,38 @@ class Stats(C.Structure):
                 ("last_pass_ms", C.c_double)]
 
 
+class CCache(C.Structure):
+    """cc_cache: a paged int8 cache in device memory (KVCache builds it)."""
+    _fields_ = [("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("n_pages", C.c_int32),
+                ("max_pages", C.c_int32), ("slots", C.c_int32), ("rope_rows", C.c_int32), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("bounds", C.c_void_p), ("page_table", C.c_void_p), ("rope", C.c_void_p)]
+
+
+class CSampling(C.Structure):
+    """cc_sampling: what each row of a call asks for (Sampling builds it)."""
+    _fields_ = [("temp", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("rep", C.c_void_p), ("freq", C.c_void_p), ("pres", C.c_void_p), ("freq_cap", C.c_float),
+                ("pen_at", C.c_void_p), ("pen_ids", C.c_void_p), ("pen_counts", C.c_void_p), ("n_pen", C.c_int32),
+                ("bias_at", C.c_void_p), ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("n_bias", C.c_int32),
+                ("mask", C.c_void_p), ("mask_words", C.c_int32), ("n_masks", C.c_int32), ("mask_of", C.c_void_p),
+                ("u", C.c_void_p)]
+
+
 _lib = None
+_torch_first = False   # torch was there when the library was loaded: they share one HIP runtime
 
 
 def load():
     """Loads libccdecode.so; raises if it is not built (no fallback)."""
-    global _lib
+    global _lib, _torch_first
     if _lib is not None:
         return _lib
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(f"{LIB_PATH} is missing: build it with `python -m chattorrent_amd.build`")
+    _torch_first = "torch" in sys.modules
     L = C.CDLL(LIB_PATH)
     P = C.c_void_p
-    i32, i64, u64 = C.c_int32, C.c_int64, C.c_uint64
+    i32, i64, u64, size = C.c_int32, C.c_int64, C.c_uint64, C.c_size_t
     sig = {
         "cc_create": (i32, [C.POINTER(Dims), C.POINTER(Opts), C.POINTER(P)]),
         "cc_destroy": (None, [P]),
@@ -98,6 +119,15 @@ def load():
         "cc_read_logits": (i32, [P, i32, P]),
         "cc_mtp_draft": (i32, [P, i32, i32, i32, i32, i32, P]),
         "cc_decode_steps": (i32, [P, C.POINTER(Job), i32, i32, i32, P, P]),
+        "cc_cache_of": (i32, [P, i32, C.POINTER(CCache)]),
+        "cc_bounds_bytes": (size, [C.POINTER(CCache)]),
+        "cc_kv_append": (i32, [P, P, P, i32, P, i64, P, i64, P]),
+        "cc_kv_bounds": (i32, [P, P, P, i32, P]),
+        "cc_attend_workspace": (size, [P, P, P, i32, i32, i32]),
+        "cc_attend_pages": (i32, [P, P, P, i32, i32, i32, i32, i32, P, i64, P, i64, P, size, P]),
+        "cc_logits_adjust": (i32, [P, P, i64, i32, i32, P, P, i64, P]),
+        "cc_sample_workspace": (size, [i32, i32]),
+        "cc_sample": (i32, [P, P, i64, i32, i32, P, P, P, P, size, P]),
         "cc_profile": (i32, [P, i32]),
         "cc_profile_read": (i32, [P, i32, C.POINTER(C.c_double), C.POINTER(C.c_int64), C.POINTER(C.c_double)]),
     }
@@ -120,6 +150,183 @@ class CCError(RuntimeError):
         super().__init__(msg)
         self.status = status
         self.kind = STATUS_NAMES[status] if 0 <= status < len(STATUS_NAMES) else str(status)
+
+
+# --- device buffers: the operators on the caller's own memory -------------------------
+# They take torch tensors (a call then runs on torch's current stream) or DeviceArrays.
+
+def _hip():
+    """The HIP runtime that the library itself uses."""
+    load()
+    h = C.CDLL("libamdhip64.so.7")
+    h.hipMalloc.argtypes = [C.POINTER(C.c_void_p), C.c_size_t]
+    h.hipFree.argtypes = [C.c_void_p]
+    h.hipMemcpy.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int]
+    return h
+
+
+class DeviceArray:
+    """A C-contiguous array in device memory, for callers without torch."""
+
+    def __init__(self, shape, dtype):
+        self.shape, self.dtype = tuple(int(n) for n in np.atleast_1d(shape)), np.dtype(dtype)
+        self.nbytes = int(np.prod(self.shape)) * self.dtype.itemsize
+        self._h, p = _hip(), C.c_void_p()
+        if self._h.hipMalloc(C.byref(p), max(self.nbytes, 16)):
+            raise MemoryError(f"no device memory for {self.nbytes} bytes")
+        self._p = p.value
+
+    @classmethod
+    def of(cls, a):
+        """A copy of a numpy array on the device."""
+        a = np.ascontiguousarray(a)
+        out = cls(a.shape, a.dtype)
+        out.set(a)
+        return out
+
+    def set(self, a):
+        a = np.ascontiguousarray(a, self.dtype)
+        if a.shape != self.shape:
+            raise ValueError(f"shape {a.shape}, not {self.shape}")
+        self._copy(self._p, a.ctypes.data, 1)
+
+    def numpy(self):
+        """A copy on the host, once everything on the device is done."""
+        out = np.empty(self.shape, self.dtype)
+        self._copy(out.ctypes.data, self._p, 2)
+        return out
+
+    def _copy(self, to, of, kind):
+        if self._h.hipDeviceSynchronize() or (self.nbytes and self._h.hipMemcpy(to, of, self.nbytes, kind)):
+            raise RuntimeError("a copy between host and device failed")
+
+    def data_ptr(self):
+        return self._p
+
+    def stride(self, dim):
+        return int(np.prod(self.shape[dim:][1:])) if dim >= 0 else self.stride(dim + len(self.shape))
+
+    def __del__(self):
+        if getattr(self, "_p", None):
+            self._h.hipFree(self._p)
+            self._p = None
+
+
+def _is_torch(t):
+    torch = sys.modules.get("torch")
+    return torch is not None and isinstance(t, torch.Tensor)
+
+
+def _dtype(t):
+    return str(t.dtype).rsplit(".", 1)[-1]
+
+
+class _Buffers:
+    """Buffers that one C struct points into: checked, kept alive, on one device."""
+
+    def __init__(self):
+        self.kept, self.device = [], None
+
+    def take(self, t, name, dtypes, shape, nullable=True):
+        """The pointer of a contiguous device array of one of `dtypes` and of `shape` (None: any extent)."""
+        if t is None and nullable:
+            return None
+        if _dtype(t) not in dtypes:
+            raise ValueError(f"{name}: {' or '.join(dtypes)}, not {t.dtype}")
+        if len(t.shape) != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, not {shape}")
+        if _is_torch(t):
+            if not t.is_cuda or not t.is_contiguous():
+                raise ValueError(f"{name}: a contiguous tensor on the GPU")
+            if self.device is not None and t.device.index != self.device:
+                raise ValueError(f"{name}: on another GPU than the others")
+            self.device = t.device.index
+        self.kept.append(t)
+        return t.data_ptr()
+
+
+class KVCache(_Buffers):
+    """A paged int8 cache in the caller's device memory, K and V of one layer,
+    laid out as include/ccdecode.h says (cc_cache): k, v uint8 [pages, kv heads,
+    64*D + 64*D/32*4], page_table int32 [slots, pages a slot], rope f32
+    [positions, rot_dim/2, 2], and key bounds uint8 [pages, kv heads*(2*D +
+    D/8)] or None. KVCache.of_context gives a context's own."""
+
+    def __init__(self, k, v, page_table, rope, head_dim, bounds=None):
+        super().__init__()
+        D = int(head_dim)
+        n_pages, n_kv = int(k.shape[0]), int(k.shape[1])
+        block = 64 * D + 64 * (D // 32) * 4
+        self.c = CCache(n_kv_heads=n_kv, head_dim=D, rot_dim=2 * int(rope.shape[1]), n_pages=n_pages,
+                        max_pages=int(page_table.shape[1]), slots=int(page_table.shape[0]),
+                        rope_rows=int(rope.shape[0]),
+                        k=self.take(k, "k", ("uint8", "int8"), (n_pages, n_kv, block), False),
+                        v=self.take(v, "v", ("uint8", "int8"), (n_pages, n_kv, block), False),
+                        page_table=self.take(page_table, "page_table", ("int32", "uint32"), (None, None), False),
+                        rope=self.take(rope, "rope", ("float32",), (None, None, 2), False),
+                        bounds=self.take(bounds, "bounds", ("uint8", "int8"), (n_pages, n_kv * (2 * D + D // 8))))
+        self.ref = C.byref(self.c)
+
+    @classmethod
+    def of_context(cls, ctx, layer, bounds=None):
+        """The context's own cache of block `layer`; `bounds`: key bounds of the caller's."""
+        self = cls.__new__(cls)
+        _Buffers.__init__(self)
+        self.c = CCache()
+        ctx._chk(ctx.lib.cc_cache_of(ctx.h, layer, C.byref(self.c)))
+        self.kept.append(ctx)
+        self.device = ctx.opts.device if _is_torch(bounds) else None
+        self.c.bounds = self.take(bounds, "bounds", ("uint8", "int8"),
+                                  (self.c.n_pages, int(ctx.lib.cc_bounds_bytes(C.byref(self.c)))))
+        self.ref = C.byref(self.c)
+        return self
+
+
+class Sampling(_Buffers):
+    """What the rows of a call ask for (cc_sampling): device arrays, None where
+    no row asks for it. temp, top_p, min_p, rep, freq, pres f32 [rows]; top_k
+    int32 [rows]; u f64 [rows]; the history pen_at int32 [rows + 1], pen_ids
+    int32 [entries], pen_counts int32 [entries] or None (1 each); bias_at,
+    bias_ids likewise and bias f32 [entries]; mask 32-bit words [masks,
+    ceil(vocab/32) or more] and mask_of int32 [rows]."""
+
+    def __init__(self, rows, vocab, temp=None, top_k=None, top_p=None, min_p=None, rep=None, freq=None, pres=None,
+                 freq_cap=1.5, pen_at=None, pen_ids=None, pen_counts=None, bias_at=None, bias_ids=None, bias=None,
+                 mask=None, mask_of=None, u=None):
+        super().__init__()
+        self.rows, self.vocab = int(rows), int(vocab)
+        n_pen = 0 if pen_ids is None else int(pen_ids.shape[0])
+        n_bias = 0 if bias_ids is None else int(bias_ids.shape[0])
+        f32, i32, row = ("float32",), ("int32", "uint32"), (self.rows,)
+        if mask is not None and int(mask.shape[1]) * 32 < self.vocab:
+            raise ValueError(f"mask: {mask.shape[1]} words are fewer than the vocabulary takes")
+        self.c = CSampling(
+            temp=self.take(temp, "temp", f32, row), top_k=self.take(top_k, "top_k", i32, row),
+            top_p=self.take(top_p, "top_p", f32, row), min_p=self.take(min_p, "min_p", f32, row),
+            rep=self.take(rep, "rep", f32, row), freq=self.take(freq, "freq", f32, row),
+            pres=self.take(pres, "pres", f32, row), freq_cap=freq_cap,
+            pen_at=self.take(pen_at, "pen_at", i32, (self.rows + 1,)),
+            pen_ids=self.take(pen_ids, "pen_ids", i32, (n_pen,)),
+            pen_counts=self.take(pen_counts, "pen_counts", i32, (n_pen,)), n_pen=n_pen,
+            bias_at=self.take(bias_at, "bias_at", i32, (self.rows + 1,)),
+            bias_ids=self.take(bias_ids, "bias_ids", i32, (n_bias,)),
+            bias=self.take(bias, "bias", f32, (n_bias,)), n_bias=n_bias,
+            mask=self.take(mask, "mask", i32, (None, None)), mask_words=0 if mask is None else int(mask.shape[1]),
+            n_masks=0 if mask is None else int(mask.shape[0]), mask_of=self.take(mask_of, "mask_of", i32, row),
+            u=self.take(u, "u", ("float64",), row))
+        self.ref = C.byref(self.c)
+
+
+def _job_rows(jobs):
+    """(slot, past, n) of each job as int32 [jobs, 3], and the rows they hold."""
+    a = np.asarray(jobs)
+    if a.dtype != np.int32:
+        if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
+            raise ValueError("jobs: 32-bit integers (slot, past, n)")
+        a = a.astype(np.int32)
+    if a.ndim != 2 or a.shape[1] != 3:
+        raise ValueError("jobs: one (slot, past, n) each")
+    return np.ascontiguousarray(a), int(a[:, 2].sum(dtype=np.int64))
 
 
 def layer_kinds(d):
@@ -369,3 +576,101 @@ class Context:
         out = np.empty_like(q)
         self._chk(self.lib.cc_op_attend(self.h, layer, slot, _p(q), q.shape[0], past, _p(out)))
         return out
+
+    # --- operators on the caller's device buffers --------------------------------------
+    def _on(self, stream, *tensors):
+        """The stream of a call on `tensors`: the one given, else torch's current one, else the context's."""
+        torch_ones = [t for t in tensors if _is_torch(t)]
+        for t in torch_ones:
+            if not t.is_cuda or t.device.index != self.opts.device:
+                raise ValueError(f"a tensor on {t.device}, not on the context's GPU ({self.opts.device})")
+        if stream is None and torch_ones:
+            if not _torch_first:
+                raise RuntimeError("import torch before the library is loaded: they would hold two HIP runtimes")
+            stream = sys.modules["torch"].cuda.current_stream(self.opts.device).cuda_stream or 1   # 0: the legacy stream
+        return stream
+
+    def _rows(self, t, name, rows, width):
+        """Pointer and row stride of f32 rows [rows, width], whose elements lie beside each other."""
+        if _dtype(t) != "float32" or len(t.shape) != 2 or t.shape[0] != rows or (width is not None and t.shape[1] != width):
+            raise ValueError(f"{name}: f32 [{rows}, {width}], not {t.dtype} {tuple(t.shape)}")
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"{name}: a row's values must lie beside each other")
+        return t.data_ptr(), max(t.stride(0), t.shape[1]) if rows == 1 else t.stride(0)
+
+    def _new(self, like, shape, dtype):
+        if _is_torch(like):
+            torch = sys.modules["torch"]
+            return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
+        return DeviceArray(shape, dtype)
+
+    def _same_device(self, held):
+        if held.device is not None and held.device != self.opts.device:
+            raise ValueError(f"buffers on GPU {held.device}, not on the context's ({self.opts.device})")
+
+    def kv_append(self, cache, jobs, k, v, stream=None):
+        """cc_kv_append: the jobs' rows (slot, past, n) of k (before RoPE) and v,
+        f32 [rows, kv heads * D], into the cache's pages, and the key bounds of
+        the pages they complete."""
+        self._same_device(cache)
+        stream = self._on(stream, k, v)
+        a, rows = _job_rows(jobs)
+        width = cache.c.n_kv_heads * cache.c.head_dim
+        kp, ldk = self._rows(k, "k", rows, width)
+        vp, ldv = self._rows(v, "v", rows, width)
+        self._chk(self.lib.cc_kv_append(self.h, cache.ref, a.ctypes.data, len(a), kp, ldk, vp, ldv, stream))
+
+    def kv_bounds(self, cache, jobs, stream=None):
+        """cc_kv_bounds: key bounds of the pages within the jobs' rows, from the cache."""
+        self._same_device(cache)
+        stream = self._on(stream, *(t for t in cache.kept if _is_torch(t)))
+        a, _ = _job_rows(jobs)
+        self._chk(self.lib.cc_kv_bounds(self.h, cache.ref, a.ctypes.data, len(a), stream))
+
+    def attend_pages(self, cache, jobs, q, budget, sink=1, recent=2, out=None, stream=None):
+        """cc_attend_pages: attention of the jobs' rows, q f32 [rows, heads * D]
+        before RoPE, over at most `budget` pages a row and kv head. Returns the
+        rows' output (`out`, or a new array)."""
+        self._same_device(cache)
+        stream = self._on(stream, q, out)
+        a, rows = _job_rows(jobs)
+        qp, ldq = self._rows(q, "q", rows, None)
+        D, width = cache.c.head_dim, int(q.shape[1])
+        if width % D:
+            raise ValueError(f"q: rows of {width} values are not whole heads of {D}")
+        if out is None:
+            out = self._new(q, (rows, width), "float32")
+        op, ldo = self._rows(out, "out", rows, width)
+        need = self.lib.cc_attend_workspace(self.h, cache.ref, a.ctypes.data, len(a), width // D, budget)
+        if not need:
+            raise CCError(CC_EARG, self.lib.cc_last_error(self.h).decode())
+        ws = self._new(q, (need,), "uint8")
+        self._chk(self.lib.cc_attend_pages(self.h, cache.ref, a.ctypes.data, len(a), width // D, budget, sink, recent,
+                                           qp, ldq, op, ldo, ws.data_ptr(), need, stream))
+        return out
+
+    def adjust_logits(self, logits, sampling, out=None, stream=None):
+        """cc_logits_adjust: the rows with penalties, biases and masks, in `out`
+        (logits itself, another array, or a new one)."""
+        self._same_device(sampling)
+        stream = self._on(stream, logits, out)
+        if out is None:
+            out = self._new(logits, (sampling.rows, sampling.vocab), "float32")
+        lp, ld = self._rows(logits, "logits", sampling.rows, sampling.vocab)
+        op, ldo = self._rows(out, "out", sampling.rows, sampling.vocab)
+        self._chk(self.lib.cc_logits_adjust(self.h, lp, ld, sampling.rows, sampling.vocab, sampling.ref, op, ldo, stream))
+        return out
+
+    def sample(self, logits, sampling, stream=None):
+        """cc_sample: a token of each row of logits and the probability it was
+        drawn with, int32 and f32 [rows]."""
+        self._same_device(sampling)
+        stream = self._on(stream, logits)
+        rows, V = sampling.rows, sampling.vocab
+        lp, ld = self._rows(logits, "logits", rows, V)
+        ids, probs = self._new(logits, (rows,), "int32"), self._new(logits, (rows,), "float32")
+        need = self.lib.cc_sample_workspace(rows, V)
+        ws = self._new(logits, (max(need, 16),), "uint8")
+        self._chk(self.lib.cc_sample(self.h, lp, ld, rows, V, sampling.ref, ids.data_ptr(), probs.data_ptr(),
+                                     ws.data_ptr(), need, stream))
+        return ids, probs

@@ -19,6 +19,7 @@
 #include "../../include/ccdecode.h"
 #include "common.h"
 #include "kernels.h"
+#include "ops.h"
 
 namespace {
 
@@ -2220,6 +2221,317 @@ cc_status cc_op_attend(cc_ctx* ctx, int32_t layer, int32_t slot, const float* q,
     HIPCHK(hipMemcpy(out, dctx, (size_t)n * qd * 4, hipMemcpyDeviceToHost));
     for (void* v : {(void*)dr, (void*)dctx, (void*)dXp}) (void)hipFree(v);
     return CC_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------ operators on the caller's buffers ---
+namespace {
+
+// The context's GPU is current for the calls below; the caller's is again after.
+struct DeviceGuard {
+    int before = -1;
+    hipError_t err = hipSuccess;
+    explicit DeviceGuard(int device) {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device);
+        else if (err == hipSuccess) before = -1;   // nothing to put back
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+bool ok_width(int D) { return D == 64 || D == 128 || D == 256; }
+bool is_aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
+cc_status cache_dev(cc_ctx* ctx, const cc_cache* c, CacheDev& d) {
+    if (!ok_width(c->head_dim)) return fail(ctx, CC_EARG, "cache: head_dim must be 64, 128 or 256");
+    if (c->rot_dim < 2 || c->rot_dim > c->head_dim || c->rot_dim % 2)
+        return fail(ctx, CC_EARG, "cache: rot_dim must be even, 2 .. head_dim");
+    if (c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->n_pages < 1 || c->slots < 1 || c->rope_rows < 1 || c->max_pages < 1 ||
+        c->max_pages > 32768)
+        return fail(ctx, CC_EARG, "cache: n_kv_heads 1 .. 1024, max_pages 1 .. 32768, n_pages, slots and rope_rows positive");
+    if (!c->k || !c->v || !c->page_table || !c->rope) return fail(ctx, CC_EARG, "cache: k, v, page_table and rope must be set");
+    if (!is_aligned(c->k, 16) || !is_aligned(c->v, 16) || !is_aligned(c->bounds, 16) || !is_aligned(c->rope, 8) ||
+        !is_aligned(c->page_table, 4))
+        return fail(ctx, CC_EARG, "cache: k, v and bounds must be 16-byte aligned, rope 8");
+    d.k = (uint8_t*)c->k;
+    d.v = (uint8_t*)c->v;
+    d.bounds = (uint8_t*)c->bounds;
+    d.page_table = c->page_table;
+    d.rope = c->rope;
+    d.nKV = c->n_kv_heads;
+    d.D = c->head_dim;
+    d.ng = c->head_dim / 32;
+    d.rot = c->rot_dim;
+    d.n_pages = c->n_pages;
+    d.max_pages = c->max_pages;
+    d.blk = 64 * d.D + 64 * d.ng * 4;
+    d.bblk = (int)cc_bounds_bytes(c);
+    return CC_OK;
+}
+
+cc_status check_rows(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t njobs, int64_t* rows, bool once) {
+    if (!jobs || njobs < 1) return fail(ctx, CC_EARG, "jobs: at least one");
+    const int64_t cap = std::min((int64_t)c->max_pages * 64, (int64_t)c->rope_rows);
+    std::vector<bool> seen(once ? (size_t)c->slots : 0, false);
+    *rows = 0;
+    for (int j = 0; j < njobs; j++) {
+        const cc_rows& r = jobs[j];
+        if (r.slot < 0 || r.slot >= c->slots || r.past < 0 || r.n < 1 || (int64_t)r.past + r.n > cap)
+            return fail(ctx, CC_EARG, "job " + std::to_string(j) + ": slot within the cache, past >= 0, n >= 1 and past + n at most " +
+                                          std::to_string(cap) + " (the slot's pages and the rope table)");
+        if (once) {
+            if (seen[r.slot]) return fail(ctx, CC_EARG, "slot " + std::to_string(r.slot) + " twice in one call");
+            seen[r.slot] = true;
+        }
+        *rows += r.n;
+    }
+    return CC_OK;
+}
+
+// The jobs in launches of at most OP_JOBS (and, with rows as units, at most
+// OP_ROWS rows); units(job) > 0 is the job's work. f(jobs) launches.
+constexpr int OP_ROWS = 65535;   // a grid's third dimension
+template <class U, class F>
+hipError_t each_batch(const cc_rows* jobs, int32_t njobs, int64_t cap, U&& units, F&& f) {
+    OpJobs b;
+    int64_t row0 = 0;
+    for (int j = 0; j < njobs; j++) {
+        const int64_t u = units(jobs[j]);
+        if (u > 0) {
+            if (b.n == OP_JOBS || (b.n > 0 && b.units + u > cap)) {
+                const hipError_t e = f(b);
+                if (e != hipSuccess) return e;
+                b.n = b.rows = b.units = 0;
+            }
+            b.j[b.n++] = OpJob{jobs[j].slot, jobs[j].past, jobs[j].n, (int32_t)row0, b.units};
+            b.rows += jobs[j].n;
+            b.units += (int32_t)u;
+        }
+        row0 += jobs[j].n;
+    }
+    return b.n ? f(b) : hipSuccess;
+}
+
+// How a call of `rows` rows (of its largest launch) is laid out. Work of a row
+// and kv head is cut over workgroups until there are about two for each
+// compute unit, and a workgroup's pages are at most one index a lane of its
+// four waves.
+AttendPlan attend_plan(int ncu, const cc_cache* c, int64_t rows, int max_seen, int n_heads, int budget) {
+    AttendPlan p;
+    p.group = n_heads / c->n_kv_heads;
+    p.tiles = ceil_div(p.group, 16);
+    p.max_seen = max_seen;
+    p.budget = budget;
+    p.scored = max_seen > budget;
+    const int kept = std::min(max_seen, budget);
+    const int64_t units = rows * c->n_kv_heads * p.tiles;
+    const int64_t want = std::max<int64_t>(1, (2 * (int64_t)ncu + units - 1) / units);
+    p.per = (int)std::max<int64_t>(ATTEND_WAVES, std::min<int64_t>(ATTEND_PER, (kept + want - 1) / want));
+    p.splits = ceil_div(kept, p.per);
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    p.scores = 0;
+    p.partials = up(p.scored ? (size_t)rows * c->n_kv_heads * max_seen * 4 : 0);
+    p.counters = p.partials + up(p.splits > 1 ? (size_t)units * p.splits * std::min(16, p.group) * (c->head_dim + 2) * 4 : 0);
+    p.bytes = p.counters + up((size_t)units * 4);
+    return p;
+}
+
+cc_status attend_args(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t njobs, int32_t n_heads, int32_t budget,
+                      AttendPlan& p, int64_t* total) {
+    cc_status st = check_rows(ctx, c, jobs, njobs, total, false);
+    if (st != CC_OK) return st;
+    if (n_heads < 1 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 1024)
+        return fail(ctx, CC_EARG, "n_heads must be a multiple of the cache's n_kv_heads");
+    if ((int64_t)c->n_kv_heads * ceil_div(n_heads / c->n_kv_heads, 16) > 65535 || *total > (1 << 30))
+        return fail(ctx, CC_EARG, "too many heads or rows in one call");
+    if (budget < 1) return fail(ctx, CC_EARG, "budget must be at least one page");
+    int max_seen = 0;
+    int64_t most = 0;
+    for (int j = 0; j < njobs; j++) {
+        if (jobs[j].n > OP_ROWS) return fail(ctx, CC_EARG, "a job of more than 65535 rows");
+        max_seen = std::max(max_seen, (jobs[j].past + jobs[j].n - 1) / 64 + 1);
+    }
+    (void)each_batch(jobs, njobs, OP_ROWS, [](const cc_rows& r) { return (int64_t)r.n; }, [&](const OpJobs& b) {
+        most = std::max<int64_t>(most, b.rows);
+        return hipSuccess;
+    });
+    p = attend_plan(ctx->ncu, c, most, max_seen, n_heads, budget);
+    return CC_OK;
+}
+
+cc_status sampling_dev(cc_ctx* ctx, const cc_sampling* s, int64_t vocab, SamplingDev& d) {
+    if ((s->rep || s->freq || s->pres) && !s->pen_at) return fail(ctx, CC_EARG, "sampling: rep, freq and pres need a history (pen_at)");
+    if (s->n_pen < 0 || s->n_bias < 0 || s->n_masks < 0) return fail(ctx, CC_EARG, "sampling: n_pen, n_bias and n_masks must not be negative");
+    if (s->pen_at && s->n_pen > 0 && !s->pen_ids) return fail(ctx, CC_EARG, "sampling: pen_at needs pen_ids");
+    if (s->bias_at && s->n_bias > 0 && (!s->bias_ids || !s->bias)) return fail(ctx, CC_EARG, "sampling: bias_at needs bias_ids and bias");
+    if (s->mask && !s->mask_of) return fail(ctx, CC_EARG, "sampling: mask needs mask_of");
+    if (s->mask && (int64_t)s->mask_words * 32 < vocab) return fail(ctx, CC_EARG, "sampling: mask_words is at least ceil(vocab/32)");
+    if (!(s->freq_cap >= 0.0f)) return fail(ctx, CC_EARG, "sampling: freq_cap must not be negative");
+    d = SamplingDev{s->temp, s->top_p, s->min_p, s->rep, s->freq, s->pres, s->bias, s->top_k,
+                    s->n_pen ? s->pen_at : nullptr, s->pen_ids, s->pen_counts, s->n_bias ? s->bias_at : nullptr,
+                    s->bias_ids, s->mask_of, s->mask, s->u, s->freq_cap, s->n_pen, s->n_bias, s->n_masks, s->mask_words};
+    return CC_OK;
+}
+
+cc_status check_logits(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, int32_t vocab) {
+    if (!logits || rows < 1 || rows > 65535 || vocab < 1 || vocab > (1 << 20) || ld < vocab || ld > ((int64_t)1 << 31))
+        return fail(ctx, CC_EARG, "logits: 1 .. 65535 rows of 1 .. 2^20 logits, ld at least vocab, in a device buffer");
+    return CC_OK;
+}
+
+// A C entry lets no exception out.
+template <class F>
+cc_status guarded(cc_ctx* ctx, F&& f) {
+    try {
+        const DeviceGuard dev(ctx->o.device);
+        if (dev.err != hipSuccess) return fail(ctx, CC_EDEVICE, std::string("hipSetDevice: ") + hipGetErrorString(dev.err));
+        return f();
+    } catch (...) {
+        return CC_EOOM;
+    }
+}
+
+cc_status launched(cc_ctx* ctx, const char* what, hipError_t e) {
+    return e == hipSuccess ? CC_OK : fail(ctx, CC_EDEVICE, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" {
+
+cc_status cc_cache_of(cc_ctx* ctx, int32_t layer, cc_cache* out) {
+    if (!ctx || !out) return CC_EARG;
+    const int li = layer - ctx->L0;
+    if (li < 0 || li >= (int)ctx->layers.size()) return fail(ctx, CC_EARG, "layer not held");
+    if (!ctx->layers[li].kpool) return fail(ctx, CC_EARG, "a linear_attention block keeps no KV");
+    *out = cc_cache{ctx->geom.nKV, ctx->D, ctx->rot, ctx->n_pages, ctx->max_pages, (int32_t)ctx->owned.size(), ctx->tbl_cap,
+                    ctx->layers[li].kpool, ctx->layers[li].vpool, nullptr, ctx->page_table, ctx->tbl};
+    return CC_OK;
+}
+
+size_t cc_bounds_bytes(const cc_cache* cache) {
+    if (!cache || !ok_width(cache->head_dim) || cache->n_kv_heads < 1 || cache->n_kv_heads > 1024) return 0;
+    return (size_t)cache->n_kv_heads * (2 * cache->head_dim + 4 * (cache->head_dim / 32));
+}
+
+cc_status cc_kv_append(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, const float* k, int64_t ldk,
+                       const float* v, int64_t ldv, void* stream) {
+    if (!ctx) return CC_EARG;
+    if (!cache || !k || !v) return fail(ctx, CC_EARG, "append: cache, k and v must be set");
+    return guarded(ctx, [&]() -> cc_status {
+        CacheDev c;
+        cc_status st = cache_dev(ctx, cache, c);
+        if (st != CC_OK) return st;
+        int64_t rows = 0;
+        st = check_rows(ctx, cache, jobs, njobs, &rows, true);
+        if (st != CC_OK) return st;
+        const int64_t width = (int64_t)c.nKV * c.D;
+        if (ldk < width || ldv < width) return fail(ctx, CC_EARG, "append: ldk and ldv are at least n_kv_heads * head_dim");
+        if (rows > (1 << 30)) return fail(ctx, CC_EARG, "append: too many rows in one call");
+        const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+        return launched(ctx, "append", each_batch(jobs, njobs, INT32_MAX,
+            [](const cc_rows& r) { return (int64_t)(r.past + r.n - 1) / 64 - r.past / 64 + 1; },
+            [&](const OpJobs& b) { return launch_kv_append(s, c, b, k, ldk, v, ldv); }));
+    });
+}
+
+cc_status cc_kv_bounds(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, void* stream) {
+    if (!ctx) return CC_EARG;
+    if (!cache || !cache->bounds) return fail(ctx, CC_EARG, "bounds: a cache with bounds");
+    return guarded(ctx, [&]() -> cc_status {
+        CacheDev c;
+        cc_status st = cache_dev(ctx, cache, c);
+        if (st != CC_OK) return st;
+        int64_t rows = 0;
+        st = check_rows(ctx, cache, jobs, njobs, &rows, true);
+        if (st != CC_OK) return st;
+        const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+        return launched(ctx, "bounds", each_batch(jobs, njobs, INT32_MAX,
+            [](const cc_rows& r) { return (int64_t)(r.past + r.n) / 64 - (r.past + 63) / 64; },
+            [&](const OpJobs& b) { return launch_kv_bounds(s, c, b); }));
+    });
+}
+
+size_t cc_attend_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
+                           int32_t budget) {
+    if (!ctx || !cache) return 0;
+    try {
+        CacheDev c;
+        AttendPlan p;
+        int64_t rows = 0;
+        if (cache_dev(ctx, cache, c) != CC_OK || attend_args(ctx, cache, jobs, njobs, n_heads, budget, p, &rows) != CC_OK) return 0;
+        return p.bytes;
+    } catch (...) {
+        return 0;
+    }
+}
+
+cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
+                          int32_t budget, int32_t sink, int32_t recent, const float* q, int64_t ldq, float* out,
+                          int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!ctx) return CC_EARG;
+    if (!cache || !q || !out) return fail(ctx, CC_EARG, "attend: cache, q and out must be set");
+    return guarded(ctx, [&]() -> cc_status {
+        CacheDev c;
+        cc_status st = cache_dev(ctx, cache, c);
+        if (st != CC_OK) return st;
+        AttendPlan p;
+        int64_t rows = 0;
+        st = attend_args(ctx, cache, jobs, njobs, n_heads, budget, p, &rows);
+        if (st != CC_OK) return st;
+        if (sink < 0 || recent < 1 || (int64_t)sink + recent > budget)
+            return fail(ctx, CC_EARG, "attend: sink >= 0, recent >= 1 and sink + recent <= budget");
+        p.sink = sink;
+        p.recent = recent;
+        if (p.scored && !c.bounds) return fail(ctx, CC_EARG, "attend: a row sees more pages than its budget: the cache needs bounds");
+        const int64_t width = (int64_t)n_heads * c.D;
+        if (ldq < width || ldo < width) return fail(ctx, CC_EARG, "attend: ldq and ldo are at least n_heads * head_dim");
+        if (!workspace || workspace_bytes < p.bytes || !is_aligned(workspace, 16))
+            return fail(ctx, CC_EARG, "attend: a workspace of " + std::to_string(p.bytes) + " bytes, 16-byte aligned");
+        const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+        return launched(ctx, "attend", each_batch(jobs, njobs, OP_ROWS, [](const cc_rows& r) { return (int64_t)r.n; },
+            [&](const OpJobs& b) { return launch_attend_pages(s, c, b, p, q, ldq, out, ldo, (uint8_t*)workspace); }));
+    });
+}
+
+cc_status cc_logits_adjust(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, int32_t vocab,
+                           const cc_sampling* sampling, float* out, int64_t ldo, void* stream) {
+    if (!ctx) return CC_EARG;
+    if (!sampling || !out) return fail(ctx, CC_EARG, "adjust: sampling and out must be set");
+    return guarded(ctx, [&]() -> cc_status {
+        SamplingDev d;
+        cc_status st = check_logits(ctx, logits, ld, rows, vocab);
+        if (st == CC_OK) st = sampling_dev(ctx, sampling, vocab, d);
+        if (st != CC_OK) return st;
+        if (ldo < vocab || (out == logits && ldo != ld)) return fail(ctx, CC_EARG, "adjust: ldo is at least vocab, and ld where out is logits");
+        return launched(ctx, "adjust", launch_logits_adjust(stream ? (hipStream_t)stream : ctx->stream, logits, ld, rows, vocab,
+                                                            d, out, ldo));
+    });
+}
+
+size_t cc_sample_workspace(int32_t rows, int32_t vocab) {
+    return rows < 1 || rows > 65535 || vocab < 1 || vocab > (1 << 20) ? 0 : sample_workspace(rows, vocab);
+}
+
+cc_status cc_sample(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, int32_t vocab, const cc_sampling* sampling,
+                    int32_t* ids, float* probs, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!ctx) return CC_EARG;
+    if (!sampling || !ids) return fail(ctx, CC_EARG, "sample: sampling and ids must be set");
+    return guarded(ctx, [&]() -> cc_status {
+        SamplingDev d;
+        cc_status st = check_logits(ctx, logits, ld, rows, vocab);
+        if (st == CC_OK) st = sampling_dev(ctx, sampling, vocab, d);
+        if (st != CC_OK) return st;
+        if (d.temp && !d.u) return fail(ctx, CC_EARG, "sample: a temperature needs random numbers (u)");
+        const size_t need = sample_workspace(rows, vocab);
+        if (!workspace || workspace_bytes < need || !is_aligned(workspace, 16))
+            return fail(ctx, CC_EARG, "sample: a workspace of " + std::to_string(need) + " bytes, 16-byte aligned");
+        return launched(ctx, "sample", launch_sample(stream ? (hipStream_t)stream : ctx->stream, logits, ld, rows, vocab, d,
+                                                     ids, probs, (uint8_t*)workspace));
+    });
 }
 
 }  // extern "C"

@@ -1,0 +1,738 @@
+// Operators on a paged int8 cache in device memory (cc_cache): appending rows
+// with the key bounds of the pages they complete, and attention over the pages
+// that a cheap score selects. The cache is laid out as the pass lays its own
+// out (common.h, KV geometry), so they run on a context's cache as well.
+#include "common.h"
+#include "ops.h"
+#include <algorithm>
+
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+
+// The job that holds unit u (uniform: u comes from the block's index).
+__device__ static inline OpJob job_of(const OpJobs& jobs, int u) {
+    int lo = 0, hi = jobs.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (jobs.j[mid].first <= u) lo = mid;
+        else hi = mid;
+    }
+    return jobs.j[lo];
+}
+
+// ================================================================= append ===
+// Rows of keys and values into their pages, and key bounds.
+//
+// A workgroup takes one (page that a job's rows touch, kv head, K or V). A
+// lane holds 8 consecutive channels of a row, so D/8 lanes hold the row, a
+// 32-channel group is 4 neighbouring lanes (its largest magnitude two
+// exchanges away) and a wave takes 512/D rows at a time. RoPE, amax, scale =
+// amax/127, inv = 1/scale, rint, clamp: the f32 steps of the pass's own store,
+// so the codes and scales are its bits.
+//
+// Key bounds (a page's, made when its 64th row is stored): per channel the
+// largest and the smallest of the page's 64 dequantised keys, as codes against
+// B = (largest magnitude in the 32-channel group)/127, the largest rounded up
+// and the smallest down. Rows that were there before are read back from the
+// page. Layout of a page's bounds: per kv head 2*D code bytes, channel d's
+// largest (w = 0) or smallest (w = 1) at (2w + (d%32)/16)*(D/2) + 16*(d/32) +
+// d%16, so that a lane of the score's matrix operand reads D/2 bytes in one
+// run; then, after all kv heads' codes, B as f32 [kv heads][D/32].
+__device__ static inline void bound_code(float mx, float mn, float B, int8_t& hi, int8_t& lo) {
+    hi = lo = 0;
+    if (!(B > 0.0f)) return;
+    hi = (int8_t)(int)fminf(fmaxf(ceilf(mx / B), -127.0f), 127.0f);
+    lo = (int8_t)(int)fminf(fmaxf(floorf(mn / B), -127.0f), 127.0f);
+}
+
+// VEC: the rows' groups of 8 channels are 16-byte aligned and RoPE's halves
+// are whole groups.
+template <int D, bool VEC>
+__global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, const float* __restrict__ k, int64_t ldk,
+                                                   const float* __restrict__ v, int64_t ldv, int only) {
+    constexpr int G8 = D / 8, RPW = 64 / G8, NG = D / 32;
+    __shared__ float red[2][4][D];
+    const OpJob jb = job_of(jobs, blockIdx.x);
+    const int head = blockIdx.y, which = blockIdx.z;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // bounds alone (`only`): the job's whole pages, each with 64 rows that were there before
+    const int p = (jb.past + (only ? 63 : 0)) / 64 + ((int)blockIdx.x - jb.first);
+    const int s0 = only ? 64 : max(jb.past - 64 * p, 0), s1 = only ? 64 : min(jb.past + jb.n - 64 * p, 64);
+    const uint32_t page = c.page_table[(size_t)jb.slot * c.max_pages + p];
+    if (page >= (uint32_t)c.n_pages) return;
+    uint8_t* blk = (which ? c.v : c.k) + ((size_t)page * c.nKV + head) * c.blk;
+    const int g = lane & (G8 - 1), rr = lane / G8;
+    const int half = c.rot >> 1;
+    const bool bounds = which == 0 && c.bounds != nullptr && s1 == 64;
+    float mx[8], mn[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        mx[e] = -INFINITY;
+        mn[e] = INFINITY;
+    }
+    // rows that the page held before
+    if (bounds)
+        for (int s = wave * RPW + rr; s < s0; s += 4 * RPW) {
+            const uint2 u = *(const uint2*)(blk + (size_t)s * D + kpos(8 * g, D));
+            const float sc = *(const float*)(blk + 64 * D + ((size_t)s * NG + (g >> 2)) * 4);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int code = (int)(((e < 4 ? u.x : u.y) >> (8 * (e & 3))) & 0xffu) - 128;
+                const float x = (float)code * sc;
+                mx[e] = fmaxf(mx[e], x);
+                mn[e] = fminf(mn[e], x);
+            }
+        }
+    const float* src = (which ? v : k) + (size_t)head * D;
+    const int64_t ld = which ? ldv : ldk;
+    for (int sb = s0 + wave * RPW; sb < s1; sb += 4 * RPW) {   // uniform in the wave: lanes exchange below
+        const int s = sb + rr;
+        const bool live = s < s1;
+        const int pos = 64 * p + (live ? s : s0);
+        const float* x = src + (jb.row0 + pos - jb.past) * ld + 8 * g;
+        float r[8];
+        if (VEC) {
+            const float4 a = *(const float4*)x, b = *(const float4*)(x + 4);
+            r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
+            r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+            if (which == 0 && 8 * g < c.rot) {
+                const bool low = 8 * g < half;
+                const float* y = x + (low ? half : -half);
+                const float4 ya = *(const float4*)y, yb = *(const float4*)(y + 4);
+                const float o[8] = {ya.x, ya.y, ya.z, ya.w, yb.x, yb.y, yb.z, yb.w};
+                const float4* t = (const float4*)(c.rope + ((size_t)pos * half + 8 * g - (low ? 0 : half)) * 2);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float4 cs = t[e >> 1];
+                    r[e] = low ? r[e] * cs.x - o[e] * cs.y : r[e] * cs.x + o[e] * cs.y;
+                    r[e + 1] = low ? r[e + 1] * cs.z - o[e + 1] * cs.w : r[e + 1] * cs.z + o[e + 1] * cs.w;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int d = 8 * g + e;
+                r[e] = x[e];
+                if (which == 0 && d < c.rot) {
+                    const float* t = c.rope + ((size_t)pos * half + (d < half ? d : d - half)) * 2;
+                    const float o = x[e + (d < half ? half : -half)];
+                    r[e] = d < half ? r[e] * t[0] - o * t[1] : r[e] * t[0] + o * t[1];
+                }
+            }
+        }
+        float amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(r[e]));
+        amax = fmaxf(amax, __shfl_xor(amax, 1));
+        amax = fmaxf(amax, __shfl_xor(amax, 2));
+        const float scale = amax / 127.0f;
+        const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+        if (!live) continue;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int code = (int)fminf(fmaxf(__builtin_rintf(r[e] * inv), -127.0f), 127.0f);
+            w[e >> 2] |= (uint32_t)((code ^ 0x80) & 0xff) << (8 * (e & 3));
+            const float x8 = (float)code * scale;
+            mx[e] = fmaxf(mx[e], x8);
+            mn[e] = fminf(mn[e], x8);
+        }
+        if (which == 0) {
+            *(uint2*)(blk + (size_t)s * D + kpos(8 * g, D)) = make_uint2(w[0], w[1]);
+            if ((g & 3) == 0) *(float*)(blk + 64 * D + ((size_t)s * NG + (g >> 2)) * 4) = scale;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) blk[vcode_at(8 * g + e, s, D)] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+            if ((g & 3) == 0) *(float*)(blk + 64 * D + (size_t)vscale_at(g >> 2, s, NG) * 4) = scale;
+        }
+    }
+    if (!bounds) return;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        for (int o = G8; o < 64; o <<= 1) {
+            mx[e] = fmaxf(mx[e], __shfl_xor(mx[e], o));
+            mn[e] = fminf(mn[e], __shfl_xor(mn[e], o));
+        }
+        if (rr == 0) {
+            red[0][wave][8 * g + e] = mx[e];
+            red[1][wave][8 * g + e] = mn[e];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= G8) return;
+    float amax = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int d = 8 * g + e;
+        mx[e] = fmaxf(fmaxf(red[0][0][d], red[0][1][d]), fmaxf(red[0][2][d], red[0][3][d]));
+        mn[e] = fminf(fminf(red[1][0][d], red[1][1][d]), fminf(red[1][2][d], red[1][3][d]));
+        amax = fmaxf(amax, fmaxf(fabsf(mx[e]), fabsf(mn[e])));
+    }
+    amax = fmaxf(amax, __shfl_xor(amax, 1));
+    amax = fmaxf(amax, __shfl_xor(amax, 2));
+    const float B = amax / 127.0f;
+    uint32_t w[2][2] = {{0, 0}, {0, 0}};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        int8_t hi, lo;
+        bound_code(mx[e], mn[e], B, hi, lo);
+        w[0][e >> 2] |= (uint32_t)(uint8_t)hi << (8 * (e & 3));
+        w[1][e >> 2] |= (uint32_t)(uint8_t)lo << (8 * (e & 3));
+    }
+    uint8_t* b = c.bounds + (size_t)page * c.bblk;
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+        *(uint2*)(b + head * 2 * D + (2 * q + ((g & 3) >> 1)) * (D / 2) + 16 * (g >> 2) + 8 * (g & 1)) =
+            make_uint2(w[q][0], w[q][1]);
+    if ((g & 3) == 0) *(float*)(b + c.nKV * 2 * D + (head * NG + (g >> 2)) * 4) = B;
+}
+
+template <int D>
+static void append_d(hipStream_t st, dim3 grid, bool vec, const CacheDev& c, const OpJobs& jobs, const float* k,
+                     int64_t ldk, const float* v, int64_t ldv, int only) {
+    if (vec) hipLaunchKernelGGL((k_kv_append<D, true>), grid, dim3(256), 0, st, c, jobs, k, ldk, v, ldv, only);
+    else hipLaunchKernelGGL((k_kv_append<D, false>), grid, dim3(256), 0, st, c, jobs, k, ldk, v, ldv, only);
+}
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+hipError_t launch_kv_append(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const float* k, int64_t ldk,
+                            const float* v, int64_t ldv) {
+    const bool vec = aligned16(k) && aligned16(v) && aligned16(c.rope) && ldk % 4 == 0 && ldv % 4 == 0 && c.rot % 16 == 0;
+    const dim3 grid(jobs.units, c.nKV, 2);
+    if (c.D == 64) append_d<64>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
+    else if (c.D == 128) append_d<128>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
+    else append_d<256>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_bounds(hipStream_t st, const CacheDev& c, const OpJobs& jobs) {
+    const dim3 grid(jobs.units, c.nKV, 1);
+    if (c.D == 64) append_d<64>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
+    else if (c.D == 128) append_d<128>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
+    else append_d<256>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
+    return hipGetLastError();
+}
+
+// ========================================================== selected pages ===
+// The rows' query heads of one tile (16 heads of a kv head's group), rotated
+// to the row's position: the f32 steps of rope_cs.
+template <int D>
+__device__ static inline float rotated(const float* __restrict__ q, int d, const float* __restrict__ cs, int rot) {
+    const float x = q[d];
+    if (d >= rot) return x;
+    const int half = rot >> 1;
+    if (d < half) return x * cs[2 * d] - q[d + half] * cs[2 * d + 1];
+    return x * cs[2 * (d - half)] + q[d - half] * cs[2 * (d - half) + 1];
+}
+
+// Order-preserving bits of an f32.
+__device__ static inline uint32_t order_bits(float v) {
+    const uint32_t b = f2u(v);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+// The score of a page for a row and kv head: an upper bound, in 8 bits, of
+// q . k over the page's keys, the largest over the head's query heads:
+//   sum_b T_b * B_b * (sum_{d in b} qc > 0 ? qc * hi : qc * lo),
+// qc, T the query in 8 bits per 32 channels as a key is stored, hi, lo, B the
+// page's key bounds. With the query's positive codes beside its negative ones
+// the inner sum of a 32-channel group is one 64-wide dot product, [q+ | q-] .
+// [hi | lo]: one v_mfma_i32_16x16x64_i8 for 16 query heads and 16 pages, exact.
+// The groups' sums meet in f64 (T * B is exact there), and the score is that
+// sum rounded to f32, so which pages a row keeps does not depend on an order
+// of summation.
+//
+// A wave takes SCORE_TILES tiles of 16 pages, 4 waves of a workgroup the pages
+// one after another of one row and kv head, reading 2*D + 4*D/32 bytes a page:
+// what bounds it at many pages. The rows of a job read the same bounds; the
+// later ones find them in L2.
+constexpr int SCORE_TILES = 2;
+template <int NG>
+__global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, AttendPlan p, const float* __restrict__ q,
+                                                    int64_t ldq, float* __restrict__ scores,
+                                                    uint32_t* __restrict__ counters, int n_counters) {
+    constexpr int D = 32 * NG;
+    __shared__ __align__(16) int8_t qc[16][D];
+    __shared__ float qs[16][NG];
+    // the attention launch that follows counts its finished workgroups
+    {
+        const int at = ((blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+        for (int i = at; i < n_counters; i += gridDim.x * gridDim.y * gridDim.z * 256) counters[i] = 0;
+    }
+    const int row = blockIdx.z, kvh = blockIdx.y;
+    const OpJob jb = job_of(jobs, row);
+    const int pos = jb.past + row - jb.first, seen = (pos >> 6) + 1;
+    const int page0 = blockIdx.x * (64 * SCORE_TILES), page1 = seen - p.recent;
+    if (seen <= p.budget || page0 >= page1 || page0 + 64 * SCORE_TILES <= p.sink) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, kb = lane >> 4;
+    const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
+    const float* cs = c.rope + (size_t)pos * c.rot;
+    const float* qr = q + (jb.row0 + row - jb.first) * ldq + (size_t)kvh * p.group * D;
+    u32x4 b[SCORE_TILES][NG];
+    float B[SCORE_TILES][NG];
+    int pg[SCORE_TILES];
+#pragma unroll
+    for (int t = 0; t < SCORE_TILES; t++) {
+        pg[t] = page0 + (wave * SCORE_TILES + t) * 16 + l16;
+        const uint32_t id = pg[t] < page1 ? pt[pg[t]] : 0u;
+        const uint8_t* at = c.bounds + (size_t)(id < (uint32_t)c.n_pages ? id : 0u) * c.bblk;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            b[t][g] = *(const u32x4_a4*)(at + kvh * 2 * D + kb * (D / 2) + 16 * g);
+            B[t][g] = *(const float*)(at + c.nKV * 2 * D + (kvh * NG + g) * 4);
+        }
+        if (id >= (uint32_t)c.n_pages) pg[t] = page1;   // a page index outside the cache: never kept for its score
+    }
+    float best[SCORE_TILES];
+#pragma unroll
+    for (int t = 0; t < SCORE_TILES; t++) best[t] = -INFINITY;
+    for (int h0 = 0; h0 < p.group; h0 += 16) {
+        const int gt = min(16, p.group - h0);
+        if (h0) __syncthreads();
+        for (int i = threadIdx.x; i < 16 * D; i += 256) {   // 32 lanes hold a group of channels
+            const int h = i / D, d = i & (D - 1);
+            const float x = h < gt ? rotated<D>(qr + (size_t)(h0 + h) * D, d, cs, c.rot) : 0.0f;
+            float amax = fabsf(x);
+            for (int o = 1; o < 32; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+            const float scale = amax / 127.0f;
+            const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+            qc[h][d] = (int8_t)(int)fminf(fmaxf(__builtin_rintf(x * inv), -127.0f), 127.0f);
+            if ((d & 31) == 0) qs[h][d >> 5] = scale;
+        }
+        __syncthreads();
+        // the lane's operand: head l16, codes 32g + 16(kb % 2) .., the positive (kb < 2) or the negative ones
+        u32x4 a[NG];
+        float T[4][NG];
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const u32x4 w = *(const u32x4*)&qc[l16][32 * g + 16 * (kb & 1)];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t neg = ((w[e] >> 7) & 0x01010101u) * 0xffu;
+                a[g][e] = w[e] & (kb < 2 ? ~neg : neg);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) T[r][g] = qs[4 * kb + r][g];
+        }
+#pragma unroll
+        for (int t = 0; t < SCORE_TILES; t++) {
+            double acc[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                i32x4 d = {0, 0, 0, 0};
+                d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a[g]),
+                                                          __builtin_bit_cast(i32x4, b[t][g]), d, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[r] = fma((double)T[r][g] * (double)B[t][g], (double)d[r], acc[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (4 * kb + r < gt) best[t] = fmaxf(best[t], (float)acc[r]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < SCORE_TILES; t++) {
+        best[t] = fmaxf(best[t], __shfl_xor(best[t], 16));
+        best[t] = fmaxf(best[t], __shfl_xor(best[t], 32));
+        const int page = page0 + (wave * SCORE_TILES + t) * 16 + l16;
+        if (kb == 0 && page < page1)
+            scores[((size_t)row * c.nKV + kvh) * p.max_seen + page] = pg[t] < page1 ? best[t] : -INFINITY;
+    }
+}
+
+// The pages that a row and kv head keep, ascending: entries [e0, e1) of them
+// into list (LDS). Entry order: the first `sink` pages, the `need` best of the
+// pages [a, z) by score (ties to the lower page), the last `recent`. The
+// `need`-th largest score comes from four passes over its bits from the top,
+// 8 at a time, with a count of the scores that share the bits so far; then
+// every thread ranks a run of pages.
+__device__ static inline void kept_pages(const float* __restrict__ sc, int a, int z, int need, int sink, int e0, int e1,
+                                         int recent0, uint16_t* list, uint32_t* hist, uint32_t* s_sel) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    uint32_t prefix = 0, left = (uint32_t)need;
+    for (int sh = 24; sh >= 0 && need > 0; sh -= 8) {
+        hist[t] = 0;
+        __syncthreads();
+        for (int i = a + t; i < z; i += 256) {
+            const uint32_t k = order_bits(sc[i]);
+            if (sh == 24 || (k >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(k >> sh) & 255u], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {
+            // lane l: digits 255 - 4l .. 252 - 4l, from the largest down
+            uint32_t n[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                n[e] = hist[255 - 4 * lane - e];
+                sum += n[e];
+            }
+            uint32_t before = sum;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t x = __shfl_up(before, o);
+                if (lane >= o) before += x;
+            }
+            before -= sum;
+            if (before < left && left <= before + sum) {
+                int e = 0;
+                while (before + n[e] < left) before += n[e++];
+                s_sel[0] = prefix | ((uint32_t)(255 - 4 * lane - e) << sh);
+                s_sel[1] = left - before;
+            }
+        }
+        __syncthreads();
+        prefix = s_sel[0];
+        left = s_sel[1];
+    }
+    // prefix: the need-th largest score's bits; `left` of the pages that have them are kept
+    if (need == 0) z = a;
+    const int per = (z - a + 255) / 256, i0 = a + t * per, i1 = min(i0 + per, z);
+    uint32_t gt = 0, eq = 0;
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = order_bits(sc[i]);
+        gt += k > prefix;
+        eq += k == prefix;
+    }
+    uint32_t bg = gt, be = eq;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_up(bg, o), y = __shfl_up(be, o);
+        if (lane >= o) {
+            bg += x;
+            be += y;
+        }
+    }
+    if (lane == 63) {
+        hist[wave] = bg;
+        hist[4 + wave] = be;
+    }
+    __syncthreads();
+    bg -= gt;
+    be -= eq;
+    for (int w = 0; w < wave; w++) {
+        bg += hist[w];
+        be += hist[4 + w];
+    }
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = order_bits(sc[i]);
+        const bool keep = k > prefix || (k == prefix && be < left);
+        if (keep) {
+            const int e = sink + (int)(bg + min(be, left));
+            if (e >= e0 && e < e1) list[e - e0] = (uint16_t)i;
+        }
+        bg += k > prefix;
+        be += k == prefix;
+    }
+    for (int e = e0 + t; e < e1; e += 256) {
+        if (e < sink) list[e - e0] = (uint16_t)e;
+        if (e >= sink + need) list[e - e0] = (uint16_t)(recent0 + e - sink - need);
+    }
+}
+
+// Attention of a row's query heads (a tile of up to 16 of one kv head's) over
+// its kept pages, split over workgroups of `per` pages and those over four
+// waves. A wave walks its pages as the pass's attention does (online softmax
+// in log2 units; S^T = K . Q^T with the query as an f16 pair; O^T += V^T .
+// (p * s) with p * s as an f16 pair; one page of codes in flight), but its
+// pages come from a list. The waves' parts meet in LDS, the workgroups' in the
+// workspace: the last workgroup of a (row, tile) to finish joins them in split
+// order, whichever it is, so a row's result does not depend on it.
+template <int NG>
+__global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c, OpJobs jobs, AttendPlan p,
+                                                                      const float* __restrict__ q, int64_t ldq,
+                                                                      const float* __restrict__ scores,
+                                                                      float* __restrict__ partials,
+                                                                      uint32_t* __restrict__ counters,
+                                                                      float* __restrict__ out, int64_t ldo) {
+    constexpr int D = 32 * NG, DT = D / 16, SCL = NG > 4 ? NG / 4 : 1;
+    constexpr int OW = 16 * D + 32;   // floats of a wave's part: O [16][D], max [16], sum [16]
+    __shared__ __align__(16) float smem[ATTEND_WAVES * OW];
+    __shared__ uint16_t list[ATTEND_PER];
+    __shared__ uint32_t hist[256], s_sel[2];
+    const int row = blockIdx.z, split = blockIdx.x, kvh = blockIdx.y % c.nKV, tile = blockIdx.y / c.nKV;
+    const OpJob jb = job_of(jobs, row);
+    const int pos = jb.past + row - jb.first, seen = (pos >> 6) + 1;
+    const int kept = min(seen, p.budget);
+    const int splits = (kept + p.per - 1) / p.per;   // of this row
+    if (split >= splits) return;
+    const int e0 = split * p.per, e1 = min(e0 + p.per, kept);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j4 = lane >> 4, l16 = lane & 15;
+    const int h0 = tile * 16, gt = min(16, p.group - h0);
+    const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
+    // the query heads, rotated, in LDS (a wave's scale slices and part come there later)
+    {
+        const float* cs = c.rope + (size_t)pos * c.rot;
+        const float* qr = q + (jb.row0 + row - jb.first) * ldq + (size_t)(kvh * p.group + h0) * D;
+        for (int i = tid; i < 16 * D; i += 256)
+            smem[i] = i < gt * D ? rotated<D>(qr + (size_t)(i / D) * D, i & (D - 1), cs, c.rot) : 0.0f;
+    }
+    if (seen > p.budget) {
+        kept_pages(scores + ((size_t)row * c.nKV + kvh) * p.max_seen, p.sink, seen - p.recent,
+                   p.budget - p.sink - p.recent, p.sink, e0, e1, seen - p.recent, list, hist, s_sel);
+    } else {
+        for (int e = e0 + tid; e < e1; e += 256) list[e - e0] = (uint16_t)e;
+    }
+    __syncthreads();
+    half8_t qh[NG], ql[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            _Float16 hi, lo;
+            split_hilo(smem[l16 * D + 32 * g + 8 * j4 + e], hi, lo);
+            qh[g][e] = hi;
+            ql[g][e] = lo;
+        }
+    __syncthreads();   // every wave has its query: the space is free
+    // this wave's entries of the list, their pages' indices one a lane
+    const int n = e1 - e0, w0 = (n * wave) / ATTEND_WAVES, w1 = (n * (wave + 1)) / ATTEND_WAVES, nw = w1 - w0;
+    const int lp = lane < nw ? (int)list[w0 + lane] : 0;
+    const uint32_t pgv = lane < nw ? pt[lp] : 0u;
+    float* ksl = smem + wave * OW;
+    float* vsl = ksl + 256 * SCL;
+    const float score_scale = 1.4426950408889634f / sqrtf((float)D);
+    const size_t pstride = (size_t)c.nKV * c.blk, hoff = (size_t)kvh * c.blk;
+    auto page_rsrc = [&](const uint8_t* pool, int i) {
+        const uint32_t pg = __builtin_amdgcn_readlane(pgv, i);
+        const bool ok = pg < (uint32_t)c.n_pages;   // an index outside the cache: the page reads as zero, and is masked
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(pool + (ok ? (size_t)pg * pstride + hoff : 0)), 0,
+                                                 ok ? c.blk : 0, 0x00020000);
+    };
+    const int vk = l16 * D + (D / 4) * j4, vv = j4 * D * 16 + l16 * 16;
+    int vso[SCL];
+#pragma unroll
+    for (int s = 0; s < SCL; s++) {
+        const int e = 256 * s + lane * 4, b = e >> 6, jb4 = (e >> 4) & 3;
+        vso[s] = 4 * ((jb4 * NG + b) * 16 + (e & 15));
+    }
+    float mrow = -INFINITY, lsum = 0.0f;
+    bool shifted = true;
+    float4_t o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) o[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+    u32x4 kc[4][NG / 2], vc[DT], kst[SCL], vst[SCL];
+    auto load_k = [&](__amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv) {
+#pragma unroll
+        for (int s = 0; s < SCL; s++) {
+            // D = 64: a scale block is 512 bytes; lanes past it read zero
+            kst[s] = __builtin_amdgcn_raw_buffer_load_b128(rk, lane * 16, 64 * D + 1024 * s, 0);
+            vst[s] = __builtin_amdgcn_raw_buffer_load_b128(rv, vso[s], 64 * D, 0);
+        }
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+            for (int s = 0; s < NG / 2; s++)
+                kc[tt][s] = __builtin_amdgcn_raw_buffer_load_b128(rk, vk, tt * 16 * D + 16 * s, 0);
+    };
+    auto load_v = [&](__amdgpu_buffer_rsrc_t rv) {
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) vc[dt] = __builtin_amdgcn_raw_buffer_load_b128(rv, vv, dt * 256, 0);
+    };
+    auto page = [&](int i) {
+        const int in = i + 1 < nw ? i + 1 : i;
+        const int p64 = 64 * __builtin_amdgcn_readlane(lp, i);
+        const bool bad = (uint32_t)__builtin_amdgcn_readlane(pgv, i) >= (uint32_t)c.n_pages;
+        const int last = bad ? -1 : pos;   // the last token that counts
+        bool big = false;
+#pragma unroll
+        for (int s = 0; s < SCL; s++) {
+            *(u32x4*)&ksl[256 * s + lane * 4] = kst[s];
+            u32x4 v = vst[s];
+            if (p64 + 63 > last) {   // tokens past the row: whatever scale lies there, NaN too, goes in as zero
+                const int t0 = p64 + 16 * (lane & 3) + 4 * (((256 * s + lane * 4) >> 4) & 3);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (t0 + e > last) v[e] = 0u;
+            }
+            big = big || pv_big(v);
+            *(u32x4*)&vsl[256 * s + lane * 4] = v;
+        }
+        const bool pbig = __builtin_amdgcn_ballot_w64(big) != 0;
+        float pr[4][4];
+        float pm = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++) {
+            float ks[4 * NG];
+#pragma unroll
+            for (int s = 0; s < NG; s++) {
+                const float4 f = *(const float4*)&ksl[(tt * 16 + 4 * j4) * NG + 4 * s];
+                ks[4 * s] = f.x; ks[4 * s + 1] = f.y; ks[4 * s + 2] = f.z; ks[4 * s + 3] = f.w;
+            }
+            float4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const u32x4 w = kc[tt][g >> 1];
+                const half8_t kf = (g & 1) ? dequant8_biased(w[2], w[3]) : dequant8_biased(w[0], w[1]);
+                float4_t pp = {0.f, 0.f, 0.f, 0.f};
+                pp = mfma16x16x32(kf, qh[g], pp);
+                pp = mfma16x16x32(kf, ql[g], pp);
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(ks[r * NG + g], pp[r], acc[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) pr[tt][r] = acc[r] * score_scale;
+        }
+        if (p64 + 63 > last) {
+#pragma unroll
+            for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (p64 + tt * 16 + 4 * j4 + r > last) pr[tt][r] = -INFINITY;
+        }
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) pm = fmaxf(pm, pr[tt][r]);
+        const auto rvn = page_rsrc(c.v, in);
+        load_k(page_rsrc(c.k, in), rvn);
+        __builtin_amdgcn_sched_barrier(0);
+        pm = fmaxf(pm, __shfl_xor(pm, 16));
+        pm = fmaxf(pm, __shfl_xor(pm, 32));
+        const float mnew = fmaxf(mrow, pm);
+        const bool drop = pbig || !(fabsf(mnew) < PV_MAX_SCORE);
+        const float shrink = drop && shifted ? PV_UNSHIFT : 1.0f;
+        shifted = shifted && !drop;
+        const float alpha = (mrow == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrow - mnew)) * shrink;
+        lsum *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) o[dt][r] *= alpha;
+        const float msub = (mnew == -INFINITY ? 0.0f : mnew) - (shifted ? PV_SHIFT_LOG2 : 0.0f);
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float e = __builtin_amdgcn_exp2f(pr[tt][r] - msub);
+                pr[tt][r] = e;
+                lsum += e;
+            }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < NG; b++) {
+            float sv[16];
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const float4 f = *(const float4*)&vsl[b * 64 + 16 * j4 + 4 * s];
+                sv[4 * s] = f.x; sv[4 * s + 1] = f.y; sv[4 * s + 2] = f.z; sv[4 * s + 3] = f.w;
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                u32x4 phw, plw;
+#pragma unroll
+                for (int ii = 0; ii < 8; ii += 2) {
+                    const int tt = 2 * ks + (ii >> 2), r = ii & 3;
+                    uint32_t h, l;
+                    split_hilo2(pr[tt][r] * sv[4 * tt + r], pr[tt][r + 1] * sv[4 * tt + r + 1], h, l);
+                    phw[ii >> 1] = h;
+                    plw[ii >> 1] = l;
+                }
+                const half8_t ph = __builtin_bit_cast(half8_t, phw), pl = __builtin_bit_cast(half8_t, plw);
+#pragma unroll
+                for (int dd = 0; dd < 2; dd++) {
+                    const int dt = 2 * b + dd;
+                    const u32x4 w = vc[dt];
+                    const half8_t vf = ks ? dequant8_biased(w[2], w[3]) : dequant8_biased(w[0], w[1]);
+                    o[dt] = mfma16x16x32(vf, ph, o[dt]);
+                    o[dt] = mfma16x16x32(vf, pl, o[dt]);
+                }
+            }
+        }
+        mrow = mnew;
+        load_v(rvn);
+    };
+    if (nw > 0) {
+        const auto rv = page_rsrc(c.v, 0);
+        load_k(page_rsrc(c.k, 0), rv);
+        load_v(rv);
+        for (int i = 0; i < nw; i++) page(i);
+    }
+    lsum += __shfl_xor(lsum, 16);
+    lsum += __shfl_xor(lsum, 32);
+    {
+        const float un = shifted ? PV_UNSHIFT : 1.0f;
+        float* part = smem + wave * OW;   // its scale slices are this wave's own and done with
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) *(float4_t*)(part + l16 * D + dt * 16 + 4 * j4) = o[dt] * un;
+        if (j4 == 0) {
+            part[16 * D + l16] = mrow;
+            part[16 * D + 16 + l16] = lsum * un;
+        }
+    }
+    __syncthreads();
+    // the four waves' parts of the tile's heads
+    float* dst = out + (jb.row0 + row - jb.first) * ldo + (size_t)(kvh * p.group + h0) * D;
+    const size_t unit = ((size_t)row * c.nKV + kvh) * p.tiles + tile;
+    const int gw = min(16, p.group);
+    float* mine = partials + (unit * p.splits + split) * ((size_t)gw * (D + 2));
+    for (int i = tid; i < gt * D; i += 256) {
+        const int h = i / D, d = i & (D - 1);
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < ATTEND_WAVES; w++) m = fmaxf(m, smem[w * OW + 16 * D + h]);
+        const float ms = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < ATTEND_WAVES; w++) {
+            const float* part = smem + w * OW;
+            const float f = __builtin_amdgcn_exp2f(part[16 * D + h] - ms);
+            l = __builtin_fmaf(part[16 * D + 16 + h], f, l);
+            x = __builtin_fmaf(part[h * D + d], f, x);
+        }
+        if (splits == 1) {
+            dst[(size_t)h * D + d] = l > 0.0f ? x / l : 0.0f;
+        } else {
+            mine[(size_t)h * (D + 2) + 2 + d] = x;
+            if (d == 0) {
+                mine[(size_t)h * (D + 2)] = m;
+                mine[(size_t)h * (D + 2) + 1] = l;
+            }
+        }
+    }
+    if (splits == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_sel[0] = atomicAdd(&counters[unit], 1u);
+    __syncthreads();
+    if (s_sel[0] != (uint32_t)(splits - 1)) return;
+    __threadfence();
+    const float* all = partials + unit * p.splits * ((size_t)gw * (D + 2));
+    for (int i = tid; i < gt * D; i += 256) {
+        const int h = i / D, d = i & (D - 1);
+        const float* part = all + (size_t)h * (D + 2);
+        const size_t step = (size_t)gw * (D + 2);
+        float m = -INFINITY;
+        for (int s = 0; s < splits; s++) m = fmaxf(m, __builtin_nontemporal_load(part + s * step));
+        const float ms = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, x = 0.0f;
+        for (int s = 0; s < splits; s++) {
+            const float f = __builtin_amdgcn_exp2f(__builtin_nontemporal_load(part + s * step) - ms);
+            l = __builtin_fmaf(__builtin_nontemporal_load(part + s * step + 1), f, l);
+            x = __builtin_fmaf(__builtin_nontemporal_load(part + s * step + 2 + d), f, x);
+        }
+        dst[(size_t)h * D + d] = l > 0.0f ? x / l : 0.0f;
+    }
+}
+
+template <int NG>
+static void attend_ng(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& p, const float* q,
+                      int64_t ldq, float* out, int64_t ldo, uint8_t* ws) {
+    float* scores = (float*)(ws + p.scores);
+    float* partials = (float*)(ws + p.partials);
+    uint32_t* counters = (uint32_t*)(ws + p.counters);
+    if (p.scored || p.splits > 1) {
+        const int n_counters = p.splits > 1 ? jobs.rows * c.nKV * p.tiles : 0;
+        const int bx = p.scored ? (p.max_seen - p.recent + 64 * SCORE_TILES - 1) / (64 * SCORE_TILES) : 1;
+        hipLaunchKernelGGL((k_page_score<NG>), dim3(std::max(bx, 1), c.nKV, jobs.rows), dim3(256), 0, st, c, jobs, p, q,
+                           ldq, scores, counters, n_counters);
+    }
+    hipLaunchKernelGGL((k_attend_pages<NG>), dim3(p.splits, c.nKV * p.tiles, jobs.rows), dim3(256), 0, st, c, jobs, p,
+                       q, ldq, scores, partials, counters, out, ldo);
+}
+
+hipError_t launch_attend_pages(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& p,
+                               const float* q, int64_t ldq, float* out, int64_t ldo, uint8_t* ws) {
+    if (c.ng == 2) attend_ng<2>(st, c, jobs, p, q, ldq, out, ldo, ws);
+    else if (c.ng == 4) attend_ng<4>(st, c, jobs, p, q, ldq, out, ldo, ws);
+    else attend_ng<8>(st, c, jobs, p, q, ldq, out, ldo, ws);
+    return hipGetLastError();
+}

@@ -191,6 +191,16 @@ __device__ static inline void split_hilo2(float x0, float x1, uint32_t& hi, uint
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
+// Whether any of four V scales (f32 bits) is too large for the shifted P.V
+// split (p * s * PV_SHIFT would overflow f16) — or not finite.
+__device__ static inline bool pv_big(u32x4 v) {
+    bool b = false;
+#pragma unroll
+    for (int e = 0; e < 4; e++) b = b || !(__uint_as_float(v[e]) <= PV_SCALE_MAX);
+    return b;
+}
+
+
 __device__ static inline float wave_max(float v) {
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     return v;
@@ -198,4 +208,31 @@ __device__ static inline float wave_max(float v) {
 __device__ static inline float wave_sum(float v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
+}
+
+// ============================================================ KV geometry ===
+// One (page, kv head) block of the pool, blk = 64*D + 64*ng*4 bytes:
+//   K: codes [64 tokens][D] with column d at (D/4)*((d%32)/8) + 8*(d/32) + d%8,
+//      so one lane's fragment bytes for every group are contiguous; then f32
+//      scales [64 tokens][ng].
+//   V: codes [4][D][16]: with v = vpos(s) = 16*((s%16)/4) + 4*(s/16) + s%4,
+//      token s's code for channel d sits in 16-byte row (v/16, d) at byte
+//      v%16, so a lane's P·V fragment (16 tokens of one channel) is one
+//      contiguous 16-byte load, and one token's D codes lie in D*16 bytes
+//      (a new token dirties 16 lines of 128 B at D = 128, not the 64 of a
+//      [D][64] layout); then f32 scales [4][ng][16] at the same positions.
+// Codes are stored biased (code ^ 0x80, i.e. code + 128) so the MFMA dequant
+// puts them under an f16 exponent directly; they are the reference's store_kv
+// codes bit for bit once converted back (k_kv_ref: cc_read_kv, cc_write_kv).
+__host__ __device__ static inline int kpos(int d, int D) { return (D / 4) * ((d & 31) >> 3) + 8 * (d >> 5) + (d & 7); }
+__host__ __device__ static inline int vpos(int s) { return 16 * ((s & 15) >> 2) + 4 * (s >> 4) + (s & 3); }
+// byte of V code (channel d, token s) in its block, and float of V scale
+// (group b, token s) after the codes
+__host__ __device__ static inline int vcode_at(int d, int s, int D) {
+    const int v = vpos(s);
+    return ((v >> 4) * D + d) * 16 + (v & 15);
+}
+__host__ __device__ static inline int vscale_at(int b, int s, int ng) {
+    const int v = vpos(s);
+    return ((v >> 4) * ng + b) * 16 + (v & 15);
 }

@@ -1614,33 +1614,6 @@ void launch_fin_swiglu(hipStream_t st, const float* part, int splits, int M, int
     CHECK_LAUNCH();
 }
 
-// ============================================================ KV geometry ===
-// One (page, kv head) block of the pool, blk = 64*D + 64*ng*4 bytes:
-//   K: codes [64 tokens][D] with column d at (D/4)*((d%32)/8) + 8*(d/32) + d%8,
-//      so one lane's fragment bytes for every group are contiguous; then f32
-//      scales [64 tokens][ng].
-//   V: codes [4][D][16]: with v = vpos(s) = 16*((s%16)/4) + 4*(s/16) + s%4,
-//      token s's code for channel d sits in 16-byte row (v/16, d) at byte
-//      v%16, so a lane's P·V fragment (16 tokens of one channel) is one
-//      contiguous 16-byte load, and one token's D codes lie in D*16 bytes
-//      (a new token dirties 16 lines of 128 B at D = 128, not the 64 of a
-//      [D][64] layout); then f32 scales [4][ng][16] at the same positions.
-// Codes are stored biased (code ^ 0x80, i.e. code + 128) so the MFMA dequant
-// puts them under an f16 exponent directly; they are the reference's store_kv
-// codes bit for bit once converted back (k_kv_ref: cc_read_kv, cc_write_kv).
-__host__ __device__ static inline int kpos(int d, int D) { return (D / 4) * ((d & 31) >> 3) + 8 * (d >> 5) + (d & 7); }
-__host__ __device__ static inline int vpos(int s) { return 16 * ((s & 15) >> 2) + 4 * (s >> 4) + (s & 3); }
-// byte of V code (channel d, token s) in its block, and float of V scale
-// (group b, token s) after the codes
-__host__ __device__ static inline int vcode_at(int d, int s, int D) {
-    const int v = vpos(s);
-    return ((v >> 4) * D + d) * 16 + (v & 15);
-}
-__host__ __device__ static inline int vscale_at(int b, int s, int ng) {
-    const int v = vpos(s);
-    return ((v >> 4) * ng + b) * 16 + (v & 15);
-}
-
 // store_kv (web/model/kernels.js:1024-1073) for a row's K and V, plus RoPE on
 // its Q (kernels.js:1093-1129) into the attention operand, after the q|k|v
 // splits are summed.
@@ -2525,15 +2498,6 @@ void launch_lin_norm(hipStream_t st, const float* core, const float* lraw, const
 // mask, and a still fully masked row (max -inf) just takes alpha = 0, p = 0.
 // One work item of a wave: its (job, kv head, m-tile) over the chunk's pages,
 // with the wave's LDS slices for the page's K and V scale blocks.
-// Whether any of four V scales (f32 bits) is too large for the shifted P.V
-// split (p * s * PV_SHIFT would overflow f16) — or not finite.
-__device__ static inline bool pv_big(u32x4 v) {
-    bool b = false;
-#pragma unroll
-    for (int e = 0; e < 4; e++) b = b || !(__uint_as_float(v[e]) <= PV_SCALE_MAX);
-    return b;
-}
-
 template <int NG>
 __device__ __forceinline__ void attn_item(const AttnItem& it, const uint4* __restrict__ Qp,
                                           const uint8_t* __restrict__ kpool, const uint8_t* __restrict__ vpool,

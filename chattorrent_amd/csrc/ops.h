@@ -1,0 +1,67 @@
+// Launchers of the operators on the caller's own device buffers
+// (cache_ops.hip: paged cache; logit_ops.hip: logits and sampling). Shapes are
+// validated by the caller (api.hip) before a launch; each launcher returns its
+// launch's error.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+// ------------------------------------------------------------ paged cache ---
+// A paged int8 cache (cc_cache): blk bytes per (page, kv head) block, bblk
+// bytes of key bounds per page (all kv heads).
+struct CacheDev {
+    uint8_t* k = nullptr;
+    uint8_t* v = nullptr;
+    uint8_t* bounds = nullptr;
+    const uint32_t* page_table = nullptr;
+    const float* rope = nullptr;
+    int nKV = 0, D = 0, ng = 0, rot = 0, n_pages = 0, max_pages = 0, blk = 0, bblk = 0;
+};
+
+// A launch's jobs, by value in its kernel arguments (no table to upload, and a
+// captured launch keeps them): `first` is the job's first unit of work and
+// row0 its first row of the call.
+constexpr int OP_JOBS = 128;
+struct OpJob {
+    int32_t slot, past, n, row0, first;
+};
+struct OpJobs {
+    int n = 0, rows = 0, units = 0;
+    OpJob j[OP_JOBS];
+};
+
+// units: pages that the jobs' rows touch.
+hipError_t launch_kv_append(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const float* k, int64_t ldk,
+                            const float* v, int64_t ldv);
+// units: pages that lie in the jobs' rows as a whole.
+hipError_t launch_kv_bounds(hipStream_t st, const CacheDev& c, const OpJobs& jobs);
+
+// How cc_attend_pages lays a call out: work of a row and kv head is `splits`
+// workgroups for each 16 query heads (`tiles`), `per` kept pages each.
+constexpr int ATTEND_WAVES = 4, ATTEND_PER = 64 * ATTEND_WAVES;   // one page index a lane
+struct AttendPlan {
+    int group = 0, tiles = 0, splits = 0, per = 0;
+    int max_seen = 0;             // the most pages that a row sees
+    int budget = 0, sink = 0, recent = 0;
+    bool scored = false;          // a row sees more pages than it keeps
+    size_t scores = 0, partials = 0, counters = 0, bytes = 0;   // offsets into the workspace, and its size
+};
+// units: rows.
+hipError_t launch_attend_pages(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& p,
+                               const float* q, int64_t ldq, float* out, int64_t ldo, uint8_t* ws);
+
+// -------------------------------------------------------- logits, sampling ---
+// cc_sampling with its pointers typed; null: that part is off.
+struct SamplingDev {
+    const float *temp, *top_p, *min_p, *rep, *freq, *pres, *bias;
+    const int32_t *top_k, *pen_at, *pen_ids, *pen_counts, *bias_at, *bias_ids, *mask_of;
+    const uint32_t* mask;
+    const double* u;
+    float freq_cap;
+    int n_pen, n_bias, n_masks, mask_words;
+};
+hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s,
+                                float* out, int64_t ldo);
+size_t sample_workspace(int rows, int V);
+hipError_t launch_sample(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s,
+                         int32_t* ids, float* probs, uint8_t* ws);

@@ -304,6 +304,160 @@ cc_status cc_op_rmsnorm(cc_ctx* ctx, const float* x, const float* w, int32_t T, 
 cc_status cc_op_attend(cc_ctx* ctx, int32_t layer, int32_t slot, const float* q, int32_t n,
                        int32_t past, float* out);
 
+/* ---- Operators on the caller's device buffers: one decode step of long
+ * chats, from the paged cache to the token, for callers that run their own
+ * blocks or sample rows themselves. They stand beside cc_topk_noalloc: every
+ * buffer is device memory of the context's GPU that the caller owns, nothing
+ * is allocated or copied, and a call runs asynchronously on `stream` (a
+ * hipStream_t; NULL: the context's stream), in kernels alone, so it can be
+ * captured into a HIP graph (its jobs and pointers are then the captured
+ * ones). The context gives the GPU and holds the error message; calls on one
+ * context from two threads must not overlap. Calls on several streams may
+ * overlap on the GPU as long as they share no workspace and no rows that one
+ * of them writes. No counterpart in the reference, whose cache ops are inside
+ * its pass and whose sampler runs on the host (web/model/sampling.js). ---- */
+
+/* A paged int8 cache, K and V of one layer. Each (page of 64 tokens, kv head)
+ * is a block of 64*D code bytes (code + 128) and then 64*D/32 f32 scales, one
+ * per token and 32 channels; `k` and `v` are [n_pages][n_kv_heads] blocks:
+ *   K: token t, channel d at t*D + (D/4)*((d%32)/8) + 8*(d/32) + d%8, scale of
+ *      group g at t*D/32 + g;
+ *   V: with u = 16*((t%16)/4) + 4*(t/16) + t%4, code at ((u/16)*D + d)*16 +
+ *      u%16, scale at ((u/16)*D/32 + g)*16 + u%16.
+ * page_table [slots][max_pages]: a slot's pages in token order (an index of
+ * n_pages or more is no page: rows are not stored there, and its tokens are
+ * masked). rope [rope_rows][rot_dim/2][2]: cos and sin of each position, f32.
+ * bounds (may be NULL): key bounds, n_pages * cc_bounds_bytes(cache) bytes:
+ * per page and kv head 2*D int8 codes, channel d's largest (w = 0) and
+ * smallest (w = 1) key of the page's 64 tokens at (2w + (d%32)/16)*(D/2) +
+ * 16*(d/32) + d%16, then, after all kv heads' codes, f32 scales
+ * [n_kv_heads][D/32]. k, v and bounds are 16-byte aligned; D (head_dim) is 64,
+ * 128 or 256; rot_dim is even, at most D; max_pages at most 32768. */
+typedef struct cc_cache {
+    int32_t n_kv_heads, head_dim, rot_dim;
+    int32_t n_pages, max_pages, slots, rope_rows;
+    void* k;
+    void* v;
+    void* bounds;
+    const uint32_t* page_table;
+    const float* rope;
+} cc_cache;
+/* The context's own cache of block `layer` (bounds NULL: the caller may set
+ * its own). Its pages are the context's to give: cc_step, cc_fill_random_kv
+ * and cc_release change the page table on the context's stream. */
+cc_status cc_cache_of(cc_ctx* ctx, int32_t layer, cc_cache* out);
+/* Bytes of key bounds a page takes; 0 for a head_dim that is not supported. */
+size_t cc_bounds_bytes(const cc_cache* cache);
+
+/* `n` rows of a slot from position `past`. The rows of a call's jobs lie
+ * behind each other in job order. Host memory, read during the call. */
+typedef struct cc_rows {
+    int32_t slot, past, n;
+} cc_rows;
+
+/* Stores the jobs' rows: k, rotated to its position, and v, both f32 [rows]
+ * [n_kv_heads * D] with ldk and ldv floats from row to row, in 32-channel
+ * groups of int8 codes as store_kv rounds them (web/model/kernels.js:1024-1073:
+ * the pass's own bits). Where the cache has bounds, a page whose last row is
+ * among them gets its key bounds, from its 64 rows as the cache holds them:
+ * per 32 channels B = (largest magnitude)/127, the largest key of a channel as
+ * ceil(key/B), the smallest as floor(key/B), both within +-127. The page's
+ * earlier rows are those stored before. The slots' pages must be in the page
+ * table. CC_EARG: a slot twice in a call, rows past max_pages*64 or rope_rows. */
+cc_status cc_kv_append(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, const float* k,
+                       int64_t ldk, const float* v, int64_t ldv, void* stream);
+/* Key bounds of the pages that lie within the jobs' rows as a whole, from what
+ * the cache holds: for rows that another path stored (cc_step). */
+cc_status cc_kv_bounds(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, void* stream);
+
+/* Attention of the jobs' rows over selected pages. Row i of a job is at
+ * position past + i and sees the tokens up to its own (stored before). q f32
+ * [rows][n_heads * D] before RoPE, ldq floats from row to row; out alike, with
+ * ldo. Query head h reads kv head h / (n_heads / n_kv_heads).
+ * A row sees P = (past + i)/64 + 1 pages. Up to `budget` it reads them all.
+ * Else each kv head of it reads `budget` of them: the first `sink`, the last
+ * `recent`, and the best of the others by score, ties to the lower page. With
+ * the rotated query in 8 bits as store_kv rounds a key (codes c, scales T per
+ * 32 channels) and a page's bounds (hi, lo, B), a query head's score is the
+ *   sum over groups g of T_g * B_g * sum over d in g of max(c*hi, c*lo),
+ * and the kv head's the largest over its query heads, rounded to f32.
+ * out = softmax(q . k / sqrt(D)) v over the tokens read.
+ * 0 <= sink, 1 <= recent, sink + recent <= budget. cache->bounds is needed
+ * where a row sees more than `budget` pages: the pages before the row's last
+ * `recent` have theirs. `workspace`: cc_attend_workspace bytes, 16-byte
+ * aligned, of any contents; two calls that may overlap need two. */
+size_t cc_attend_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
+                           int32_t budget);
+cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
+                          int32_t budget, int32_t sink, int32_t recent, const float* q, int64_t ldq, float* out,
+                          int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
+
+/* What a call asks of each of its rows: device arrays [rows], or NULL where
+ * none asks for it. The meaning is the reference's sampler's
+ * (web/model/sampling.js:57-215) with two more cuts, biases and masks.
+ *   temp       0 or below: greedy
+ *   top_k      0 or below, or vocab and more: off
+ *   top_p      1 and more: off;  min_p  0: off (at most 1 counts)
+ *   rep, freq, pres   penalties of the tokens in the row's history (1, 0 and 0:
+ *              none); one token's frequency penalty is at most freq_cap
+ *   pen_at [rows+1], pen_ids [n_pen], pen_counts [n_pen] or NULL: row r's
+ *              history is the entries [pen_at[r], pen_at[r+1]); an entry counts
+ *              pen_counts, or 1, and an id's entries add up (0 or below: no
+ *              entry)
+ *   bias_at [rows+1], bias_ids, bias [n_bias]: added to the row's logits; of an
+ *              id's entries the last counts
+ *   mask [n_masks][mask_words], mask_of [rows]: bit t%32 of word t/32 allows
+ *              token t to the rows of that mask (mask_of out of range: every
+ *              token); mask_words >= ceil(vocab/32)
+ *   u          the random numbers, in [0, 1)
+ * Ids outside the vocabulary and entries outside the lists are passed over. */
+typedef struct cc_sampling {
+    const float* temp;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* rep;
+    const float* freq;
+    const float* pres;
+    float freq_cap;
+    const int32_t* pen_at;
+    const int32_t* pen_ids;
+    const int32_t* pen_counts;
+    int32_t n_pen;
+    const int32_t* bias_at;
+    const int32_t* bias_ids;
+    const float* bias;
+    int32_t n_bias;
+    const uint32_t* mask;
+    int32_t mask_words, n_masks;
+    const int32_t* mask_of;
+    const double* u;
+} cc_sampling;
+
+/* The rows' logits with penalties, biases and masks: with c a token's count
+ * in the row's history, x > 0 ? x / rep : x * rep, less pres + min(freq * c,
+ * freq_cap), where c > 0; plus its bias; -inf where the mask bars it (whatever
+ * the logit, NaN too). In f64 steps, rounded to f32 once; untouched logits keep
+ * their bits. logits f32 [rows][vocab], ld floats from row to row; out alike
+ * with ldo, and may be logits itself (same ld). vocab at most 2^20. */
+cc_status cc_logits_adjust(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, int32_t vocab,
+                           const cc_sampling* sampling, float* out, int64_t ldo, void* stream);
+/* Draws a token of each row of logits, which stay as they are. Of the adjusted
+ * row a (a NaN counts as -inf), s = f32(a / temp), a finite value stays finite;
+ * kept are, in this order, the s that reach the top_k-th largest, of those the
+ * s that reach the largest value above (and with) which lies top_p of their
+ * weight exp(s), and of those exp(s - max) >= min_p; equal values are kept or
+ * cut together. The token is the first, in id order, at which the running sum
+ * of the kept weights is above u times their sum. Weights are held to 2^-42 of
+ * the largest one, their sums exactly. ids gets the token, probs (may be NULL)
+ * the probability it was drawn with. Greedy: the first maximum of a, 1. A row
+ * with nothing above -inf: -1, 0. `workspace`: cc_sample_workspace bytes,
+ * 16-byte aligned, of any contents; two calls that may overlap need two. */
+size_t cc_sample_workspace(int32_t rows, int32_t vocab);
+cc_status cc_sample(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, int32_t vocab,
+                    const cc_sampling* sampling, int32_t* ids, float* probs, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif
