@@ -543,7 +543,8 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
                 for (int e = 0; e < 4; e++)
                     if (t0 + e > last) v[e] = 0u;
             }
-            big = big || pv_big(v);
+            // at D = 64 the upper lanes hold no scale of this page's (but a stale one, perhaps)
+            big = big || (256 * s + lane * 4 < 64 * NG && pv_big(v));
             *(u32x4*)&vsl[256 * s + lane * 4] = v;
         }
         const bool pbig = __builtin_amdgcn_ballot_w64(big) != 0;
