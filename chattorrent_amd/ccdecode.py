@@ -123,7 +123,7 @@ def load():
         "cc_bounds_bytes": (size, [C.POINTER(CCache)]),
         "cc_kv_append": (i32, [P, P, P, i32, P, i64, P, i64, P]),
         "cc_kv_bounds": (i32, [P, P, P, i32, P]),
-        "cc_attend_workspace": (size, [P, P, P, i32, i32, i32]),
+        "cc_attend_workspace": (size, [P, P, i32, i32, i32]),
         "cc_attend_pages": (i32, [P, P, P, i32, i32, i32, i32, i32, P, i64, P, i64, P, size, P]),
         "cc_logits_adjust": (i32, [P, P, i64, i32, i32, P, P, i64, P]),
         "cc_sample_workspace": (size, [i32, i32]),
@@ -641,7 +641,7 @@ class Context:
         if out is None:
             out = self._new(q, (rows, width), "float32")
         op, ldo = self._rows(out, "out", rows, width)
-        need = self.lib.cc_attend_workspace(self.h, cache.ref, a.ctypes.data, len(a), width // D, budget)
+        need = self.lib.cc_attend_workspace(self.h, cache.ref, rows, width // D, budget) if rows else 0
         if not need:
             raise CCError(CC_EARG, self.lib.cc_last_error(self.h).decode())
         ws = self._new(q, (need,), "uint8")

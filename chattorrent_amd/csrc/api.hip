@@ -2315,11 +2315,14 @@ hipError_t each_batch(const cc_rows* jobs, int32_t njobs, int64_t cap, U&& units
     return b.n ? f(b) : hipSuccess;
 }
 
-// How a call of `rows` rows (of its largest launch) is laid out. Work of a row
-// and kv head is cut over workgroups until there are about two for each
-// compute unit, and a workgroup's pages are at most one index a lane of its
-// four waves.
-AttendPlan attend_plan(int ncu, const cc_cache* c, int64_t rows, int max_seen, int n_heads, int budget) {
+// How a launch of `rows` rows is laid out. Work of a row and kv head is cut
+// over workgroups until there are about two for each compute unit (at most 64
+// cuts), and a workgroup's pages are at most one index a lane of its four
+// waves. The workspace's parts are sized for `ws_rows` rows that see up to
+// ws_seen pages: with u units of work there are at most 2 * ncu + u parts, or
+// u * ceil(kept / ATTEND_PER), and fewer pages or rows take no more.
+AttendPlan attend_plan(int ncu, const cc_cache* c, int64_t rows, int max_seen, int64_t ws_rows, int ws_seen, int n_heads,
+                       int budget) {
     AttendPlan p;
     p.group = n_heads / c->n_kv_heads;
     p.tiles = ceil_div(p.group, 16);
@@ -2328,37 +2331,26 @@ AttendPlan attend_plan(int ncu, const cc_cache* c, int64_t rows, int max_seen, i
     p.scored = max_seen > budget;
     const int kept = std::min(max_seen, budget);
     const int64_t units = rows * c->n_kv_heads * p.tiles;
-    const int64_t want = std::max<int64_t>(1, (2 * (int64_t)ncu + units - 1) / units);
+    const int64_t want = std::min<int64_t>(64, std::max<int64_t>(1, (2 * (int64_t)ncu + units - 1) / units));
     p.per = (int)std::max<int64_t>(ATTEND_WAVES, std::min<int64_t>(ATTEND_PER, (kept + want - 1) / want));
     p.splits = ceil_div(kept, p.per);
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const int64_t ws_units = ws_rows * c->n_kv_heads * p.tiles;
+    const int64_t parts = std::max<int64_t>(2 * (int64_t)ncu + ws_units,
+                                            ws_units * ceil_div(std::min(ws_seen, budget), ATTEND_PER));
     p.scores = 0;
-    p.partials = up(p.scored ? (size_t)rows * c->n_kv_heads * max_seen * 4 : 0);
-    p.counters = p.partials + up(p.splits > 1 ? (size_t)units * p.splits * std::min(16, p.group) * (c->head_dim + 2) * 4 : 0);
-    p.bytes = p.counters + up((size_t)units * 4);
+    p.partials = up(ws_seen > budget ? (size_t)ws_rows * c->n_kv_heads * ws_seen * 4 : 0);
+    p.counters = p.partials + up((size_t)parts * std::min(16, p.group) * (c->head_dim + 2) * 4);
+    p.bytes = p.counters + up((size_t)ws_units * 4);
     return p;
 }
 
-cc_status attend_args(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t njobs, int32_t n_heads, int32_t budget,
-                      AttendPlan& p, int64_t* total) {
-    cc_status st = check_rows(ctx, c, jobs, njobs, total, false);
-    if (st != CC_OK) return st;
+cc_status attend_shape(cc_ctx* ctx, const cc_cache* c, int64_t rows, int32_t n_heads, int32_t budget) {
     if (n_heads < 1 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 1024)
         return fail(ctx, CC_EARG, "n_heads must be a multiple of the cache's n_kv_heads");
-    if ((int64_t)c->n_kv_heads * ceil_div(n_heads / c->n_kv_heads, 16) > 65535 || *total > (1 << 30))
+    if ((int64_t)c->n_kv_heads * ceil_div(n_heads / c->n_kv_heads, 16) > 65535 || rows < 1 || rows > (1 << 30))
         return fail(ctx, CC_EARG, "too many heads or rows in one call");
     if (budget < 1) return fail(ctx, CC_EARG, "budget must be at least one page");
-    int max_seen = 0;
-    int64_t most = 0;
-    for (int j = 0; j < njobs; j++) {
-        if (jobs[j].n > OP_ROWS) return fail(ctx, CC_EARG, "a job of more than 65535 rows");
-        max_seen = std::max(max_seen, (jobs[j].past + jobs[j].n - 1) / 64 + 1);
-    }
-    (void)each_batch(jobs, njobs, OP_ROWS, [](const cc_rows& r) { return (int64_t)r.n; }, [&](const OpJobs& b) {
-        most = std::max<int64_t>(most, b.rows);
-        return hipSuccess;
-    });
-    p = attend_plan(ctx->ncu, c, most, max_seen, n_heads, budget);
     return CC_OK;
 }
 
@@ -2455,15 +2447,13 @@ cc_status cc_kv_bounds(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, 
     });
 }
 
-size_t cc_attend_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
-                           int32_t budget) {
+size_t cc_attend_workspace(cc_ctx* ctx, const cc_cache* cache, int32_t rows, int32_t n_heads, int32_t budget) {
     if (!ctx || !cache) return 0;
     try {
         CacheDev c;
-        AttendPlan p;
-        int64_t rows = 0;
-        if (cache_dev(ctx, cache, c) != CC_OK || attend_args(ctx, cache, jobs, njobs, n_heads, budget, p, &rows) != CC_OK) return 0;
-        return p.bytes;
+        if (cache_dev(ctx, cache, c) != CC_OK || attend_shape(ctx, cache, rows, n_heads, budget) != CC_OK) return 0;
+        const int r = std::min(rows, OP_ROWS);
+        return attend_plan(ctx->ncu, cache, r, cache->max_pages, r, cache->max_pages, n_heads, budget).bytes;
     } catch (...) {
         return 0;
     }
@@ -2478,22 +2468,33 @@ cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* job
         CacheDev c;
         cc_status st = cache_dev(ctx, cache, c);
         if (st != CC_OK) return st;
-        AttendPlan p;
         int64_t rows = 0;
-        st = attend_args(ctx, cache, jobs, njobs, n_heads, budget, p, &rows);
+        st = check_rows(ctx, cache, jobs, njobs, &rows, false);
+        if (st == CC_OK) st = attend_shape(ctx, cache, rows, n_heads, budget);
         if (st != CC_OK) return st;
         if (sink < 0 || recent < 1 || (int64_t)sink + recent > budget)
             return fail(ctx, CC_EARG, "attend: sink >= 0, recent >= 1 and sink + recent <= budget");
-        p.sink = sink;
-        p.recent = recent;
-        if (p.scored && !c.bounds) return fail(ctx, CC_EARG, "attend: a row sees more pages than its budget: the cache needs bounds");
+        int max_seen = 0;
+        for (int j = 0; j < njobs; j++) {
+            if (jobs[j].n > OP_ROWS) return fail(ctx, CC_EARG, "attend: a job of more than 65535 rows");
+            max_seen = std::max(max_seen, (jobs[j].past + jobs[j].n - 1) / 64 + 1);
+        }
+        if (max_seen > budget && !c.bounds)
+            return fail(ctx, CC_EARG, "attend: a row sees more pages than its budget: the cache needs bounds");
         const int64_t width = (int64_t)n_heads * c.D;
         if (ldq < width || ldo < width) return fail(ctx, CC_EARG, "attend: ldq and ldo are at least n_heads * head_dim");
-        if (!workspace || workspace_bytes < p.bytes || !is_aligned(workspace, 16))
-            return fail(ctx, CC_EARG, "attend: a workspace of " + std::to_string(p.bytes) + " bytes, 16-byte aligned");
+        const int64_t ws_rows = std::min<int64_t>(rows, OP_ROWS);
+        const size_t need = attend_plan(ctx->ncu, cache, ws_rows, max_seen, ws_rows, cache->max_pages, n_heads, budget).bytes;
+        if (!workspace || workspace_bytes < need || !is_aligned(workspace, 16))
+            return fail(ctx, CC_EARG, "attend: a workspace of " + std::to_string(need) + " bytes, 16-byte aligned");
         const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
         return launched(ctx, "attend", each_batch(jobs, njobs, OP_ROWS, [](const cc_rows& r) { return (int64_t)r.n; },
-            [&](const OpJobs& b) { return launch_attend_pages(s, c, b, p, q, ldq, out, ldo, (uint8_t*)workspace); }));
+            [&](const OpJobs& b) {
+                AttendPlan p = attend_plan(ctx->ncu, cache, b.rows, max_seen, ws_rows, cache->max_pages, n_heads, budget);
+                p.sink = sink;
+                p.recent = recent;
+                return launch_attend_pages(s, c, b, p, q, ldq, out, ldo, (uint8_t*)workspace);
+            }));
     });
 }
 

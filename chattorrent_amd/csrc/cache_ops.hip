@@ -45,8 +45,44 @@ __device__ static inline void bound_code(float mx, float mn, float B, int8_t& hi
     lo = (int8_t)(int)fminf(fmaxf(floorf(mn / B), -127.0f), 127.0f);
 }
 
-// VEC: the rows' groups of 8 channels are 16-byte aligned and RoPE's halves
-// are whole groups.
+// Channels d0 .. d0 + 7 of one head of a row x, rotated with the position's
+// (cos, sin) pairs cs: the f32 steps of rope_cs (rot 0: as they are). vec: x
+// is 16-byte aligned at groups of 4 channels, as is cs, and RoPE's halves are
+// whole groups of 8.
+__device__ static inline void rotated8(const float* __restrict__ x, int d0, const float* __restrict__ cs, int rot,
+                                       bool vec, float (&r)[8]) {
+    const int half = rot >> 1;
+    if (vec) {
+        const float4 a = *(const float4*)(x + d0), b = *(const float4*)(x + d0 + 4);
+        r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
+        r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
+        if (d0 < rot) {
+            const bool low = d0 < half;
+            const float* y = x + d0 + (low ? half : -half);
+            const float4 ya = *(const float4*)y, yb = *(const float4*)(y + 4);
+            const float o[8] = {ya.x, ya.y, ya.z, ya.w, yb.x, yb.y, yb.z, yb.w};
+            const float4* t = (const float4*)(cs + 2 * (d0 - (low ? 0 : half)));
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float4 c = t[e >> 1];
+                r[e] = low ? r[e] * c.x - o[e] * c.y : r[e] * c.x + o[e] * c.y;
+                r[e + 1] = low ? r[e + 1] * c.z - o[e + 1] * c.w : r[e + 1] * c.z + o[e + 1] * c.w;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int d = d0 + e;
+        r[e] = x[d];
+        if (d < rot) {
+            const float* t = cs + 2 * (d < half ? d : d - half);
+            const float o = x[d < half ? d + half : d - half];
+            r[e] = d < half ? r[e] * t[0] - o * t[1] : r[e] * t[0] + o * t[1];
+        }
+    }
+}
+
 template <int D, bool VEC>
 __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, const float* __restrict__ k, int64_t ldk,
                                                    const float* __restrict__ v, int64_t ldv, int only) {
@@ -62,7 +98,6 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
     if (page >= (uint32_t)c.n_pages) return;
     uint8_t* blk = (which ? c.v : c.k) + ((size_t)page * c.nKV + head) * c.blk;
     const int g = lane & (G8 - 1), rr = lane / G8;
-    const int half = c.rot >> 1;
     const bool bounds = which == 0 && c.bounds != nullptr && s1 == 64;
     float mx[8], mn[8];
 #pragma unroll
@@ -89,37 +124,8 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
         const int s = sb + rr;
         const bool live = s < s1;
         const int pos = 64 * p + (live ? s : s0);
-        const float* x = src + (jb.row0 + pos - jb.past) * ld + 8 * g;
         float r[8];
-        if (VEC) {
-            const float4 a = *(const float4*)x, b = *(const float4*)(x + 4);
-            r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
-            r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
-            if (which == 0 && 8 * g < c.rot) {
-                const bool low = 8 * g < half;
-                const float* y = x + (low ? half : -half);
-                const float4 ya = *(const float4*)y, yb = *(const float4*)(y + 4);
-                const float o[8] = {ya.x, ya.y, ya.z, ya.w, yb.x, yb.y, yb.z, yb.w};
-                const float4* t = (const float4*)(c.rope + ((size_t)pos * half + 8 * g - (low ? 0 : half)) * 2);
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const float4 cs = t[e >> 1];
-                    r[e] = low ? r[e] * cs.x - o[e] * cs.y : r[e] * cs.x + o[e] * cs.y;
-                    r[e + 1] = low ? r[e + 1] * cs.z - o[e + 1] * cs.w : r[e + 1] * cs.z + o[e + 1] * cs.w;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int d = 8 * g + e;
-                r[e] = x[e];
-                if (which == 0 && d < c.rot) {
-                    const float* t = c.rope + ((size_t)pos * half + (d < half ? d : d - half)) * 2;
-                    const float o = x[e + (d < half ? half : -half)];
-                    r[e] = d < half ? r[e] * t[0] - o * t[1] : r[e] * t[0] + o * t[1];
-                }
-            }
-        }
+        rotated8(src + (jb.row0 + pos - jb.past) * ld, 8 * g, c.rope + (size_t)pos * c.rot, which == 0 ? c.rot : 0, VEC, r);
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(r[e]));
@@ -215,17 +221,6 @@ hipError_t launch_kv_bounds(hipStream_t st, const CacheDev& c, const OpJobs& job
 }
 
 // ========================================================== selected pages ===
-// The rows' query heads of one tile (16 heads of a kv head's group), rotated
-// to the row's position: the f32 steps of rope_cs.
-template <int D>
-__device__ static inline float rotated(const float* __restrict__ q, int d, const float* __restrict__ cs, int rot) {
-    const float x = q[d];
-    if (d >= rot) return x;
-    const int half = rot >> 1;
-    if (d < half) return x * cs[2 * d] - q[d + half] * cs[2 * d + 1];
-    return x * cs[2 * (d - half)] + q[d - half] * cs[2 * (d - half) + 1];
-}
-
 // Order-preserving bits of an f32.
 __device__ static inline uint32_t order_bits(float v) {
     const uint32_t b = f2u(v);
@@ -241,16 +236,15 @@ __device__ static inline uint32_t order_bits(float v) {
 // [hi | lo]: one v_mfma_i32_16x16x64_i8 for 16 query heads and 16 pages, exact.
 // The groups' sums meet in f64 (T * B is exact there), and the score is that
 // sum rounded to f32, so which pages a row keeps does not depend on an order
-// of summation.
+// of summation. Kept as the score's order-preserving bits.
 //
 // A wave takes SCORE_TILES tiles of 16 pages, 4 waves of a workgroup the pages
-// one after another of one row and kv head, reading 2*D + 4*D/32 bytes a page:
-// what bounds it at many pages. The rows of a job read the same bounds; the
-// later ones find them in L2.
+// one after another of one row and kv head, reading 2*D + 4*D/32 bytes a page.
+// The rows of a job read the same bounds; the later ones find them in L2.
 constexpr int SCORE_TILES = 2;
 template <int NG>
 __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, AttendPlan p, const float* __restrict__ q,
-                                                    int64_t ldq, float* __restrict__ scores,
+                                                    int64_t ldq, uint32_t* __restrict__ scores,
                                                     uint32_t* __restrict__ counters, int n_counters) {
     constexpr int D = 32 * NG;
     __shared__ __align__(16) int8_t qc[16][D];
@@ -290,18 +284,28 @@ __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, Att
     for (int h0 = 0; h0 < p.group; h0 += 16) {
         const int gt = min(16, p.group - h0);
         if (h0) __syncthreads();
-        for (int i = threadIdx.x; i < 16 * D; i += 256) {   // 32 lanes hold a group of channels
-            const int h = i / D, d = i & (D - 1);
-            const float x = h < gt ? rotated<D>(qr + (size_t)(h0 + h) * D, d, cs, c.rot) : 0.0f;
-            float amax = fabsf(x);
-            for (int o = 1; o < 32; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+        for (int i = threadIdx.x; i < gt * (D / 8); i += 256) {   // 8 channels a thread, a group of 32 in 4 lanes
+            const int h = i / (D / 8), d0 = 8 * (i & (D / 8 - 1));
+            float r[8];
+            rotated8(qr + (size_t)(h0 + h) * D, d0, cs, c.rot, p.vec, r);
+            float amax = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(r[e]));
+            amax = fmaxf(amax, __shfl_xor(amax, 1));
+            amax = fmaxf(amax, __shfl_xor(amax, 2));
             const float scale = amax / 127.0f;
             const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
-            qc[h][d] = (int8_t)(int)fminf(fmaxf(__builtin_rintf(x * inv), -127.0f), 127.0f);
-            if ((d & 31) == 0) qs[h][d >> 5] = scale;
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                w[e >> 2] |= (uint32_t)(uint8_t)(int8_t)(int)fminf(fmaxf(__builtin_rintf(r[e] * inv), -127.0f), 127.0f)
+                             << (8 * (e & 3));
+            *(uint2*)&qc[h][d0] = make_uint2(w[0], w[1]);
+            if ((d0 & 31) == 0) qs[h][d0 >> 5] = scale;
         }
         __syncthreads();
-        // the lane's operand: head l16, codes 32g + 16(kb % 2) .., the positive (kb < 2) or the negative ones
+        // the lane's operand: head l16, codes 32g + 16(kb % 2) .., the positive (kb < 2) or the negative ones;
+        // rows of heads past the tile's come from whatever lies there, and are left out below
         u32x4 a[NG];
         float T[4][NG];
 #pragma unroll
@@ -337,7 +341,7 @@ __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, Att
         best[t] = fmaxf(best[t], __shfl_xor(best[t], 32));
         const int page = page0 + (wave * SCORE_TILES + t) * 16 + l16;
         if (kb == 0 && page < page1)
-            scores[((size_t)row * c.nKV + kvh) * p.max_seen + page] = pg[t] < page1 ? best[t] : -INFINITY;
+            scores[((size_t)row * c.nKV + kvh) * p.max_seen + page] = order_bits(pg[t] < page1 ? best[t] : -INFINITY);
     }
 }
 
@@ -346,18 +350,34 @@ __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, Att
 // pages [a, z) by score (ties to the lower page), the last `recent`. The
 // `need`-th largest score comes from four passes over its bits from the top,
 // 8 at a time, with a count of the scores that share the bits so far; then
-// every thread ranks a run of pages.
-__device__ static inline void kept_pages(const float* __restrict__ sc, int a, int z, int need, int sink, int e0, int e1,
-                                         int recent0, uint16_t* list, uint32_t* hist, uint32_t* s_sel) {
+// every thread ranks a run of pages. KEEP: a thread's run is at most
+// SELECT_REG pages, held in registers throughout.
+constexpr int SELECT_REG = 4;
+template <bool KEEP>
+__device__ static inline void best_pages(const uint32_t* __restrict__ sc, int a, int z, uint32_t need, int sink, int e0,
+                                         int e1, uint16_t* list, uint32_t* hist, uint32_t* s_sel) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    uint32_t prefix = 0, left = (uint32_t)need;
-    for (int sh = 24; sh >= 0 && need > 0; sh -= 8) {
+    const int per = KEEP ? SELECT_REG : (z - a + 255) / 256, i0 = a + t * per, i1 = min(i0 + per, z);
+    uint32_t reg[SELECT_REG];
+    if (KEEP)
+#pragma unroll
+        for (int e = 0; e < SELECT_REG; e++) reg[e] = i0 + e < i1 ? sc[i0 + e] : 0u;
+    auto each = [&](auto&& f) {
+        if (KEEP) {
+#pragma unroll
+            for (int e = 0; e < SELECT_REG; e++)
+                if (i0 + e < i1) f(i0 + e, reg[e]);
+        } else {
+            for (int i = i0; i < i1; i++) f(i, sc[i]);
+        }
+    };
+    uint32_t prefix = 0, left = need;
+    for (int sh = 24; sh >= 0; sh -= 8) {
         hist[t] = 0;
         __syncthreads();
-        for (int i = a + t; i < z; i += 256) {
-            const uint32_t k = order_bits(sc[i]);
+        each([&](int, uint32_t k) {
             if (sh == 24 || (k >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(k >> sh) & 255u], 1u);
-        }
+        });
         __syncthreads();
         if (wave == 0) {
             // lane l: digits 255 - 4l .. 252 - 4l, from the largest down
@@ -385,14 +405,11 @@ __device__ static inline void kept_pages(const float* __restrict__ sc, int a, in
         left = s_sel[1];
     }
     // prefix: the need-th largest score's bits; `left` of the pages that have them are kept
-    if (need == 0) z = a;
-    const int per = (z - a + 255) / 256, i0 = a + t * per, i1 = min(i0 + per, z);
     uint32_t gt = 0, eq = 0;
-    for (int i = i0; i < i1; i++) {
-        const uint32_t k = order_bits(sc[i]);
+    each([&](int, uint32_t k) {
         gt += k > prefix;
         eq += k == prefix;
-    }
+    });
     uint32_t bg = gt, be = eq;
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t x = __shfl_up(bg, o), y = __shfl_up(be, o);
@@ -412,20 +429,14 @@ __device__ static inline void kept_pages(const float* __restrict__ sc, int a, in
         bg += hist[w];
         be += hist[4 + w];
     }
-    for (int i = i0; i < i1; i++) {
-        const uint32_t k = order_bits(sc[i]);
-        const bool keep = k > prefix || (k == prefix && be < left);
-        if (keep) {
+    each([&](int i, uint32_t k) {
+        if (k > prefix || (k == prefix && be < left)) {
             const int e = sink + (int)(bg + min(be, left));
             if (e >= e0 && e < e1) list[e - e0] = (uint16_t)i;
         }
         bg += k > prefix;
         be += k == prefix;
-    }
-    for (int e = e0 + t; e < e1; e += 256) {
-        if (e < sink) list[e - e0] = (uint16_t)e;
-        if (e >= sink + need) list[e - e0] = (uint16_t)(recent0 + e - sink - need);
-    }
+    });
 }
 
 // Attention of a row's query heads (a tile of up to 16 of one kv head's) over
@@ -433,13 +444,16 @@ __device__ static inline void kept_pages(const float* __restrict__ sc, int a, in
 // waves. A wave walks its pages as the pass's attention does (online softmax
 // in log2 units; S^T = K . Q^T with the query as an f16 pair; O^T += V^T .
 // (p * s) with p * s as an f16 pair; one page of codes in flight), but its
-// pages come from a list. The waves' parts meet in LDS, the workgroups' in the
-// workspace: the last workgroup of a (row, tile) to finish joins them in split
-// order, whichever it is, so a row's result does not depend on it.
+// pages come from a list, and a page's V scales enter p * s relative to the
+// power of two below the largest of them, so that f16 holds them whatever the
+// values' magnitude (O is carried relative to the last page's). The waves'
+// parts meet in LDS, the workgroups' in the workspace: the last workgroup of a
+// (row, tile) to finish joins them in split order, whichever it is, so a row's
+// result does not depend on it.
 template <int NG>
 __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c, OpJobs jobs, AttendPlan p,
                                                                       const float* __restrict__ q, int64_t ldq,
-                                                                      const float* __restrict__ scores,
+                                                                      const uint32_t* __restrict__ scores,
                                                                       float* __restrict__ partials,
                                                                       uint32_t* __restrict__ counters,
                                                                       float* __restrict__ out, int64_t ldo) {
@@ -448,6 +462,7 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     __shared__ __align__(16) float smem[ATTEND_WAVES * OW];
     __shared__ uint16_t list[ATTEND_PER];
     __shared__ uint32_t hist[256], s_sel[2];
+    static_assert(ATTEND_WAVES * OW >= 2 * 16 * ATTEND_SPLITS, "the join's weights take the parts' place");
     const int row = blockIdx.z, split = blockIdx.x, kvh = blockIdx.y % c.nKV, tile = blockIdx.y / c.nKV;
     const OpJob jb = job_of(jobs, row);
     const int pos = jb.past + row - jb.first, seen = (pos >> 6) + 1;
@@ -462,31 +477,49 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     {
         const float* cs = c.rope + (size_t)pos * c.rot;
         const float* qr = q + (jb.row0 + row - jb.first) * ldq + (size_t)(kvh * p.group + h0) * D;
-        for (int i = tid; i < 16 * D; i += 256)
-            smem[i] = i < gt * D ? rotated<D>(qr + (size_t)(i / D) * D, i & (D - 1), cs, c.rot) : 0.0f;
+        for (int i = tid; i < gt * (D / 8); i += 256) {
+            const int h = i / (D / 8), d0 = 8 * (i & (D / 8 - 1));
+            float r[8];
+            rotated8(qr + (size_t)h * D, d0, cs, c.rot, p.vec, r);
+            *(float4*)&smem[h * D + d0] = make_float4(r[0], r[1], r[2], r[3]);
+            *(float4*)&smem[h * D + d0 + 4] = make_float4(r[4], r[5], r[6], r[7]);
+        }
     }
     if (seen > p.budget) {
-        kept_pages(scores + ((size_t)row * c.nKV + kvh) * p.max_seen, p.sink, seen - p.recent,
-                   p.budget - p.sink - p.recent, p.sink, e0, e1, seen - p.recent, list, hist, s_sel);
+        const uint32_t* sc = scores + ((size_t)row * c.nKV + kvh) * p.max_seen;
+        const int a = p.sink, z = seen - p.recent, need = p.budget - p.sink - p.recent;
+        if (need > 0) {
+            if (z - a <= 256 * SELECT_REG) best_pages<true>(sc, a, z, need, p.sink, e0, e1, list, hist, s_sel);
+            else best_pages<false>(sc, a, z, need, p.sink, e0, e1, list, hist, s_sel);
+        }
+        for (int e = e0 + tid; e < e1; e += 256) {
+            if (e < p.sink) list[e - e0] = (uint16_t)e;
+            if (e >= p.sink + need) list[e - e0] = (uint16_t)(z + e - p.sink - need);
+        }
     } else {
         for (int e = e0 + tid; e < e1; e += 256) list[e - e0] = (uint16_t)e;
     }
     __syncthreads();
-    half8_t qh[NG], ql[NG];
-#pragma unroll
-    for (int g = 0; g < NG; g++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            _Float16 hi, lo;
-            split_hilo(smem[l16 * D + 32 * g + 8 * j4 + e], hi, lo);
-            qh[g][e] = hi;
-            ql[g][e] = lo;
-        }
-    __syncthreads();   // every wave has its query: the space is free
     // this wave's entries of the list, their pages' indices one a lane
     const int n = e1 - e0, w0 = (n * wave) / ATTEND_WAVES, w1 = (n * (wave + 1)) / ATTEND_WAVES, nw = w1 - w0;
     const int lp = lane < nw ? (int)list[w0 + lane] : 0;
     const uint32_t pgv = lane < nw ? pt[lp] : 0u;
+    half8_t qh[NG], ql[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 f = *(const float4*)&smem[l16 * D + 32 * g + 8 * j4 + e];
+            const float x[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                _Float16 hi, lo;
+                split_hilo(l16 < gt ? x[i] : 0.0f, hi, lo);
+                qh[g][e + i] = hi;
+                ql[g][e + i] = lo;
+            }
+        }
+    __syncthreads();   // every wave has its query: the space is free
     float* ksl = smem + wave * OW;
     float* vsl = ksl + 256 * SCL;
     const float score_scale = 1.4426950408889634f / sqrtf((float)D);
@@ -502,10 +535,11 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
 #pragma unroll
     for (int s = 0; s < SCL; s++) {
         const int e = 256 * s + lane * 4, b = e >> 6, jb4 = (e >> 4) & 3;
-        vso[s] = 4 * ((jb4 * NG + b) * 16 + (e & 15));
+        vso[s] = e < 64 * NG ? 4 * ((jb4 * NG + b) * 16 + (e & 15)) : c.blk;   // D = 64: the upper lanes read zero
     }
     float mrow = -INFINITY, lsum = 0.0f;
-    bool shifted = true;
+    bool shifted = true;   // p carries 2^PV_SHIFT_LOG2 until a running max leaves no room for it
+    int ev = -127, etop = -127;   // O is relative to 2^ev; the largest ev yet
     float4_t o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -513,7 +547,6 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     auto load_k = [&](__amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv) {
 #pragma unroll
         for (int s = 0; s < SCL; s++) {
-            // D = 64: a scale block is 512 bytes; lanes past it read zero
             kst[s] = __builtin_amdgcn_raw_buffer_load_b128(rk, lane * 16, 64 * D + 1024 * s, 0);
             vst[s] = __builtin_amdgcn_raw_buffer_load_b128(rv, vso[s], 64 * D, 0);
         }
@@ -532,22 +565,32 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
         const int p64 = 64 * __builtin_amdgcn_readlane(lp, i);
         const bool bad = (uint32_t)__builtin_amdgcn_readlane(pgv, i) >= (uint32_t)c.n_pages;
         const int last = bad ? -1 : pos;   // the last token that counts
-        bool big = false;
+        uint32_t top = 0;
 #pragma unroll
         for (int s = 0; s < SCL; s++) {
             *(u32x4*)&ksl[256 * s + lane * 4] = kst[s];
-            u32x4 v = vst[s];
             if (p64 + 63 > last) {   // tokens past the row: whatever scale lies there, NaN too, goes in as zero
                 const int t0 = p64 + 16 * (lane & 3) + 4 * (((256 * s + lane * 4) >> 4) & 3);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (t0 + e > last) v[e] = 0u;
+                    if (t0 + e > last) vst[s][e] = 0u;
             }
-            // at D = 64 the upper lanes hold no scale of this page's (but a stale one, perhaps)
-            big = big || (256 * s + lane * 4 < 64 * NG && pv_big(v));
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = max(top, vst[s][e]);   // scales are not negative
+        }
+        // the largest V scale's exponent (all zero: as before), and every scale relative to it; O has room for values
+        // 2^60 times as large as this page's
+        const uint32_t mx = wave_max_u32(top);
+        const int en = max(mx ? min((int)(mx >> 23) - 127, 127) : ev, etop - 60);
+        etop = max(etop, en);
+        const float down = u2f((uint32_t)(en < 127 ? 127 - en : 1) << 23) * (en < 127 ? 1.0f : 0.5f);   // 2^-en
+#pragma unroll
+        for (int s = 0; s < SCL; s++) {
+            u32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = f2u(u2f(vst[s][e]) * down);
             *(u32x4*)&vsl[256 * s + lane * 4] = v;
         }
-        const bool pbig = __builtin_amdgcn_ballot_w64(big) != 0;
         float pr[4][4];
         float pm = -INFINITY;
 #pragma unroll
@@ -589,15 +632,17 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
         pm = fmaxf(pm, __shfl_xor(pm, 16));
         pm = fmaxf(pm, __shfl_xor(pm, 32));
         const float mnew = fmaxf(mrow, pm);
-        const bool drop = pbig || !(fabsf(mnew) < PV_MAX_SCORE);
+        const bool drop = !(fabsf(mnew) < PV_MAX_SCORE);
         const float shrink = drop && shifted ? PV_UNSHIFT : 1.0f;
         shifted = shifted && !drop;
         const float alpha = (mrow == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrow - mnew)) * shrink;
         lsum *= alpha;
+        const float alpha_o = ldexpf(alpha, ev - en);
+        ev = en;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) o[dt][r] *= alpha;
+            for (int r = 0; r < 4; r++) o[dt][r] *= alpha_o;
         const float msub = (mnew == -INFINITY ? 0.0f : mnew) - (shifted ? PV_SHIFT_LOG2 : 0.0f);
 #pragma unroll
         for (int tt = 0; tt < 4; tt++)
@@ -650,74 +695,103 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     lsum += __shfl_xor(lsum, 16);
     lsum += __shfl_xor(lsum, 32);
     {
-        const float un = shifted ? PV_UNSHIFT : 1.0f;
+        const float un = shifted ? PV_UNSHIFT : 1.0f, up = ldexpf(un, ev);
         float* part = smem + wave * OW;   // its scale slices are this wave's own and done with
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) *(float4_t*)(part + l16 * D + dt * 16 + 4 * j4) = o[dt] * un;
+        for (int dt = 0; dt < DT; dt++) *(float4_t*)(part + l16 * D + dt * 16 + 4 * j4) = o[dt] * up;
         if (j4 == 0) {
             part[16 * D + l16] = mrow;
             part[16 * D + 16 + l16] = lsum * un;
         }
     }
     __syncthreads();
-    // the four waves' parts of the tile's heads
+    // the four waves' parts of the tile's heads, two channels a thread
     float* dst = out + (jb.row0 + row - jb.first) * ldo + (size_t)(kvh * p.group + h0) * D;
     const size_t unit = ((size_t)row * c.nKV + kvh) * p.tiles + tile;
     const int gw = min(16, p.group);
-    float* mine = partials + (unit * p.splits + split) * ((size_t)gw * (D + 2));
-    for (int i = tid; i < gt * D; i += 256) {
-        const int h = i / D, d = i & (D - 1);
+    const size_t part_floats = (size_t)gw * (D + 2);   // of a split: O [gw][D], then (max, sum) [gw]
+    float* mine = partials + (unit * p.splits + split) * part_floats;
+    for (int i = tid; i < gt * (D / 2); i += 256) {
+        const int h = i / (D / 2), d = 2 * (i & (D / 2 - 1));
         float m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < ATTEND_WAVES; w++) m = fmaxf(m, smem[w * OW + 16 * D + h]);
         const float ms = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, x = 0.0f;
+        float l = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
         for (int w = 0; w < ATTEND_WAVES; w++) {
             const float* part = smem + w * OW;
             const float f = __builtin_amdgcn_exp2f(part[16 * D + h] - ms);
+            const float2 xy = *(const float2*)(part + h * D + d);
             l = __builtin_fmaf(part[16 * D + 16 + h], f, l);
-            x = __builtin_fmaf(part[h * D + d], f, x);
+            x = __builtin_fmaf(xy.x, f, x);
+            y = __builtin_fmaf(xy.y, f, y);
         }
         if (splits == 1) {
             dst[(size_t)h * D + d] = l > 0.0f ? x / l : 0.0f;
+            dst[(size_t)h * D + d + 1] = l > 0.0f ? y / l : 0.0f;
         } else {
-            mine[(size_t)h * (D + 2) + 2 + d] = x;
-            if (d == 0) {
-                mine[(size_t)h * (D + 2)] = m;
-                mine[(size_t)h * (D + 2) + 1] = l;
-            }
+            leave64(mine + (size_t)h * D + d, (unsigned long long)f2u(y) << 32 | f2u(x));
+            if (d == 0) leave64(mine + (size_t)gw * D + 2 * h, (unsigned long long)f2u(l) << 32 | f2u(m));
         }
     }
     if (splits == 1) return;
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) s_sel[0] = atomicAdd(&counters[unit], 1u);
-    __syncthreads();
-    if (s_sel[0] != (uint32_t)(splits - 1)) return;
-    __threadfence();
-    const float* all = partials + unit * p.splits * ((size_t)gw * (D + 2));
-    for (int i = tid; i < gt * D; i += 256) {
-        const int h = i / D, d = i & (D - 1);
-        const float* part = all + (size_t)h * (D + 2);
-        const size_t step = (size_t)gw * (D + 2);
-        float m = -INFINITY;
-        for (int s = 0; s < splits; s++) m = fmaxf(m, __builtin_nontemporal_load(part + s * step));
-        const float ms = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, x = 0.0f;
-        for (int s = 0; s < splits; s++) {
-            const float f = __builtin_amdgcn_exp2f(__builtin_nontemporal_load(part + s * step) - ms);
-            l = __builtin_fmaf(__builtin_nontemporal_load(part + s * step + 1), f, l);
-            x = __builtin_fmaf(__builtin_nontemporal_load(part + s * step + 2 + d), f, x);
+    if (!finished_last(&counters[unit], splits, s_sel)) return;
+    // the splits' weights: 16 threads a head, over its splits
+    const float* all = partials + unit * p.splits * part_floats;
+    float* wt = smem;                          // [splits][16]
+    float* total = smem + 16 * ATTEND_SPLITS;  // [16]
+    {
+        const int h = tid >> 4, s0 = tid & 15;
+        float m[ATTEND_SPLITS / 16], l[ATTEND_SPLITS / 16], mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < ATTEND_SPLITS / 16; e++) {
+            const int s = s0 + 16 * e;
+            const unsigned long long v =
+                h < gt && s < splits ? left64(all + s * part_floats + (size_t)gw * D + 2 * h) : (unsigned long long)f2u(-INFINITY);
+            m[e] = u2f((uint32_t)v);
+            l[e] = u2f((uint32_t)(v >> 32));
+            mx = fmaxf(mx, m[e]);
         }
+        for (int x = 1; x < 16; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+        const float ms = mx == -INFINITY ? 0.0f : mx;
+        // the sum in split order within a thread's splits, then across the threads: an order of its own, always the same
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < ATTEND_SPLITS / 16; e++) {
+            const float f = __builtin_amdgcn_exp2f(m[e] - ms);
+            sum = __builtin_fmaf(l[e], f, sum);
+            if (s0 + 16 * e < splits) wt[(s0 + 16 * e) * 16 + h] = f;
+        }
+        for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor(sum, x);
+        if (s0 == 0) total[h] = sum;
+    }
+    __syncthreads();
+    for (int i = tid; i < gt * (D / 2); i += 256) {
+        const int h = i / (D / 2), d = 2 * (i & (D / 2 - 1));
+        const float* part = all + (size_t)h * D + d;
+        float x = 0.0f, y = 0.0f;
+        for (int s = 0; s < splits; s += 8) {   // eight loads in flight
+            unsigned long long v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = s + e < splits ? left64(part + (size_t)(s + e) * part_floats) : 0ull;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float f = s + e < splits ? wt[(s + e) * 16 + h] : 0.0f;
+                x = __builtin_fmaf(u2f((uint32_t)v[e]), f, x);
+                y = __builtin_fmaf(u2f((uint32_t)(v[e] >> 32)), f, y);
+            }
+        }
+        const float l = total[h];
         dst[(size_t)h * D + d] = l > 0.0f ? x / l : 0.0f;
+        dst[(size_t)h * D + d + 1] = l > 0.0f ? y / l : 0.0f;
     }
 }
 
 template <int NG>
 static void attend_ng(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& p, const float* q,
                       int64_t ldq, float* out, int64_t ldo, uint8_t* ws) {
-    float* scores = (float*)(ws + p.scores);
+    uint32_t* scores = (uint32_t*)(ws + p.scores);
     float* partials = (float*)(ws + p.partials);
     uint32_t* counters = (uint32_t*)(ws + p.counters);
     if (p.scored || p.splits > 1) {
@@ -730,8 +804,10 @@ static void attend_ng(hipStream_t st, const CacheDev& c, const OpJobs& jobs, con
                        q, ldq, scores, partials, counters, out, ldo);
 }
 
-hipError_t launch_attend_pages(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& p,
+hipError_t launch_attend_pages(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& plan,
                                const float* q, int64_t ldq, float* out, int64_t ldo, uint8_t* ws) {
+    AttendPlan p = plan;
+    p.vec = aligned16(q) && aligned16(c.rope) && ldq % 4 == 0 && c.rot % 16 == 0;
     if (c.ng == 2) attend_ng<2>(st, c, jobs, p, q, ldq, out, ldo, ws);
     else if (c.ng == 4) attend_ng<4>(st, c, jobs, p, q, ldq, out, ldo, ws);
     else attend_ng<8>(st, c, jobs, p, q, ldq, out, ldo, ws);

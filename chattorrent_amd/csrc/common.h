@@ -201,6 +201,49 @@ __device__ static inline bool pv_big(u32x4 v) {
 }
 
 
+// The largest of a wave's words as unsigned integers, in a scalar register:
+// within rows of 16 lanes by DPP, the four rows' by readlane.
+__device__ static inline uint32_t wave_max_u32(uint32_t x) {
+    auto mx = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true));    // lane ^ 1
+    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));    // lane ^ 2
+    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));   // 7 - lane of the eight
+    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));   // 15 - lane of the row
+    return mx(mx((uint32_t)__builtin_amdgcn_readlane((int)x, 0), (uint32_t)__builtin_amdgcn_readlane((int)x, 16)),
+              mx((uint32_t)__builtin_amdgcn_readlane((int)x, 32), (uint32_t)__builtin_amdgcn_readlane((int)x, 48)));
+}
+
+// Words that the workgroups of a launch leave for the one of them that
+// finishes last, wherever on the chip it runs. The eight L2s are not coherent
+// with each other, and a device-scope fence makes them so by writing back the
+// whole L2: with every workgroup doing it, 512 workgroups took 80 us longer.
+// These words instead are stored and loaded with device scope themselves
+// (sc1: past the L2, one access each), and a workgroup counts itself as
+// finished once its own stores are complete (vmcnt 0 in every wave, then the
+// workgroup's barrier), so nothing else has to be written back or dropped.
+__device__ static inline void leave64(void* p, unsigned long long v) {
+    __hip_atomic_store((unsigned long long*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ static inline void leave32(void* p, uint32_t v) {
+    __hip_atomic_store((uint32_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ static inline unsigned long long left64(const void* p) {
+    return __hip_atomic_load((const unsigned long long*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ static inline uint32_t left32(const void* p) {
+    return __hip_atomic_load((const uint32_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// True, for the whole workgroup, in the last of `n` workgroups to call it.
+// counter is zero before the launch.
+__device__ static inline bool finished_last(uint32_t* counter, int n, uint32_t* s_last) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        *s_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(n - 1);
+    __syncthreads();
+    return *s_last != 0;
+}
+
 __device__ static inline float wave_max(float v) {
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     return v;

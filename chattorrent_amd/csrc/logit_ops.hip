@@ -190,7 +190,7 @@ __device__ static inline float scaled_logit(float a, double inv_temp) {
     if (!(a > -INFINITY)) return -INFINITY;   // NaN too
     if (a == INFINITY) return a;
     const float s = (float)((double)a * inv_temp);
-    return fminf(fmaxf(s, -3.4028234663852886e38f), 3.4028234663852886e38f);
+    return fminf(fmaxf(s, -3.4028234663852886e38f), 3.4028234663852886e38f) + 0.0f;   // -0 is 0
 }
 __device__ static inline double weight(float s, float m) {
     return s == m ? 1.0 : exp((double)s - (double)m);
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_max(const float* __restrict__ x
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 if (!(a[j][e] > -INFINITY)) continue;
-                const uint32_t t = c * LG_CH + 4 * (LG_T * j + threadIdx.x) + e, o = ordered(a[j][e]);
+                const uint32_t t = c * LG_CH + 4 * (LG_T * j + threadIdx.x) + e, o = ordered(a[j][e] + 0.0f);   // -0 is 0
                 const u64 k = ((u64)o << 32) | (0xffffffffu - t);
                 best = k > best ? k : best;
                 least = o < least ? o : least;
@@ -407,18 +407,6 @@ __device__ static inline void draw_row(const float* __restrict__ x, int V, const
     draw_in_chunk<VEC>(x, V, s, r, c * LG_CH, cnt, last, red, left, total, kept, id, prob);
 }
 
-// Counts this workgroup as finished; true for the row's last one, which then
-// sees what the others wrote.
-__device__ static inline bool last_of_row(uint32_t* counter, int groups, uint32_t* s_last) {
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) *s_last = atomicAdd(counter, 1u) == (uint32_t)(groups - 1);
-    __syncthreads();
-    if (!*s_last) return false;
-    __threadfence();
-    return true;
-}
-
 template <bool VEC>
 __global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                       SampleWs w, int32_t* __restrict__ ids,
@@ -461,9 +449,9 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ 
                 }
         }
         sum = block_sum64(sum, red);
-        if (tid == 0) w.mass[at] = sum;
-        if (!last_of_row(&info->done[0], w.groups, &s_last)) return;
-        draw_row<VEC>(xr, V, s, r, w, row, tid < w.groups ? w.mass[(size_t)row * w.groups + tid] : 0, cnt, last, red,
+        if (tid == 0) leave64(&w.mass[at], sum);
+        if (!finished_last(&info->done[0], w.groups, &s_last)) return;
+        draw_row<VEC>(xr, V, s, r, w, row, tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0, cnt, last, red,
                       found, kept, ids + row, prob);
         return;
     }
@@ -489,23 +477,31 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ 
             }
     }
     __syncthreads();
-    for (int b = tid; b < SM_BINS; b += LG_T) {
-        w.hcount[at * SM_BINS + b] = hcount[b];
-        if (weigh) w.hmass[at * SM_BINS + b] = hmass[b];
-    }
-    if (!last_of_row(&info->done[0], w.groups, &s_last)) return;
     // thread t: bins 2t and 2t + 1
+    leave64(&w.hcount[at * SM_BINS + 2 * tid], (u64)hcount[2 * tid + 1] << 32 | hcount[2 * tid]);
+    if (weigh) {
+        leave64(&w.hmass[at * SM_BINS + 2 * tid], hmass[2 * tid]);
+        leave64(&w.hmass[at * SM_BINS + 2 * tid + 1], hmass[2 * tid + 1]);
+    }
+    if (!finished_last(&info->done[0], w.groups, &s_last)) return;
     u64 n[2] = {0, 0}, ms[2] = {0, 0};
-    for (int i = 0; i < w.groups; i++) {
-        const size_t o = ((size_t)row * w.groups + i) * SM_BINS + 2 * tid;
-        const uint2 c2 = *(const uint2*)(w.hcount + o);
-        n[0] += c2.x;
-        n[1] += c2.y;
-        if (weigh) {
-            const ulonglong2 m2 = *(const ulonglong2*)(w.hmass + o);
-            ms[0] += m2.x;
-            ms[1] += m2.y;
+    for (int i0 = 0; i0 < w.groups; i0 += 8) {   // eight workgroups' loads in flight
+        u64 c2[8], m2[8][2];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const size_t o = ((size_t)row * w.groups + min(i0 + i, w.groups - 1)) * SM_BINS + 2 * tid;
+            c2[i] = left64(&w.hcount[o]);
+            m2[i][0] = weigh ? left64(&w.hmass[o]) : 0;
+            m2[i][1] = weigh ? left64(&w.hmass[o + 1]) : 0;
         }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i0 + i < w.groups) {
+                n[0] += c2[i] & 0xffffffffu;
+                n[1] += c2[i] >> 32;
+                ms[0] += m2[i][0];
+                ms[1] += m2[i][1];
+            }
     }
     const u64 nb = block_before64(n[0] + n[1], red);
     const u64 mb = block_before64(ms[0] + ms[1], red);
@@ -650,22 +646,22 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(const float* __restrict__ x
             for (int e = 0; e < 4; e++)
                 if ((in >> (4 * j + e)) & 1u) {
                     if (mine < SM_CAND)
-                        cand[mine] = make_uint2(ordered(a[j][e]), (uint32_t)(c * LG_CH + 4 * (LG_T * j + tid) + e));
+                        leave64(&cand[mine], (u64)(c * LG_CH + 4 * (LG_T * j + tid) + e) << 32 | ordered(a[j][e]));
                     mine++;
                 }
         __syncthreads();
     }
     sum = block_sum64(sum, red);
-    if (tid == 0) w.mass[(size_t)row * w.groups + g] = sum;
-    if (!last_of_row(&info->done[1], w.groups, &s_last)) return;
-    const uint32_t n = info->n_cand;
+    if (tid == 0) leave64(&w.mass[(size_t)row * w.groups + g], sum);
+    if (!finished_last(&info->done[1], w.groups, &s_last)) return;
+    const uint32_t n = left32(&info->n_cand);
     const u64 above = info->above, mass_above = info->mass_above;
     uint32_t cut = 0;
-    gmass[tid] = tid < w.groups ? w.mass[(size_t)row * w.groups + tid] : 0;
+    gmass[tid] = tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0;
     auto weigh_key = [&](uint32_t key) { return whole_weight(weight(unordered(key), d.m)); };
     if (n <= SM_CAND) {
         uint32_t* keys = (uint32_t*)lists;
-        for (uint32_t i = tid; i < n; i += LG_T) keys[i] = cand[i].x;
+        for (uint32_t i = tid; i < n; i += LG_T) keys[i] = left32(&cand[i].x);
         __syncthreads();
         if (ask.k > 0)
             cut = find_cut((u64)ask.k - above, 0, hist, found, [&](auto&& f) {
@@ -686,9 +682,9 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(const float* __restrict__ x
         }
         __syncthreads();
         for (uint32_t i = tid; i < n; i += LG_T) {
-            const uint2 kv = cand[i];
-            const double q = weight(unordered(kv.x), d.m);
-            if (kv.x >= cut && q >= ask.min_p) atomicAdd(&gmass[kv.y / (uint32_t)(LG_CH * w.span)], whole_weight(q));
+            const double q = weight(unordered(keys[i]), d.m);
+            if (keys[i] >= cut && q >= ask.min_p)
+                atomicAdd(&gmass[left32(&cand[i].y) / (uint32_t)(LG_CH * w.span)], whole_weight(q));
         }
     } else {
         // too many values share the cut's bins: the same, in passes over the row

@@ -39,11 +39,13 @@ hipError_t launch_kv_bounds(hipStream_t st, const CacheDev& c, const OpJobs& job
 // How cc_attend_pages lays a call out: work of a row and kv head is `splits`
 // workgroups for each 16 query heads (`tiles`), `per` kept pages each.
 constexpr int ATTEND_WAVES = 4, ATTEND_PER = 64 * ATTEND_WAVES;   // one page index a lane
+constexpr int ATTEND_SPLITS = 128;   // 32768 pages in workgroups of ATTEND_PER
 struct AttendPlan {
     int group = 0, tiles = 0, splits = 0, per = 0;
     int max_seen = 0;             // the most pages that a row sees
     int budget = 0, sink = 0, recent = 0;
     bool scored = false;          // a row sees more pages than it keeps
+    bool vec = false;             // 16-byte loads of the query and the rope table
     size_t scores = 0, partials = 0, counters = 0, bytes = 0;   // offsets into the workspace, and its size
 };
 // units: rows.

@@ -384,10 +384,10 @@ cc_status cc_kv_bounds(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, 
  * out = softmax(q . k / sqrt(D)) v over the tokens read.
  * 0 <= sink, 1 <= recent, sink + recent <= budget. cache->bounds is needed
  * where a row sees more than `budget` pages: the pages before the row's last
- * `recent` have theirs. `workspace`: cc_attend_workspace bytes, 16-byte
- * aligned, of any contents; two calls that may overlap need two. */
-size_t cc_attend_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
-                           int32_t budget);
+ * `recent` have theirs. `workspace`: cc_attend_workspace bytes (for a
+ * call of up to `rows` rows; 0: it would be refused), 16-byte aligned, of any
+ * contents; two calls that may overlap need two. */
+size_t cc_attend_workspace(cc_ctx* ctx, const cc_cache* cache, int32_t rows, int32_t n_heads, int32_t budget);
 cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
                           int32_t budget, int32_t sink, int32_t recent, const float* q, int64_t ldq, float* out,
                           int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
