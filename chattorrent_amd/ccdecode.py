@@ -126,7 +126,7 @@ def load():
         "cc_attend_workspace": (size, [P, P, i32, i32, i32]),
         "cc_attend_pages": (i32, [P, P, P, i32, i32, i32, i32, i32, P, i64, P, i64, P, size, P]),
         "cc_logits_adjust": (i32, [P, P, i64, i32, i32, P, P, i64, P]),
-        "cc_sample_workspace": (size, [i32, i32]),
+        "cc_sample_workspace": (size, [i32, i32, P]),
         "cc_sample": (i32, [P, P, i64, i32, i32, P, P, P, P, size, P]),
         "cc_profile": (i32, [P, i32]),
         "cc_profile_read": (i32, [P, i32, C.POINTER(C.c_double), C.POINTER(C.c_int64), C.POINTER(C.c_double)]),
@@ -669,7 +669,7 @@ class Context:
         rows, V = sampling.rows, sampling.vocab
         lp, ld = self._rows(logits, "logits", rows, V)
         ids, probs = self._new(logits, (rows,), "int32"), self._new(logits, (rows,), "float32")
-        need = self.lib.cc_sample_workspace(rows, V)
+        need = self.lib.cc_sample_workspace(rows, V, sampling.ref)
         ws = self._new(logits, (max(need, 16),), "uint8")
         self._chk(self.lib.cc_sample(self.h, lp, ld, rows, V, sampling.ref, ids.data_ptr(), probs.data_ptr(),
                                      ws.data_ptr(), need, stream))

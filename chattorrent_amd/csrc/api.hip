@@ -2513,8 +2513,11 @@ cc_status cc_logits_adjust(cc_ctx* ctx, const float* logits, int64_t ld, int32_t
     });
 }
 
-size_t cc_sample_workspace(int32_t rows, int32_t vocab) {
-    return rows < 1 || rows > 65535 || vocab < 1 || vocab > (1 << 20) ? 0 : sample_workspace(rows, vocab);
+static bool sample_cuts(const cc_sampling* s) { return s->temp && (s->top_k || s->top_p || s->min_p); }
+
+size_t cc_sample_workspace(int32_t rows, int32_t vocab, const cc_sampling* sampling) {
+    if (!sampling || rows < 1 || rows > 65535 || vocab < 1 || vocab > (1 << 20)) return 0;
+    return sample_workspace(rows, vocab, sample_cuts(sampling));
 }
 
 cc_status cc_sample(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, int32_t vocab, const cc_sampling* sampling,
@@ -2527,7 +2530,7 @@ cc_status cc_sample(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, 
         if (st == CC_OK) st = sampling_dev(ctx, sampling, vocab, d);
         if (st != CC_OK) return st;
         if (d.temp && !d.u) return fail(ctx, CC_EARG, "sample: a temperature needs random numbers (u)");
-        const size_t need = sample_workspace(rows, vocab);
+        const size_t need = sample_workspace(rows, vocab, sample_cuts(sampling));
         if (!workspace || workspace_bytes < need || !is_aligned(workspace, 16))
             return fail(ctx, CC_EARG, "sample: a workspace of " + std::to_string(need) + " bytes, 16-byte aligned");
         return launched(ctx, "sample", launch_sample(stream ? (hipStream_t)stream : ctx->stream, logits, ld, rows, vocab, d,

@@ -52,7 +52,7 @@ __device__ static inline bool gather_lists(const SamplingDev& s, const RowPens& 
                                            int32_t* last) {
     if (r.p0 >= r.p1 && r.b0 >= r.b1) return false;
     __syncthreads();   // the previous chunk's readers are done
-    for (int i = threadIdx.x; i < CH; i += LG_T) cnt[i] = last[i] = 0;
+    for (int i = 4 * threadIdx.x; i < CH; i += 4 * LG_T) *(int4*)(cnt + i) = *(int4*)(last + i) = make_int4(0, 0, 0, 0);
     __syncthreads();
     for (int i = r.p0 + (int)threadIdx.x; i < r.p1; i += LG_T) {
         const uint32_t at = (uint32_t)s.pen_ids[i] - (uint32_t)base;
@@ -157,8 +157,8 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 // ================================================================= sample ===
 // With a the adjusted row (a NaN counts as -inf) and temp > 0:
 //   s = f32(a / temp) (a finite value stays finite), m = max s,
-//   w = exp(s - m) as a whole number of 2^-42 (f64 exp, rounded once), so that
-//   sums of weights are exact integers and do not depend on their order;
+//   w = exp(s - m) as a whole number of 2^-42, so that sums of weights are
+//   exact integers and do not depend on their order;
 //   kept by top-k: s >= the k-th largest s (ties stay);
 //   kept by top-p: s >= the largest value t for which the kept weights of
 //   s >= t reach p of all kept weights (ties stay);
@@ -167,21 +167,27 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 //   ids, is above u * sum; prob = exp(s - m) / sum.
 // temp <= 0 (or null): the first maximum of a, prob 1. No token left: -1, 0.
 //
-// A row is cut over workgroups (`span` chunks each), in two or three launches:
-//   k_sample_max   every workgroup's largest and smallest value;
-//   k_sample_mass  with the row's m known, every workgroup's weight. The last
-//                  workgroup of a row to finish knows them all: it finds the
-//                  one that the token falls into and the token in it. A row
-//                  with top-k or top-p instead gets a histogram of m - s in
-//                  SM_BINS bins from every workgroup (counts, weights), and the
-//                  last one finds the bins that the cuts fall into;
-//   k_sample_cut   (only where a row may have top-k or top-p) the values of
-//                  those bins, a few hundred of a row as a rule, are gathered;
-//                  the last workgroup takes them 8 bits at a time to the cuts'
-//                  exact values, and draws.
+// Calls without top-k, top-p and min-p take two launches and read the logits
+// once:
+//   k_sample_weights  the weight of every chunk, relative to its own maximum;
+//   k_sample_pick     a workgroup a row: the chunk that the token falls into,
+//                     and the token in it.
+// The others take three, a row cut over workgroups of `span` chunks:
+//   k_sample_scale    writes s to the workspace, with every workgroup's largest
+//                     and smallest value: lists, masks and the division once;
+//   k_sample_mass     with the row's m known, a histogram of m - s in SM_BINS
+//                     bins (counts for top-k, weights for top-p) of every
+//                     workgroup; the row's last workgroup to finish adds them
+//                     and finds the bins that the cuts fall into. (A row
+//                     without a cut: the weights, and the last one draws.)
+//   k_sample_cut      the values of those bins are gathered; the row's last
+//                     workgroup finds the cuts' exact values among them and
+//                     draws. Where everything up to the cut's bin is at most
+//                     SM_SMALL values, all of it is gathered, and each value
+//                     counts the larger ones; else 8 bits at a time.
 // A row whose cut falls among more than SM_CAND values (nearly equal logits) is
 // drawn by its last workgroup alone, in passes over the row.
-constexpr int SM_BINS = 512, SM_CAND = 8192, SM_CHUNKS = (1 << 20) / LG_CH;
+constexpr int SM_BINS = 512, SM_CAND = 8192, SM_SMALL = 512, SM_CHUNKS = (1 << 20) / LG_CH;
 constexpr float SM_REACH = 32.0f;            // the histogram's last bin takes everything below m - 32
 constexpr double SM_ONE = 4398046511104.0;   // 2^42: a row of 2^20 tokens sums to at most 2^62
 typedef unsigned long long u64;
@@ -192,10 +198,37 @@ __device__ static inline float scaled_logit(float a, double inv_temp) {
     const float s = (float)((double)a * inv_temp);
     return fminf(fmaxf(s, -3.4028234663852886e38f), 3.4028234663852886e38f) + 0.0f;   // -0 is 0
 }
-__device__ static inline double weight(float s, float m) {
-    return s == m ? 1.0 : exp((double)s - (double)m);
+
+// 2^(j/16), j = 0 .. 15, in LDS: a lane's lookup meets no bank conflict.
+__device__ static inline void exp_table(double* T) {
+    static constexpr double two16[16] = {
+        1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.1892071150027210, 1.2418578120734840,
+        1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407,
+        1.6104903319492543, 1.6817928305074290, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+    if (threadIdx.x < 16) T[threadIdx.x] = two16[threadIdx.x];
 }
-__device__ static inline u64 whole_weight(double w) { return (u64)(w * SM_ONE + 0.5); }
+// The weight exp(s - m) in [0, 1], s <= m, to about 2^-50: x = (16 e + j) ln2/16
+// + r with |r| <= ln2/32, where six terms of exp(r) are left off by r^7/5040 <
+// 2^-51. Under x = -30 it is less than half a 2^-42 and counts as nothing.
+__device__ static inline double weight(float s, float m, const double* T) {
+    if (s == m) return 1.0;
+    const double x = (double)s - (double)m;
+    if (!(x > -30.0)) return 0.0;
+    const double n = rint(x * 23.083120654223414);   // 16 / ln 2
+    const int i = (int)n;
+    const double r = fma(n, -0.043321698784996580, x);
+    double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p * T[i & 15], i >> 4);
+}
+// w in [0, 1] to the nearest 2^-42: 2^10 + w has that step.
+__device__ static inline u64 whole_weight(double w) {
+    return __builtin_bit_cast(u64, w + 1024.0) - __builtin_bit_cast(u64, 1024.0);
+}
 
 __device__ static inline uint32_t ordered(float v) {
     const uint32_t b = f2u(v);
@@ -203,35 +236,52 @@ __device__ static inline uint32_t ordered(float v) {
 }
 __device__ static inline float unordered(uint32_t k) { return u2f((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
-__device__ static inline u64 wave_sum64(u64 v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+// A lane's 64-bit value from another lane by DPP (zero where there is none).
+template <int CTRL, int ROWS = 0xf>
+__device__ static inline u64 dpp64(u64 v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return (u64)hi << 32 | lo;
 }
-// Over the workgroup, to every thread: the sum, the sum of the threads before, the largest.
-__device__ static inline u64 block_sum64(u64 v, u64* red) {
-    v = wave_sum64(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
+__device__ static inline u64 lane64(u64 v, int lane) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
+// The sum over a wave's lanes up to this one: within rows of 16 lanes by
+// shifts (1, 2, 4, 8), then the rows' sums before.
+__device__ static inline u64 wave_scan64(u64 v) {
+    v += dpp64<0x111>(v);
+    v += dpp64<0x112>(v);
+    v += dpp64<0x114>(v);
+    v += dpp64<0x118>(v);
+    const u64 a = lane64(v, 15), b = a + lane64(v, 31), c = b + lane64(v, 47);
+    const int row = (threadIdx.x & 63) >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+__device__ static inline u64 wave_max64(u64 v) {
+    auto mx = [](u64 a, u64 b) { return a > b ? a : b; };
+    v = mx(v, dpp64<0xB1>(v));
+    v = mx(v, dpp64<0x4E>(v));
+    v = mx(v, dpp64<0x141>(v));
+    v = mx(v, dpp64<0x140>(v));
+    return mx(mx(lane64(v, 0), lane64(v, 16)), mx(lane64(v, 32), lane64(v, 48)));
+}
+// Over the workgroup, to every thread: the sum; the sum of the threads before
+// (red then holds the waves' sums); the largest.
 __device__ static inline u64 block_before64(u64 v, u64* red) {
-    u64 inc = v;
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = __shfl_up(inc, o);
-        if ((int)(threadIdx.x & 63) >= o) inc += y;
-    }
+    u64 inc = wave_scan64(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = inc;
     __syncthreads();
     for (int w = 0; w < (int)(threadIdx.x >> 6); w++) inc += red[w];
     return inc - v;
 }
+__device__ static inline u64 block_sum64(u64 v, u64* red) {
+    block_before64(v, red);
+    return red[0] + red[1] + red[2] + red[3];
+}
 __device__ static inline u64 block_max64(u64 v, u64* red) {
-    for (int o = 32; o > 0; o >>= 1) {
-        const u64 y = __shfl_xor(v, o);
-        v = y > v ? y : v;
-    }
+    v = wave_max64(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -239,14 +289,16 @@ __device__ static inline u64 block_max64(u64 v, u64* red) {
     return a > b ? a : b;
 }
 
-// The workspace of a call: per row and workgroup (groups of them) the largest
-// key and the smallest value, the weight, the histogram; per row what the cuts
-// found, two counters of finished workgroups and the gathered values.
+// The workspace of a call. Without cuts: per row and chunk the largest key and
+// the weight. With: per row and workgroup (`groups` of them) the largest key,
+// the smallest value, the weight and the histogram; per row the scaled logits,
+// what the cuts found, two counters of finished workgroups and the gathered
+// values.
 struct SampleInfo {
-    int32_t lo, hi;        // the bins that the cuts fall into
+    int32_t lo, hi;        // the bins whose values are gathered
     uint32_t above;        // values in the bins before lo
     uint32_t n_cand;       // gathered values (more than SM_CAND: not all of them were)
-    u64 mass_above;        // their weight
+    u64 mass_above;        // the weight of the bins before lo
     u64 want;              // top-p without top-k: the weight to reach
     uint32_t done[2], pad[2];
 };
@@ -258,6 +310,8 @@ struct SampleWs {
     uint32_t* hcount; // [rows][groups][SM_BINS]
     SampleInfo* info; // [rows]
     uint2* cand;      // [rows][SM_CAND] ordered(s), token
+    float* s;         // [rows][lds]
+    int64_t lds;
     int groups, span;
 };
 
@@ -278,29 +332,156 @@ struct RowAsk {
     }
 };
 
+__device__ static inline u64 best_key(float a, uint32_t token) {
+    return a > -INFINITY ? (u64)ordered(a + 0.0f) << 32 | (0xffffffffu - token) : 0;   // -0 is 0
+}
+__device__ static inline u64 target_of(double u, u64 total) {
+    const u64 t = (u64)fmax(u * (double)total, 0.0);
+    return t < total - 1 ? t : total - 1;
+}
+
+// Of a chunk's scaled logits v (in adjusted_chunk's order), the token with
+// `left` of the kept weights of the chunk before it. Called by the whole
+// workgroup; mw(v) is a value's kept weight; hit(token, v) is called once.
+template <class W, class H>
+__device__ static inline void draw_in_chunk(const float (&v)[LG_J][4], int base, u64 left, u64* red, W&& mw, H&& hit) {
+#pragma unroll
+    for (int j = 0; j < LG_J; j++) {   // runs of 4 * LG_T tokens, one after another
+        u64 m[4], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            m[e] = mw(v[j][e]);
+            sum += m[e];
+        }
+        u64 before = block_before64(sum, red);
+        const u64 run = red[0] + red[1] + red[2] + red[3];
+        if (left < run) {   // the same for every thread
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (before <= left && left < before + m[e]) hit(base + 4 * (LG_T * j + (int)threadIdx.x) + e, v[j][e]);
+                before += m[e];
+            }
+            return;
+        }
+        left -= run;
+    }
+}
+
+// ---- without cuts
 template <bool VEC>
-__global__ __launch_bounds__(LG_T) void k_sample_max(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
-                                                     SampleWs w) {
+__global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
+                                                         SampleWs w) {
+    __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
+    __shared__ double T[16];
+    __shared__ u64 red[4];
+    const int row = blockIdx.y, c = blockIdx.x;
+    exp_table(T);
+    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
+    float a[LG_J][4];
+    adjusted_chunk<VEC>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
+    u64 best = 0;
+#pragma unroll
+    for (int j = 0; j < LG_J; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const u64 k = best_key(a[j][e], c * LG_CH + 4 * (LG_T * j + threadIdx.x) + e);
+            best = k > best ? k : best;
+        }
+    best = block_max64(best, red);
+    u64 sum = 0;
+    if (best && temp > 0.0) {
+        const float m = scaled_logit(unordered((uint32_t)(best >> 32)), inv);
+#pragma unroll
+        for (int j = 0; j < LG_J; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum += whole_weight(weight(scaled_logit(a[j][e], inv), m, T));
+        sum = block_sum64(sum, red);
+    }
+    if (threadIdx.x == 0) {
+        w.best[(size_t)row * w.groups + c] = best;
+        w.mass[(size_t)row * w.groups + c] = sum;
+    }
+}
+
+// The chunks' weights relative to the row's maximum m are theirs times
+// exp(m_c - m), rounded to whole numbers again.
+template <bool VEC>
+__global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
+                                                      SampleWs w, int32_t* __restrict__ ids, float* __restrict__ probs) {
+    __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
+    __shared__ double T[16];
+    __shared__ u64 red[4], found[2];
+    __shared__ float s_m;
+    const int row = blockIdx.x, tid = threadIdx.x;
+    exp_table(T);
+    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
+    const u64 mine = tid < w.groups ? w.best[(size_t)row * w.groups + tid] : 0;
+    const u64 local = tid < w.groups ? w.mass[(size_t)row * w.groups + tid] : 0;
+    const u64 key = block_max64(mine, red);
+    if (!key || !(temp > 0.0)) {
+        if (tid == 0) {
+            ids[row] = key ? (int32_t)(0xffffffffu - (uint32_t)key) : -1;
+            if (probs) probs[row] = key ? 1.0f : 0.0f;
+        }
+        return;
+    }
+    const float m = scaled_logit(unordered((uint32_t)(key >> 32)), inv);
+    const float mc = mine ? scaled_logit(unordered((uint32_t)(mine >> 32)), inv) : -INFINITY;
+    const double f = weight(mc, m, T);
+    const u64 mass = (u64)rint((double)local * f);
+    const u64 before = block_before64(mass, red);
+    const u64 total = red[0] + red[1] + red[2] + red[3];
+    const u64 target = target_of(s.u ? s.u[row] : 0.0, total);
+    if (before <= target && target < before + mass) {
+        const u64 left = (u64)((double)(target - before) / f);
+        found[0] = tid;
+        found[1] = left < local - 1 ? left : local - 1;
+        s_m = mc;
+    }
+    __syncthreads();
+    const int c = (int)found[0];
+    const u64 left = found[1];
+    const float m_c = s_m;
+    float a[LG_J][4];
+    adjusted_chunk<VEC>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
+#pragma unroll
+    for (int j = 0; j < LG_J; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) a[j][e] = scaled_logit(a[j][e], inv);
+    draw_in_chunk(a, c * LG_CH, left, red, [&](float v) { return whole_weight(weight(v, m_c, T)); }, [&](int t, float v) {
+        ids[row] = t;
+        if (probs) probs[row] = (float)(weight(v, m, T) * SM_ONE / (double)total);
+    });
+}
+
+// ---- with cuts
+template <bool VEC>
+__global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
+                                                       SampleWs w) {
     __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
     __shared__ u64 red[4];
     const int row = blockIdx.y, g = blockIdx.x;
     if (g == 0 && threadIdx.x < sizeof(SampleInfo) / 4) ((uint32_t*)(w.info + row))[threadIdx.x] = 0;
     const RowPens r = row_pens(s, row);
+    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
     u64 best = 0;
     uint32_t least = 0xffffffffu;
     for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
         float a[LG_J][4];
         adjusted_chunk<VEC>(x + row * ldx, V, s, r, c * LG_CH, cnt, last, a);
 #pragma unroll
-        for (int j = 0; j < LG_J; j++)
+        for (int j = 0; j < LG_J; j++) {
+            const int t = c * LG_CH + 4 * (LG_T * j + (int)threadIdx.x);
+            float v[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (!(a[j][e] > -INFINITY)) continue;
-                const uint32_t t = c * LG_CH + 4 * (LG_T * j + threadIdx.x) + e, o = ordered(a[j][e] + 0.0f);   // -0 is 0
-                const u64 k = ((u64)o << 32) | (0xffffffffu - t);
+                const u64 k = best_key(a[j][e], t + e);
                 best = k > best ? k : best;
-                least = o < least ? o : least;
+                if (k && (uint32_t)(k >> 32) < least) least = (uint32_t)(k >> 32);
+                v[e] = scaled_logit(a[j][e], inv);
             }
+            if (t < V) *(float4*)(w.s + row * w.lds + t) = make_float4(v[0], v[1], v[2], v[3]);
+        }
     }
     best = block_max64(best, red);
     const u64 low = block_max64(~(u64)least, red);
@@ -310,10 +491,20 @@ __global__ __launch_bounds__(LG_T) void k_sample_max(const float* __restrict__ x
     }
 }
 
+// A chunk of a row's scaled logits.
+__device__ static inline void scaled_chunk(const float* __restrict__ s, int V, int base, float (&v)[LG_J][4]) {
+#pragma unroll
+    for (int j = 0; j < LG_J; j++) {
+        const int t = base + 4 * (LG_T * j + (int)threadIdx.x);
+        const float4 f = t < V ? *(const float4*)(s + t) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        v[j][0] = f.x; v[j][1] = f.y; v[j][2] = f.z; v[j][3] = f.w;
+    }
+}
+
 // What a row's workgroups share about its draw.
 struct RowDraw {
     float m, bins;      // the largest s; bins per unit of m - s
-    u64 key;            // the row's best (k_sample_max)
+    u64 key;            // the row's best (k_sample_scale)
 };
 __device__ static inline RowDraw row_draw(const SampleWs& w, int row, const RowAsk& ask, u64* red) {
     u64 best = 0, low = 0;
@@ -335,53 +526,16 @@ __device__ static inline int bin_of(float s, const RowDraw& d) {
     return s == d.m ? 0 : (int)fminf((d.m - s) * d.bins, (float)(SM_BINS - 1));
 }
 
-// Draws from the chunk at `base` the token with `left` of the kept weights of
-// the chunk before it. Called by the whole workgroup.
-template <bool VEC, class K>
-__device__ static inline void draw_in_chunk(const float* __restrict__ x, int V, const SamplingDev& s, const RowPens& r,
-                                            int base, int32_t* cnt, int32_t* last, u64* red, u64 left, u64 total,
-                                            K&& kept, int32_t* id, float* prob) {
-    float a[LG_J][4];
-    adjusted_chunk<VEC>(x, V, s, r, base, cnt, last, a);
-#pragma unroll
-    for (int j = 0; j < LG_J; j++) {   // runs of 4 * LG_T tokens, one after another
-        u64 mw[4], sum = 0;
-        double w[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            w[e] = 0.0;
-            mw[e] = kept(a[j][e], w[e]) ? whole_weight(w[e]) : 0;
-            sum += mw[e];
-        }
-        u64 before = block_before64(sum, red);
-        const u64 run = red[0] + red[1] + red[2] + red[3];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (before <= left && left < before + mw[e]) {
-                *id = base + 4 * (LG_T * j + (int)threadIdx.x) + e;
-                if (prob) *prob = (float)(w[e] * SM_ONE / (double)total);
-            }
-            before += mw[e];
-        }
-        if (left < run) return;   // the same for every thread
-        left -= run;
-    }
-}
-
-__device__ static inline u64 target_of(double u, u64 total) {
-    const u64 t = (u64)fmax(u * (double)total, 0.0);
-    return t < total - 1 ? t : total - 1;
-}
-
 // The last workgroup of a row, with the workgroups' kept weights known: mass
 // (this thread's workgroup of the row) -> the token.
-template <bool VEC, class K>
-__device__ static inline void draw_row(const float* __restrict__ x, int V, const SamplingDev& s, const RowPens& r,
-                                       const SampleWs& w, int row, u64 mass, int32_t* cnt, int32_t* last, u64* red,
-                                       u64* found, K&& kept, int32_t* id, float* prob) {
+template <class W>
+__device__ static inline void draw_row(const float* __restrict__ sr, int V, const SamplingDev& s, const SampleWs& w, int row,
+                                       u64 mass, float m, const double* T, u64* red, u64* found, W&& mw, int32_t* id,
+                                       float* prob) {
     const u64 before = block_before64(mass, red);
     const u64 total = red[0] + red[1] + red[2] + red[3];
     const u64 target = target_of(s.u ? s.u[row] : 0.0, total);
+    __syncthreads();
     if (before <= target && target < before + mass) {
         found[0] = threadIdx.x;
         found[1] = target - before;
@@ -389,32 +543,32 @@ __device__ static inline void draw_row(const float* __restrict__ x, int V, const
     __syncthreads();
     int c = (int)found[0] * w.span;
     u64 left = found[1];
+    float v[LG_J][4];
     for (int i = 1; i < w.span; i++, c++) {   // the workgroup's chunk that holds it
-        float a[LG_J][4];
-        adjusted_chunk<VEC>(x, V, s, r, c * LG_CH, cnt, last, a);
+        scaled_chunk(sr, V, c * LG_CH, v);
         u64 sum = 0;
 #pragma unroll
         for (int j = 0; j < LG_J; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                double q;
-                if (kept(a[j][e], q)) sum += whole_weight(q);
-            }
+            for (int e = 0; e < 4; e++) sum += mw(v[j][e]);
         sum = block_sum64(sum, red);
         if (left < sum) break;
         left -= sum;
     }
-    draw_in_chunk<VEC>(x, V, s, r, c * LG_CH, cnt, last, red, left, total, kept, id, prob);
+    scaled_chunk(sr, V, c * LG_CH, v);
+    draw_in_chunk(v, c * LG_CH, left, red, mw, [&](int t, float q) {
+        *id = t;
+        if (prob) *prob = (float)(weight(q, m, T) * SM_ONE / (double)total);
+    });
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
-                                                      SampleWs w, int32_t* __restrict__ ids,
+__global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, SampleWs w, int32_t* __restrict__ ids,
                                                       float* __restrict__ probs) {
-    __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
     __shared__ u64 hmass[SM_BINS], red[4], found[2];
     __shared__ uint32_t hcount[SM_BINS], s_last;
+    __shared__ double T[16];
     const int row = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
+    exp_table(T);
     const RowAsk ask(s, row, V);
     const RowDraw d = row_draw(w, row, ask, red);
     float* prob = probs ? probs + row : nullptr;
@@ -425,34 +579,28 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ 
         }
         return;
     }
-    const RowPens r = row_pens(s, row);
-    const float* xr = x + row * ldx;
+    const float* sr = w.s + row * w.lds;
     SampleInfo* info = w.info + row;
     const size_t at = (size_t)row * w.groups + g;
-    auto kept = [&](float a, double& q) {
-        const float v = scaled_logit(a, ask.inv);
-        if (!(v > -INFINITY)) return false;
-        q = weight(v, d.m);
-        return q >= ask.min_p;
-    };
     if (!ask.cut) {
+        auto mw = [&](float v) {
+            const double q = weight(v, d.m, T);
+            return q >= ask.min_p ? whole_weight(q) : 0;
+        };
         u64 sum = 0;
         for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
-            float a[LG_J][4];
-            adjusted_chunk<VEC>(xr, V, s, r, c * LG_CH, cnt, last, a);
+            float v[LG_J][4];
+            scaled_chunk(sr, V, c * LG_CH, v);
 #pragma unroll
             for (int j = 0; j < LG_J; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    double q;
-                    if (kept(a[j][e], q)) sum += whole_weight(q);
-                }
+                for (int e = 0; e < 4; e++) sum += mw(v[j][e]);
         }
         sum = block_sum64(sum, red);
         if (tid == 0) leave64(&w.mass[at], sum);
         if (!finished_last(&info->done[0], w.groups, &s_last)) return;
-        draw_row<VEC>(xr, V, s, r, w, row, tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0, cnt, last, red,
-                      found, kept, ids + row, prob);
+        draw_row(sr, V, s, w, row, tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0, d.m, T, red, found, mw,
+                 ids + row, prob);
         return;
     }
     // the histogram; weights only where top-p needs them
@@ -463,17 +611,16 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ 
     }
     __syncthreads();
     for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
-        float a[LG_J][4];
-        adjusted_chunk<VEC>(xr, V, s, r, c * LG_CH, cnt, last, a);
+        float v[LG_J][4];
+        scaled_chunk(sr, V, c * LG_CH, v);
 #pragma unroll
         for (int j = 0; j < LG_J; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float v = scaled_logit(a[j][e], ask.inv);
-                if (!(v > -INFINITY)) continue;
-                const int b = bin_of(v, d);
+                if (!(v[j][e] > -INFINITY)) continue;
+                const int b = bin_of(v[j][e], d);
                 atomicAdd(&hcount[b], 1u);
-                if (weigh) atomicAdd(&hmass[b], whole_weight(weight(v, d.m)));
+                if (weigh) atomicAdd(&hmass[b], whole_weight(weight(v[j][e], d.m, T)));
             }
     }
     __syncthreads();
@@ -508,21 +655,19 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ 
     const u64 total = red[0] + red[1] + red[2] + red[3];
     // the bin in which a running sum (of counts or weights) first reaches `want`
     auto reach = [&](u64 before, const u64* v, u64 want) {
+        __syncthreads();
         if (tid == 0) found[0] = SM_BINS - 1;
         __syncthreads();
         if (before < want && want <= before + v[0] + v[1]) found[0] = 2 * tid + (before + v[0] < want ? 1 : 0);
         __syncthreads();
-        const int b = (int)found[0];
-        __syncthreads();
-        return b;
+        return (int)found[0];
     };
     // a sum over the bins before b
     auto ahead = [&](u64 before, const u64* v, int b) {
+        __syncthreads();
         if (tid == b >> 1) found[0] = before + ((b & 1) ? v[0] : 0);
         __syncthreads();
-        const u64 r2 = found[0];
-        __syncthreads();
-        return r2;
+        return found[0];
     };
     int lo = SM_BINS - 1, hi = SM_BINS - 1;
     u64 want = 0, base = total;
@@ -536,6 +681,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ 
         lo = p < lo ? p : lo;
         if (ask.k == 0) hi = lo;
     }
+    // few enough up to and with hi: all of them are gathered
+    if (ahead(nb, n, hi + 1 < SM_BINS ? hi + 1 : hi) + (hi + 1 < SM_BINS ? 0 : SM_SMALL + 1) <= SM_SMALL) lo = 0;
     const u64 above = ahead(nb, n, lo), mass_above = weigh ? ahead(mb, ms, lo) : 0;
     if (tid == 0) {
         info->lo = lo;
@@ -547,8 +694,9 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(const float* __restrict__ 
 }
 
 // The value (as ordered bits, at least `floor`) at which the sum over the
-// values from the top first reaches `want`, 8 bits at a time: of(i, key) calls
-// are made by `each` for every value with its key and what it adds.
+// values from the top first reaches `want`, 8 bits at a time: `each` calls its
+// argument for every value with its key and what it adds. 0 (everything is
+// kept) if they all sum to less.
 template <class E>
 __device__ static inline uint32_t find_cut(u64 want, uint32_t floor, u64* hist, u64* sel, E&& each) {
     uint32_t prefix = 0;
@@ -573,12 +721,7 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t floor, u64* hist, 
                 v[e] = hist[255 - 4 * lane - e];
                 sum += v[e];
             }
-            u64 before = sum;
-            for (int o = 1; o < 64; o <<= 1) {
-                const u64 y = __shfl_up(before, o);
-                if (lane >= o) before += y;
-            }
-            before -= sum;
+            u64 before = wave_scan64(sum) - sum;
             if (before < left && left <= before + sum) {
                 int e = 0;
                 while (before + v[e] < left) before += v[e++];
@@ -590,46 +733,48 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t floor, u64* hist, 
         prefix = (uint32_t)sel[0];
         left = sel[1];
     }
-    return prefix;   // fewer than `want` in all: 0, everything is kept
+    return prefix;
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(LG_T) void k_sample_cut(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
-                                                     SampleWs w, int32_t* __restrict__ ids, float* __restrict__ probs) {
-    __shared__ __align__(16) int32_t lists[2 * LG_CH];   // the history counts and last biases; later the gathered keys
-    __shared__ u64 gmass[LG_T], hist[256], red[4], found[2];
+__global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, SampleWs w, int32_t* __restrict__ ids,
+                                                     float* __restrict__ probs) {
+    __shared__ uint32_t keys[SM_CAND];
+    __shared__ u64 gmass[LG_T], hist[256], red[4], found[2], wts[SM_SMALL];
+    __shared__ uint32_t tok[SM_SMALL];
     __shared__ uint32_t s_last, s_n, s_at;
-    static_assert(SM_CAND <= 2 * LG_CH, "the gathered keys take the lists' place");
+    __shared__ double T[16];
     static_assert(SM_CHUNKS <= LG_T, "a thread a workgroup of the row");
-    int32_t *cnt = lists, *last = lists + LG_CH;
+    static_assert(SM_SMALL == 2 * LG_T, "two values a thread");
     const int row = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
     const RowAsk ask(s, row, V);
     if (!ask.cut) return;
+    exp_table(T);
     const RowDraw d = row_draw(w, row, ask, red);
     if (d.key == 0) return;
-    const RowPens r = row_pens(s, row);
-    const float* xr = x + row * ldx;
+    const float* sr = w.s + row * w.lds;
     SampleInfo* info = w.info + row;
     const int lo = info->lo, hi = info->hi;
     uint2* cand = w.cand + (size_t)row * SM_CAND;
+    const bool from_hist = ask.top_p < 1.0 && !(ask.min_p > 0.0);   // the bins before lo: their weights are in the histogram
     u64 sum = 0;
+    if (from_hist) {
+        const u64* h = w.hmass + ((size_t)row * w.groups + g) * SM_BINS;
+        for (int b = tid; b < lo; b += LG_T) sum += h[b];
+    }
     for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
-        float a[LG_J][4];
-        adjusted_chunk<VEC>(xr, V, s, r, c * LG_CH, cnt, last, a);
+        float v[LG_J][4];
+        scaled_chunk(sr, V, c * LG_CH, v);
         uint32_t in = 0;
 #pragma unroll
         for (int j = 0; j < LG_J; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float v = scaled_logit(a[j][e], ask.inv);
-                a[j][e] = v;
-                if (!(v > -INFINITY)) continue;
-                const int b = bin_of(v, d);
-                if (b < lo) {
-                    const double q = weight(v, d.m);
-                    if (q >= ask.min_p) sum += whole_weight(q);
-                } else if (b <= hi) {
-                    in |= 1u << (4 * j + e);
+                const float q = v[j][e];
+                const int b = q > -INFINITY ? bin_of(q, d) : SM_BINS;
+                if (b >= lo && b <= hi) in |= 1u << (4 * j + e);
+                if (b < lo && !from_hist) {
+                    const double x = weight(q, d.m, T);
+                    if (x >= ask.min_p) sum += whole_weight(x);
                 }
             }
         // the workgroup's place among the gathered values, then each thread's
@@ -646,7 +791,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(const float* __restrict__ x
             for (int e = 0; e < 4; e++)
                 if ((in >> (4 * j + e)) & 1u) {
                     if (mine < SM_CAND)
-                        leave64(&cand[mine], (u64)(c * LG_CH + 4 * (LG_T * j + tid) + e) << 32 | ordered(a[j][e]));
+                        leave64(&cand[mine], (u64)(c * LG_CH + 4 * (LG_T * j + tid) + e) << 32 | ordered(v[j][e]));
                     mine++;
                 }
         __syncthreads();
@@ -656,11 +801,82 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(const float* __restrict__ x
     if (!finished_last(&info->done[1], w.groups, &s_last)) return;
     const uint32_t n = left32(&info->n_cand);
     const u64 above = info->above, mass_above = info->mass_above;
+    auto weigh_key = [&](uint32_t key) { return whole_weight(weight(unordered(key), d.m, T)); };
+    float* prob = probs ? probs + row : nullptr;
+    if (lo == 0 && n <= SM_SMALL) {
+        // every value that may be kept is here, two a thread: it is kept if fewer than k are larger, if the larger ones
+        // that top-k keeps have not reached p of the weight, and if it reaches min_p
+        uint32_t kv[2];
+        u64 mv[2];
+        bool in[2];
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const uint32_t i = tid + q * LG_T;
+            const u64 c2 = i < n ? left64(&cand[i]) : 0;
+            keys[i] = kv[q] = (uint32_t)c2;      // 0: no value has these bits (-inf is left out)
+            tok[i] = (uint32_t)(c2 >> 32);
+            mv[q] = i < n ? weigh_key(kv[q]) : 0;
+            wts[i] = mv[q];
+            in[q] = i < n;
+        }
+        __syncthreads();
+        if (ask.k > 0) {
+            uint32_t larger[2] = {0, 0};
+            for (uint32_t i = 0; i < n; i++) {
+                larger[0] += keys[i] > kv[0];
+                larger[1] += keys[i] > kv[1];
+            }
+            in[0] = in[0] && larger[0] < (uint32_t)ask.k;
+            in[1] = in[1] && larger[1] < (uint32_t)ask.k;
+        }
+        if (ask.top_p < 1.0) {
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+                if (!in[q]) wts[tid + q * LG_T] = 0;
+            u64 want = info->want;
+            if (ask.k > 0)
+                want = (u64)fmax(ceil(ask.top_p * (double)block_sum64((in[0] ? mv[0] : 0) + (in[1] ? mv[1] : 0), red)), 1.0);
+            __syncthreads();
+            u64 over[2] = {0, 0};
+            for (uint32_t i = 0; i < n; i++) {
+                const u64 x = wts[i];
+                const uint32_t kk = keys[i];
+                over[0] += kk > kv[0] ? x : 0;
+                over[1] += kk > kv[1] ? x : 0;
+            }
+            in[0] = in[0] && over[0] < want;
+            in[1] = in[1] && over[1] < want;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            if (in[q] && !(weight(unordered(kv[q]), d.m, T) >= ask.min_p)) in[q] = false;
+            if (!in[q]) mv[q] = 0;
+            wts[tid + q * LG_T] = mv[q];
+        }
+        const u64 total = block_sum64(mv[0] + mv[1], red);
+        __syncthreads();
+        const u64 target = target_of(s.u ? s.u[row] : 0.0, total);
+        u64 before[2] = {0, 0};
+        const uint32_t t0 = tok[tid], t1 = tok[tid + LG_T];
+        for (uint32_t i = 0; i < n; i++) {
+            const u64 x = wts[i];
+            const uint32_t tt = tok[i];
+            before[0] += tt < t0 ? x : 0;
+            before[1] += tt < t1 ? x : 0;
+        }
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+            if (before[q] <= target && target < before[q] + mv[q]) {
+                ids[row] = (int32_t)(q ? t1 : t0);
+                if (prob) *prob = (float)(weight(unordered(kv[q]), d.m, T) * SM_ONE / (double)total);
+            }
+        return;
+    }
     uint32_t cut = 0;
     gmass[tid] = tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0;
-    auto weigh_key = [&](uint32_t key) { return whole_weight(weight(unordered(key), d.m)); };
     if (n <= SM_CAND) {
-        uint32_t* keys = (uint32_t*)lists;
         for (uint32_t i = tid; i < n; i += LG_T) keys[i] = left32(&cand[i].x);
         __syncthreads();
         if (ask.k > 0)
@@ -682,7 +898,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(const float* __restrict__ x
         }
         __syncthreads();
         for (uint32_t i = tid; i < n; i += LG_T) {
-            const double q = weight(unordered(keys[i]), d.m);
+            const double q = weight(unordered(keys[i]), d.m, T);
             if (keys[i] >= cut && q >= ask.min_p)
                 atomicAdd(&gmass[left32(&cand[i].y) / (uint32_t)(LG_CH * w.span)], whole_weight(q));
         }
@@ -691,15 +907,13 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(const float* __restrict__ x
         const int chunks = (V + LG_CH - 1) / LG_CH;
         auto all = [&](auto&& f) {
             for (int c = 0; c < chunks; c++) {
-                float a[LG_J][4];
-                adjusted_chunk<VEC>(xr, V, s, r, c * LG_CH, cnt, last, a);
+                float v[LG_J][4];
+                scaled_chunk(sr, V, c * LG_CH, v);
 #pragma unroll
                 for (int j = 0; j < LG_J; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float v = scaled_logit(a[j][e], ask.inv);
-                        if (v > -INFINITY) f(ordered(v), c);
-                    }
+                    for (int e = 0; e < 4; e++)
+                        if (v[j][e] > -INFINITY) f(ordered(v[j][e]), c);
             }
         };
         if (ask.k > 0)
@@ -721,18 +935,17 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(const float* __restrict__ x
         gmass[tid] = 0;
         __syncthreads();
         all([&](uint32_t key, int c) {
-            const double q = weight(unordered(key), d.m);
+            const double q = weight(unordered(key), d.m, T);
             if (key >= cut && q >= ask.min_p) atomicAdd(&gmass[c / w.span], whole_weight(q));
         });
     }
     __syncthreads();
-    auto kept = [&](float a, double& q) {
-        const float v = scaled_logit(a, ask.inv);
-        if (!(v > -INFINITY) || ordered(v) < cut) return false;
-        q = weight(v, d.m);
-        return q >= ask.min_p;
+    auto mw = [&](float v) {
+        if (!(v > -INFINITY) || ordered(v) < cut) return (u64)0;
+        const double q = weight(v, d.m, T);
+        return q >= ask.min_p ? whole_weight(q) : 0;
     };
-    draw_row<VEC>(xr, V, s, r, w, row, gmass[tid], cnt, last, red, found, kept, ids + row, probs ? probs + row : nullptr);
+    draw_row(sr, V, s, w, row, gmass[tid], d.m, T, red, found, mw, ids + row, prob);
 }
 
 // Chunks a workgroup takes: one while the call has few workgroups, more where
@@ -744,9 +957,11 @@ static int sample_span(int rows, int V) {
     return span;
 }
 
-static size_t sample_layout(int rows, int V, uint8_t* at, SampleWs& w) {
-    w.span = sample_span(rows, V);
+// cuts: the call has top-k, top-p or min-p.
+static size_t sample_layout(int rows, int V, bool cuts, uint8_t* at, SampleWs& w) {
     const int chunks = (V + LG_CH - 1) / LG_CH;
+    w = SampleWs{};
+    w.span = cuts ? sample_span(rows, V) : 1;
     w.groups = (chunks + w.span - 1) / w.span;
     size_t n = 0;
     auto take = [&](size_t bytes) {
@@ -756,34 +971,43 @@ static size_t sample_layout(int rows, int V, uint8_t* at, SampleWs& w) {
     };
     const size_t gr = (size_t)rows * w.groups;
     w.best = (u64*)take(gr * 8);
-    w.least = (float*)take(gr * 4);
     w.mass = (u64*)take(gr * 8);
+    if (!cuts) return n;
+    w.least = (float*)take(gr * 4);
     w.hmass = (u64*)take(gr * SM_BINS * 8);
     w.hcount = (uint32_t*)take(gr * SM_BINS * 4);
     w.info = (SampleInfo*)take((size_t)rows * sizeof(SampleInfo));
     w.cand = (uint2*)take((size_t)rows * SM_CAND * 8);
+    w.lds = (V + 3) & ~3;
+    w.s = (float*)take((size_t)rows * w.lds * 4);
     return n;
 }
 
-size_t sample_workspace(int rows, int V) {
+static bool has_cuts(const SamplingDev& s) { return s.temp && (s.top_k || s.top_p || s.min_p); }
+
+size_t sample_workspace(int rows, int V, bool cuts) {
     SampleWs w;
-    return sample_layout(rows, V, nullptr, w);
+    return sample_layout(rows, V, cuts, nullptr, w);
 }
 
 template <bool VEC>
 static void sample_vec(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s, int32_t* ids,
                        float* probs, const SampleWs& w) {
     const dim3 grid(w.groups, rows);
-    hipLaunchKernelGGL(k_sample_max<VEC>, grid, dim3(LG_T), 0, st, x, ldx, V, s, w);
-    hipLaunchKernelGGL(k_sample_mass<VEC>, grid, dim3(LG_T), 0, st, x, ldx, V, s, w, ids, probs);
-    if (s.temp && (s.top_k || s.top_p))
-        hipLaunchKernelGGL(k_sample_cut<VEC>, grid, dim3(LG_T), 0, st, x, ldx, V, s, w, ids, probs);
+    if (!has_cuts(s)) {
+        hipLaunchKernelGGL(k_sample_weights<VEC>, grid, dim3(LG_T), 0, st, x, ldx, V, s, w);
+        hipLaunchKernelGGL(k_sample_pick<VEC>, dim3(rows), dim3(LG_T), 0, st, x, ldx, V, s, w, ids, probs);
+        return;
+    }
+    hipLaunchKernelGGL(k_sample_scale<VEC>, grid, dim3(LG_T), 0, st, x, ldx, V, s, w);
+    hipLaunchKernelGGL(k_sample_mass, grid, dim3(LG_T), 0, st, V, s, w, ids, probs);
+    if (s.top_k || s.top_p) hipLaunchKernelGGL(k_sample_cut, grid, dim3(LG_T), 0, st, V, s, w, ids, probs);
 }
 
 hipError_t launch_sample(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s,
                          int32_t* ids, float* probs, uint8_t* ws) {
     SampleWs w;
-    sample_layout(rows, V, ws, w);
+    sample_layout(rows, V, has_cuts(s), ws, w);
     if (vec_rows(x, ldx)) sample_vec<true>(st, x, ldx, rows, V, s, ids, probs, w);
     else sample_vec<false>(st, x, ldx, rows, V, s, ids, probs, w);
     return hipGetLastError();

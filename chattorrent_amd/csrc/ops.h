@@ -64,6 +64,7 @@ struct SamplingDev {
 };
 hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s,
                                 float* out, int64_t ldo);
-size_t sample_workspace(int rows, int V);
+// cuts: the call has a temperature with top-k, top-p or min-p.
+size_t sample_workspace(int rows, int V, bool cuts);
 hipError_t launch_sample(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s,
                          int32_t* ids, float* probs, uint8_t* ws);

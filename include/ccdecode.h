@@ -451,9 +451,10 @@ cc_status cc_logits_adjust(cc_ctx* ctx, const float* logits, int64_t ld, int32_t
  * of the kept weights is above u times their sum. Weights are held to 2^-42 of
  * the largest one, their sums exactly. ids gets the token, probs (may be NULL)
  * the probability it was drawn with. Greedy: the first maximum of a, 1. A row
- * with nothing above -inf: -1, 0. `workspace`: cc_sample_workspace bytes,
- * 16-byte aligned, of any contents; two calls that may overlap need two. */
-size_t cc_sample_workspace(int32_t rows, int32_t vocab);
+ * with nothing above -inf: -1, 0. `workspace`: cc_sample_workspace bytes
+ * (0: the shape would be refused), 16-byte aligned, of any contents; two calls
+ * that may overlap need two. */
+size_t cc_sample_workspace(int32_t rows, int32_t vocab, const cc_sampling* sampling);
 cc_status cc_sample(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, int32_t vocab,
                     const cc_sampling* sampling, int32_t* ids, float* probs, void* workspace, size_t workspace_bytes,
                     void* stream);

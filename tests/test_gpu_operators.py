@@ -733,7 +733,7 @@ def test_a_captured_step_replays(ctx, hip):
     ask = Ask(rng, 2, V, temp=0.9, top_p=0.8, top_k=200, history=40, rep=1.1, u=[0.3, 0.8])
     sampling = ask.device()
     need = lib.cc_attend_workspace(ctx.h, cache.ref, 2, heads, budget)
-    need2 = lib.cc_sample_workspace(2, V)
+    need2 = lib.cc_sample_workspace(2, V, sampling.ref)
     graphs = []
     for g in range(2):
         ws, ws2 = DeviceArray((need,), np.uint8), DeviceArray((need2,), np.uint8)
@@ -876,9 +876,10 @@ def test_refusals_of_the_logits_operators(ctx):
     refuses(ctx, "freq_cap", lambda: ctx.adjust_logits(x, Sampling(2, 100, freq_cap=-1.0)))
     refuses(ctx, "pen_ids", lambda: Sampling(2, 100, pen_ids=dev(np.zeros(4, np.int64))))
     ids, ws = dev(np.zeros(2, np.int32)), dev(np.zeros(1 << 20, np.uint8))
-    need = lib.cc_sample_workspace(2, 100)
+    need = lib.cc_sample_workspace(2, 100, plain.ref)
     assert 0 < need <= 1 << 20
-    assert lib.cc_sample_workspace(0, 100) == 0 and lib.cc_sample_workspace(2, (1 << 20) + 1) == 0
+    assert lib.cc_sample_workspace(0, 100, plain.ref) == 0 and lib.cc_sample_workspace(2, (1 << 20) + 1, plain.ref) == 0
+    assert lib.cc_sample_workspace(2, 100, None) == 0
 
     def sample(rows=2, V=100, ld=100, ws_=ws.data_ptr(), n=need):
         return lib.cc_sample(ctx.h, x.data_ptr(), ld, rows, V, plain.ref, ids.data_ptr(), None, ws_, n, None)
