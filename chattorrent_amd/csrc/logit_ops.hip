@@ -192,43 +192,62 @@ constexpr float SM_REACH = 32.0f;            // the histogram's last bin takes e
 constexpr double SM_ONE = 4398046511104.0;   // 2^42: a row of 2^20 tokens sums to at most 2^62
 typedef unsigned long long u64;
 
-__device__ static inline float scaled_logit(float a, double inv_temp) {
-    if (!(a > -INFINITY)) return -INFINITY;   // NaN too
-    if (a == INFINITY) return a;
-    const float s = (float)((double)a * inv_temp);
-    return fminf(fmaxf(s, -3.4028234663852886e38f), 3.4028234663852886e38f) + 0.0f;   // -0 is 0
+// s of an adjusted logit. inv = 1/temp; only above 1 can a finite value leave
+// the range (a branch on it is uniform).
+__device__ static inline float scaled_logit(float a, double inv) {
+    a = fmaxf(a, -INFINITY);   // NaN: -inf
+    float s = (float)((double)a * inv);
+    if (inv > 1.0 && fabsf(a) < INFINITY) s = fminf(fmaxf(s, -3.4028234663852886e38f), 3.4028234663852886e38f);
+    return s + 0.0f;   // -0 is 0
 }
 
-// 2^(j/16), j = 0 .. 15, in LDS: a lane's lookup meets no bank conflict.
+// 2^(j/32), j = 0 .. 31, in LDS: 256 bytes, so a lane's lookup meets no bank
+// conflict.
 __device__ static inline void exp_table(double* T) {
-    static constexpr double two16[16] = {
-        1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.1892071150027210, 1.2418578120734840,
-        1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407,
-        1.6104903319492543, 1.6817928305074290, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
-    if (threadIdx.x < 16) T[threadIdx.x] = two16[threadIdx.x];
+    static constexpr double two32[32] = {
+        1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+        1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+        1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467,
+        1.4768261459394993, 1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649,
+        1.681792830507429, 1.7186192981224779, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103,
+        1.9152065613971474, 1.9571441241754002};
+    if (threadIdx.x < 32) T[threadIdx.x] = two32[threadIdx.x];
 }
-// The weight exp(s - m) in [0, 1], s <= m, to about 2^-50: x = (16 e + j) ln2/16
-// + r with |r| <= ln2/32, where six terms of exp(r) are left off by r^7/5040 <
-// 2^-51. Under x = -30 it is less than half a 2^-42 and counts as nothing.
-__device__ static inline double weight(float s, float m, const double* T) {
-    if (s == m) return 1.0;
-    const double x = (double)s - (double)m;
-    if (!(x > -30.0)) return 0.0;
-    const double n = rint(x * 23.083120654223414);   // 16 / ln 2
+// exp(s - m) in [0, 1], s <= m, in pieces: x = (32 e + j) ln2/32 + r with |r| <=
+// ln2/64, exp(r) to five terms (left off: r^6/720 < 2^-48) and 2^e * 2^(j/32)
+// with the exponent put into the table's entry. Under x = -30 the weight is
+// less than half a 2^-42 and counts as nothing. (fmin also takes inf - inf,
+// a NaN, to 0: the weight of +inf is 1.)
+struct ExpParts {
+    double p, t;
+    bool some;
+};
+__device__ static inline ExpParts exp_parts(float s, double m, const double* T) {
+    const double x = fmin((double)s - m, 0.0);
+    const double n = rint(x * 46.16624130844683);   // 32 / ln 2
     const int i = (int)n;
-    const double r = fma(n, -0.043321698784996580, x);
-    double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
+    const double r = fma(n, -0.02166084939249829, x);
+    double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
     p = fma(p, r, 1.0 / 6.0);
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0);
-    return ldexp(p * T[i & 15], i >> 4);
+    const u64 b = __builtin_bit_cast(u64, T[i & 31]);
+    const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)(i >> 5) << 20);
+    return ExpParts{p, __builtin_bit_cast(double, (u64)hi << 32 | (uint32_t)b), x > -30.0};
 }
-// w in [0, 1] to the nearest 2^-42: 2^10 + w has that step.
-__device__ static inline u64 whole_weight(double w) {
-    return __builtin_bit_cast(u64, w + 1024.0) - __builtin_bit_cast(u64, 1024.0);
+__device__ static inline double weight(float s, float m, const double* T) {
+    const ExpParts e = exp_parts(s, (double)m, T);
+    return e.some ? e.p * e.t : 0.0;
 }
+// The weight to the nearest 2^-42, as a whole number above SM_BASE: 2^10 + w
+// has that step.
+constexpr u64 SM_BASE = 0x4090000000000000ull;   // the bits of 1024.0
+__device__ static inline u64 based_weight(float s, double m, const double* T) {
+    const ExpParts e = exp_parts(s, m, T);
+    return e.some ? __builtin_bit_cast(u64, fma(e.p, e.t, 1024.0)) : SM_BASE;
+}
+__device__ static inline u64 whole_weight(float s, float m, const double* T) { return based_weight(s, (double)m, T) - SM_BASE; }
 
 __device__ static inline uint32_t ordered(float v) {
     const uint32_t b = f2u(v);
@@ -335,6 +354,18 @@ struct RowAsk {
 __device__ static inline u64 best_key(float a, uint32_t token) {
     return a > -INFINITY ? (u64)ordered(a + 0.0f) << 32 | (0xffffffffu - token) : 0;   // -0 is 0
 }
+// The first largest of values given in the order of their tokens (-0 is 0, a
+// NaN nothing).
+struct FirstMax {
+    float v = -INFINITY;
+    uint32_t t = 0;
+    __device__ void take(float a, uint32_t token) {
+        const bool more = a > v;
+        v = more ? a : v;
+        t = more ? token : t;
+    }
+    __device__ u64 key() const { return best_key(v, t); }
+};
 __device__ static inline u64 target_of(double u, u64 total) {
     const u64 t = (u64)fmax(u * (double)total, 0.0);
     return t < total - 1 ? t : total - 1;
@@ -372,30 +403,27 @@ template <bool VEC>
 __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                          SampleWs w) {
     __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
-    __shared__ double T[16];
+    __shared__ double T[32];
     __shared__ u64 red[4];
     const int row = blockIdx.y, c = blockIdx.x;
     exp_table(T);
     const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
     float a[LG_J][4];
     adjusted_chunk<VEC>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
-    u64 best = 0;
+    FirstMax first;
 #pragma unroll
     for (int j = 0; j < LG_J; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const u64 k = best_key(a[j][e], c * LG_CH + 4 * (LG_T * j + threadIdx.x) + e);
-            best = k > best ? k : best;
-        }
-    best = block_max64(best, red);
+        for (int e = 0; e < 4; e++) first.take(a[j][e], c * LG_CH + 4 * (LG_T * j + threadIdx.x) + e);
+    const u64 best = block_max64(first.key(), red);
     u64 sum = 0;
     if (best && temp > 0.0) {
         const float m = scaled_logit(unordered((uint32_t)(best >> 32)), inv);
 #pragma unroll
         for (int j = 0; j < LG_J; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) sum += whole_weight(weight(scaled_logit(a[j][e], inv), m, T));
-        sum = block_sum64(sum, red);
+            for (int e = 0; e < 4; e++) sum += based_weight(scaled_logit(a[j][e], inv), (double)m, T);
+        sum = block_sum64(sum - LG_J * 4 * SM_BASE, red);
     }
     if (threadIdx.x == 0) {
         w.best[(size_t)row * w.groups + c] = best;
@@ -409,7 +437,7 @@ template <bool VEC>
 __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                       SampleWs w, int32_t* __restrict__ ids, float* __restrict__ probs) {
     __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
-    __shared__ double T[16];
+    __shared__ double T[32];
     __shared__ u64 red[4], found[2];
     __shared__ float s_m;
     const int row = blockIdx.x, tid = threadIdx.x;
@@ -448,7 +476,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
     for (int j = 0; j < LG_J; j++)
 #pragma unroll
         for (int e = 0; e < 4; e++) a[j][e] = scaled_logit(a[j][e], inv);
-    draw_in_chunk(a, c * LG_CH, left, red, [&](float v) { return whole_weight(weight(v, m_c, T)); }, [&](int t, float v) {
+    draw_in_chunk(a, c * LG_CH, left, red, [&](float v) { return whole_weight(v, m_c, T); }, [&](int t, float v) {
         ids[row] = t;
         if (probs) probs[row] = (float)(weight(v, m, T) * SM_ONE / (double)total);
     });
@@ -464,8 +492,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
     if (g == 0 && threadIdx.x < sizeof(SampleInfo) / 4) ((uint32_t*)(w.info + row))[threadIdx.x] = 0;
     const RowPens r = row_pens(s, row);
     const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
-    u64 best = 0;
-    uint32_t least = 0xffffffffu;
+    FirstMax first;
+    float least = INFINITY;
     for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
         float a[LG_J][4];
         adjusted_chunk<VEC>(x + row * ldx, V, s, r, c * LG_CH, cnt, last, a);
@@ -475,19 +503,18 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
             float v[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const u64 k = best_key(a[j][e], t + e);
-                best = k > best ? k : best;
-                if (k && (uint32_t)(k >> 32) < least) least = (uint32_t)(k >> 32);
+                first.take(a[j][e], t + e);
+                least = a[j][e] > -INFINITY ? fminf(least, a[j][e]) : least;
                 v[e] = scaled_logit(a[j][e], inv);
             }
             if (t < V) *(float4*)(w.s + row * w.lds + t) = make_float4(v[0], v[1], v[2], v[3]);
         }
     }
-    best = block_max64(best, red);
-    const u64 low = block_max64(~(u64)least, red);
+    const u64 best = block_max64(first.key(), red);
+    const u64 low = block_max64(~(u64)ordered(least), red);
     if (threadIdx.x == 0) {
         w.best[(size_t)row * w.groups + g] = best;
-        w.least[(size_t)row * w.groups + g] = best ? unordered((uint32_t)~low) : INFINITY;
+        w.least[(size_t)row * w.groups + g] = unordered((uint32_t)~low);
     }
 }
 
@@ -566,7 +593,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
                                                       float* __restrict__ probs) {
     __shared__ u64 hmass[SM_BINS], red[4], found[2];
     __shared__ uint32_t hcount[SM_BINS], s_last;
-    __shared__ double T[16];
+    __shared__ double T[32];
     const int row = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
     exp_table(T);
     const RowAsk ask(s, row, V);
@@ -584,8 +611,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
     const size_t at = (size_t)row * w.groups + g;
     if (!ask.cut) {
         auto mw = [&](float v) {
-            const double q = weight(v, d.m, T);
-            return q >= ask.min_p ? whole_weight(q) : 0;
+            return ask.min_p > 0.0 && !(weight(v, d.m, T) >= ask.min_p) ? 0 : whole_weight(v, d.m, T);
         };
         u64 sum = 0;
         for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
@@ -620,7 +646,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
                 if (!(v[j][e] > -INFINITY)) continue;
                 const int b = bin_of(v[j][e], d);
                 atomicAdd(&hcount[b], 1u);
-                if (weigh) atomicAdd(&hmass[b], whole_weight(weight(v[j][e], d.m, T)));
+                if (weigh) atomicAdd(&hmass[b], whole_weight(v[j][e], d.m, T));
             }
     }
     __syncthreads();
@@ -693,16 +719,17 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
     }
 }
 
-// The value (as ordered bits, at least `floor`) at which the sum over the
-// values from the top first reaches `want`, 8 bits at a time: `each` calls its
-// argument for every value with its key and what it adds. 0 (everything is
-// kept) if they all sum to less.
+// The value (as ordered bits) at which the sum over the values from the top
+// first reaches `want`, 8 bits at a time below the bits that all keys (in
+// [kmin, kmax]) share: `each` calls its argument for every value with its key
+// and what it adds. kmin (everything is kept) if they all sum to less.
 template <class E>
-__device__ static inline uint32_t find_cut(u64 want, uint32_t floor, u64* hist, u64* sel, E&& each) {
-    uint32_t prefix = 0;
-    u64 left = want;
+__device__ static inline uint32_t find_cut(u64 want, uint32_t kmin, uint32_t kmax, u64* hist, u64* sel, E&& each) {
     const int tid = threadIdx.x, lane = tid & 63;
-    for (int sh = 24; sh >= 0; sh -= 8) {
+    uint32_t prefix = 0;   // of key - kmin
+    u64 left = want;
+    const int bits = kmax > kmin ? 32 - __clz(kmax - kmin) : 0;
+    for (int sh = ((bits + 7) >> 3 << 3) - 8; sh >= 0; sh -= 8) {
         __syncthreads();
         hist[tid] = 0;
         if (tid == 0) {
@@ -711,7 +738,8 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t floor, u64* hist, 
         }
         __syncthreads();
         each([&](uint32_t key, u64 adds) {
-            if (key >= floor && (sh == 24 || (key >> (sh + 8)) == (prefix >> (sh + 8)))) atomicAdd(&hist[(key >> sh) & 255u], adds);
+            const uint32_t k = key - kmin;
+            if (sh == 24 || (k >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(k >> sh) & 255u], adds);
         });
         __syncthreads();
         if (tid < 64) {   // lane l: digits 255 - 4l .. 252 - 4l
@@ -733,16 +761,17 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t floor, u64* hist, 
         prefix = (uint32_t)sel[0];
         left = sel[1];
     }
-    return prefix;
+    return kmin + prefix;
 }
 
 __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, SampleWs w, int32_t* __restrict__ ids,
                                                      float* __restrict__ probs) {
     __shared__ uint32_t keys[SM_CAND];
+    __shared__ uint8_t group[SM_CAND];   // the workgroup of the row that a value came from
     __shared__ u64 gmass[LG_T], hist[256], red[4], found[2], wts[SM_SMALL];
     __shared__ uint32_t tok[SM_SMALL];
     __shared__ uint32_t s_last, s_n, s_at;
-    __shared__ double T[16];
+    __shared__ double T[32];
     static_assert(SM_CHUNKS <= LG_T, "a thread a workgroup of the row");
     static_assert(SM_SMALL == 2 * LG_T, "two values a thread");
     const int row = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
@@ -772,10 +801,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                 const float q = v[j][e];
                 const int b = q > -INFINITY ? bin_of(q, d) : SM_BINS;
                 if (b >= lo && b <= hi) in |= 1u << (4 * j + e);
-                if (b < lo && !from_hist) {
-                    const double x = weight(q, d.m, T);
-                    if (x >= ask.min_p) sum += whole_weight(x);
-                }
+                if (b < lo && !from_hist && weight(q, d.m, T) >= ask.min_p) sum += whole_weight(q, d.m, T);
             }
         // the workgroup's place among the gathered values, then each thread's
         if (tid == 0) s_n = 0;
@@ -801,7 +827,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     if (!finished_last(&info->done[1], w.groups, &s_last)) return;
     const uint32_t n = left32(&info->n_cand);
     const u64 above = info->above, mass_above = info->mass_above;
-    auto weigh_key = [&](uint32_t key) { return whole_weight(weight(unordered(key), d.m, T)); };
+    auto weigh_key = [&](uint32_t key) { return whole_weight(unordered(key), d.m, T); };
     float* prob = probs ? probs + row : nullptr;
     if (lo == 0 && n <= SM_SMALL) {
         // every value that may be kept is here, two a thread: it is kept if fewer than k are larger, if the larger ones
@@ -877,10 +903,24 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     uint32_t cut = 0;
     gmass[tid] = tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0;
     if (n <= SM_CAND) {
-        for (uint32_t i = tid; i < n; i += LG_T) keys[i] = left32(&cand[i].x);
-        __syncthreads();
+        u64 top = 0, low = 0;
+        for (uint32_t i0 = tid; i0 < n; i0 += 8 * LG_T) {   // eight loads in flight
+            u64 q[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) q[e] = i0 + e * LG_T < n ? left64(&cand[i0 + e * LG_T]) : 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (i0 + e * LG_T < n) {
+                    const uint32_t key = (uint32_t)q[e];
+                    keys[i0 + e * LG_T] = key;
+                    group[i0 + e * LG_T] = (uint8_t)((uint32_t)(q[e] >> 32) / (uint32_t)(LG_CH * w.span));
+                    top = key > top ? key : top;
+                    low = (u64)(~key) > low ? (u64)(~key) : low;
+                }
+        }
+        const uint32_t kmax = (uint32_t)block_max64(top, red), kmin = n ? ~(uint32_t)block_max64(low, red) : 0u;   // none: no cut
         if (ask.k > 0)
-            cut = find_cut((u64)ask.k - above, 0, hist, found, [&](auto&& f) {
+            cut = find_cut((u64)ask.k - above, kmin, kmax, hist, found, [&](auto&& f) {
                 for (uint32_t i = tid; i < n; i += LG_T) f(keys[i], 1ull);
             });
         if (ask.top_p < 1.0) {
@@ -891,17 +931,16 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                     if (keys[i] >= cut) in += weigh_key(keys[i]);
                 want = (u64)fmax(ceil(ask.top_p * (double)(mass_above + block_sum64(in, red))), 1.0);
             }
-            const uint32_t c2 = find_cut(want - mass_above, cut, hist, found, [&](auto&& f) {
-                for (uint32_t i = tid; i < n; i += LG_T) f(keys[i], weigh_key(keys[i]));
+            const uint32_t floor = cut;
+            const uint32_t c2 = find_cut(want - mass_above, kmin, kmax, hist, found, [&](auto&& f) {
+                for (uint32_t i = tid; i < n; i += LG_T)
+                    if (keys[i] >= floor) f(keys[i], weigh_key(keys[i]));
             });
             cut = c2 > cut ? c2 : cut;
         }
         __syncthreads();
-        for (uint32_t i = tid; i < n; i += LG_T) {
-            const double q = weight(unordered(keys[i]), d.m, T);
-            if (keys[i] >= cut && q >= ask.min_p)
-                atomicAdd(&gmass[left32(&cand[i].y) / (uint32_t)(LG_CH * w.span)], whole_weight(q));
-        }
+        for (uint32_t i = tid; i < n; i += LG_T)
+            if (keys[i] >= cut && weight(unordered(keys[i]), d.m, T) >= ask.min_p) atomicAdd(&gmass[group[i]], weigh_key(keys[i]));
     } else {
         // too many values share the cut's bins: the same, in passes over the row
         const int chunks = (V + LG_CH - 1) / LG_CH;
@@ -917,16 +956,17 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
             }
         };
         if (ask.k > 0)
-            cut = find_cut((u64)ask.k, 0, hist, found, [&](auto&& f) { all([&](uint32_t key, int) { f(key, 1ull); }); });
+            cut = find_cut((u64)ask.k, 0, 0xffffffffu, hist, found, [&](auto&& f) { all([&](uint32_t key, int) { f(key, 1ull); }); });
         if (ask.top_p < 1.0) {
             u64 in = 0;
             all([&](uint32_t key, int) {
                 if (key >= cut) in += weigh_key(key);
             });
             const u64 want = (u64)fmax(ceil(ask.top_p * (double)block_sum64(in, red)), 1.0);
-            const uint32_t c2 = find_cut(want, cut, hist, found, [&](auto&& f) {
+            const uint32_t floor = cut;
+            const uint32_t c2 = find_cut(want, 0, 0xffffffffu, hist, found, [&](auto&& f) {
                 all([&](uint32_t key, int) {
-                    if (key >= cut) f(key, weigh_key(key));
+                    if (key >= floor) f(key, weigh_key(key));
                 });
             });
             cut = c2 > cut ? c2 : cut;
@@ -935,15 +975,13 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
         gmass[tid] = 0;
         __syncthreads();
         all([&](uint32_t key, int c) {
-            const double q = weight(unordered(key), d.m, T);
-            if (key >= cut && q >= ask.min_p) atomicAdd(&gmass[c / w.span], whole_weight(q));
+            if (key >= cut && weight(unordered(key), d.m, T) >= ask.min_p) atomicAdd(&gmass[c / w.span], weigh_key(key));
         });
     }
     __syncthreads();
     auto mw = [&](float v) {
         if (!(v > -INFINITY) || ordered(v) < cut) return (u64)0;
-        const double q = weight(v, d.m, T);
-        return q >= ask.min_p ? whole_weight(q) : 0;
+        return weight(v, d.m, T) >= ask.min_p ? whole_weight(v, d.m, T) : 0;
     };
     draw_row(sr, V, s, w, row, gmass[tid], d.m, T, red, found, mw, ids + row, prob);
 }
