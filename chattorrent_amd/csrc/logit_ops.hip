@@ -173,8 +173,8 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 //   k_sample_pick     a workgroup a row: the chunk that the token falls into,
 //                     and the token in it.
 // The others take three, a row cut over workgroups of `span` chunks:
-//   k_sample_scale    writes s to the workspace, with every workgroup's largest
-//                     and smallest value: lists, masks and the division once;
+//   k_sample_scale    writes s to the workspace, with every chunk's largest and
+//                     smallest value: lists, masks and the division once;
 //   k_sample_mass     with the row's m known, a histogram of m - s in SM_BINS
 //                     bins (counts for top-k, weights for top-p) of every
 //                     workgroup; the row's last workgroup to finish adds them
@@ -255,6 +255,17 @@ __device__ static inline uint32_t ordered(float v) {
 }
 __device__ static inline float unordered(uint32_t k) { return u2f((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
+// min-p as a cut of s: the ordered bits of the smallest value whose weight
+// reaches min_p (0: none is cut; a weight under 1e-13 counts as nothing anyhow).
+__device__ static inline uint32_t min_cut(float m, double min_p, const double* T) {
+    if (!(min_p > 1e-13)) return 0;
+    if (m == INFINITY) return ordered(m);
+    uint32_t k = ordered(fminf((float)((double)m + log(min_p)), m));   // within a step or two of it
+    while (k < ordered(m) && weight(unordered(k), m, T) < min_p) k++;
+    while (weight(unordered(k - 1), m, T) >= min_p) k--;
+    return k;
+}
+
 // A lane's 64-bit value from another lane by DPP (zero where there is none).
 template <int CTRL, int ROWS = 0xf>
 __device__ static inline u64 dpp64(u64 v) {
@@ -308,22 +319,23 @@ __device__ static inline u64 block_max64(u64 v, u64* red) {
     return a > b ? a : b;
 }
 
-// The workspace of a call. Without cuts: per row and chunk the largest key and
-// the weight. With: per row and workgroup (`groups` of them) the largest key,
-// the smallest value, the weight and the histogram; per row the scaled logits,
-// what the cuts found, two counters of finished workgroups and the gathered
-// values.
+// The workspace of a call: per row and chunk the largest key, and (without
+// cuts) the weight. With cuts also the smallest value of every chunk; per row
+// and workgroup (`groups` of them) the weight and the histogram; per row the
+// scaled logits, what the cuts found, two counters of finished workgroups and
+// the gathered values.
 struct SampleInfo {
     int32_t lo, hi;        // the bins whose values are gathered
     uint32_t above;        // values in the bins before lo
     uint32_t n_cand;       // gathered values (more than SM_CAND: not all of them were)
     u64 mass_above;        // the weight of the bins before lo
     u64 want;              // top-p without top-k: the weight to reach
-    uint32_t done[2], pad[2];
+    uint32_t floor, fixed; // min-p as a value's ordered bits; whether it is the cut
+    uint32_t done[2];
 };
 struct SampleWs {
-    u64* best;        // [rows][groups] ordered(a) << 32 | ~token; 0: nothing above -inf
-    float* least;     // [rows][groups] the smallest value above -inf
+    u64* best;        // [rows][chunks] ordered(a) << 32 | ~token; 0: nothing above -inf
+    float* least;     // [rows][chunks] the smallest value above -inf
     u64* mass;        // [rows][groups]
     u64* hmass;       // [rows][groups][SM_BINS]
     uint32_t* hcount; // [rows][groups][SM_BINS]
@@ -331,7 +343,7 @@ struct SampleWs {
     uint2* cand;      // [rows][SM_CAND] ordered(s), token
     float* s;         // [rows][lds]
     int64_t lds;
-    int groups, span;
+    int chunks, groups, span;
 };
 
 struct RowAsk {
@@ -372,30 +384,52 @@ __device__ static inline u64 target_of(double u, u64 total) {
 }
 
 // Of a chunk's scaled logits v (in adjusted_chunk's order), the token with
-// `left` of the kept weights of the chunk before it. Called by the whole
-// workgroup; mw(v) is a value's kept weight; hit(token, v) is called once.
+// `left` of the kept weights of the chunk before it; false (and left less the
+// chunk's weight) if the chunk ends before. Called by the whole workgroup;
+// mw(v) is a value's kept weight; hit(token, v) is called once. runs: LDS for
+// the runs' weights by wave.
 template <class W, class H>
-__device__ static inline void draw_in_chunk(const float (&v)[LG_J][4], int base, u64 left, u64* red, W&& mw, H&& hit) {
+__device__ static inline bool draw_in_chunk(const float (&v)[LG_J][4], int base, u64& left, u64 (&runs)[LG_J][4], W&& mw,
+                                            H&& hit) {
+    const int wave = threadIdx.x >> 6;
+    u64 m[LG_J][4], inc[LG_J];
 #pragma unroll
     for (int j = 0; j < LG_J; j++) {   // runs of 4 * LG_T tokens, one after another
-        u64 m[4], sum = 0;
+        u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            m[e] = mw(v[j][e]);
-            sum += m[e];
+            m[j][e] = mw(v[j][e]);
+            sum += m[j][e];
         }
-        u64 before = block_before64(sum, red);
-        const u64 run = red[0] + red[1] + red[2] + red[3];
-        if (left < run) {   // the same for every thread
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (before <= left && left < before + m[e]) hit(base + 4 * (LG_T * j + (int)threadIdx.x) + e, v[j][e]);
-                before += m[e];
-            }
-            return;
-        }
-        left -= run;
+        inc[j] = wave_scan64(sum);
     }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63)
+#pragma unroll
+        for (int j = 0; j < LG_J; j++) runs[j][wave] = inc[j];
+    __syncthreads();
+    u64 ahead = 0;   // of the chunk's weights, before the run and wave
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < LG_J; j++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const u64 here = runs[j][q];
+            if (!found && left < ahead + here) {   // the same for every thread
+                found = true;
+                if (q == wave) {
+                    u64 before = ahead + inc[j] - (m[j][0] + m[j][1] + m[j][2] + m[j][3]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (before <= left && left < before + m[j][e]) hit(base + 4 * (LG_T * j + (int)threadIdx.x) + e, v[j][e]);
+                        before += m[j][e];
+                    }
+                }
+            }
+            ahead += here;
+        }
+    if (!found) left -= ahead;
+    return found;
 }
 
 // ---- without cuts
@@ -426,8 +460,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict
         sum = block_sum64(sum - LG_J * 4 * SM_BASE, red);
     }
     if (threadIdx.x == 0) {
-        w.best[(size_t)row * w.groups + c] = best;
-        w.mass[(size_t)row * w.groups + c] = sum;
+        w.best[(size_t)row * w.chunks + c] = best;
+        w.mass[(size_t)row * w.chunks + c] = sum;
     }
 }
 
@@ -438,13 +472,13 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
                                                       SampleWs w, int32_t* __restrict__ ids, float* __restrict__ probs) {
     __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
     __shared__ double T[32];
-    __shared__ u64 red[4], found[2];
+    __shared__ u64 red[4], found[2], runs[LG_J][4];
     __shared__ float s_m;
     const int row = blockIdx.x, tid = threadIdx.x;
     exp_table(T);
     const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
-    const u64 mine = tid < w.groups ? w.best[(size_t)row * w.groups + tid] : 0;
-    const u64 local = tid < w.groups ? w.mass[(size_t)row * w.groups + tid] : 0;
+    const u64 mine = tid < w.chunks ? w.best[(size_t)row * w.chunks + tid] : 0;
+    const u64 local = tid < w.chunks ? w.mass[(size_t)row * w.chunks + tid] : 0;
     const u64 key = block_max64(mine, red);
     if (!key || !(temp > 0.0)) {
         if (tid == 0) {
@@ -468,7 +502,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
     }
     __syncthreads();
     const int c = (int)found[0];
-    const u64 left = found[1];
+    u64 left = found[1];
     const float m_c = s_m;
     float a[LG_J][4];
     adjusted_chunk<VEC>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
@@ -476,7 +510,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
     for (int j = 0; j < LG_J; j++)
 #pragma unroll
         for (int e = 0; e < 4; e++) a[j][e] = scaled_logit(a[j][e], inv);
-    draw_in_chunk(a, c * LG_CH, left, red, [&](float v) { return whole_weight(v, m_c, T); }, [&](int t, float v) {
+    draw_in_chunk(a, c * LG_CH, left, runs, [&](float v) { return whole_weight(v, m_c, T); }, [&](int t, float v) {
         ids[row] = t;
         if (probs) probs[row] = (float)(weight(v, m, T) * SM_ONE / (double)total);
     });
@@ -488,33 +522,30 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
                                                        SampleWs w) {
     __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
     __shared__ u64 red[4];
-    const int row = blockIdx.y, g = blockIdx.x;
-    if (g == 0 && threadIdx.x < sizeof(SampleInfo) / 4) ((uint32_t*)(w.info + row))[threadIdx.x] = 0;
+    const int row = blockIdx.y, c = blockIdx.x;
+    if (c == 0 && threadIdx.x < sizeof(SampleInfo) / 4) ((uint32_t*)(w.info + row))[threadIdx.x] = 0;
     const RowPens r = row_pens(s, row);
     const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
     FirstMax first;
-    float least = INFINITY;
-    for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
-        float a[LG_J][4];
-        adjusted_chunk<VEC>(x + row * ldx, V, s, r, c * LG_CH, cnt, last, a);
+    float least = INFINITY, a[LG_J][4];
+    adjusted_chunk<VEC>(x + row * ldx, V, s, r, c * LG_CH, cnt, last, a);
 #pragma unroll
-        for (int j = 0; j < LG_J; j++) {
-            const int t = c * LG_CH + 4 * (LG_T * j + (int)threadIdx.x);
-            float v[4];
+    for (int j = 0; j < LG_J; j++) {
+        const int t = c * LG_CH + 4 * (LG_T * j + (int)threadIdx.x);
+        float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                first.take(a[j][e], t + e);
-                least = a[j][e] > -INFINITY ? fminf(least, a[j][e]) : least;
-                v[e] = scaled_logit(a[j][e], inv);
-            }
-            if (t < V) *(float4*)(w.s + row * w.lds + t) = make_float4(v[0], v[1], v[2], v[3]);
+        for (int e = 0; e < 4; e++) {
+            first.take(a[j][e], t + e);
+            least = a[j][e] > -INFINITY ? fminf(least, a[j][e]) : least;
+            v[e] = scaled_logit(a[j][e], inv);
         }
+        if (t < V) *(float4*)(w.s + row * w.lds + t) = make_float4(v[0], v[1], v[2], v[3]);
     }
     const u64 best = block_max64(first.key(), red);
     const u64 low = block_max64(~(u64)ordered(least), red);
     if (threadIdx.x == 0) {
-        w.best[(size_t)row * w.groups + g] = best;
-        w.least[(size_t)row * w.groups + g] = unordered((uint32_t)~low);
+        w.best[(size_t)row * w.chunks + c] = best;
+        w.least[(size_t)row * w.chunks + c] = unordered((uint32_t)~low);
     }
 }
 
@@ -535,10 +566,10 @@ struct RowDraw {
 };
 __device__ static inline RowDraw row_draw(const SampleWs& w, int row, const RowAsk& ask, u64* red) {
     u64 best = 0, low = 0;
-    for (int i = threadIdx.x; i < w.groups; i += LG_T) {
-        const u64 b = w.best[(size_t)row * w.groups + i];
+    for (int i = threadIdx.x; i < w.chunks; i += LG_T) {
+        const u64 b = w.best[(size_t)row * w.chunks + i];
         best = b > best ? b : best;
-        const u64 l = ~(u64)ordered(w.least[(size_t)row * w.groups + i]);
+        const u64 l = ~(u64)ordered(w.least[(size_t)row * w.chunks + i]);
         low = l > low ? l : low;
     }
     RowDraw d;
@@ -557,7 +588,7 @@ __device__ static inline int bin_of(float s, const RowDraw& d) {
 // (this thread's workgroup of the row) -> the token.
 template <class W>
 __device__ static inline void draw_row(const float* __restrict__ sr, int V, const SamplingDev& s, const SampleWs& w, int row,
-                                       u64 mass, float m, const double* T, u64* red, u64* found, W&& mw, int32_t* id,
+                                       u64 mass, float m, const double* T, u64* red, u64* found, u64 (&runs)[LG_J][4], W&& mw, int32_t* id,
                                        float* prob) {
     const u64 before = block_before64(mass, red);
     const u64 total = red[0] + red[1] + red[2] + red[3];
@@ -568,30 +599,21 @@ __device__ static inline void draw_row(const float* __restrict__ sr, int V, cons
         found[1] = target - before;
     }
     __syncthreads();
-    int c = (int)found[0] * w.span;
     u64 left = found[1];
-    float v[LG_J][4];
-    for (int i = 1; i < w.span; i++, c++) {   // the workgroup's chunk that holds it
+    for (int c = (int)found[0] * w.span, end = c + w.span; c < end; c++) {   // the workgroup's chunk that holds it
+        float v[LG_J][4];
         scaled_chunk(sr, V, c * LG_CH, v);
-        u64 sum = 0;
-#pragma unroll
-        for (int j = 0; j < LG_J; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += mw(v[j][e]);
-        sum = block_sum64(sum, red);
-        if (left < sum) break;
-        left -= sum;
+        if (draw_in_chunk(v, c * LG_CH, left, runs, mw, [&](int t, float q) {
+                *id = t;
+                if (prob) *prob = (float)(weight(q, m, T) * SM_ONE / (double)total);
+            }))
+            return;
     }
-    scaled_chunk(sr, V, c * LG_CH, v);
-    draw_in_chunk(v, c * LG_CH, left, red, mw, [&](int t, float q) {
-        *id = t;
-        if (prob) *prob = (float)(weight(q, m, T) * SM_ONE / (double)total);
-    });
 }
 
 __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, SampleWs w, int32_t* __restrict__ ids,
                                                       float* __restrict__ probs) {
-    __shared__ u64 hmass[SM_BINS], red[4], found[2];
+    __shared__ u64 hmass[SM_BINS], red[4], found[2], runs[LG_J][4];
     __shared__ uint32_t hcount[SM_BINS], s_last;
     __shared__ double T[32];
     const int row = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
@@ -610,9 +632,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
     SampleInfo* info = w.info + row;
     const size_t at = (size_t)row * w.groups + g;
     if (!ask.cut) {
-        auto mw = [&](float v) {
-            return ask.min_p > 0.0 && !(weight(v, d.m, T) >= ask.min_p) ? 0 : whole_weight(v, d.m, T);
-        };
+        const uint32_t cut = min_cut(d.m, ask.min_p, T);
+        auto mw = [&](float v) { return ordered(v) >= cut ? whole_weight(v, d.m, T) : 0; };
         u64 sum = 0;
         for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
             float v[LG_J][4];
@@ -625,12 +646,12 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
         sum = block_sum64(sum, red);
         if (tid == 0) leave64(&w.mass[at], sum);
         if (!finished_last(&info->done[0], w.groups, &s_last)) return;
-        draw_row(sr, V, s, w, row, tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0, d.m, T, red, found, mw,
+        draw_row(sr, V, s, w, row, tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0, d.m, T, red, found, runs, mw,
                  ids + row, prob);
         return;
     }
-    // the histogram; weights only where top-p needs them
-    const bool weigh = ask.top_p < 1.0;
+    // the histogram: counts for top-k, weights for top-p
+    const bool weigh = ask.top_p < 1.0, count = ask.k > 0 || !weigh;
     for (int b = tid; b < SM_BINS; b += LG_T) {
         hmass[b] = 0;
         hcount[b] = 0;
@@ -645,13 +666,13 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
             for (int e = 0; e < 4; e++) {
                 if (!(v[j][e] > -INFINITY)) continue;
                 const int b = bin_of(v[j][e], d);
-                atomicAdd(&hcount[b], 1u);
+                if (count) atomicAdd(&hcount[b], 1u);
                 if (weigh) atomicAdd(&hmass[b], whole_weight(v[j][e], d.m, T));
             }
     }
     __syncthreads();
     // thread t: bins 2t and 2t + 1
-    leave64(&w.hcount[at * SM_BINS + 2 * tid], (u64)hcount[2 * tid + 1] << 32 | hcount[2 * tid]);
+    if (count) leave64(&w.hcount[at * SM_BINS + 2 * tid], (u64)hcount[2 * tid + 1] << 32 | hcount[2 * tid]);
     if (weigh) {
         leave64(&w.hmass[at * SM_BINS + 2 * tid], hmass[2 * tid]);
         leave64(&w.hmass[at * SM_BINS + 2 * tid + 1], hmass[2 * tid + 1]);
@@ -663,7 +684,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const size_t o = ((size_t)row * w.groups + min(i0 + i, w.groups - 1)) * SM_BINS + 2 * tid;
-            c2[i] = left64(&w.hcount[o]);
+            c2[i] = count ? left64(&w.hcount[o]) : 0;
             m2[i][0] = weigh ? left64(&w.hmass[o]) : 0;
             m2[i][1] = weigh ? left64(&w.hmass[o + 1]) : 0;
         }
@@ -708,11 +729,18 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
         if (ask.k == 0) hi = lo;
     }
     // few enough up to and with hi: all of them are gathered
-    if (ahead(nb, n, hi + 1 < SM_BINS ? hi + 1 : hi) + (hi + 1 < SM_BINS ? 0 : SM_SMALL + 1) <= SM_SMALL) lo = 0;
+    if (count && hi + 1 < SM_BINS && ahead(nb, n, hi + 1) <= SM_SMALL) lo = 0;
+    // min-p cuts above what top-k and top-p cut: only its own bin is looked at
+    const uint32_t floor = min_cut(d.m, ask.min_p, T);
+    const int fb = floor ? bin_of(unordered(floor), d) : SM_BINS;
+    const bool fixed = fb < lo;
+    if (fixed) lo = hi = fb;
     const u64 above = ahead(nb, n, lo), mass_above = weigh ? ahead(mb, ms, lo) : 0;
     if (tid == 0) {
         info->lo = lo;
         info->hi = hi;
+        info->floor = floor;
+        info->fixed = fixed;
         info->above = (uint32_t)above;
         info->mass_above = mass_above;
         info->want = want;
@@ -768,7 +796,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                                                      float* __restrict__ probs) {
     __shared__ uint32_t keys[SM_CAND];
     __shared__ uint8_t group[SM_CAND];   // the workgroup of the row that a value came from
-    __shared__ u64 gmass[LG_T], hist[256], red[4], found[2], wts[SM_SMALL];
+    __shared__ u64 gmass[LG_T], hist[256], red[4], found[2], wts[SM_SMALL], runs[LG_J][4];
     __shared__ uint32_t tok[SM_SMALL];
     __shared__ uint32_t s_last, s_n, s_at;
     __shared__ double T[32];
@@ -784,7 +812,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     SampleInfo* info = w.info + row;
     const int lo = info->lo, hi = info->hi;
     uint2* cand = w.cand + (size_t)row * SM_CAND;
-    const bool from_hist = ask.top_p < 1.0 && !(ask.min_p > 0.0);   // the bins before lo: their weights are in the histogram
+    const uint32_t floor = info->floor;
+    const bool from_hist = ask.top_p < 1.0;   // the weights of the bins before lo, all above min-p's, are in the histogram
     u64 sum = 0;
     if (from_hist) {
         const u64* h = w.hmass + ((size_t)row * w.groups + g) * SM_BINS;
@@ -801,7 +830,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                 const float q = v[j][e];
                 const int b = q > -INFINITY ? bin_of(q, d) : SM_BINS;
                 if (b >= lo && b <= hi) in |= 1u << (4 * j + e);
-                if (b < lo && !from_hist && weight(q, d.m, T) >= ask.min_p) sum += whole_weight(q, d.m, T);
+                if (b < lo && !from_hist) sum += whole_weight(q, d.m, T);
             }
         // the workgroup's place among the gathered values, then each thread's
         if (tid == 0) s_n = 0;
@@ -829,7 +858,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     const u64 above = info->above, mass_above = info->mass_above;
     auto weigh_key = [&](uint32_t key) { return whole_weight(unordered(key), d.m, T); };
     float* prob = probs ? probs + row : nullptr;
-    if (lo == 0 && n <= SM_SMALL) {
+    if (lo == 0 && n <= SM_SMALL && !info->fixed) {
         // every value that may be kept is here, two a thread: it is kept if fewer than k are larger, if the larger ones
         // that top-k keeps have not reached p of the weight, and if it reaches min_p
         uint32_t kv[2];
@@ -877,8 +906,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < 2; q++) {
-            if (in[q] && !(weight(unordered(kv[q]), d.m, T) >= ask.min_p)) in[q] = false;
-            if (!in[q]) mv[q] = 0;
+            if (!in[q] || kv[q] < floor) mv[q] = 0;
             wts[tid + q * LG_T] = mv[q];
         }
         const u64 total = block_sum64(mv[0] + mv[1], red);
@@ -901,6 +929,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
         return;
     }
     uint32_t cut = 0;
+    const bool k_cuts = ask.k > 0 && !info->fixed, p_cuts = ask.top_p < 1.0 && !info->fixed;
     gmass[tid] = tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0;
     if (n <= SM_CAND) {
         u64 top = 0, low = 0;
@@ -919,11 +948,11 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                 }
         }
         const uint32_t kmax = (uint32_t)block_max64(top, red), kmin = n ? ~(uint32_t)block_max64(low, red) : 0u;   // none: no cut
-        if (ask.k > 0)
+        if (k_cuts)
             cut = find_cut((u64)ask.k - above, kmin, kmax, hist, found, [&](auto&& f) {
                 for (uint32_t i = tid; i < n; i += LG_T) f(keys[i], 1ull);
             });
-        if (ask.top_p < 1.0) {
+        if (p_cuts) {
             u64 want = info->want;
             if (ask.k > 0) {
                 u64 in = 0;
@@ -931,16 +960,17 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                     if (keys[i] >= cut) in += weigh_key(keys[i]);
                 want = (u64)fmax(ceil(ask.top_p * (double)(mass_above + block_sum64(in, red))), 1.0);
             }
-            const uint32_t floor = cut;
+            const uint32_t from = cut;
             const uint32_t c2 = find_cut(want - mass_above, kmin, kmax, hist, found, [&](auto&& f) {
                 for (uint32_t i = tid; i < n; i += LG_T)
-                    if (keys[i] >= floor) f(keys[i], weigh_key(keys[i]));
+                    if (keys[i] >= from) f(keys[i], weigh_key(keys[i]));
             });
             cut = c2 > cut ? c2 : cut;
         }
+        cut = cut > floor ? cut : floor;
         __syncthreads();
         for (uint32_t i = tid; i < n; i += LG_T)
-            if (keys[i] >= cut && weight(unordered(keys[i]), d.m, T) >= ask.min_p) atomicAdd(&gmass[group[i]], weigh_key(keys[i]));
+            if (keys[i] >= cut) atomicAdd(&gmass[group[i]], weigh_key(keys[i]));
     } else {
         // too many values share the cut's bins: the same, in passes over the row
         const int chunks = (V + LG_CH - 1) / LG_CH;
@@ -955,35 +985,33 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                         if (v[j][e] > -INFINITY) f(ordered(v[j][e]), c);
             }
         };
-        if (ask.k > 0)
+        if (k_cuts)
             cut = find_cut((u64)ask.k, 0, 0xffffffffu, hist, found, [&](auto&& f) { all([&](uint32_t key, int) { f(key, 1ull); }); });
-        if (ask.top_p < 1.0) {
+        if (p_cuts) {
             u64 in = 0;
             all([&](uint32_t key, int) {
                 if (key >= cut) in += weigh_key(key);
             });
             const u64 want = (u64)fmax(ceil(ask.top_p * (double)block_sum64(in, red)), 1.0);
-            const uint32_t floor = cut;
+            const uint32_t from = cut;
             const uint32_t c2 = find_cut(want, 0, 0xffffffffu, hist, found, [&](auto&& f) {
                 all([&](uint32_t key, int) {
-                    if (key >= floor) f(key, weigh_key(key));
+                    if (key >= from) f(key, weigh_key(key));
                 });
             });
             cut = c2 > cut ? c2 : cut;
         }
+        cut = cut > floor ? cut : floor;
         __syncthreads();
         gmass[tid] = 0;
         __syncthreads();
         all([&](uint32_t key, int c) {
-            if (key >= cut && weight(unordered(key), d.m, T) >= ask.min_p) atomicAdd(&gmass[c / w.span], weigh_key(key));
+            if (key >= cut) atomicAdd(&gmass[c / w.span], weigh_key(key));
         });
     }
     __syncthreads();
-    auto mw = [&](float v) {
-        if (!(v > -INFINITY) || ordered(v) < cut) return (u64)0;
-        return weight(v, d.m, T) >= ask.min_p ? whole_weight(v, d.m, T) : 0;
-    };
-    draw_row(sr, V, s, w, row, gmass[tid], d.m, T, red, found, mw, ids + row, prob);
+    auto mw = [&](float v) { return v > -INFINITY && ordered(v) >= cut ? whole_weight(v, d.m, T) : 0; };
+    draw_row(sr, V, s, w, row, gmass[tid], d.m, T, red, found, runs, mw, ids + row, prob);
 }
 
 // Chunks a workgroup takes: one while the call has few workgroups, more where
@@ -1008,10 +1036,11 @@ static size_t sample_layout(int rows, int V, bool cuts, uint8_t* at, SampleWs& w
         return p;
     };
     const size_t gr = (size_t)rows * w.groups;
-    w.best = (u64*)take(gr * 8);
+    w.chunks = chunks;
+    w.best = (u64*)take((size_t)rows * chunks * 8);
     w.mass = (u64*)take(gr * 8);
     if (!cuts) return n;
-    w.least = (float*)take(gr * 4);
+    w.least = (float*)take((size_t)rows * chunks * 4);
     w.hmass = (u64*)take(gr * SM_BINS * 8);
     w.hcount = (uint32_t*)take(gr * SM_BINS * 4);
     w.info = (SampleInfo*)take((size_t)rows * sizeof(SampleInfo));
@@ -1031,13 +1060,13 @@ size_t sample_workspace(int rows, int V, bool cuts) {
 template <bool VEC>
 static void sample_vec(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s, int32_t* ids,
                        float* probs, const SampleWs& w) {
-    const dim3 grid(w.groups, rows);
+    const dim3 grid(w.groups, rows), chunks(w.chunks, rows);
     if (!has_cuts(s)) {
-        hipLaunchKernelGGL(k_sample_weights<VEC>, grid, dim3(LG_T), 0, st, x, ldx, V, s, w);
+        hipLaunchKernelGGL(k_sample_weights<VEC>, chunks, dim3(LG_T), 0, st, x, ldx, V, s, w);
         hipLaunchKernelGGL(k_sample_pick<VEC>, dim3(rows), dim3(LG_T), 0, st, x, ldx, V, s, w, ids, probs);
         return;
     }
-    hipLaunchKernelGGL(k_sample_scale<VEC>, grid, dim3(LG_T), 0, st, x, ldx, V, s, w);
+    hipLaunchKernelGGL(k_sample_scale<VEC>, chunks, dim3(LG_T), 0, st, x, ldx, V, s, w);
     hipLaunchKernelGGL(k_sample_mass, grid, dim3(LG_T), 0, st, V, s, w, ids, probs);
     if (s.top_k || s.top_p) hipLaunchKernelGGL(k_sample_cut, grid, dim3(LG_T), 0, st, V, s, w, ids, probs);
 }
