@@ -3,6 +3,7 @@
 // (cc_sample).
 #include "common.h"
 #include "ops.h"
+#include <type_traits>
 
 // ================================================================= adjust ===
 // A row's adjusted logits, by chunks of the vocabulary. With c the sum of the
@@ -81,9 +82,10 @@ __device__ static inline float adjust_one(float x, const SamplingDev& s, const R
 // A chunk is LG_CH tokens, LG_PER a thread: LG_J runs of four, run j of thread
 // t at 4 * (LG_T * j + t). a: the chunk's adjusted logits of row x, in that
 // order; -inf past the vocabulary and where the mask bars the token. VEC: the
-// row's fours of logits are 16-byte aligned.
+// row's fours of logits are 16-byte aligned; LISTS: the call has histories or
+// biases (without, no LDS holds the workgroups of a CU down).
 constexpr int LG_CH = 4096, LG_J = LG_CH / (4 * LG_T);
-template <bool VEC>
+template <bool VEC, bool LISTS>
 __device__ static inline void adjusted_chunk(const float* __restrict__ x, int V, const SamplingDev& s, const RowPens& r,
                                              int base, int32_t* cnt, int32_t* last, float (&a)[LG_J][4]) {
 #pragma unroll
@@ -103,15 +105,17 @@ __device__ static inline void adjusted_chunk(const float* __restrict__ x, int V,
         const int t = base + 4 * (LG_T * j + (int)threadIdx.x);
         bits[j] = !r.mask ? 15u : t < V ? r.mask[t >> 5] >> (t & 31) : 0u;
     }
-    if (gather_lists<LG_CH>(s, r, base, cnt, last)) {
+    if (LISTS && gather_lists<LG_CH>(s, r, base, cnt, last)) {
 #pragma unroll
         for (int j = 0; j < LG_J; j++) {
             const int i = 4 * (LG_T * j + (int)threadIdx.x);
             const int4 c = *(const int4*)(cnt + i), l = *(const int4*)(last + i);
-            a[j][0] = adjust_one(a[j][0], s, r, c.x, l.x);
-            a[j][1] = adjust_one(a[j][1], s, r, c.y, l.y);
-            a[j][2] = adjust_one(a[j][2], s, r, c.z, l.z);
-            a[j][3] = adjust_one(a[j][3], s, r, c.w, l.w);
+            if ((c.x | c.y | c.z | c.w | l.x | l.y | l.z | l.w) != 0) {   // few of the fours hold a listed token
+                a[j][0] = adjust_one(a[j][0], s, r, c.x, l.x);
+                a[j][1] = adjust_one(a[j][1], s, r, c.y, l.y);
+                a[j][2] = adjust_one(a[j][2], s, r, c.z, l.z);
+                a[j][3] = adjust_one(a[j][3], s, r, c.w, l.w);
+            }
         }
     }
 #pragma unroll
@@ -121,13 +125,13 @@ __device__ static inline void adjusted_chunk(const float* __restrict__ x, int V,
             if (!((bits[j] >> e) & 1u)) a[j][e] = -INFINITY;
 }
 
-template <bool VEC>
+template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_logits_adjust(const float* x, int64_t ldx, int V, SamplingDev s, float* out,
                                                         int64_t ldo) {
-    __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
+    __shared__ __align__(16) int32_t cnt[LISTS ? LG_CH : 4], last[LISTS ? LG_CH : 4];
     const int row = blockIdx.y, base = blockIdx.x * LG_CH;
     float a[LG_J][4];
-    adjusted_chunk<VEC>(x + row * ldx, V, s, row_pens(s, row), base, cnt, last, a);
+    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), base, cnt, last, a);
 #pragma unroll
     for (int j = 0; j < LG_J; j++) {
         const int t = base + 4 * (LG_T * j + (int)threadIdx.x);
@@ -143,14 +147,22 @@ __global__ __launch_bounds__(LG_T) void k_logits_adjust(const float* x, int64_t 
 }
 
 static bool vec_rows(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 4 == 0; }
+static bool has_lists(const SamplingDev& s) { return s.pen_at || s.bias_at; }
+// f with (VEC, LISTS) as types.
+template <class F>
+static void with_forms(bool vec, bool lists, F&& f) {
+    if (vec && lists) f(std::true_type{}, std::true_type{});
+    else if (vec) f(std::true_type{}, std::false_type{});
+    else if (lists) f(std::false_type{}, std::true_type{});
+    else f(std::false_type{}, std::false_type{});
+}
 
 hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s,
                                 float* out, int64_t ldo) {
     const dim3 grid((V + LG_CH - 1) / LG_CH, rows);
-    if (vec_rows(x, ldx) && vec_rows(out, ldo))
-        hipLaunchKernelGGL(k_logits_adjust<true>, grid, dim3(LG_T), 0, st, x, ldx, V, s, out, ldo);
-    else
-        hipLaunchKernelGGL(k_logits_adjust<false>, grid, dim3(LG_T), 0, st, x, ldx, V, s, out, ldo);
+    with_forms(vec_rows(x, ldx) && vec_rows(out, ldo), has_lists(s), [&](auto vec, auto lists) {
+        hipLaunchKernelGGL((k_logits_adjust<vec.value, lists.value>), grid, dim3(LG_T), 0, st, x, ldx, V, s, out, ldo);
+    });
     return hipGetLastError();
 }
 
@@ -172,13 +184,13 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 //   k_sample_weights  the weight of every chunk, relative to its own maximum;
 //   k_sample_pick     a workgroup a row: the chunk that the token falls into,
 //                     and the token in it.
-// The others take three, a row cut over workgroups of `span` chunks:
+// The others take three:
 //   k_sample_scale    writes s to the workspace, with every chunk's largest and
 //                     smallest value: lists, masks and the division once;
 //   k_sample_mass     with the row's m known, a histogram of m - s in SM_BINS
 //                     bins (counts for top-k, weights for top-p) of every
-//                     workgroup; the row's last workgroup to finish adds them
-//                     and finds the bins that the cuts fall into. (A row
+//                     chunk; the row's last workgroup to finish adds them and
+//                     finds the bins that the cuts fall into. (A row
 //                     without a cut: the weights, and the last one draws.)
 //   k_sample_cut      the values of those bins are gathered; the row's last
 //                     workgroup finds the cuts' exact values among them and
@@ -187,7 +199,7 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 //                     counts the larger ones; else 8 bits at a time.
 // A row whose cut falls among more than SM_CAND values (nearly equal logits) is
 // drawn by its last workgroup alone, in passes over the row.
-constexpr int SM_BINS = 512, SM_CAND = 8192, SM_SMALL = 512, SM_CHUNKS = (1 << 20) / LG_CH;
+constexpr int SM_BINS = 512, SM_CAND = 4096, SM_SMALL = 512, SM_CHUNKS = (1 << 20) / LG_CH;
 constexpr float SM_REACH = 32.0f;            // the histogram's last bin takes everything below m - 32
 constexpr double SM_ONE = 4398046511104.0;   // 2^42: a row of 2^20 tokens sums to at most 2^62
 typedef unsigned long long u64;
@@ -319,11 +331,10 @@ __device__ static inline u64 block_max64(u64 v, u64* red) {
     return a > b ? a : b;
 }
 
-// The workspace of a call: per row and chunk the largest key, and (without
-// cuts) the weight. With cuts also the smallest value of every chunk; per row
-// and workgroup (`groups` of them) the weight and the histogram; per row the
-// scaled logits, what the cuts found, two counters of finished workgroups and
-// the gathered values.
+// The workspace of a call: per row and chunk the largest key and the weight;
+// with cuts also the smallest value and the histogram, and per row the scaled
+// logits, what the cuts found, two counters of finished workgroups and the
+// gathered values.
 struct SampleInfo {
     int32_t lo, hi;        // the bins whose values are gathered
     uint32_t above;        // values in the bins before lo
@@ -336,14 +347,14 @@ struct SampleInfo {
 struct SampleWs {
     u64* best;        // [rows][chunks] ordered(a) << 32 | ~token; 0: nothing above -inf
     float* least;     // [rows][chunks] the smallest value above -inf
-    u64* mass;        // [rows][groups]
-    u64* hmass;       // [rows][groups][SM_BINS]
-    uint32_t* hcount; // [rows][groups][SM_BINS]
+    u64* mass;        // [rows][chunks]
+    u64* hmass;       // [rows][chunks][SM_BINS]
+    uint32_t* hcount; // [rows][chunks][SM_BINS]
     SampleInfo* info; // [rows]
     uint2* cand;      // [rows][SM_CAND] ordered(s), token
     float* s;         // [rows][lds]
     int64_t lds;
-    int chunks, groups, span;
+    int chunks;
 };
 
 struct RowAsk {
@@ -383,18 +394,16 @@ __device__ static inline u64 target_of(double u, u64 total) {
     return t < total - 1 ? t : total - 1;
 }
 
-// Of a chunk's scaled logits v (in adjusted_chunk's order), the token with
-// `left` of the kept weights of the chunk before it; false (and left less the
-// chunk's weight) if the chunk ends before. Called by the whole workgroup;
-// mw(v) is a value's kept weight; hit(token, v) is called once. runs: LDS for
-// the runs' weights by wave.
-template <class W, class H>
-__device__ static inline bool draw_in_chunk(const float (&v)[LG_J][4], int base, u64& left, u64 (&runs)[LG_J][4], W&& mw,
-                                            H&& hit) {
+// Of the scaled logits v of N runs of 4 * LG_T tokens (a chunk's are LG_J, in
+// adjusted_chunk's order), the token with `left` of their kept weights before
+// it. Called by the whole workgroup; mw(v) is a value's kept weight;
+// hit(token, v) is called once. runs: LDS for the runs' weights by wave.
+template <int N, class W, class H>
+__device__ static inline void draw_in_runs(const float (&v)[N][4], int base, u64 left, u64 (&runs)[N][4], W&& mw, H&& hit) {
     const int wave = threadIdx.x >> 6;
-    u64 m[LG_J][4], inc[LG_J];
+    u64 m[N][4], inc[N];
 #pragma unroll
-    for (int j = 0; j < LG_J; j++) {   // runs of 4 * LG_T tokens, one after another
+    for (int j = 0; j < N; j++) {
         u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -406,12 +415,12 @@ __device__ static inline bool draw_in_chunk(const float (&v)[LG_J][4], int base,
     __syncthreads();
     if ((threadIdx.x & 63) == 63)
 #pragma unroll
-        for (int j = 0; j < LG_J; j++) runs[j][wave] = inc[j];
+        for (int j = 0; j < N; j++) runs[j][wave] = inc[j];
     __syncthreads();
-    u64 ahead = 0;   // of the chunk's weights, before the run and wave
+    u64 ahead = 0;   // of the weights, before the run and wave
     bool found = false;
 #pragma unroll
-    for (int j = 0; j < LG_J; j++)
+    for (int j = 0; j < N; j++)
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const u64 here = runs[j][q];
@@ -428,22 +437,20 @@ __device__ static inline bool draw_in_chunk(const float (&v)[LG_J][4], int base,
             }
             ahead += here;
         }
-    if (!found) left -= ahead;
-    return found;
 }
 
 // ---- without cuts
-template <bool VEC>
+template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                          SampleWs w) {
-    __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
+    __shared__ __align__(16) int32_t cnt[LISTS ? LG_CH : 4], last[LISTS ? LG_CH : 4];
     __shared__ double T[32];
     __shared__ u64 red[4];
     const int row = blockIdx.y, c = blockIdx.x;
     exp_table(T);
     const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
     float a[LG_J][4];
-    adjusted_chunk<VEC>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
+    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
     FirstMax first;
 #pragma unroll
     for (int j = 0; j < LG_J; j++)
@@ -467,10 +474,10 @@ __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict
 
 // The chunks' weights relative to the row's maximum m are theirs times
 // exp(m_c - m), rounded to whole numbers again.
-template <bool VEC>
+template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                       SampleWs w, int32_t* __restrict__ ids, float* __restrict__ probs) {
-    __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
+    __shared__ __align__(16) int32_t cnt[LISTS ? LG_CH : 4], last[LISTS ? LG_CH : 4];
     __shared__ double T[32];
     __shared__ u64 red[4], found[2], runs[LG_J][4];
     __shared__ float s_m;
@@ -502,25 +509,25 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
     }
     __syncthreads();
     const int c = (int)found[0];
-    u64 left = found[1];
+    const u64 left = found[1];
     const float m_c = s_m;
     float a[LG_J][4];
-    adjusted_chunk<VEC>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
+    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
 #pragma unroll
     for (int j = 0; j < LG_J; j++)
 #pragma unroll
         for (int e = 0; e < 4; e++) a[j][e] = scaled_logit(a[j][e], inv);
-    draw_in_chunk(a, c * LG_CH, left, runs, [&](float v) { return whole_weight(v, m_c, T); }, [&](int t, float v) {
+    draw_in_runs(a, c * LG_CH, left, runs, [&](float v) { return whole_weight(v, m_c, T); }, [&](int t, float v) {
         ids[row] = t;
         if (probs) probs[row] = (float)(weight(v, m, T) * SM_ONE / (double)total);
     });
 }
 
 // ---- with cuts
-template <bool VEC>
+template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                        SampleWs w) {
-    __shared__ __align__(16) int32_t cnt[LG_CH], last[LG_CH];
+    __shared__ __align__(16) int32_t cnt[LISTS ? LG_CH : 4], last[LISTS ? LG_CH : 4];
     __shared__ u64 red[4];
     const int row = blockIdx.y, c = blockIdx.x;
     if (c == 0 && threadIdx.x < sizeof(SampleInfo) / 4) ((uint32_t*)(w.info + row))[threadIdx.x] = 0;
@@ -528,7 +535,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
     const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
     FirstMax first;
     float least = INFINITY, a[LG_J][4];
-    adjusted_chunk<VEC>(x + row * ldx, V, s, r, c * LG_CH, cnt, last, a);
+    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, r, c * LG_CH, cnt, last, a);
 #pragma unroll
     for (int j = 0; j < LG_J; j++) {
         const int t = c * LG_CH + 4 * (LG_T * j + (int)threadIdx.x);
@@ -539,7 +546,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
             least = a[j][e] > -INFINITY ? fminf(least, a[j][e]) : least;
             v[e] = scaled_logit(a[j][e], inv);
         }
-        if (t < V) *(float4*)(w.s + row * w.lds + t) = make_float4(v[0], v[1], v[2], v[3]);
+        // past the caches' ordinary way: 1.5% of the call less than plain stores, which the kernel's end writes back
+        if (t < V) __builtin_nontemporal_store(float4_t{v[0], v[1], v[2], v[3]}, (float4_t*)(w.s + row * w.lds + t));
     }
     const u64 best = block_max64(first.key(), red);
     const u64 low = block_max64(~(u64)ordered(least), red);
@@ -549,10 +557,11 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
     }
 }
 
-// A chunk of a row's scaled logits.
-__device__ static inline void scaled_chunk(const float* __restrict__ s, int V, int base, float (&v)[LG_J][4]) {
+// N runs of a row's scaled logits, from token `base` on.
+template <int N>
+__device__ static inline void scaled_runs(const float* __restrict__ s, int V, int base, float (&v)[N][4]) {
 #pragma unroll
-    for (int j = 0; j < LG_J; j++) {
+    for (int j = 0; j < N; j++) {
         const int t = base + 4 * (LG_T * j + (int)threadIdx.x);
         const float4 f = t < V ? *(const float4*)(s + t) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         v[j][0] = f.x; v[j][1] = f.y; v[j][2] = f.z; v[j][3] = f.w;
@@ -586,9 +595,9 @@ __device__ static inline int bin_of(float s, const RowDraw& d) {
 
 // The last workgroup of a row, with the workgroups' kept weights known: mass
 // (this thread's workgroup of the row) -> the token.
-template <class W>
-__device__ static inline void draw_row(const float* __restrict__ sr, int V, const SamplingDev& s, const SampleWs& w, int row,
-                                       u64 mass, float m, const double* T, u64* red, u64* found, u64 (&runs)[LG_J][4], W&& mw, int32_t* id,
+template <int N, class W>
+__device__ static inline void draw_row(const float* __restrict__ sr, int V, const SamplingDev& s, int row, u64 mass, float m,
+                                       const double* T, u64* red, u64* found, u64 (&runs)[N][4], W&& mw, int32_t* id,
                                        float* prob) {
     const u64 before = block_before64(mass, red);
     const u64 total = red[0] + red[1] + red[2] + red[3];
@@ -599,16 +608,13 @@ __device__ static inline void draw_row(const float* __restrict__ sr, int V, cons
         found[1] = target - before;
     }
     __syncthreads();
-    u64 left = found[1];
-    for (int c = (int)found[0] * w.span, end = c + w.span; c < end; c++) {   // the workgroup's chunk that holds it
-        float v[LG_J][4];
-        scaled_chunk(sr, V, c * LG_CH, v);
-        if (draw_in_chunk(v, c * LG_CH, left, runs, mw, [&](int t, float q) {
-                *id = t;
-                if (prob) *prob = (float)(weight(q, m, T) * SM_ONE / (double)total);
-            }))
-            return;
-    }
+    const int base = (int)found[0] * (N * 4 * LG_T);
+    float v[N][4];
+    scaled_runs(sr, V, base, v);
+    draw_in_runs(v, base, found[1], runs, mw, [&](int t, float q) {
+        *id = t;
+        if (prob) *prob = (float)(weight(q, m, T) * SM_ONE / (double)total);
+    });
 }
 
 __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, SampleWs w, int32_t* __restrict__ ids,
@@ -617,6 +623,9 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
     __shared__ uint32_t hcount[SM_BINS], s_last;
     __shared__ double T[32];
     const int row = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
+    const float* sr = w.s + row * w.lds;
+    float v[LG_J][4];
+    scaled_runs(sr, V, g * LG_CH, v);   // in flight while the row's maximum is found
     exp_table(T);
     const RowAsk ask(s, row, V);
     const RowDraw d = row_draw(w, row, ask, red);
@@ -628,25 +637,20 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
         }
         return;
     }
-    const float* sr = w.s + row * w.lds;
     SampleInfo* info = w.info + row;
-    const size_t at = (size_t)row * w.groups + g;
+    const size_t at = (size_t)row * w.chunks + g;
     if (!ask.cut) {
         const uint32_t cut = min_cut(d.m, ask.min_p, T);
         auto mw = [&](float v) { return ordered(v) >= cut ? whole_weight(v, d.m, T) : 0; };
         u64 sum = 0;
-        for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
-            float v[LG_J][4];
-            scaled_chunk(sr, V, c * LG_CH, v);
 #pragma unroll
-            for (int j = 0; j < LG_J; j++)
+        for (int j = 0; j < LG_J; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) sum += mw(v[j][e]);
-        }
+            for (int e = 0; e < 4; e++) sum += mw(v[j][e]);
         sum = block_sum64(sum, red);
         if (tid == 0) leave64(&w.mass[at], sum);
-        if (!finished_last(&info->done[0], w.groups, &s_last)) return;
-        draw_row(sr, V, s, w, row, tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0, d.m, T, red, found, runs, mw,
+        if (!finished_last(&info->done[0], w.chunks, &s_last)) return;
+        draw_row(sr, V, s, row, tid < w.chunks ? left64(&w.mass[(size_t)row * w.chunks + tid]) : 0, d.m, T, red, found, runs, mw,
                  ids + row, prob);
         return;
     }
@@ -657,19 +661,15 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
         hcount[b] = 0;
     }
     __syncthreads();
-    for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
-        float v[LG_J][4];
-        scaled_chunk(sr, V, c * LG_CH, v);
 #pragma unroll
-        for (int j = 0; j < LG_J; j++)
+    for (int j = 0; j < LG_J; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (!(v[j][e] > -INFINITY)) continue;
-                const int b = bin_of(v[j][e], d);
-                if (count) atomicAdd(&hcount[b], 1u);
-                if (weigh) atomicAdd(&hmass[b], whole_weight(v[j][e], d.m, T));
-            }
-    }
+        for (int e = 0; e < 4; e++) {
+            if (!(v[j][e] > -INFINITY)) continue;
+            const int b = bin_of(v[j][e], d);
+            if (count) atomicAdd(&hcount[b], 1u);
+            if (weigh) atomicAdd(&hmass[b], whole_weight(v[j][e], d.m, T));
+        }
     __syncthreads();
     // thread t: bins 2t and 2t + 1
     if (count) leave64(&w.hcount[at * SM_BINS + 2 * tid], (u64)hcount[2 * tid + 1] << 32 | hcount[2 * tid]);
@@ -677,20 +677,20 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
         leave64(&w.hmass[at * SM_BINS + 2 * tid], hmass[2 * tid]);
         leave64(&w.hmass[at * SM_BINS + 2 * tid + 1], hmass[2 * tid + 1]);
     }
-    if (!finished_last(&info->done[0], w.groups, &s_last)) return;
+    if (!finished_last(&info->done[0], w.chunks, &s_last)) return;
     u64 n[2] = {0, 0}, ms[2] = {0, 0};
-    for (int i0 = 0; i0 < w.groups; i0 += 8) {   // eight workgroups' loads in flight
+    for (int i0 = 0; i0 < w.chunks; i0 += 8) {   // eight workgroups' loads in flight
         u64 c2[8], m2[8][2];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const size_t o = ((size_t)row * w.groups + min(i0 + i, w.groups - 1)) * SM_BINS + 2 * tid;
+            const size_t o = ((size_t)row * w.chunks + min(i0 + i, w.chunks - 1)) * SM_BINS + 2 * tid;
             c2[i] = count ? left64(&w.hcount[o]) : 0;
             m2[i][0] = weigh ? left64(&w.hmass[o]) : 0;
             m2[i][1] = weigh ? left64(&w.hmass[o + 1]) : 0;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (i0 + i < w.groups) {
+            if (i0 + i < w.chunks) {
                 n[0] += c2[i] & 0xffffffffu;
                 n[1] += c2[i] >> 32;
                 ms[0] += m2[i][0];
@@ -795,7 +795,7 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t kmin, uint32_t kma
 __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, SampleWs w, int32_t* __restrict__ ids,
                                                      float* __restrict__ probs) {
     __shared__ uint32_t keys[SM_CAND];
-    __shared__ uint8_t group[SM_CAND];   // the workgroup of the row that a value came from
+    __shared__ uint8_t group[SM_CAND];   // the chunk that a value came from
     __shared__ u64 gmass[LG_T], hist[256], red[4], found[2], wts[SM_SMALL], runs[LG_J][4];
     __shared__ uint32_t tok[SM_SMALL];
     __shared__ uint32_t s_last, s_n, s_at;
@@ -805,10 +805,12 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     const int row = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
     const RowAsk ask(s, row, V);
     if (!ask.cut) return;
+    const float* sr = w.s + row * w.lds;
+    float v[LG_J][4];
+    scaled_runs(sr, V, g * LG_CH, v);   // in flight while the row's maximum is found
     exp_table(T);
     const RowDraw d = row_draw(w, row, ask, red);
     if (d.key == 0) return;
-    const float* sr = w.s + row * w.lds;
     SampleInfo* info = w.info + row;
     const int lo = info->lo, hi = info->hi;
     uint2* cand = w.cand + (size_t)row * SM_CAND;
@@ -816,44 +818,39 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     const bool from_hist = ask.top_p < 1.0;   // the weights of the bins before lo, all above min-p's, are in the histogram
     u64 sum = 0;
     if (from_hist) {
-        const u64* h = w.hmass + ((size_t)row * w.groups + g) * SM_BINS;
+        const u64* h = w.hmass + ((size_t)row * w.chunks + g) * SM_BINS;
         for (int b = tid; b < lo; b += LG_T) sum += h[b];
     }
-    for (int c = g * w.span; c < (g + 1) * w.span && c * LG_CH < V; c++) {
-        float v[LG_J][4];
-        scaled_chunk(sr, V, c * LG_CH, v);
-        uint32_t in = 0;
+    uint32_t in = 0;
 #pragma unroll
-        for (int j = 0; j < LG_J; j++)
+    for (int j = 0; j < LG_J; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float q = v[j][e];
-                const int b = q > -INFINITY ? bin_of(q, d) : SM_BINS;
-                if (b >= lo && b <= hi) in |= 1u << (4 * j + e);
-                if (b < lo && !from_hist) sum += whole_weight(q, d.m, T);
+        for (int e = 0; e < 4; e++) {
+            const float q = v[j][e];
+            const int b = q > -INFINITY ? bin_of(q, d) : SM_BINS;
+            if (b >= lo && b <= hi) in |= 1u << (4 * j + e);
+            if (b < lo && !from_hist) sum += whole_weight(q, d.m, T);
+        }
+    // the workgroup's place among the gathered values, then each thread's
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    uint32_t mine = in ? atomicAdd(&s_n, (uint32_t)__popc(in)) : 0;
+    __syncthreads();
+    if (tid == 0 && s_n) s_at = atomicAdd(&info->n_cand, s_n);
+    __syncthreads();
+    mine += s_at;
+#pragma unroll
+    for (int j = 0; j < LG_J; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if ((in >> (4 * j + e)) & 1u) {
+                if (mine < SM_CAND)
+                    leave64(&cand[mine], (u64)(g * LG_CH + 4 * (LG_T * j + tid) + e) << 32 | ordered(v[j][e]));
+                mine++;
             }
-        // the workgroup's place among the gathered values, then each thread's
-        if (tid == 0) s_n = 0;
-        __syncthreads();
-        uint32_t mine = in ? atomicAdd(&s_n, (uint32_t)__popc(in)) : 0;
-        __syncthreads();
-        if (tid == 0 && s_n) s_at = atomicAdd(&info->n_cand, s_n);
-        __syncthreads();
-        mine += s_at;
-#pragma unroll
-        for (int j = 0; j < LG_J; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if ((in >> (4 * j + e)) & 1u) {
-                    if (mine < SM_CAND)
-                        leave64(&cand[mine], (u64)(c * LG_CH + 4 * (LG_T * j + tid) + e) << 32 | ordered(v[j][e]));
-                    mine++;
-                }
-        __syncthreads();
-    }
     sum = block_sum64(sum, red);
-    if (tid == 0) leave64(&w.mass[(size_t)row * w.groups + g], sum);
-    if (!finished_last(&info->done[1], w.groups, &s_last)) return;
+    if (tid == 0) leave64(&w.mass[(size_t)row * w.chunks + g], sum);
+    if (!finished_last(&info->done[1], w.chunks, &s_last)) return;
     const uint32_t n = left32(&info->n_cand);
     const u64 above = info->above, mass_above = info->mass_above;
     auto weigh_key = [&](uint32_t key) { return whole_weight(unordered(key), d.m, T); };
@@ -930,7 +927,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     }
     uint32_t cut = 0;
     const bool k_cuts = ask.k > 0 && !info->fixed, p_cuts = ask.top_p < 1.0 && !info->fixed;
-    gmass[tid] = tid < w.groups ? left64(&w.mass[(size_t)row * w.groups + tid]) : 0;
+    gmass[tid] = tid < w.chunks ? left64(&w.mass[(size_t)row * w.chunks + tid]) : 0;
     if (n <= SM_CAND) {
         u64 top = 0, low = 0;
         for (uint32_t i0 = tid; i0 < n; i0 += 8 * LG_T) {   // eight loads in flight
@@ -942,7 +939,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                 if (i0 + e * LG_T < n) {
                     const uint32_t key = (uint32_t)q[e];
                     keys[i0 + e * LG_T] = key;
-                    group[i0 + e * LG_T] = (uint8_t)((uint32_t)(q[e] >> 32) / (uint32_t)(LG_CH * w.span));
+                    group[i0 + e * LG_T] = (uint8_t)((uint32_t)(q[e] >> 32) / (uint32_t)LG_CH);
                     top = key > top ? key : top;
                     low = (u64)(~key) > low ? (u64)(~key) : low;
                 }
@@ -976,13 +973,13 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
         const int chunks = (V + LG_CH - 1) / LG_CH;
         auto all = [&](auto&& f) {
             for (int c = 0; c < chunks; c++) {
-                float v[LG_J][4];
-                scaled_chunk(sr, V, c * LG_CH, v);
+                float x[LG_J][4];
+                scaled_runs(sr, V, c * LG_CH, x);
 #pragma unroll
                 for (int j = 0; j < LG_J; j++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        if (v[j][e] > -INFINITY) f(ordered(v[j][e]), c);
+                        if (x[j][e] > -INFINITY) f(ordered(x[j][e]), c);
             }
         };
         if (k_cuts)
@@ -1006,43 +1003,32 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
         gmass[tid] = 0;
         __syncthreads();
         all([&](uint32_t key, int c) {
-            if (key >= cut) atomicAdd(&gmass[c / w.span], weigh_key(key));
+            if (key >= cut) atomicAdd(&gmass[c], weigh_key(key));
         });
     }
     __syncthreads();
     auto mw = [&](float v) { return v > -INFINITY && ordered(v) >= cut ? whole_weight(v, d.m, T) : 0; };
-    draw_row(sr, V, s, w, row, gmass[tid], d.m, T, red, found, runs, mw, ids + row, prob);
-}
-
-// Chunks a workgroup takes: one while the call has few workgroups, more where
-// that leaves enough of them (fewer workgroups a row to join).
-static int sample_span(int rows, int V) {
-    const int chunks = (V + LG_CH - 1) / LG_CH;
-    int span = 1;
-    while (span < 4 && (int64_t)rows * (chunks / (span * 2)) >= 512) span *= 2;
-    return span;
+    draw_row(sr, V, s, row, gmass[tid], d.m, T, red, found, runs, mw, ids + row, prob);
 }
 
 // cuts: the call has top-k, top-p or min-p.
 static size_t sample_layout(int rows, int V, bool cuts, uint8_t* at, SampleWs& w) {
     const int chunks = (V + LG_CH - 1) / LG_CH;
     w = SampleWs{};
-    w.span = cuts ? sample_span(rows, V) : 1;
-    w.groups = (chunks + w.span - 1) / w.span;
     size_t n = 0;
     auto take = [&](size_t bytes) {
         uint8_t* p = at ? at + n : nullptr;
         n += (bytes + 255) & ~(size_t)255;
         return p;
     };
-    const size_t gr = (size_t)rows * w.groups;
+    const size_t rc = (size_t)rows * chunks;
     w.chunks = chunks;
-    w.best = (u64*)take((size_t)rows * chunks * 8);
-    w.mass = (u64*)take(gr * 8);
+    w.best = (u64*)take(rc * 8);
+    w.mass = (u64*)take(rc * 8);
     if (!cuts) return n;
-    w.least = (float*)take((size_t)rows * chunks * 4);
-    w.hmass = (u64*)take(gr * SM_BINS * 8);
-    w.hcount = (uint32_t*)take(gr * SM_BINS * 4);
+    w.least = (float*)take(rc * 4);
+    w.hmass = (u64*)take(rc * SM_BINS * 8);
+    w.hcount = (uint32_t*)take(rc * SM_BINS * 4);
     w.info = (SampleInfo*)take((size_t)rows * sizeof(SampleInfo));
     w.cand = (uint2*)take((size_t)rows * SM_CAND * 8);
     w.lds = (V + 3) & ~3;
@@ -1057,25 +1043,24 @@ size_t sample_workspace(int rows, int V, bool cuts) {
     return sample_layout(rows, V, cuts, nullptr, w);
 }
 
-template <bool VEC>
-static void sample_vec(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s, int32_t* ids,
-                       float* probs, const SampleWs& w) {
-    const dim3 grid(w.groups, rows), chunks(w.chunks, rows);
-    if (!has_cuts(s)) {
-        hipLaunchKernelGGL(k_sample_weights<VEC>, chunks, dim3(LG_T), 0, st, x, ldx, V, s, w);
-        hipLaunchKernelGGL(k_sample_pick<VEC>, dim3(rows), dim3(LG_T), 0, st, x, ldx, V, s, w, ids, probs);
-        return;
-    }
-    hipLaunchKernelGGL(k_sample_scale<VEC>, chunks, dim3(LG_T), 0, st, x, ldx, V, s, w);
-    hipLaunchKernelGGL(k_sample_mass, grid, dim3(LG_T), 0, st, V, s, w, ids, probs);
-    if (s.top_k || s.top_p) hipLaunchKernelGGL(k_sample_cut, grid, dim3(LG_T), 0, st, V, s, w, ids, probs);
-}
-
 hipError_t launch_sample(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s,
                          int32_t* ids, float* probs, uint8_t* ws) {
     SampleWs w;
-    sample_layout(rows, V, has_cuts(s), ws, w);
-    if (vec_rows(x, ldx)) sample_vec<true>(st, x, ldx, rows, V, s, ids, probs, w);
-    else sample_vec<false>(st, x, ldx, rows, V, s, ids, probs, w);
+    const bool cuts = has_cuts(s);
+    sample_layout(rows, V, cuts, ws, w);
+    const dim3 chunks(w.chunks, rows);
+    with_forms(vec_rows(x, ldx), has_lists(s), [&](auto vec, auto lists) {
+        constexpr bool VEC = vec.value, LISTS = lists.value;
+        if (cuts) {
+            hipLaunchKernelGGL((k_sample_scale<VEC, LISTS>), chunks, dim3(LG_T), 0, st, x, ldx, V, s, w);
+        } else {
+            hipLaunchKernelGGL((k_sample_weights<VEC, LISTS>), chunks, dim3(LG_T), 0, st, x, ldx, V, s, w);
+            hipLaunchKernelGGL((k_sample_pick<VEC, LISTS>), dim3(rows), dim3(LG_T), 0, st, x, ldx, V, s, w, ids, probs);
+        }
+    });
+    if (cuts) {
+        hipLaunchKernelGGL(k_sample_mass, chunks, dim3(LG_T), 0, st, V, s, w, ids, probs);
+        if (s.top_k || s.top_p) hipLaunchKernelGGL(k_sample_cut, chunks, dim3(LG_T), 0, st, V, s, w, ids, probs);
+    }
     return hipGetLastError();
 }
