@@ -12,9 +12,8 @@
 //   v = x;  c > 0:  v = v > 0 ? v / rep : v * rep;  v -= pres + min(freq * c, cap)
 //   + the bias of the token's last entry;  masked out: -inf
 // in f64, rounded to f32 once (an untouched token's bits stay as they are).
-// The chunk's counts and its tokens' last bias entries are gathered in LDS, so
-// an id that occurs twice needs no order: counts add up as integers, and the
-// largest entry index wins.
+// An id that occurs twice needs no order: counts add up as integers, and of a
+// token's bias entries the largest index wins.
 constexpr int LG_T = 256;
 
 struct RowPens {
@@ -45,28 +44,7 @@ __device__ static inline RowPens row_pens(const SamplingDev& s, int row) {
     return r;
 }
 
-// The chunk [base, base + CH) of the row's lists into LDS: cnt (history
-// counts) and last (bias entry + 1), zero where there is none. False (for the
-// whole workgroup) if the row has no list. Ends with a barrier.
-template <int CH>
-__device__ static inline bool gather_lists(const SamplingDev& s, const RowPens& r, int base, int32_t* cnt,
-                                           int32_t* last) {
-    if (r.p0 >= r.p1 && r.b0 >= r.b1) return false;
-    __syncthreads();   // the previous chunk's readers are done
-    for (int i = 4 * threadIdx.x; i < CH; i += 4 * LG_T) *(int4*)(cnt + i) = *(int4*)(last + i) = make_int4(0, 0, 0, 0);
-    __syncthreads();
-    for (int i = r.p0 + (int)threadIdx.x; i < r.p1; i += LG_T) {
-        const uint32_t at = (uint32_t)s.pen_ids[i] - (uint32_t)base;
-        const int n = s.pen_counts ? s.pen_counts[i] : 1;
-        if (at < (uint32_t)CH && n > 0) atomicAdd(&cnt[at], n);
-    }
-    for (int i = r.b0 + (int)threadIdx.x; i < r.b1; i += LG_T) {
-        const uint32_t at = (uint32_t)s.bias_ids[i] - (uint32_t)base;
-        if (at < (uint32_t)CH) atomicMax(&last[at], i - r.b0 + 1);
-    }
-    __syncthreads();
-    return true;
-}
+constexpr int LG_CH = 4096;
 
 __device__ static inline float adjust_one(float x, const SamplingDev& s, const RowPens& r, int cnt, int last) {
     if (cnt <= 0 && last <= 0) return x;
@@ -83,17 +61,62 @@ __device__ static inline float adjust_one(float x, const SamplingDev& s, const R
 // t at 4 * (LG_T * j + t). a: the chunk's adjusted logits of row x, in that
 // order; -inf past the vocabulary and where the mask bars the token. VEC: the
 // row's fours of logits are 16-byte aligned; LISTS: the call has histories or
-// biases (without, no LDS holds the workgroups of a CU down).
-constexpr int LG_CH = 4096, LG_J = LG_CH / (4 * LG_T);
-template <bool VEC, bool LISTS>
+// biases (without, no LDS holds the workgroups of a CU down); NT: the
+// logits pass the caches' ordinary way.
+constexpr int LG_J = LG_CH / (4 * LG_T);
+
+// Applies the row's lists to its chunk at `base`. What a token is listed for
+// is gathered in LDS first (LG_CH words): its count in the upper half of its
+// word, its last bias entry + 1 in the lower. Where those do not fit (a row of
+// 2^16 entries, or counts of the caller's), each half of the chunk in turn
+// gets a word for either.
+__device__ static inline void apply_lists(const SamplingDev& s, const RowPens& r, int base, uint32_t* lds,
+                                          float (&a)[LG_J][4]) {
+    const int tid = threadIdx.x;
+    const bool narrow = !s.pen_counts && r.p1 - r.p0 < 65536 && r.b1 - r.b0 < 65535;
+    for (int h = 0; h < (narrow ? 1 : 2); h++) {
+        const uint32_t first = base + h * (LG_CH / 2), n = narrow ? LG_CH : LG_CH / 2;
+        __syncthreads();   // what was here is read
+        for (int i = 4 * tid; i < LG_CH; i += 4 * LG_T) *(uint4*)(lds + i) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        for (int i = r.b0 + tid; i < r.b1; i += LG_T) {
+            const uint32_t at = (uint32_t)s.bias_ids[i] - first;
+            if (at < n) atomicMax(&lds[narrow ? at : LG_CH / 2 + at], (uint32_t)(i - r.b0 + 1));
+        }
+        if (narrow && r.b0 < r.b1) __syncthreads();   // the largest of whole words, before counts come in above
+        for (int i = r.p0 + tid; i < r.p1; i += LG_T) {
+            const uint32_t at = (uint32_t)s.pen_ids[i] - first;
+            const int c = s.pen_counts ? s.pen_counts[i] : 1;
+            if (at < n && c > 0) atomicAdd(&lds[at], narrow ? 0x10000u : (uint32_t)c);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < LG_J; j++) {
+            if (!narrow && j / (LG_J / 2) != h) continue;
+            const int i = 4 * (LG_T * j + tid) - (narrow ? 0 : h * (LG_CH / 2));
+            const uint4 u = *(const uint4*)(lds + i);
+            const uint4 l = narrow ? make_uint4(u.x & 0xffffu, u.y & 0xffffu, u.z & 0xffffu, u.w & 0xffffu)
+                                   : *(const uint4*)(lds + LG_CH / 2 + i);
+            const int up = narrow ? 16 : 0;
+            if ((u.x | u.y | u.z | u.w | l.x | l.y | l.z | l.w) != 0) {   // few of the fours hold a listed token
+                a[j][0] = adjust_one(a[j][0], s, r, (int)(u.x >> up), (int)l.x);
+                a[j][1] = adjust_one(a[j][1], s, r, (int)(u.y >> up), (int)l.y);
+                a[j][2] = adjust_one(a[j][2], s, r, (int)(u.z >> up), (int)l.z);
+                a[j][3] = adjust_one(a[j][3], s, r, (int)(u.w >> up), (int)l.w);
+            }
+        }
+    }
+}
+
+template <bool VEC, bool LISTS, bool NT = false>
 __device__ static inline void adjusted_chunk(const float* __restrict__ x, int V, const SamplingDev& s, const RowPens& r,
-                                             int base, int32_t* cnt, int32_t* last, float (&a)[LG_J][4]) {
+                                             int base, uint32_t* lds, float (&a)[LG_J][4]) {
 #pragma unroll
     for (int j = 0; j < LG_J; j++) {
         const int t = base + 4 * (LG_T * j + (int)threadIdx.x);
         if (VEC && t + 3 < V) {
-            const float4 f = *(const float4*)(x + t);
-            a[j][0] = f.x; a[j][1] = f.y; a[j][2] = f.z; a[j][3] = f.w;
+            const float4_t f = NT ? __builtin_nontemporal_load((const float4_t*)(x + t)) : *(const float4_t*)(x + t);
+            a[j][0] = f[0]; a[j][1] = f[1]; a[j][2] = f[2]; a[j][3] = f[3];
         } else {
 #pragma unroll
             for (int e = 0; e < 4; e++) a[j][e] = t + e < V ? x[t + e] : -INFINITY;
@@ -105,19 +128,7 @@ __device__ static inline void adjusted_chunk(const float* __restrict__ x, int V,
         const int t = base + 4 * (LG_T * j + (int)threadIdx.x);
         bits[j] = !r.mask ? 15u : t < V ? r.mask[t >> 5] >> (t & 31) : 0u;
     }
-    if (LISTS && gather_lists<LG_CH>(s, r, base, cnt, last)) {
-#pragma unroll
-        for (int j = 0; j < LG_J; j++) {
-            const int i = 4 * (LG_T * j + (int)threadIdx.x);
-            const int4 c = *(const int4*)(cnt + i), l = *(const int4*)(last + i);
-            if ((c.x | c.y | c.z | c.w | l.x | l.y | l.z | l.w) != 0) {   // few of the fours hold a listed token
-                a[j][0] = adjust_one(a[j][0], s, r, c.x, l.x);
-                a[j][1] = adjust_one(a[j][1], s, r, c.y, l.y);
-                a[j][2] = adjust_one(a[j][2], s, r, c.z, l.z);
-                a[j][3] = adjust_one(a[j][3], s, r, c.w, l.w);
-            }
-        }
-    }
+    if (LISTS && (r.p0 < r.p1 || r.b0 < r.b1)) apply_lists(s, r, base, lds, a);
 #pragma unroll
     for (int j = 0; j < LG_J; j++)
 #pragma unroll
@@ -125,19 +136,24 @@ __device__ static inline void adjusted_chunk(const float* __restrict__ x, int V,
             if (!((bits[j] >> e) & 1u)) a[j][e] = -INFINITY;
 }
 
+// What bounds it at many rows is memory. Its loads and stores are non-temporal:
+// 128 x 248320 (254 MB in and out), in turn with two other calls' buffers,
+// takes 84 us with ordinary ones and 68 with these; up to 64 rows x 151936,
+// alone or with the sampler reading its output, the two are the same.
 template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_logits_adjust(const float* x, int64_t ldx, int V, SamplingDev s, float* out,
                                                         int64_t ldo) {
-    __shared__ __align__(16) int32_t cnt[LISTS ? LG_CH : 4], last[LISTS ? LG_CH : 4];
+    __shared__ __align__(16) uint32_t lds[LISTS ? LG_CH : 4];
     const int row = blockIdx.y, base = blockIdx.x * LG_CH;
     float a[LG_J][4];
-    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), base, cnt, last, a);
+    adjusted_chunk<VEC, LISTS, true>(x + row * ldx, V, s, row_pens(s, row), base, lds, a);
 #pragma unroll
     for (int j = 0; j < LG_J; j++) {
         const int t = base + 4 * (LG_T * j + (int)threadIdx.x);
         float* o = out + row * ldo + t;
         if (VEC && t + 3 < V) {
-            *(float4*)o = make_float4(a[j][0], a[j][1], a[j][2], a[j][3]);
+            const float4_t f = {a[j][0], a[j][1], a[j][2], a[j][3]};
+            __builtin_nontemporal_store(f, (float4_t*)o);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -443,14 +459,14 @@ __device__ static inline void draw_in_runs(const float (&v)[N][4], int base, u64
 template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                          SampleWs w) {
-    __shared__ __align__(16) int32_t cnt[LISTS ? LG_CH : 4], last[LISTS ? LG_CH : 4];
+    __shared__ __align__(16) uint32_t lds[LISTS ? LG_CH : 4];
     __shared__ double T[32];
     __shared__ u64 red[4];
     const int row = blockIdx.y, c = blockIdx.x;
     exp_table(T);
     const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
     float a[LG_J][4];
-    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
+    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, lds, a);
     FirstMax first;
 #pragma unroll
     for (int j = 0; j < LG_J; j++)
@@ -477,7 +493,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict
 template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                       SampleWs w, int32_t* __restrict__ ids, float* __restrict__ probs) {
-    __shared__ __align__(16) int32_t cnt[LISTS ? LG_CH : 4], last[LISTS ? LG_CH : 4];
+    __shared__ __align__(16) uint32_t lds[LISTS ? LG_CH : 4];
     __shared__ double T[32];
     __shared__ u64 red[4], found[2], runs[LG_J][4];
     __shared__ float s_m;
@@ -512,7 +528,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
     const u64 left = found[1];
     const float m_c = s_m;
     float a[LG_J][4];
-    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, cnt, last, a);
+    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, lds, a);
 #pragma unroll
     for (int j = 0; j < LG_J; j++)
 #pragma unroll
@@ -527,7 +543,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
 template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                        SampleWs w) {
-    __shared__ __align__(16) int32_t cnt[LISTS ? LG_CH : 4], last[LISTS ? LG_CH : 4];
+    __shared__ __align__(16) uint32_t lds[LISTS ? LG_CH : 4];
     __shared__ u64 red[4];
     const int row = blockIdx.y, c = blockIdx.x;
     if (c == 0 && threadIdx.x < sizeof(SampleInfo) / 4) ((uint32_t*)(w.info + row))[threadIdx.x] = 0;
@@ -535,7 +551,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
     const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
     FirstMax first;
     float least = INFINITY, a[LG_J][4];
-    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, r, c * LG_CH, cnt, last, a);
+    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, r, c * LG_CH, lds, a);
 #pragma unroll
     for (int j = 0; j < LG_J; j++) {
         const int t = c * LG_CH + 4 * (LG_T * j + (int)threadIdx.x);
