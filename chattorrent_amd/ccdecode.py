@@ -217,8 +217,15 @@ def _is_torch(t):
     return torch is not None and isinstance(t, torch.Tensor)
 
 
+_dtypes = {}   # a dtype object's name
+
+
 def _dtype(t):
-    return str(t.dtype).rsplit(".", 1)[-1]
+    d = t.dtype
+    name = _dtypes.get(d)
+    if name is None:
+        name = _dtypes[d] = str(d).rsplit(".", 1)[-1]
+    return name
 
 
 class _Buffers:
@@ -265,7 +272,11 @@ class KVCache(_Buffers):
                         page_table=self.take(page_table, "page_table", ("int32", "uint32"), (None, None), False),
                         rope=self.take(rope, "rope", ("float32",), (None, None, 2), False),
                         bounds=self.take(bounds, "bounds", ("uint8", "int8"), (n_pages, n_kv * (2 * D + D // 8))))
-        self.ref = C.byref(self.c)
+        self._done()
+
+    def _done(self):
+        """What every call on the cache needs of it: its struct, the width of a row, workspaces' sizes as they come up."""
+        self.ref, self.width, self.workspace = C.byref(self.c), self.c.n_kv_heads * self.c.head_dim, {}
 
     @classmethod
     def of_context(cls, ctx, layer, bounds=None):
@@ -278,7 +289,7 @@ class KVCache(_Buffers):
         self.device = ctx.opts.device if _is_torch(bounds) else None
         self.c.bounds = self.take(bounds, "bounds", ("uint8", "int8"),
                                   (self.c.n_pages, int(ctx.lib.cc_bounds_bytes(C.byref(self.c)))))
-        self.ref = C.byref(self.c)
+        self._done()
         return self
 
 
@@ -314,11 +325,11 @@ class Sampling(_Buffers):
             mask=self.take(mask, "mask", i32, (None, None)), mask_words=0 if mask is None else int(mask.shape[1]),
             n_masks=0 if mask is None else int(mask.shape[0]), mask_of=self.take(mask_of, "mask_of", i32, row),
             u=self.take(u, "u", ("float64",), row))
-        self.ref = C.byref(self.c)
+        self.ref, self.workspace = C.byref(self.c), None
 
 
 def _job_rows(jobs):
-    """(slot, past, n) of each job as int32 [jobs, 3], and the rows they hold."""
+    """(slot, past, n) of each job as int32 [jobs, 3], its address, and the rows they hold."""
     a = np.asarray(jobs)
     if a.dtype != np.int32:
         if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
@@ -326,7 +337,11 @@ def _job_rows(jobs):
         a = a.astype(np.int32)
     if a.ndim != 2 or a.shape[1] != 3:
         raise ValueError("jobs: one (slot, past, n) each")
-    return np.ascontiguousarray(a), int(a[:, 2].sum(dtype=np.int64))
+    if not a.flags.c_contiguous:
+        a = np.ascontiguousarray(a)
+    n = len(a)
+    rows = int(a[0, 2]) if n == 1 else int(np.add.reduce(a[:, 2], dtype=np.int64))
+    return a, a.__array_interface__["data"][0], n, rows
 
 
 def layer_kinds(d):
@@ -578,27 +593,35 @@ class Context:
         return out
 
     # --- operators on the caller's device buffers --------------------------------------
-    def _on(self, stream, *tensors):
-        """The stream of a call on `tensors`: the one given, else torch's current one, else the context's."""
-        torch_ones = [t for t in tensors if _is_torch(t)]
-        for t in torch_ones:
-            if not t.is_cuda or t.device.index != self.opts.device:
-                raise ValueError(f"a tensor on {t.device}, not on the context's GPU ({self.opts.device})")
-        if stream is None and torch_ones:
-            if not _torch_first:
-                raise RuntimeError("import torch before the library is loaded: they would hold two HIP runtimes")
-            stream = sys.modules["torch"].cuda.current_stream(self.opts.device).cuda_stream or 1   # 0: the legacy stream
-        return stream
+    def _on(self, stream, t, out=None):
+        """The stream of a call on `t`: the one given, else torch's current one, else the context's."""
+        if not _is_torch(t):
+            return stream
+        for x in (t,) if out is None else (t, out):
+            if x.get_device() != self.opts.device:
+                raise ValueError(f"a tensor on {x.device}, not on the context's GPU ({self.opts.device})")
+        if stream is not None:
+            return stream
+        if not _torch_first:
+            raise RuntimeError("import torch before the library is loaded: they would hold two HIP runtimes")
+        torch = sys.modules["torch"]
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # a microsecond less than making a Stream
+        of = raw(self.opts.device) if raw else torch.cuda.current_stream(self.opts.device).cuda_stream
+        return of or 1   # 0: the legacy stream
 
-    def _rows(self, t, name, rows, width):
+    @staticmethod
+    def _rows(t, name, rows, width):
         """Pointer and row stride of f32 rows [rows, width], whose elements lie beside each other."""
-        if _dtype(t) != "float32" or len(t.shape) != 2 or t.shape[0] != rows or (width is not None and t.shape[1] != width):
-            raise ValueError(f"{name}: f32 [{rows}, {width}], not {t.dtype} {tuple(t.shape)}")
-        if t.shape[1] > 1 and t.stride(1) != 1:
+        shape = t.shape
+        if len(shape) != 2 or shape[0] != rows or (width is not None and shape[1] != width) or _dtype(t) != "float32":
+            raise ValueError(f"{name}: f32 [{rows}, {width}], not {t.dtype} {tuple(shape)}")
+        if t.stride(1) != 1 and shape[1] > 1:
             raise ValueError(f"{name}: a row's values must lie beside each other")
-        return t.data_ptr(), max(t.stride(0), t.shape[1]) if rows == 1 else t.stride(0)
+        ld = t.stride(0)
+        return t.data_ptr(), ld if rows > 1 else max(ld, shape[1])
 
-    def _new(self, like, shape, dtype):
+    @staticmethod
+    def _new(like, shape, dtype):
         if _is_torch(like):
             torch = sys.modules["torch"]
             return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
@@ -614,18 +637,19 @@ class Context:
         the pages they complete."""
         self._same_device(cache)
         stream = self._on(stream, k, v)
-        a, rows = _job_rows(jobs)
-        width = cache.c.n_kv_heads * cache.c.head_dim
-        kp, ldk = self._rows(k, "k", rows, width)
-        vp, ldv = self._rows(v, "v", rows, width)
-        self._chk(self.lib.cc_kv_append(self.h, cache.ref, a.ctypes.data, len(a), kp, ldk, vp, ldv, stream))
+        a, at, n, rows = _job_rows(jobs)
+        kp, ldk = self._rows(k, "k", rows, cache.width)
+        vp, ldv = self._rows(v, "v", rows, cache.width)
+        st = self.lib.cc_kv_append(self.h, cache.ref, at, n, kp, ldk, vp, ldv, stream)
+        if st:
+            self._chk(st)
 
     def kv_bounds(self, cache, jobs, stream=None):
         """cc_kv_bounds: key bounds of the pages within the jobs' rows, from the cache."""
         self._same_device(cache)
-        stream = self._on(stream, *(t for t in cache.kept if _is_torch(t)))
-        a, _ = _job_rows(jobs)
-        self._chk(self.lib.cc_kv_bounds(self.h, cache.ref, a.ctypes.data, len(a), stream))
+        stream = self._on(stream, cache.kept[-1])
+        a, at, n, _ = _job_rows(jobs)
+        self._chk(self.lib.cc_kv_bounds(self.h, cache.ref, at, n, stream))
 
     def attend_pages(self, cache, jobs, q, budget, sink=1, recent=2, out=None, stream=None):
         """cc_attend_pages: attention of the jobs' rows, q f32 [rows, heads * D]
@@ -633,20 +657,28 @@ class Context:
         rows' output (`out`, or a new array)."""
         self._same_device(cache)
         stream = self._on(stream, q, out)
-        a, rows = _job_rows(jobs)
+        a, at, n, rows = _job_rows(jobs)
         qp, ldq = self._rows(q, "q", rows, None)
         D, width = cache.c.head_dim, int(q.shape[1])
-        if width % D:
+        heads = width // D
+        if heads * D != width:
             raise ValueError(f"q: rows of {width} values are not whole heads of {D}")
         if out is None:
             out = self._new(q, (rows, width), "float32")
         op, ldo = self._rows(out, "out", rows, width)
-        need = self.lib.cc_attend_workspace(self.h, cache.ref, rows, width // D, budget) if rows else 0
-        if not need:
-            raise CCError(CC_EARG, self.lib.cc_last_error(self.h).decode())
+        need = cache.workspace.get((rows, heads, budget))
+        if need is None:
+            need = self.lib.cc_attend_workspace(self.h, cache.ref, rows, heads, budget) if rows else 0
+            if not need:
+                raise CCError(CC_EARG, self.lib.cc_last_error(self.h).decode() if rows else "jobs: at least one")
+            if len(cache.workspace) > 1000:
+                cache.workspace.clear()
+            cache.workspace[rows, heads, budget] = need
         ws = self._new(q, (need,), "uint8")
-        self._chk(self.lib.cc_attend_pages(self.h, cache.ref, a.ctypes.data, len(a), width // D, budget, sink, recent,
-                                           qp, ldq, op, ldo, ws.data_ptr(), need, stream))
+        st = self.lib.cc_attend_pages(self.h, cache.ref, at, n, heads, budget, sink, recent, qp, ldq, op, ldo,
+                                      ws.data_ptr(), need, stream)
+        if st:
+            self._chk(st)
         return out
 
     def adjust_logits(self, logits, sampling, out=None, stream=None):
@@ -654,11 +686,14 @@ class Context:
         (logits itself, another array, or a new one)."""
         self._same_device(sampling)
         stream = self._on(stream, logits, out)
+        rows, V = sampling.rows, sampling.vocab
+        lp, ld = self._rows(logits, "logits", rows, V)
         if out is None:
-            out = self._new(logits, (sampling.rows, sampling.vocab), "float32")
-        lp, ld = self._rows(logits, "logits", sampling.rows, sampling.vocab)
-        op, ldo = self._rows(out, "out", sampling.rows, sampling.vocab)
-        self._chk(self.lib.cc_logits_adjust(self.h, lp, ld, sampling.rows, sampling.vocab, sampling.ref, op, ldo, stream))
+            out = self._new(logits, (rows, V), "float32")
+        op, ldo = self._rows(out, "out", rows, V)
+        st = self.lib.cc_logits_adjust(self.h, lp, ld, rows, V, sampling.ref, op, ldo, stream)
+        if st:
+            self._chk(st)
         return out
 
     def sample(self, logits, sampling, stream=None):
@@ -669,8 +704,12 @@ class Context:
         rows, V = sampling.rows, sampling.vocab
         lp, ld = self._rows(logits, "logits", rows, V)
         ids, probs = self._new(logits, (rows,), "int32"), self._new(logits, (rows,), "float32")
-        need = self.lib.cc_sample_workspace(rows, V, sampling.ref)
+        if sampling.workspace is None:
+            sampling.workspace = self.lib.cc_sample_workspace(rows, V, sampling.ref)
+        need = sampling.workspace
         ws = self._new(logits, (max(need, 16),), "uint8")
-        self._chk(self.lib.cc_sample(self.h, lp, ld, rows, V, sampling.ref, ids.data_ptr(), probs.data_ptr(),
-                                     ws.data_ptr(), need, stream))
+        st = self.lib.cc_sample(self.h, lp, ld, rows, V, sampling.ref, ids.data_ptr(), probs.data_ptr(), ws.data_ptr(),
+                                need, stream)
+        if st:
+            self._chk(st)
         return ids, probs

@@ -2291,9 +2291,8 @@ cc_status check_rows(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_
     return CC_OK;
 }
 
-// The jobs in launches of at most OP_JOBS (and, with rows as units, at most
-// OP_ROWS rows); units(job) > 0 is the job's work. f(jobs) launches.
-constexpr int OP_ROWS = 65535;   // a grid's third dimension
+// The jobs in launches of at most OP_JOBS of them and `cap` units of work;
+// units(job) > 0 is the job's work (at most cap). f(jobs) launches.
 template <class U, class F>
 hipError_t each_batch(const cc_rows* jobs, int32_t njobs, int64_t cap, U&& units, F&& f) {
     OpJobs b;
@@ -2314,6 +2313,29 @@ hipError_t each_batch(const cc_rows* jobs, int32_t njobs, int64_t cap, U&& units
     }
     return b.n ? f(b) : hipSuccess;
 }
+// The same with rows as units: a job may go over several launches.
+template <class F>
+hipError_t each_row_batch(const cc_rows* jobs, int32_t njobs, int64_t cap, F&& f) {
+    OpJobs b;
+    int64_t row0 = 0;
+    for (int j = 0; j < njobs; j++)
+        for (int i = 0; i < jobs[j].n;) {
+            if (b.n == OP_JOBS || b.rows == cap) {
+                const hipError_t e = f(b);
+                if (e != hipSuccess) return e;
+                b.n = b.rows = b.units = 0;
+            }
+            const int n = (int)std::min<int64_t>(jobs[j].n - i, cap - b.rows);
+            b.j[b.n++] = OpJob{jobs[j].slot, jobs[j].past + i, n, (int32_t)row0, b.rows};
+            b.rows += n;
+            b.units = b.rows;
+            i += n;
+            row0 += n;
+        }
+    return b.n ? f(b) : hipSuccess;
+}
+constexpr int64_t OP_BLOCKS = 1 << 24;   // workgroups of a launch: its grid is under 2^32 threads
+constexpr int OP_ROWS = 8192;            // attention rows of a launch
 
 // How a launch of `rows` rows is laid out. Work of a row and kv head is cut
 // over workgroups until there are about two for each compute unit (at most 64
@@ -2345,11 +2367,20 @@ AttendPlan attend_plan(int ncu, const cc_cache* c, int64_t rows, int max_seen, i
     return p;
 }
 
+// Rows of a launch: its workgroups (up to ATTEND_SPLITS a row and 16 query
+// heads, or one for each 64 pages scored) stay within OP_BLOCKS.
+int64_t attend_rows(const cc_cache* c, int64_t rows, int n_heads) {
+    const int64_t heads = (int64_t)c->n_kv_heads * ceil_div(n_heads / c->n_kv_heads, 16);
+    const int64_t parts = std::max(ATTEND_SPLITS, ceil_div(c->max_pages, 64));
+    return std::min(rows, std::min<int64_t>(OP_ROWS, OP_BLOCKS / (heads * parts) - 1));
+}
+
 cc_status attend_shape(cc_ctx* ctx, const cc_cache* c, int64_t rows, int32_t n_heads, int32_t budget) {
     if (n_heads < 1 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 1024)
         return fail(ctx, CC_EARG, "n_heads must be a multiple of the cache's n_kv_heads");
-    if ((int64_t)c->n_kv_heads * ceil_div(n_heads / c->n_kv_heads, 16) > 65535 || rows < 1 || rows > (1 << 30))
-        return fail(ctx, CC_EARG, "too many heads or rows in one call");
+    if (rows < 1 || rows > (1 << 30)) return fail(ctx, CC_EARG, "attend: 1 .. 2^30 rows in a call");
+    if ((int64_t)c->n_kv_heads * ceil_div(n_heads / c->n_kv_heads, 16) > 1024)
+        return fail(ctx, CC_EARG, "attend: at most 1024 tiles of 16 query heads of a kv head");
     if (budget < 1) return fail(ctx, CC_EARG, "budget must be at least one page");
     return CC_OK;
 }
@@ -2424,7 +2455,7 @@ cc_status cc_kv_append(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, 
         if (ldk < width || ldv < width) return fail(ctx, CC_EARG, "append: ldk and ldv are at least n_kv_heads * head_dim");
         if (rows > (1 << 30)) return fail(ctx, CC_EARG, "append: too many rows in one call");
         const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
-        return launched(ctx, "append", each_batch(jobs, njobs, INT32_MAX,
+        return launched(ctx, "append", each_batch(jobs, njobs, OP_BLOCKS / 4,
             [](const cc_rows& r) { return (int64_t)(r.past + r.n - 1) / 64 - r.past / 64 + 1; },
             [&](const OpJobs& b) { return launch_kv_append(s, c, b, k, ldk, v, ldv); }));
     });
@@ -2441,7 +2472,7 @@ cc_status cc_kv_bounds(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, 
         st = check_rows(ctx, cache, jobs, njobs, &rows, true);
         if (st != CC_OK) return st;
         const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
-        return launched(ctx, "bounds", each_batch(jobs, njobs, INT32_MAX,
+        return launched(ctx, "bounds", each_batch(jobs, njobs, OP_BLOCKS / 4,
             [](const cc_rows& r) { return (int64_t)(r.past + r.n) / 64 - (r.past + 63) / 64; },
             [&](const OpJobs& b) { return launch_kv_bounds(s, c, b); }));
     });
@@ -2452,7 +2483,7 @@ size_t cc_attend_workspace(cc_ctx* ctx, const cc_cache* cache, int32_t rows, int
     try {
         CacheDev c;
         if (cache_dev(ctx, cache, c) != CC_OK || attend_shape(ctx, cache, rows, n_heads, budget) != CC_OK) return 0;
-        const int r = std::min(rows, OP_ROWS);
+        const int r = (int)attend_rows(cache, rows, n_heads);
         return attend_plan(ctx->ncu, cache, r, cache->max_pages, r, cache->max_pages, n_heads, budget).bytes;
     } catch (...) {
         return 0;
@@ -2476,25 +2507,23 @@ cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* job
             return fail(ctx, CC_EARG, "attend: sink >= 0, recent >= 1 and sink + recent <= budget");
         int max_seen = 0;
         for (int j = 0; j < njobs; j++) {
-            if (jobs[j].n > OP_ROWS) return fail(ctx, CC_EARG, "attend: a job of more than 65535 rows");
             max_seen = std::max(max_seen, (jobs[j].past + jobs[j].n - 1) / 64 + 1);
         }
         if (max_seen > budget && !c.bounds)
             return fail(ctx, CC_EARG, "attend: a row sees more pages than its budget: the cache needs bounds");
         const int64_t width = (int64_t)n_heads * c.D;
         if (ldq < width || ldo < width) return fail(ctx, CC_EARG, "attend: ldq and ldo are at least n_heads * head_dim");
-        const int64_t ws_rows = std::min<int64_t>(rows, OP_ROWS);
+        const int64_t ws_rows = attend_rows(cache, rows, n_heads);
         const size_t need = attend_plan(ctx->ncu, cache, ws_rows, max_seen, ws_rows, cache->max_pages, n_heads, budget).bytes;
         if (!workspace || workspace_bytes < need || !is_aligned(workspace, 16))
             return fail(ctx, CC_EARG, "attend: a workspace of " + std::to_string(need) + " bytes, 16-byte aligned");
         const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
-        return launched(ctx, "attend", each_batch(jobs, njobs, OP_ROWS, [](const cc_rows& r) { return (int64_t)r.n; },
-            [&](const OpJobs& b) {
-                AttendPlan p = attend_plan(ctx->ncu, cache, b.rows, max_seen, ws_rows, cache->max_pages, n_heads, budget);
-                p.sink = sink;
-                p.recent = recent;
-                return launch_attend_pages(s, c, b, p, q, ldq, out, ldo, (uint8_t*)workspace);
-            }));
+        return launched(ctx, "attend", each_row_batch(jobs, njobs, ws_rows, [&](const OpJobs& b) {
+            AttendPlan p = attend_plan(ctx->ncu, cache, b.rows, max_seen, ws_rows, cache->max_pages, n_heads, budget);
+            p.sink = sink;
+            p.recent = recent;
+            return launch_attend_pages(s, c, b, p, q, ldq, out, ldo, (uint8_t*)workspace);
+        }));
     });
 }
 

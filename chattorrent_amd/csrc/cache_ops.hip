@@ -227,6 +227,24 @@ __device__ static inline uint32_t order_bits(float v) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+// A workgroup's unit of work: part `part` of a row and head. Workgroups go
+// round the eight XCDs in launch order, each with its own L2, so an XCD gets
+// a run of the units in (head, row, part) order: the rows of a job, which
+// read the same bounds and many of the same pages, meet in one L2. row < 0: none.
+struct OpWork {
+    int row, head, part;
+};
+__device__ static inline OpWork op_work(int rows, int heads, int parts) {
+    const int per = (int)gridDim.x >> 3, w = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+    OpWork o{-1, 0, 0};
+    if (w >= rows * heads * parts) return o;
+    o.part = w % parts;
+    o.row = (w / parts) % rows;
+    o.head = w / parts / rows;
+    return o;
+}
+static int op_blocks(int64_t units) { return (int)((units + 7) / 8 * 8); }
+
 // The score of a page for a row and kv head: an upper bound, in 8 bits, of
 // q . k over the page's keys, the largest over the head's query heads:
 //   sum_b T_b * B_b * (sum_{d in b} qc > 0 ? qc * hi : qc * lo),
@@ -238,10 +256,11 @@ __device__ static inline uint32_t order_bits(float v) {
 // sum rounded to f32, so which pages a row keeps does not depend on an order
 // of summation. Kept as the score's order-preserving bits.
 //
-// A wave takes SCORE_TILES tiles of 16 pages, 4 waves of a workgroup the pages
-// one after another of one row and kv head, reading 2*D + 4*D/32 bytes a page.
-// The rows of a job read the same bounds; the later ones find them in L2.
-constexpr int SCORE_TILES = 2;
+// A wave takes a tile of 16 pages, the 4 waves of a workgroup 64 pages one
+// after another of one row and kv head, reading 2*D + 4*D/32 bytes a page. (Two
+// tiles a wave: the same at head_dim 128, 128 verify rows at 256 3% slower.)
+// The rows of a job read the same bounds (op_work puts them on one L2).
+constexpr int SCORE_PAGES = 64;
 template <int NG>
 __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, AttendPlan p, const float* __restrict__ q,
                                                     int64_t ldq, uint32_t* __restrict__ scores,
@@ -250,37 +269,32 @@ __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, Att
     __shared__ __align__(16) int8_t qc[16][D];
     __shared__ float qs[16][NG];
     // the attention launch that follows counts its finished workgroups
-    {
-        const int at = ((blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
-        for (int i = at; i < n_counters; i += gridDim.x * gridDim.y * gridDim.z * 256) counters[i] = 0;
-    }
-    const int row = blockIdx.z, kvh = blockIdx.y;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n_counters; i += gridDim.x * 256) counters[i] = 0;
+    const OpWork wk = op_work(jobs.rows, c.nKV, p.score_blocks);
+    const int row = wk.row, kvh = wk.head;
+    if (row < 0) return;
     const OpJob jb = job_of(jobs, row);
     const int pos = jb.past + row - jb.first, seen = (pos >> 6) + 1;
-    const int page0 = blockIdx.x * (64 * SCORE_TILES), page1 = seen - p.recent;
-    if (seen <= p.budget || page0 >= page1 || page0 + 64 * SCORE_TILES <= p.sink) return;
+    const int page0 = wk.part * SCORE_PAGES, page1 = seen - p.recent;
+    if (seen <= p.budget || page0 >= page1 || page0 + SCORE_PAGES <= p.sink) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, kb = lane >> 4;
     const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
     const float* cs = c.rope + (size_t)pos * c.rot;
     const float* qr = q + (jb.row0 + row - jb.first) * ldq + (size_t)kvh * p.group * D;
-    u32x4 b[SCORE_TILES][NG];
-    float B[SCORE_TILES][NG];
-    int pg[SCORE_TILES];
-#pragma unroll
-    for (int t = 0; t < SCORE_TILES; t++) {
-        pg[t] = page0 + (wave * SCORE_TILES + t) * 16 + l16;
-        const uint32_t id = pg[t] < page1 ? pt[pg[t]] : 0u;
-        const uint8_t* at = c.bounds + (size_t)(id < (uint32_t)c.n_pages ? id : 0u) * c.bblk;
+    const int page = page0 + wave * 16 + l16;
+    const uint32_t id = page < page1 ? pt[page] : 0u;
+    const bool there = id < (uint32_t)c.n_pages;   // a page index outside the cache: never kept for its score
+    u32x4 b[NG];
+    float B[NG];
+    {
+        const uint8_t* at = c.bounds + (size_t)(there ? id : 0u) * c.bblk;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            b[t][g] = *(const u32x4_a4*)(at + kvh * 2 * D + kb * (D / 2) + 16 * g);
-            B[t][g] = *(const float*)(at + c.nKV * 2 * D + (kvh * NG + g) * 4);
+            b[g] = *(const u32x4_a4*)(at + kvh * 2 * D + kb * (D / 2) + 16 * g);
+            B[g] = *(const float*)(at + c.nKV * 2 * D + (kvh * NG + g) * 4);
         }
-        if (id >= (uint32_t)c.n_pages) pg[t] = page1;   // a page index outside the cache: never kept for its score
     }
-    float best[SCORE_TILES];
-#pragma unroll
-    for (int t = 0; t < SCORE_TILES; t++) best[t] = -INFINITY;
+    float best = -INFINITY;
     for (int h0 = 0; h0 < p.group; h0 += 16) {
         const int gt = min(16, p.group - h0);
         if (h0) __syncthreads();
@@ -306,43 +320,29 @@ __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, Att
         __syncthreads();
         // the lane's operand: head l16, codes 32g + 16(kb % 2) .., the positive (kb < 2) or the negative ones;
         // rows of heads past the tile's come from whatever lies there, and are left out below
-        u32x4 a[NG];
-        float T[4][NG];
+        double acc[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             const u32x4 w = *(const u32x4*)&qc[l16][32 * g + 16 * (kb & 1)];
+            u32x4 a;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t neg = ((w[e] >> 7) & 0x01010101u) * 0xffu;
-                a[g][e] = w[e] & (kb < 2 ? ~neg : neg);
+                a[e] = w[e] & (kb < 2 ? ~neg : neg);
             }
+            i32x4 d = {0, 0, 0, 0};
+            d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b[g]), d, 0, 0, 0);
 #pragma unroll
-            for (int r = 0; r < 4; r++) T[r][g] = qs[4 * kb + r][g];
+            for (int r = 0; r < 4; r++) acc[r] = fma((double)qs[4 * kb + r][g] * (double)B[g], (double)d[r], acc[r]);
         }
 #pragma unroll
-        for (int t = 0; t < SCORE_TILES; t++) {
-            double acc[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                i32x4 d = {0, 0, 0, 0};
-                d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a[g]),
-                                                          __builtin_bit_cast(i32x4, b[t][g]), d, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; r++) acc[r] = fma((double)T[r][g] * (double)B[t][g], (double)d[r], acc[r]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (4 * kb + r < gt) best[t] = fmaxf(best[t], (float)acc[r]);
-        }
+        for (int r = 0; r < 4; r++)
+            if (4 * kb + r < gt) best = fmaxf(best, (float)acc[r]);
     }
-#pragma unroll
-    for (int t = 0; t < SCORE_TILES; t++) {
-        best[t] = fmaxf(best[t], __shfl_xor(best[t], 16));
-        best[t] = fmaxf(best[t], __shfl_xor(best[t], 32));
-        const int page = page0 + (wave * SCORE_TILES + t) * 16 + l16;
-        if (kb == 0 && page < page1)
-            scores[((size_t)row * c.nKV + kvh) * p.max_seen + page] = order_bits(pg[t] < page1 ? best[t] : -INFINITY);
-    }
+    best = fmaxf(best, __shfl_xor(best, 16));
+    best = fmaxf(best, __shfl_xor(best, 32));
+    if (kb == 0 && page < page1)
+        scores[((size_t)row * c.nKV + kvh) * p.max_seen + page] = order_bits(there ? best : -INFINITY);
 }
 
 // The pages that a row and kv head keep, ascending: entries [e0, e1) of them
@@ -352,10 +352,41 @@ __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, Att
 // 8 at a time, with a count of the scores that share the bits so far; then
 // every thread ranks a run of pages. KEEP: a thread's run is at most
 // SELECT_REG pages, held in registers throughout.
+// Up to 256 pages (one a thread) are ranked by counting instead: the larger
+// scores, and the equal ones of lower pages, out of LDS; no passes (141 pages:
+// MEASURED).
+// mine, id: page a + threadIdx.x's score and index in the cache.
+__device__ static inline void best_few_pages(uint32_t mine, uint32_t id, int a, int n, uint32_t need, int sink, int e0, int e1,
+                                             uint16_t* list, uint32_t* ids, uint64_t* keys, uint32_t* s_sel) {
+    const int t = threadIdx.x, wave = t >> 6;
+    const uint64_t key = t < n ? (uint64_t)mine << 32 | (uint32_t)(255 - t) : 0;   // unique: the lower page is the larger
+    keys[t] = key;
+    __syncthreads();
+    uint32_t rank = 0;
+    for (int i = 0; i < n; i += 8) {   // past n: zeros, larger than none
+        ulonglong2 k[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) k[e] = *(const ulonglong2*)(keys + i + 2 * e);
+#pragma unroll
+        for (int e = 0; e < 4; e++) rank += (k[e].x > key) + (k[e].y > key);
+    }
+    const bool keep = t < n && rank < need;
+    const uint64_t in = __ballot(keep);
+    if ((t & 63) == 0) s_sel[wave] = (uint32_t)__popcll(in);
+    __syncthreads();
+    int e = sink + __popcll(in & ((1ull << (t & 63)) - 1));
+    for (int w = 0; w < wave; w++) e += (int)s_sel[w];
+    if (keep && e >= e0 && e < e1) {
+        list[e - e0] = (uint16_t)(a + t);
+        ids[e - e0] = id;
+    }
+}
+
 constexpr int SELECT_REG = 4;
 template <bool KEEP>
 __device__ static inline void best_pages(const uint32_t* __restrict__ sc, int a, int z, uint32_t need, int sink, int e0,
-                                         int e1, uint16_t* list, uint32_t* hist, uint32_t* s_sel) {
+                                         int e1, const uint32_t* __restrict__ pt, uint16_t* list, uint32_t* ids,
+                                         uint32_t* hist, uint32_t* s_sel) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int per = KEEP ? SELECT_REG : (z - a + 255) / 256, i0 = a + t * per, i1 = min(i0 + per, z);
     uint32_t reg[SELECT_REG];
@@ -432,7 +463,10 @@ __device__ static inline void best_pages(const uint32_t* __restrict__ sc, int a,
     each([&](int i, uint32_t k) {
         if (k > prefix || (k == prefix && be < left)) {
             const int e = sink + (int)(bg + min(be, left));
-            if (e >= e0 && e < e1) list[e - e0] = (uint16_t)i;
+            if (e >= e0 && e < e1) {
+                list[e - e0] = (uint16_t)i;
+                ids[e - e0] = pt[i];
+            }
         }
         bg += k > prefix;
         be += k == prefix;
@@ -460,10 +494,14 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     constexpr int D = 32 * NG, DT = D / 16, SCL = NG > 4 ? NG / 4 : 1;
     constexpr int OW = 16 * D + 32;   // floats of a wave's part: O [16][D], max [16], sum [16]
     __shared__ __align__(16) float smem[ATTEND_WAVES * OW];
-    __shared__ uint16_t list[ATTEND_PER];
-    __shared__ uint32_t hist[256], s_sel[2];
+    __shared__ uint16_t list[ATTEND_PER];   // the kept pages, and their indices in the cache
+    __shared__ uint32_t ids[ATTEND_PER];
+    __shared__ __align__(16) uint32_t hist[512];
+    __shared__ uint32_t s_sel[4];
     static_assert(ATTEND_WAVES * OW >= 2 * 16 * ATTEND_SPLITS, "the join's weights take the parts' place");
-    const int row = blockIdx.z, split = blockIdx.x, kvh = blockIdx.y % c.nKV, tile = blockIdx.y / c.nKV;
+    const OpWork wk = op_work(jobs.rows, c.nKV * p.tiles, p.splits);
+    const int row = wk.row, split = wk.part, kvh = wk.head / p.tiles, tile = wk.head % p.tiles;
+    if (row < 0) return;
     const OpJob jb = job_of(jobs, row);
     const int pos = jb.past + row - jb.first, seen = (pos >> 6) + 1;
     const int kept = min(seen, p.budget);
@@ -473,6 +511,20 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j4 = lane >> 4, l16 = lane & 15;
     const int h0 = tile * 16, gt = min(16, p.group - h0);
     const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
+    // what the kept pages are found from, in flight while the query is rotated
+    const int a = p.sink, z = seen - p.recent, need = p.budget - p.sink - p.recent;
+    const uint32_t* sc = scores + ((size_t)row * c.nKV + kvh) * p.max_seen;
+    const bool few = seen > p.budget && need > 0 && z - a <= 256;
+    const uint32_t few_score = few && tid < z - a ? sc[a + tid] : 0u, few_id = few && tid < z - a ? pt[a + tid] : 0u;
+    // the other entries: the first and the last pages, or all of them
+    int end_page = -1;
+    uint32_t end_id = 0;
+    if (tid < e1 - e0) {
+        const int e = e0 + tid;
+        if (seen <= p.budget || e < a) end_page = e;
+        else if (e >= a + need) end_page = z + e - a - need;
+        if (end_page >= 0) end_id = pt[end_page];
+    }
     // the query heads, rotated, in LDS (a wave's scale slices and part come there later)
     {
         const float* cs = c.rope + (size_t)pos * c.rot;
@@ -485,25 +537,20 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
             *(float4*)&smem[h * D + d0 + 4] = make_float4(r[4], r[5], r[6], r[7]);
         }
     }
-    if (seen > p.budget) {
-        const uint32_t* sc = scores + ((size_t)row * c.nKV + kvh) * p.max_seen;
-        const int a = p.sink, z = seen - p.recent, need = p.budget - p.sink - p.recent;
-        if (need > 0) {
-            if (z - a <= 256 * SELECT_REG) best_pages<true>(sc, a, z, need, p.sink, e0, e1, list, hist, s_sel);
-            else best_pages<false>(sc, a, z, need, p.sink, e0, e1, list, hist, s_sel);
-        }
-        for (int e = e0 + tid; e < e1; e += 256) {
-            if (e < p.sink) list[e - e0] = (uint16_t)e;
-            if (e >= p.sink + need) list[e - e0] = (uint16_t)(z + e - p.sink - need);
-        }
-    } else {
-        for (int e = e0 + tid; e < e1; e += 256) list[e - e0] = (uint16_t)e;
+    if (end_page >= 0) {
+        list[tid] = (uint16_t)end_page;
+        ids[tid] = end_id;
+    }
+    if (few) best_few_pages(few_score, few_id, a, z - a, need, a, e0, e1, list, ids, (uint64_t*)hist, s_sel);
+    else if (seen > p.budget && need > 0) {
+        if (z - a <= 256 * SELECT_REG) best_pages<true>(sc, a, z, need, a, e0, e1, pt, list, ids, hist, s_sel);
+        else best_pages<false>(sc, a, z, need, a, e0, e1, pt, list, ids, hist, s_sel);
     }
     __syncthreads();
-    // this wave's entries of the list, their pages' indices one a lane
+    // this wave's entries of the list, one a lane
     const int n = e1 - e0, w0 = (n * wave) / ATTEND_WAVES, w1 = (n * (wave + 1)) / ATTEND_WAVES, nw = w1 - w0;
     const int lp = lane < nw ? (int)list[w0 + lane] : 0;
-    const uint32_t pgv = lane < nw ? pt[lp] : 0u;
+    const uint32_t pgv = lane < nw ? ids[w0 + lane] : 0u;
     half8_t qh[NG], ql[NG];
 #pragma unroll
     for (int g = 0; g < NG; g++)
@@ -796,17 +843,17 @@ static void attend_ng(hipStream_t st, const CacheDev& c, const OpJobs& jobs, con
     uint32_t* counters = (uint32_t*)(ws + p.counters);
     if (p.scored || p.splits > 1) {
         const int n_counters = p.splits > 1 ? jobs.rows * c.nKV * p.tiles : 0;
-        const int bx = p.scored ? (p.max_seen - p.recent + 64 * SCORE_TILES - 1) / (64 * SCORE_TILES) : 1;
-        hipLaunchKernelGGL((k_page_score<NG>), dim3(std::max(bx, 1), c.nKV, jobs.rows), dim3(256), 0, st, c, jobs, p, q,
-                           ldq, scores, counters, n_counters);
+        hipLaunchKernelGGL((k_page_score<NG>), dim3(op_blocks((int64_t)jobs.rows * c.nKV * p.score_blocks)), dim3(256), 0, st,
+                           c, jobs, p, q, ldq, scores, counters, n_counters);
     }
-    hipLaunchKernelGGL((k_attend_pages<NG>), dim3(p.splits, c.nKV * p.tiles, jobs.rows), dim3(256), 0, st, c, jobs, p,
-                       q, ldq, scores, partials, counters, out, ldo);
+    hipLaunchKernelGGL((k_attend_pages<NG>), dim3(op_blocks((int64_t)jobs.rows * c.nKV * p.tiles * p.splits)), dim3(256), 0, st,
+                       c, jobs, p, q, ldq, scores, partials, counters, out, ldo);
 }
 
 hipError_t launch_attend_pages(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& plan,
                                const float* q, int64_t ldq, float* out, int64_t ldo, uint8_t* ws) {
     AttendPlan p = plan;
+    p.score_blocks = p.scored ? (p.max_seen - p.recent + SCORE_PAGES - 1) / SCORE_PAGES : 1;
     p.vec = aligned16(q) && aligned16(c.rope) && ldq % 4 == 0 && c.rot % 16 == 0;
     if (c.ng == 2) attend_ng<2>(st, c, jobs, p, q, ldq, out, ldo, ws);
     else if (c.ng == 4) attend_ng<4>(st, c, jobs, p, q, ldq, out, ldo, ws);

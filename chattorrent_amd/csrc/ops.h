@@ -45,6 +45,7 @@ struct AttendPlan {
     int max_seen = 0;             // the most pages that a row sees
     int budget = 0, sink = 0, recent = 0;
     bool scored = false;          // a row sees more pages than it keeps
+    int score_blocks = 1;         // workgroups that score a row and kv head's pages
     bool vec = false;             // 16-byte loads of the query and the rope table
     size_t scores = 0, partials = 0, counters = 0, bytes = 0;   // offsets into the workspace, and its size
 };
