@@ -240,14 +240,16 @@ class _Buffers:
             return None
         if _dtype(t) not in dtypes:
             raise ValueError(f"{name}: {' or '.join(dtypes)}, not {t.dtype}")
-        if len(t.shape) != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
-            raise ValueError(f"{name}: shape {tuple(t.shape)}, not {shape}")
+        have = tuple(t.shape)
+        if have != shape and (len(have) != len(shape) or any(w is not None and n != w for n, w in zip(have, shape))):
+            raise ValueError(f"{name}: shape {have}, not {shape}")
         if _is_torch(t):
-            if not t.is_cuda or not t.is_contiguous():
+            device = t.get_device()
+            if device < 0 or not t.is_contiguous():
                 raise ValueError(f"{name}: a contiguous tensor on the GPU")
-            if self.device is not None and t.device.index != self.device:
+            if self.device is not None and device != self.device:
                 raise ValueError(f"{name}: on another GPU than the others")
-            self.device = t.device.index
+            self.device = device
         self.kept.append(t)
         return t.data_ptr()
 

@@ -87,7 +87,8 @@ template <int D, bool VEC>
 __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, const float* __restrict__ k, int64_t ldk,
                                                    const float* __restrict__ v, int64_t ldv, int only) {
     constexpr int G8 = D / 8, RPW = 64 / G8, NG = D / 32;
-    __shared__ float red[2][4][D];
+    __shared__ __align__(16) uint8_t lds[64 * D];   // V: a whole page's codes; K: the waves' ranges
+    float* red = (float*)lds;                       // [2][4][D]
     const OpJob jb = job_of(jobs, blockIdx.x);
     const int head = blockIdx.y, which = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
     if (page >= (uint32_t)c.n_pages) return;
     uint8_t* blk = (which ? c.v : c.k) + ((size_t)page * c.nKV + head) * c.blk;
     const int g = lane & (G8 - 1), rr = lane / G8;
-    const bool bounds = which == 0 && c.bounds != nullptr && s1 == 64;
+    const bool bounds = which == 0 && c.bounds != nullptr && s1 == 64, whole = which == 1 && s1 - s0 == 64;
     float mx[8], mn[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -148,9 +149,17 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
             if ((g & 3) == 0) *(float*)(blk + 64 * D + ((size_t)s * NG + (g >> 2)) * 4) = scale;
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) blk[vcode_at(8 * g + e, s, D)] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+            for (int e = 0; e < 8; e++) {
+                const uint8_t code = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+                if (whole) lds[vcode_at(8 * g + e, s, D)] = code;
+                else blk[vcode_at(8 * g + e, s, D)] = code;
+            }
             if ((g & 3) == 0) *(float*)(blk + 64 * D + (size_t)vscale_at(g >> 2, s, NG) * 4) = scale;
         }
+    }
+    if (whole) {
+        __syncthreads();
+        for (int i = 16 * threadIdx.x; i < 64 * D; i += 16 * 256) *(uint4*)(blk + i) = *(const uint4*)(lds + i);
     }
     if (!bounds) return;
 #pragma unroll
@@ -160,8 +169,8 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
             mn[e] = fminf(mn[e], __shfl_xor(mn[e], o));
         }
         if (rr == 0) {
-            red[0][wave][8 * g + e] = mx[e];
-            red[1][wave][8 * g + e] = mn[e];
+            red[wave * D + 8 * g + e] = mx[e];
+            red[(4 + wave) * D + 8 * g + e] = mn[e];
         }
     }
     __syncthreads();
@@ -170,8 +179,8 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const int d = 8 * g + e;
-        mx[e] = fmaxf(fmaxf(red[0][0][d], red[0][1][d]), fmaxf(red[0][2][d], red[0][3][d]));
-        mn[e] = fminf(fminf(red[1][0][d], red[1][1][d]), fminf(red[1][2][d], red[1][3][d]));
+        mx[e] = fmaxf(fmaxf(red[d], red[D + d]), fmaxf(red[2 * D + d], red[3 * D + d]));
+        mn[e] = fminf(fminf(red[4 * D + d], red[5 * D + d]), fminf(red[6 * D + d], red[7 * D + d]));
         amax = fmaxf(amax, fmaxf(fabsf(mx[e]), fabsf(mn[e])));
     }
     amax = fmaxf(amax, __shfl_xor(amax, 1));
