@@ -87,8 +87,7 @@ template <int D, bool VEC>
 __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, const float* __restrict__ k, int64_t ldk,
                                                    const float* __restrict__ v, int64_t ldv, int only) {
     constexpr int G8 = D / 8, RPW = 64 / G8, NG = D / 32;
-    __shared__ __align__(16) uint8_t lds[64 * D];   // V: a whole page's codes; K: the waves' ranges
-    float* red = (float*)lds;                       // [2][4][D]
+    __shared__ float red[2][4][D];
     const OpJob jb = job_of(jobs, blockIdx.x);
     const int head = blockIdx.y, which = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -99,7 +98,7 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
     if (page >= (uint32_t)c.n_pages) return;
     uint8_t* blk = (which ? c.v : c.k) + ((size_t)page * c.nKV + head) * c.blk;
     const int g = lane & (G8 - 1), rr = lane / G8;
-    const bool bounds = which == 0 && c.bounds != nullptr && s1 == 64, whole = which == 1 && s1 - s0 == 64;
+    const bool bounds = which == 0 && c.bounds != nullptr && s1 == 64;
     float mx[8], mn[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -121,6 +120,36 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
         }
     const float* src = (which ? v : k) + (size_t)head * D;
     const int64_t ld = which ? ldv : ldk;
+    if (which == 1 && s1 - s0 == 64) {
+        // a whole page of V: a thread takes 8 channels of 4 tokens in a row, whose codes of a channel lie beside each other,
+        // and 4 neighbours in a wave (D <= 128) fill a channel's 16 bytes. (4000 rows of 8 x 128: 20 us with a byte a
+        // store, 15.5 with these; two rows of K at a time: no better.)
+        for (int i = threadIdx.x; i < 16 * G8; i += 256) {
+            const int g8 = i & (G8 - 1), r = i / G8, t = 16 * (r & 3) + 4 * (r >> 2);   // tokens t .. t + 3
+            uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            float sc[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                float x[8];
+                rotated8(src + (jb.row0 + 64 * p + t + q - jb.past) * ld, 8 * g8, nullptr, 0, VEC, x);
+                float amax = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
+                amax = fmaxf(amax, __shfl_xor(amax, 1));
+                amax = fmaxf(amax, __shfl_xor(amax, 2));
+                sc[q] = amax / 127.0f;
+                const float inv = sc[q] > 0.0f ? 1.0f / sc[q] : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    w[e] |= (uint32_t)(((int)fminf(fmaxf(__builtin_rintf(x[e] * inv), -127.0f), 127.0f) ^ 0x80) & 0xff) << (8 * q);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) *(uint32_t*)(blk + vcode_at(8 * g8 + e, t, D)) = w[e];
+            if ((g8 & 3) == 0)
+                *(float4*)(blk + 64 * D + (size_t)vscale_at(g8 >> 2, t, NG) * 4) = make_float4(sc[0], sc[1], sc[2], sc[3]);
+        }
+        return;
+    }
     for (int sb = s0 + wave * RPW; sb < s1; sb += 4 * RPW) {   // uniform in the wave: lanes exchange below
         const int s = sb + rr;
         const bool live = s < s1;
@@ -149,17 +178,9 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
             if ((g & 3) == 0) *(float*)(blk + 64 * D + ((size_t)s * NG + (g >> 2)) * 4) = scale;
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint8_t code = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
-                if (whole) lds[vcode_at(8 * g + e, s, D)] = code;
-                else blk[vcode_at(8 * g + e, s, D)] = code;
-            }
+            for (int e = 0; e < 8; e++) blk[vcode_at(8 * g + e, s, D)] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
             if ((g & 3) == 0) *(float*)(blk + 64 * D + (size_t)vscale_at(g >> 2, s, NG) * 4) = scale;
         }
-    }
-    if (whole) {
-        __syncthreads();
-        for (int i = 16 * threadIdx.x; i < 64 * D; i += 16 * 256) *(uint4*)(blk + i) = *(const uint4*)(lds + i);
     }
     if (!bounds) return;
 #pragma unroll
@@ -169,8 +190,8 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
             mn[e] = fminf(mn[e], __shfl_xor(mn[e], o));
         }
         if (rr == 0) {
-            red[wave * D + 8 * g + e] = mx[e];
-            red[(4 + wave) * D + 8 * g + e] = mn[e];
+            red[0][wave][8 * g + e] = mx[e];
+            red[1][wave][8 * g + e] = mn[e];
         }
     }
     __syncthreads();
@@ -179,8 +200,8 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const int d = 8 * g + e;
-        mx[e] = fmaxf(fmaxf(red[d], red[D + d]), fmaxf(red[2 * D + d], red[3 * D + d]));
-        mn[e] = fminf(fminf(red[4 * D + d], red[5 * D + d]), fminf(red[6 * D + d], red[7 * D + d]));
+        mx[e] = fmaxf(fmaxf(red[0][0][d], red[0][1][d]), fmaxf(red[0][2][d], red[0][3][d]));
+        mn[e] = fminf(fminf(red[1][0][d], red[1][1][d]), fminf(red[1][2][d], red[1][3][d]));
         amax = fmaxf(amax, fmaxf(fabsf(mx[e]), fabsf(mn[e])));
     }
     amax = fmaxf(amax, __shfl_xor(amax, 1));
@@ -362,8 +383,7 @@ __global__ __launch_bounds__(256) void k_page_score(CacheDev c, OpJobs jobs, Att
 // every thread ranks a run of pages. KEEP: a thread's run is at most
 // SELECT_REG pages, held in registers throughout.
 // Up to 256 pages (one a thread) are ranked by counting instead: the larger
-// scores, and the equal ones of lower pages, out of LDS; no passes (141 pages:
-// MEASURED).
+// keys out of LDS, no passes (of 141 pages: 2.4 us instead of 3.9).
 // mine, id: page a + threadIdx.x's score and index in the cache.
 __device__ static inline void best_few_pages(uint32_t mine, uint32_t id, int a, int n, uint32_t need, int sink, int e0, int e1,
                                              uint16_t* list, uint32_t* ids, uint64_t* keys, uint32_t* s_sel) {
