@@ -285,13 +285,29 @@ __device__ static inline float unordered(uint32_t k) { return u2f((k & 0x8000000
 
 // min-p as a cut of s: the ordered bits of the smallest value whose weight
 // reaches min_p (0: none is cut; a weight under 1e-13 counts as nothing anyhow).
+// Mostly m + log(min_p) to a step; but next to zero an f32 step is so short
+// that millions of values share a weight (min_p 1 and m 0: all of the 10^9 from
+// -2^-54 up weigh 1), so the search's steps double and then halve: 64 at most.
 __device__ static inline uint32_t min_cut(float m, double min_p, const double* T) {
     if (!(min_p > 1e-13)) return 0;
     if (m == INFINITY) return ordered(m);
-    uint32_t k = ordered(fminf((float)((double)m + log(min_p)), m));   // within a step or two of it
-    while (k < ordered(m) && weight(unordered(k), m, T) < min_p) k++;
-    while (weight(unordered(k - 1), m, T) >= min_p) k--;
-    return k;
+    const uint32_t top = ordered(m), least = ordered((float)((double)m - 31.0)) - 1;   // it weighs nothing
+    auto cut = [&](uint32_t k) { return k <= least || (k < top && weight(unordered(k), m, T) < min_p); };
+    uint32_t lo = ordered(fminf((float)((double)m + log(min_p)), m)), hi = lo;
+    for (uint32_t step = 1; cut(hi); step *= 2) {
+        lo = hi;
+        hi = step < top - hi ? hi + step : top;
+    }
+    for (uint32_t step = 1; !cut(lo); step *= 2) {
+        hi = lo;
+        lo = step < lo - least ? lo - step : least;
+    }
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (cut(mid)) lo = mid;
+        else hi = mid;
+    }
+    return hi;
 }
 
 // A lane's 64-bit value from another lane by DPP (zero where there is none).

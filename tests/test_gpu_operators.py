@@ -670,6 +670,21 @@ def test_sample_among_nearly_equal_logits(ctx, spread):
         check_sample(ctx, Ask(rng, rows, V, u=rng.random(rows), temp=1.0, **kw), x)
 
 
+@pytest.mark.parametrize("top", [0.0, 1e-30, -1e-40, 1e-8, 2.0 ** 26, -3.4028234663852886e38])
+def test_sample_with_min_p_at_its_end(ctx, top):
+    """min-p at and next to 1, where next to zero a great many f32 values share the largest weight, and where a step of f32 at the
+    largest value is longer than the whole range of weights."""
+    rng = np.random.default_rng(35)
+    V = 3000
+    x = np.full((4, V), np.float32(top))
+    x[:, ::3] = np.nextafter(np.float32(top), np.float32(-np.inf))
+    x[:, 1::3] = -np.inf if top < -1e38 else np.float32(top - 2 * max(1.0, abs(top)))
+    x[2:, 5] = x[2:, 8] = 0.0 if -1e-39 < top < 0 else top
+    for p in (1.0, 0.999999, 0.5):
+        for kw in (dict(), dict(top_k=40), dict(top_p=0.9)):
+            check_sample(ctx, Ask(rng, 4, V, u=rng.random(4), temp=1.0, min_p=p, **kw), x)
+
+
 def test_sample_follows_its_distribution(ctx):
     """4096 draws of one row: each token's share within five standard deviations of its weight."""
     rng = np.random.default_rng(34)
