@@ -596,16 +596,17 @@ class Context:
 
     # --- operators on the caller's device buffers --------------------------------------
     def _on(self, stream, t, out=None):
-        """The stream of a call on `t`: the one given, else torch's current one, else the context's."""
+        """The stream of a call on `t`: the one given, else torch's current one, else the context's. (0 is
+        torch's default stream where t is torch's.)"""
         if not _is_torch(t):
             return stream
         for x in (t,) if out is None else (t, out):
             if x.get_device() != self.opts.device:
                 raise ValueError(f"a tensor on {x.device}, not on the context's GPU ({self.opts.device})")
-        if stream is not None:
-            return stream
         if not _torch_first:
             raise RuntimeError("import torch before the library is loaded: they would hold two HIP runtimes")
+        if stream is not None:
+            return stream or 1
         torch = sys.modules["torch"]
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # a microsecond less than making a Stream
         of = raw(self.opts.device) if raw else torch.cuda.current_stream(self.opts.device).cuda_stream
@@ -623,11 +624,17 @@ class Context:
         return t.data_ptr(), ld if rows > 1 else max(ld, shape[1])
 
     @staticmethod
-    def _new(like, shape, dtype):
-        if _is_torch(like):
-            torch = sys.modules["torch"]
+    def _new(like, shape, dtype, given=None):
+        """An array for a call on `like`. On a stream that was given, torch allocates for that stream: its memory goes to
+        another tensor as soon as it is let go, which only the stream's own order makes safe."""
+        if not _is_torch(like):
+            return DeviceArray(shape, dtype)
+        torch = sys.modules["torch"]
+        if given is None:
             return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
-        return DeviceArray(shape, dtype)
+        s = torch.cuda.ExternalStream(given, like.device) if given > 1 else torch.cuda.default_stream(like.device)
+        with torch.cuda.stream(s):
+            return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
 
     def _same_device(self, held):
         if held.device is not None and held.device != self.opts.device:
@@ -658,7 +665,7 @@ class Context:
         before RoPE, over at most `budget` pages a row and kv head. Returns the
         rows' output (`out`, or a new array)."""
         self._same_device(cache)
-        stream = self._on(stream, q, out)
+        given, stream = stream, self._on(stream, q, out)
         a, at, n, rows = _job_rows(jobs)
         qp, ldq = self._rows(q, "q", rows, None)
         D, width = cache.c.head_dim, int(q.shape[1])
@@ -666,7 +673,7 @@ class Context:
         if heads * D != width:
             raise ValueError(f"q: rows of {width} values are not whole heads of {D}")
         if out is None:
-            out = self._new(q, (rows, width), "float32")
+            out = self._new(q, (rows, width), "float32", given)
         op, ldo = self._rows(out, "out", rows, width)
         need = cache.workspace.get((rows, heads, budget))
         if need is None:
@@ -676,7 +683,7 @@ class Context:
             if len(cache.workspace) > 1000:
                 cache.workspace.clear()
             cache.workspace[rows, heads, budget] = need
-        ws = self._new(q, (need,), "uint8")
+        ws = self._new(q, (need,), "uint8", given)
         st = self.lib.cc_attend_pages(self.h, cache.ref, at, n, heads, budget, sink, recent, qp, ldq, op, ldo,
                                       ws.data_ptr(), need, stream)
         if st:
@@ -687,11 +694,11 @@ class Context:
         """cc_logits_adjust: the rows with penalties, biases and masks, in `out`
         (logits itself, another array, or a new one)."""
         self._same_device(sampling)
-        stream = self._on(stream, logits, out)
+        given, stream = stream, self._on(stream, logits, out)
         rows, V = sampling.rows, sampling.vocab
         lp, ld = self._rows(logits, "logits", rows, V)
         if out is None:
-            out = self._new(logits, (rows, V), "float32")
+            out = self._new(logits, (rows, V), "float32", given)
         op, ldo = self._rows(out, "out", rows, V)
         st = self.lib.cc_logits_adjust(self.h, lp, ld, rows, V, sampling.ref, op, ldo, stream)
         if st:
@@ -702,14 +709,14 @@ class Context:
         """cc_sample: a token of each row of logits and the probability it was
         drawn with, int32 and f32 [rows]."""
         self._same_device(sampling)
-        stream = self._on(stream, logits)
+        given, stream = stream, self._on(stream, logits)
         rows, V = sampling.rows, sampling.vocab
         lp, ld = self._rows(logits, "logits", rows, V)
-        ids, probs = self._new(logits, (rows,), "int32"), self._new(logits, (rows,), "float32")
+        ids, probs = self._new(logits, (rows,), "int32", given), self._new(logits, (rows,), "float32", given)
         if sampling.workspace is None:
             sampling.workspace = self.lib.cc_sample_workspace(rows, V, sampling.ref)
         need = sampling.workspace
-        ws = self._new(logits, (max(need, 16),), "uint8")
+        ws = self._new(logits, (max(need, 16),), "uint8", given)
         st = self.lib.cc_sample(self.h, lp, ld, rows, V, sampling.ref, ids.data_ptr(), probs.data_ptr(), ws.data_ptr(),
                                 need, stream)
         if st:

@@ -5,6 +5,9 @@ streams, in captured graphs and on a context's own cache; and a run of them
 together."""
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -12,6 +15,7 @@ import pytest
 from chattorrent_amd import configs
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 U32 = 2.0 ** -24      # half a step of f32, relative to the value
 
 
@@ -706,6 +710,39 @@ def hip(gpu):
     h = _Hip()
     yield h
     h.free()
+
+
+TORCH_STREAMS = """
+import numpy as np, torch
+from chattorrent_amd import ccdecode as cc, configs
+ctx = cc.Context(configs.with_layers(configs.SMOLLM2, 1), n_max=256, t_max=8, slots=2)
+V = 1 << 20
+x = torch.randn(2, V, device="cuda")
+ask = cc.Sampling(2, V, temp=torch.ones(2, device="cuda"), u=torch.tensor([0.3, 0.6], dtype=torch.float64, device="cuda"))
+here = [t.clone() for t in (*ctx.sample(x, ask), ctx.adjust_logits(x, ask))]
+torch.cuda.synchronize()
+side = torch.cuda.Stream()
+for stream in (side.cuda_stream, 0):
+    got = [*ctx.sample(x, ask, stream=stream), ctx.adjust_logits(x, ask, stream=stream)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(here, got)), stream
+    at = got[2].data_ptr()
+    del got
+    again = torch.empty(2, V, device="cuda")
+    # what is let go is given on to the stream that wrote it, and to no other
+    assert (again.data_ptr() != at) == (stream != 0), stream
+    with torch.cuda.stream(side):
+        other = torch.empty(2, V, device="cuda")
+    assert (other.data_ptr() == at) == (stream != 0), stream
+    del again, other
+print("held")
+"""
+
+
+def test_torch_memory_of_a_call_belongs_to_its_stream(gpu):
+    r = subprocess.run([sys.executable, "-c", TORCH_STREAMS], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True,
+                       timeout=110)
+    assert r.returncode == 0 and r.stdout.strip().endswith("held"), r.stdout
 
 
 def test_operators_on_two_streams_at_once(ctx, hip):
