@@ -30,7 +30,7 @@ EXPORTS = [
     "cc_stats_get", "cc_op_matmul_q8", "cc_op_store_kv", "cc_op_round_f16", "cc_op_topk", "cc_op_rmsnorm",
     "cc_op_attend", "cc_profile", "cc_profile_read", "cc_read_logits", "cc_mtp_draft", "cc_topk_noalloc",
     "cc_decode_steps", "cc_cache_of", "cc_bounds_bytes", "cc_kv_append", "cc_kv_bounds", "cc_attend_workspace",
-    "cc_attend_pages", "cc_logits_adjust", "cc_sample_workspace", "cc_sample",
+    "cc_attend_pages", "cc_logits_adjust", "cc_sample_workspace", "cc_sample", "cc_sample_pass",
 ]
 
 
@@ -128,6 +128,7 @@ def load():
         "cc_logits_adjust": (i32, [P, P, i64, i32, i32, P, P, i64, P]),
         "cc_sample_workspace": (size, [i32, i32, P]),
         "cc_sample": (i32, [P, P, i64, i32, i32, P, P, P, P, size, P]),
+        "cc_sample_pass": (i32, [P, i32, P, P, P]),
         "cc_profile": (i32, [P, i32]),
         "cc_profile_read": (i32, [P, i32, C.POINTER(C.c_double), C.POINTER(C.c_int64), C.POINTER(C.c_double)]),
     }
@@ -252,6 +253,20 @@ class _Buffers:
             self.device = device
         self.kept.append(t)
         return t.data_ptr()
+
+
+class _HostArray:
+    """A wish of cc_sample_pass, in host memory and in the type that Sampling takes."""
+
+    def __init__(self, name, a):
+        kind = {"u": np.float64, "mask": np.uint32}.get(name, np.float32)
+        if name in ("top_k", "pen_at", "pen_ids", "pen_counts", "bias_at", "bias_ids", "mask_of"):
+            kind = np.int32
+        self.a = np.ascontiguousarray(a, kind)
+        self.shape, self.dtype = self.a.shape, self.a.dtype
+
+    def data_ptr(self):
+        return self.a.ctypes.data
 
 
 class KVCache(_Buffers):
@@ -593,6 +608,16 @@ class Context:
         out = np.empty_like(q)
         self._chk(self.lib.cc_op_attend(self.h, layer, slot, _p(q), q.shape[0], past, _p(out)))
         return out
+
+    def sample_pass(self, rows, **wishes):
+        """cc_sample_pass: a token of each of the last pass's `rows` sampled rows
+        and its probability, drawn on the device. The wishes are Sampling's, in
+        host memory (numpy arrays, lists)."""
+        s = Sampling(rows, self.d["vocab"], **{n: a if a is None or n == "freq_cap" else _HostArray(n, a)
+                                               for n, a in wishes.items()})
+        ids, probs = np.empty(rows, np.int32), np.empty(rows, np.float32)
+        self._chk(self.lib.cc_sample_pass(self.h, rows, s.ref, _p(ids), _p(probs)))
+        return ids, probs
 
     # --- operators on the caller's device buffers --------------------------------------
     def _on(self, stream, t, out=None):

@@ -141,6 +141,8 @@ struct cc_ctx {
     uint8_t* d_meta = nullptr;
     uint8_t* h_meta = nullptr;
     size_t meta_bytes = 0;
+    uint8_t* smp = nullptr;        // cc_sample_pass: its wishes, rows and workspace, grown to the largest call
+    size_t smp_bytes = 0;
     void* h_out = nullptr;         // results, pinned: kernels write them here
     std::vector<hipEvent_t> out_ev;   // one a piece of a large pass's rows
     size_t out_bytes = 0;
@@ -2564,6 +2566,81 @@ cc_status cc_sample(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, 
             return fail(ctx, CC_EARG, "sample: a workspace of " + std::to_string(need) + " bytes, 16-byte aligned");
         return launched(ctx, "sample", launch_sample(stream ? (hipStream_t)stream : ctx->stream, logits, ld, rows, vocab, d,
                                                      ids, probs, (uint8_t*)workspace));
+    });
+}
+
+cc_status cc_sample_pass(cc_ctx* ctx, int32_t rows, const cc_sampling* sampling, int32_t* ids, float* probs) {
+    if (!ctx) return CC_EARG;
+    if (!sampling || !ids) return fail(ctx, CC_EARG, "sample: sampling and ids must be set");
+    if (!ctx->logits || rows < 1 || rows != ctx->head_rows) return fail(ctx, CC_EARG, "rows must be the last pass's sampled rows");
+    return guarded(ctx, [&]() -> cc_status {
+        SamplingDev d;
+        const int V = ctx->d.vocab;
+        cc_status st = check_logits(ctx, ctx->logits, V, rows, V);
+        if (st == CC_OK) st = sampling_dev(ctx, sampling, V, d);
+        if (st != CC_OK) return st;
+        if (d.temp && !d.u) return fail(ctx, CC_EARG, "sample: a temperature needs random numbers (u)");
+        // the wishes behind each other, then what the call writes
+        std::vector<uint8_t> host;
+        auto put = [&](const void* p, size_t n) {
+            const size_t at = host.size();
+            if (p) host.insert(host.end(), (const uint8_t*)p, (const uint8_t*)p + n);
+            host.resize((host.size() + 15) & ~(size_t)15);
+            return at;
+        };
+        const size_t r4 = (size_t)rows * 4, pen = (size_t)d.n_pen * 4, bias = (size_t)d.n_bias * 4;
+        struct { const void** to; size_t at; } moved[16];
+        int n = 0;
+        auto move = [&](auto& p, size_t bytes) {
+            if (!p) return;
+            moved[n].at = put(p, bytes);
+            moved[n++].to = (const void**)&p;
+        };
+        move(d.temp, r4);
+        move(d.top_k, r4);
+        move(d.top_p, r4);
+        move(d.min_p, r4);
+        move(d.rep, r4);
+        move(d.freq, r4);
+        move(d.pres, r4);
+        move(d.pen_at, r4 + 4);
+        move(d.pen_ids, pen);
+        move(d.pen_counts, pen);
+        move(d.bias_at, r4 + 4);
+        move(d.bias_ids, bias);
+        move(d.bias, bias);
+        move(d.mask_of, r4);
+        move(d.mask, (size_t)d.n_masks * d.mask_words * 4);
+        move(d.u, 2 * r4);
+        auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+        const int planes = gemm_planes(ctx->d.tied ? ctx->wte : ctx->lm_head, rows, ctx->ncu);
+        const size_t out = up(host.size()), sum = out + up(2 * r4);
+        const size_t work = sum + (planes > 1 ? up((size_t)rows * V * 4) : 0);
+        const size_t need = work + sample_workspace(rows, V, sample_cuts(sampling));
+        if (need > ctx->smp_bytes) {
+            HIPCHK(dfree(ctx, ctx->smp, ctx->smp_bytes, &ctx->scratch_bytes));
+            ctx->smp = nullptr;
+            ctx->smp_bytes = 0;
+            HIPCHK(dalloc(ctx, &ctx->smp, need, &ctx->scratch_bytes));
+            ctx->smp_bytes = need;
+        }
+        if (!host.empty()) HIPCHK(hipMemcpyAsync(ctx->smp, host.data(), host.size(), hipMemcpyHostToDevice, ctx->stream));
+        for (int i = 0; i < n; i++) *moved[i].to = ctx->smp + moved[i].at;
+        const float* x = ctx->logits;
+        if (planes > 1) {   // the head's planes, added in plane order
+            launch_sum_splits(ctx->stream, ctx->logits, planes, rows, V, (float*)(ctx->smp + sum));
+            x = (const float*)(ctx->smp + sum);
+        }
+        const hipError_t e = launch_sample(ctx->stream, x, V, rows, V, d, (int32_t*)(ctx->smp + out), (float*)(ctx->smp + out + r4),
+                                           ctx->smp + work);
+        if (e != hipSuccess) {
+            (void)hipStreamSynchronize(ctx->stream);   // it may still read `host`
+            return launched(ctx, "sample", e);
+        }
+        HIPCHK(hipStreamSynchronize(ctx->stream));
+        HIPCHK(hipMemcpy(ids, ctx->smp + out, r4, hipMemcpyDeviceToHost));
+        if (probs) HIPCHK(hipMemcpy(probs, ctx->smp + out + r4, r4, hipMemcpyDeviceToHost));
+        return CC_OK;
     });
 }
 

@@ -459,6 +459,13 @@ cc_status cc_sample(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, 
                     const cc_sampling* sampling, int32_t* ids, float* probs, void* workspace, size_t workspace_bytes,
                     void* stream);
 
+/* cc_sample over the last pass's `rows` sampled rows (those cc_read_logits
+ * reads), for samplers that need whole rows: the token is drawn where the
+ * logits are, where the reference reads the rows back (web/model/stage.js:
+ * 1428-1436). `sampling` holds HOST pointers here, read during the call; ids
+ * and probs (may be NULL) are host memory, written when the call returns. */
+cc_status cc_sample_pass(cc_ctx* ctx, int32_t rows, const cc_sampling* sampling, int32_t* ids, float* probs);
+
 #ifdef __cplusplus
 }
 #endif
