@@ -2407,6 +2407,17 @@ cc_status check_logits(cc_ctx* ctx, const float* logits, int64_t ld, int32_t row
     return CC_OK;
 }
 
+// Whether rows of n floats at a, lda apart, and at b, ldb apart, share memory
+// (rows beside each other in one array do not; rows of two strides that mesh
+// are taken to).
+bool rows_meet(const float* a, int64_t lda, const float* b, int64_t ldb, int64_t rows, int64_t n) {
+    const int64_t A = (int64_t)(uintptr_t)a, B = (int64_t)(uintptr_t)b, w = n * 4;
+    if (A >= B + (rows - 1) * ldb * 4 + w || B >= A + (rows - 1) * lda * 4 + w) return false;
+    if (lda != ldb) return true;
+    const int64_t off = ((B - A) % (lda * 4) + lda * 4) % (lda * 4);
+    return off < w || off + w > lda * 4;
+}
+
 // A C entry lets no exception out.
 template <class F>
 cc_status guarded(cc_ctx* ctx, F&& f) {
@@ -2515,6 +2526,7 @@ cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* job
             return fail(ctx, CC_EARG, "attend: a row sees more pages than its budget: the cache needs bounds");
         const int64_t width = (int64_t)n_heads * c.D;
         if (ldq < width || ldo < width) return fail(ctx, CC_EARG, "attend: ldq and ldo are at least n_heads * head_dim");
+        if (rows_meet(q, ldq, out, ldo, rows, width)) return fail(ctx, CC_EARG, "attend: out must not share memory with q");
         const int64_t ws_rows = attend_rows(cache, rows, n_heads);
         const size_t need = attend_plan(ctx->ncu, cache, ws_rows, max_seen, ws_rows, cache->max_pages, n_heads, budget).bytes;
         if (!workspace || workspace_bytes < need || !is_aligned(workspace, 16))
@@ -2539,6 +2551,8 @@ cc_status cc_logits_adjust(cc_ctx* ctx, const float* logits, int64_t ld, int32_t
         if (st == CC_OK) st = sampling_dev(ctx, sampling, vocab, d);
         if (st != CC_OK) return st;
         if (ldo < vocab || (out == logits && ldo != ld)) return fail(ctx, CC_EARG, "adjust: ldo is at least vocab, and ld where out is logits");
+        if (out != logits && rows_meet(logits, ld, out, ldo, rows, vocab))
+            return fail(ctx, CC_EARG, "adjust: out is logits itself or shares no memory with it");
         return launched(ctx, "adjust", launch_logits_adjust(stream ? (hipStream_t)stream : ctx->stream, logits, ld, rows, vocab,
                                                             d, out, ldo));
     });
@@ -2631,8 +2645,10 @@ cc_status cc_sample_pass(cc_ctx* ctx, int32_t rows, const cc_sampling* sampling,
             launch_sum_splits(ctx->stream, ctx->logits, planes, rows, V, (float*)(ctx->smp + sum));
             x = (const float*)(ctx->smp + sum);
         }
-        const hipError_t e = launch_sample(ctx->stream, x, V, rows, V, d, (int32_t*)(ctx->smp + out), (float*)(ctx->smp + out + r4),
-                                           ctx->smp + work);
+        hipError_t e = take_launch_error();
+        if (e == hipSuccess)
+            e = launch_sample(ctx->stream, x, V, rows, V, d, (int32_t*)(ctx->smp + out), (float*)(ctx->smp + out + r4),
+                              ctx->smp + work);
         if (e != hipSuccess) {
             (void)hipStreamSynchronize(ctx->stream);   // it may still read `host`
             return launched(ctx, "sample", e);

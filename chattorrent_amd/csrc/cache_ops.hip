@@ -224,10 +224,9 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
 }
 
 template <int D>
-static void append_d(hipStream_t st, dim3 grid, bool vec, const CacheDev& c, const OpJobs& jobs, const float* k,
-                     int64_t ldk, const float* v, int64_t ldv, int only) {
-    if (vec) hipLaunchKernelGGL((k_kv_append<D, true>), grid, dim3(256), 0, st, c, jobs, k, ldk, v, ldv, only);
-    else hipLaunchKernelGGL((k_kv_append<D, false>), grid, dim3(256), 0, st, c, jobs, k, ldk, v, ldv, only);
+static hipError_t append_d(hipStream_t st, dim3 grid, bool vec, const CacheDev& c, const OpJobs& jobs, const float* k,
+                           int64_t ldk, const float* v, int64_t ldv, int only) {
+    return op_launch(vec ? k_kv_append<D, true> : k_kv_append<D, false>, grid, dim3(256), st, c, jobs, k, ldk, v, ldv, only);
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -236,18 +235,16 @@ hipError_t launch_kv_append(hipStream_t st, const CacheDev& c, const OpJobs& job
                             const float* v, int64_t ldv) {
     const bool vec = aligned16(k) && aligned16(v) && aligned16(c.rope) && ldk % 4 == 0 && ldv % 4 == 0 && c.rot % 16 == 0;
     const dim3 grid(jobs.units, c.nKV, 2);
-    if (c.D == 64) append_d<64>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
-    else if (c.D == 128) append_d<128>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
-    else append_d<256>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
-    return hipGetLastError();
+    if (c.D == 64) return append_d<64>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
+    if (c.D == 128) return append_d<128>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
+    return append_d<256>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
 }
 
 hipError_t launch_kv_bounds(hipStream_t st, const CacheDev& c, const OpJobs& jobs) {
     const dim3 grid(jobs.units, c.nKV, 1);
-    if (c.D == 64) append_d<64>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
-    else if (c.D == 128) append_d<128>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
-    else append_d<256>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
-    return hipGetLastError();
+    if (c.D == 64) return append_d<64>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
+    if (c.D == 128) return append_d<128>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
+    return append_d<256>(st, grid, false, c, jobs, nullptr, 0, nullptr, 0, 1);
 }
 
 // ========================================================== selected pages ===
@@ -865,18 +862,19 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
 }
 
 template <int NG>
-static void attend_ng(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& p, const float* q,
-                      int64_t ldq, float* out, int64_t ldo, uint8_t* ws) {
+static hipError_t attend_ng(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& p, const float* q,
+                            int64_t ldq, float* out, int64_t ldo, uint8_t* ws) {
     uint32_t* scores = (uint32_t*)(ws + p.scores);
     float* partials = (float*)(ws + p.partials);
     uint32_t* counters = (uint32_t*)(ws + p.counters);
     if (p.scored || p.splits > 1) {
         const int n_counters = p.splits > 1 ? jobs.rows * c.nKV * p.tiles : 0;
-        hipLaunchKernelGGL((k_page_score<NG>), dim3(op_blocks((int64_t)jobs.rows * c.nKV * p.score_blocks)), dim3(256), 0, st,
-                           c, jobs, p, q, ldq, scores, counters, n_counters);
+        const hipError_t e = op_launch(k_page_score<NG>, dim3(op_blocks((int64_t)jobs.rows * c.nKV * p.score_blocks)),
+                                       dim3(256), st, c, jobs, p, q, ldq, scores, counters, n_counters);
+        if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((k_attend_pages<NG>), dim3(op_blocks((int64_t)jobs.rows * c.nKV * p.tiles * p.splits)), dim3(256), 0, st,
-                       c, jobs, p, q, ldq, scores, partials, counters, out, ldo);
+    return op_launch(k_attend_pages<NG>, dim3(op_blocks((int64_t)jobs.rows * c.nKV * p.tiles * p.splits)), dim3(256), st, c,
+                     jobs, p, q, ldq, scores, partials, counters, out, ldo);
 }
 
 hipError_t launch_attend_pages(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& plan,
@@ -884,8 +882,7 @@ hipError_t launch_attend_pages(hipStream_t st, const CacheDev& c, const OpJobs& 
     AttendPlan p = plan;
     p.score_blocks = p.scored ? (p.max_seen - p.recent + SCORE_PAGES - 1) / SCORE_PAGES : 1;
     p.vec = aligned16(q) && aligned16(c.rope) && ldq % 4 == 0 && c.rot % 16 == 0;
-    if (c.ng == 2) attend_ng<2>(st, c, jobs, p, q, ldq, out, ldo, ws);
-    else if (c.ng == 4) attend_ng<4>(st, c, jobs, p, q, ldq, out, ldo, ws);
-    else attend_ng<8>(st, c, jobs, p, q, ldq, out, ldo, ws);
-    return hipGetLastError();
+    if (c.ng == 2) return attend_ng<2>(st, c, jobs, p, q, ldq, out, ldo, ws);
+    if (c.ng == 4) return attend_ng<4>(st, c, jobs, p, q, ldq, out, ldo, ws);
+    return attend_ng<8>(st, c, jobs, p, q, ldq, out, ldo, ws);
 }

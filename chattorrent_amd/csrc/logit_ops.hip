@@ -166,20 +166,19 @@ static bool vec_rows(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 
 static bool has_lists(const SamplingDev& s) { return s.pen_at || s.bias_at; }
 // f with (VEC, LISTS) as types.
 template <class F>
-static void with_forms(bool vec, bool lists, F&& f) {
-    if (vec && lists) f(std::true_type{}, std::true_type{});
-    else if (vec) f(std::true_type{}, std::false_type{});
-    else if (lists) f(std::false_type{}, std::true_type{});
-    else f(std::false_type{}, std::false_type{});
+static hipError_t with_forms(bool vec, bool lists, F&& f) {
+    if (vec && lists) return f(std::true_type{}, std::true_type{});
+    if (vec) return f(std::true_type{}, std::false_type{});
+    if (lists) return f(std::false_type{}, std::true_type{});
+    return f(std::false_type{}, std::false_type{});
 }
 
 hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int rows, int V, const SamplingDev& s,
                                 float* out, int64_t ldo) {
     const dim3 grid((V + LG_CH - 1) / LG_CH, rows);
-    with_forms(vec_rows(x, ldx) && vec_rows(out, ldo), has_lists(s), [&](auto vec, auto lists) {
-        hipLaunchKernelGGL((k_logits_adjust<vec.value, lists.value>), grid, dim3(LG_T), 0, st, x, ldx, V, s, out, ldo);
+    return with_forms(vec_rows(x, ldx) && vec_rows(out, ldo), has_lists(s), [&](auto vec, auto lists) {
+        return op_launch(k_logits_adjust<vec.value, lists.value>, grid, dim3(LG_T), st, x, ldx, V, s, out, ldo);
     });
-    return hipGetLastError();
 }
 
 // ================================================================= sample ===
@@ -1081,18 +1080,14 @@ hipError_t launch_sample(hipStream_t st, const float* x, int64_t ldx, int rows, 
     const bool cuts = has_cuts(s);
     sample_layout(rows, V, cuts, ws, w);
     const dim3 chunks(w.chunks, rows);
-    with_forms(vec_rows(x, ldx), has_lists(s), [&](auto vec, auto lists) {
+    return with_forms(vec_rows(x, ldx), has_lists(s), [&](auto vec, auto lists) {
         constexpr bool VEC = vec.value, LISTS = lists.value;
-        if (cuts) {
-            hipLaunchKernelGGL((k_sample_scale<VEC, LISTS>), chunks, dim3(LG_T), 0, st, x, ldx, V, s, w);
-        } else {
-            hipLaunchKernelGGL((k_sample_weights<VEC, LISTS>), chunks, dim3(LG_T), 0, st, x, ldx, V, s, w);
-            hipLaunchKernelGGL((k_sample_pick<VEC, LISTS>), dim3(rows), dim3(LG_T), 0, st, x, ldx, V, s, w, ids, probs);
-        }
+        hipError_t e = op_launch(cuts ? k_sample_scale<VEC, LISTS> : k_sample_weights<VEC, LISTS>, chunks, dim3(LG_T), st, x, ldx,
+                                 V, s, w);
+        if (e != hipSuccess) return e;
+        if (!cuts) return op_launch(k_sample_pick<VEC, LISTS>, dim3(rows), dim3(LG_T), st, x, ldx, V, s, w, ids, probs);
+        e = op_launch(k_sample_mass, chunks, dim3(LG_T), st, V, s, w, ids, probs);
+        if (e != hipSuccess || !(s.top_k || s.top_p)) return e;
+        return op_launch(k_sample_cut, chunks, dim3(LG_T), st, V, s, w, ids, probs);
     });
-    if (cuts) {
-        hipLaunchKernelGGL(k_sample_mass, chunks, dim3(LG_T), 0, st, V, s, w, ids, probs);
-        if (s.top_k || s.top_p) hipLaunchKernelGGL(k_sample_cut, chunks, dim3(LG_T), 0, st, V, s, w, ids, probs);
-    }
-    return hipGetLastError();
 }

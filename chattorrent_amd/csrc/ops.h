@@ -6,6 +6,25 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <tuple>
+#include <type_traits>
+
+// Launches `k` and returns this launch's own error. (hipGetLastError would
+// also tell of one that an earlier call of the caller's left behind, for work
+// that has been queued well.)
+template <class... P, class... A>
+hipError_t op_launch(void (*k)(P...), dim3 grid, dim3 block, hipStream_t st, A&&... a) {
+    std::tuple<std::decay_t<P>...> args(static_cast<A&&>(a)...);
+    const hipError_t e = std::apply(
+        [&](auto&... x) {
+            void* at[] = {(void*)&x...};
+            return hipLaunchKernel((const void*)k, grid, block, at, 0, st);
+        },
+        args);
+    if (e != hipSuccess) (void)hipGetLastError();   // told by the return value
+    return e;
+}
+
 // ------------------------------------------------------------ paged cache ---
 // A paged int8 cache (cc_cache): blk bytes per (page, kv head) block, bblk
 // bytes of key bounds per page (all kv heads).

@@ -373,7 +373,7 @@ cc_status cc_kv_bounds(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, 
 /* Attention of the jobs' rows over selected pages. Row i of a job is at
  * position past + i and sees the tokens up to its own (stored before). q f32
  * [rows][n_heads * D] before RoPE, ldq floats from row to row; out alike, with
- * ldo. Query head h reads kv head h / (n_heads / n_kv_heads).
+ * ldo, in memory of its own. Query head h reads kv head h / (n_heads / n_kv_heads).
  * A row sees P = (past + i)/64 + 1 pages. Up to `budget` it reads them all.
  * Else each kv head of it reads `budget` of them: the first `sink`, the last
  * `recent`, and the best of the others by score, ties to the lower page. With
@@ -439,7 +439,8 @@ typedef struct cc_sampling {
  * freq_cap), where c > 0; plus its bias; -inf where the mask bars it (whatever
  * the logit, NaN too). In f64 steps, rounded to f32 once; untouched logits keep
  * their bits. logits f32 [rows][vocab], ld floats from row to row; out alike
- * with ldo, and may be logits itself (same ld). vocab at most 2^20. */
+ * with ldo, and may be logits itself (same ld), or else shares no memory with
+ * it. vocab at most 2^20. */
 cc_status cc_logits_adjust(cc_ctx* ctx, const float* logits, int64_t ld, int32_t rows, int32_t vocab,
                            const cc_sampling* sampling, float* out, int64_t ldo, void* stream);
 /* Draws a token of each row of logits, which stay as they are. Of the adjusted
