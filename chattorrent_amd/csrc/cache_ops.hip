@@ -577,6 +577,18 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     const int n = e1 - e0, w0 = (n * wave) / ATTEND_WAVES, w1 = (n * (wave + 1)) / ATTEND_WAVES, nw = w1 - w0;
     const int lp = lane < nw ? (int)list[w0 + lane] : 0;
     const uint32_t pgv = lane < nw ? ids[w0 + lane] : 0u;
+    // the lane's head (none past the tile's: zero) as an f16 pair, with its largest value brought to 2^3 .. 2^4 by a power
+    // of two, so that f16 holds it whatever the query's magnitude; the scores take the power back
+    float qmax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * NG; i += 4) {
+        const float4 f = *(const float4*)&smem[l16 * D + 32 * (i >> 3) + 8 * j4 + (i & 4)];
+        qmax = fmaxf(qmax, fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))));
+    }
+    qmax = fmaxf(qmax, __shfl_xor(qmax, 16));
+    qmax = fmaxf(qmax, __shfl_xor(qmax, 32));
+    const int eq = max((int)(f2u(qmax) >> 23) - 127, -120) - 3;
+    const float qdown = u2f((uint32_t)(127 - eq) << 23);
     half8_t qh[NG], ql[NG];
 #pragma unroll
     for (int g = 0; g < NG; g++)
@@ -587,7 +599,7 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 _Float16 hi, lo;
-                split_hilo(l16 < gt ? x[i] : 0.0f, hi, lo);
+                split_hilo(l16 < gt ? x[i] * qdown : 0.0f, hi, lo);
                 qh[g][e + i] = hi;
                 ql[g][e + i] = lo;
             }
@@ -595,7 +607,7 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     __syncthreads();   // every wave has its query: the space is free
     float* ksl = smem + wave * OW;
     float* vsl = ksl + 256 * SCL;
-    const float score_scale = 1.4426950408889634f / sqrtf((float)D);
+    const float score_scale = 1.4426950408889634f / sqrtf((float)D) * u2f((uint32_t)(127 + eq) << 23);
     const size_t pstride = (size_t)c.nKV * c.blk, hoff = (size_t)kvh * c.blk;
     auto page_rsrc = [&](const uint8_t* pool, int i) {
         const uint32_t pg = __builtin_amdgcn_readlane(pgv, i);
@@ -801,8 +813,8 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
             y = __builtin_fmaf(xy.y, f, y);
         }
         if (splits == 1) {
-            dst[(size_t)h * D + d] = l > 0.0f ? x / l : 0.0f;
-            dst[(size_t)h * D + d + 1] = l > 0.0f ? y / l : 0.0f;
+            dst[(size_t)h * D + d] = l != 0.0f ? x / l : 0.0f;
+            dst[(size_t)h * D + d + 1] = l != 0.0f ? y / l : 0.0f;
         } else {
             leave64(mine + (size_t)h * D + d, (unsigned long long)f2u(y) << 32 | f2u(x));
             if (d == 0) leave64(mine + (size_t)gw * D + 2 * h, (unsigned long long)f2u(l) << 32 | f2u(m));
@@ -856,8 +868,8 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
             }
         }
         const float l = total[h];
-        dst[(size_t)h * D + d] = l > 0.0f ? x / l : 0.0f;
-        dst[(size_t)h * D + d + 1] = l > 0.0f ? y / l : 0.0f;
+        dst[(size_t)h * D + d] = l != 0.0f ? x / l : 0.0f;
+        dst[(size_t)h * D + d + 1] = l != 0.0f ? y / l : 0.0f;
     }
 }
 

@@ -444,6 +444,111 @@ def test_attend_extreme_scores_and_values(ctx):
     assert not ctx.attend_pages(cache, [(0, 249, 1)], dev(q), 8).numpy().any()
 
 
+def of_random_pages(rng, nkv, D, pages, kinds=None):
+    """A chat of whole pages of random codes and scales; kinds: only that many different pages of keys."""
+    ref = Plain(rng, nkv, D, D, pages, 1, pages)
+    for pool in (ref.k, ref.v):
+        pool[..., :64 * D] = rng.integers(1, 256, pool[..., :64 * D].shape)
+        pool.view(np.float32)[..., 16 * D:] = np.abs(rng.standard_normal((pages, nkv, 2 * D))) * 0.01 + 0.002
+    at = np.arange(pages)
+    if kinds:
+        at = ref.table[0, np.arange(pages) % kinds]
+        ref.k[ref.table[0]] = ref.k[at]
+    for i in range(pages):
+        if kinds and i >= kinds:
+            ref.bounds[ref.table[0, i]] = ref.bounds[at[i]]
+        else:
+            ref.make_bounds(ref.table[0, i])
+    return ref
+
+
+@pytest.mark.parametrize("pages,budget,sink,recent,kinds,nkv,D", [
+    (259, 20, 1, 2, None, 2, 64), (260, 20, 1, 2, None, 1, 128),      # 256 and 257 pages to choose from
+    (1027, 64, 1, 2, None, 1, 64), (1028, 64, 1, 2, 5, 1, 64),        # 1024, and 1025 of which many score the same
+    (700, 650, 1, 2, None, 1, 64), (2600, 900, 3, 5, None, 1, 64),    # long lists, over many workgroups
+    (400, 40, 39, 1, None, 1, 64), (300, 30, 0, 1, 2, 1, 64)])
+def test_attend_over_many_pages(ctx, pages, budget, sink, recent, kinds, nkv, D):
+    rng = np.random.default_rng(pages)
+    ref = of_random_pages(rng, nkv, D, pages, kinds)
+    cache = ref.device()
+    jobs = [(0, 64 * pages - 30, 2), (0, 64 * (pages // 2), 1)]
+    q = rng.standard_normal((3, 3 * nkv * D)).astype(np.float32)
+    want, vmax, smax = ref.attend(jobs, q, 3 * nkv, budget, sink, recent)
+    got = ctx.attend_pages(cache, jobs, dev(q), budget, sink=sink, recent=recent).numpy()
+    # beside attend_bound: a lane adds 16 weights a page of up to 64 pages one after another, and as many products
+    off, bound = np.abs(got - want).max(1), attend_bound(D, vmax, smax) + 2 * vmax * 16 * 64 * U32
+    assert (off <= bound).all(), (off, bound)
+
+
+@pytest.mark.parametrize("D,size", [(64, 1e6), (64, 1e-9), (128, 3e30), (256, 1e-30), (128, 65504.0)])
+def test_attend_queries_of_any_magnitude(ctx, D, size):
+    """Queries past f16's range and below it, against keys whose scales bring the scores back to order 1."""
+    rng = np.random.default_rng(25)
+    ref = of_random_pages(rng, 1, D, 9)
+    ref.k.view(np.float32)[..., 16 * D:] /= np.float32(size)
+    cache = ref.device()
+    q = (rng.standard_normal((2, 4 * D)) * size).astype(np.float32)
+    jobs = [(0, 500, 2)]
+    want, vmax, smax = ref.attend(jobs, q, 4, 9, 0, 1)
+    assert 0.1 < smax.min() and smax.max() < 1e3
+    got = ctx.attend_pages(cache, jobs, dev(q), 9).numpy()
+    assert (np.abs(got - want).max(1) <= attend_bound(D, vmax, smax)).all()
+
+
+def test_attend_queries_that_are_no_numbers(ctx):
+    """A head whose query holds NaN or infinity gives NaN; the other heads and rows what they give without it."""
+    rng = np.random.default_rng(26)
+    ref = of_random_pages(rng, 2, 64, 40)
+    cache = ref.device()
+    q = rng.standard_normal((3, 4 * 64)).astype(np.float32)
+    jobs = [(0, 2400, 3)]
+    for budget in (40, 8):
+        clean = ctx.attend_pages(cache, jobs, dev(q), budget).numpy().reshape(3, 4, 64)
+        bad = q.reshape(3, 4, 64).copy()
+        bad[0, 2:, 7] = np.nan
+        bad[2, :2, 30] = np.inf
+        got = ctx.attend_pages(cache, jobs, dev(bad.reshape(3, -1)), budget).numpy().reshape(3, 4, 64)
+        assert np.isnan(got[0, 2:]).all() and np.isnan(got[2, :2]).all()
+        for rows in (np.s_[0, :2], np.s_[1], np.s_[2, 2:]):
+            assert same_bits(got[rows], clean[rows])
+
+
+def test_attend_more_rows_than_a_launch_takes(ctx):
+    """8300 rows of one job: each row's bits are those of calls of fewer."""
+    rng = np.random.default_rng(27)
+    ref = of_random_pages(rng, 1, 64, 130)
+    cache = ref.device()
+    q = rng.standard_normal((8300, 64)).astype(np.float32)
+    whole = ctx.attend_pages(cache, [(0, 17, 8300)], dev(q), 4).numpy()
+    for i in range(0, 8300, 1660):
+        part = ctx.attend_pages(cache, [(0, 17 + i, 1660)], dev(q[i:i + 1660]), 4).numpy()
+        assert same_bits(whole[i:i + 1660], part), i
+
+
+def test_a_cache_of_more_than_4_gib(ctx):
+    """Pages whose bytes lie past 2^31 and 2^32: appended to, scored and read as those of a small cache."""
+    from chattorrent_amd.ccdecode import DeviceArray, KVCache
+    rng = np.random.default_rng(28)
+    nkv, D, n = 8, 256, 30000
+    small = Plain(rng, nkv, D, D, 6, 1, 6)
+    small.table[0] = np.arange(6)
+    near = small.device()
+    block = 64 * D + 8 * D
+    assert 14563 * nkv * block < 2 ** 31 < 14650 * nkv * block < 29127 * nkv * block < 2 ** 32 < 29250 * nkv * block
+    pools = [DeviceArray((n, nkv, block), "uint8") for _ in range(2)]
+    far_table = np.array([[29999, 3, 14800, 29400, 14650, 29250]], np.int32)
+    far = KVCache(pools[0], pools[1], dev(far_table), small.d[3], D,
+                  bounds=DeviceArray((n, nkv * (2 * D + D // 8)), "uint8"))
+    k, v = (dev(rng.standard_normal((380, nkv * D)).astype(np.float32)) for _ in range(2))
+    q = dev(rng.standard_normal((2, 2 * nkv * D)).astype(np.float32))
+    for budget in (6, 3):
+        got = []
+        for cache in (near, far):
+            ctx.kv_append(cache, [(0, 0, 380)], k, v)
+            got.append(ctx.attend_pages(cache, [(0, 378, 2)], q, budget).numpy())
+        assert same_bits(*got)
+
+
 def test_attend_twice_gives_the_same_bits(ctx):
     """Split workgroups are joined in split order, whichever ends last."""
     rng = np.random.default_rng(24)
@@ -687,6 +792,22 @@ def test_sample_with_min_p_at_its_end(ctx, top):
     for p in (1.0, 0.999999, 0.5):
         for kw in (dict(), dict(top_k=40), dict(top_p=0.9)):
             check_sample(ctx, Ask(rng, 4, V, u=rng.random(4), temp=1.0, min_p=p, **kw), x)
+
+
+def test_the_largest_vocabulary_and_long_lists(ctx):
+    """2^20 logits a row, odd ones beside; more than 2^16 entries in a row's lists, many of one token."""
+    rng = np.random.default_rng(36)
+    V = 1 << 20
+    x = (rng.standard_normal((2, V)) * 2).astype(np.float32)
+    for kw in (dict(), dict(temp=1.0), dict(temp=0.8, top_k=1000, top_p=0.95)):
+        check_sample(ctx, Ask(rng, 2, V, u=rng.random(2), history=70000, rep=1.1, freq=0.01, pres=0.3, biases=100, masks=1, **kw), x)
+    V = 9001
+    x = (rng.standard_normal((2, V)) * 2).astype(np.float32)
+    for kw in (dict(history=70000, rep=1.1, freq=0.01, biases=70000), dict(history=70000, counts=True, freq=0.01, biases=9)):
+        ask = Ask(rng, 2, V, **kw)
+        got = ctx.adjust_logits(dev(x), ask.device()).numpy()
+        with np.errstate(over="ignore", invalid="ignore"):
+            assert np.array_equal(got, ask.adjust(x).astype(np.float32), equal_nan=True)
 
 
 def test_sample_follows_its_distribution(ctx):
