@@ -219,6 +219,8 @@ constexpr float SM_REACH = 32.0f;            // the histogram's last bin takes e
 constexpr double SM_ONE = 4398046511104.0;   // 2^42: a row of 2^20 tokens sums to at most 2^62
 typedef unsigned long long u64;
 
+// 1 / temp, never 0: a barred token's -inf stays so at an infinite temperature.
+__device__ static inline double inverse(double temp) { return temp > 0.0 ? fmax(1.0 / temp, 1e-300) : 1.0; }
 // s of an adjusted logit. inv = 1/temp; only above 1 can a finite value leave
 // the range (a branch on it is uniform).
 __device__ static inline float scaled_logit(float a, double inv) {
@@ -395,12 +397,13 @@ struct RowAsk {
     __device__ RowAsk(const SamplingDev& s, int row, int V) {
         const double temp = s.temp ? (double)s.temp[row] : 0.0;
         greedy = !(temp > 0.0);
-        inv = greedy ? 1.0 : 1.0 / temp;
+        inv = inverse(temp);
         k = s.top_k ? s.top_k[row] : 0;
         if (k >= V || k < 0) k = 0;
         top_p = s.top_p ? (double)s.top_p[row] : 1.0;
         if (!(top_p < 1.0)) top_p = 1.0;
-        min_p = s.min_p ? fmin((double)s.min_p[row], 1.0) : 0.0;   // the maximum itself stays
+        min_p = s.min_p ? (double)s.min_p[row] : 0.0;
+        if (min_p > 1.0) min_p = 1.0;   // the maximum itself stays
         cut = !greedy && (k > 0 || top_p < 1.0);
     }
 };
@@ -479,7 +482,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict
     __shared__ u64 red[4];
     const int row = blockIdx.y, c = blockIdx.x;
     exp_table(T);
-    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
+    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = inverse(temp);
     float a[LG_J][4];
     adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, lds, a);
     FirstMax first;
@@ -514,7 +517,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
     __shared__ float s_m;
     const int row = blockIdx.x, tid = threadIdx.x;
     exp_table(T);
-    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
+    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = inverse(temp);
     const u64 mine = tid < w.chunks ? w.best[(size_t)row * w.chunks + tid] : 0;
     const u64 local = tid < w.chunks ? w.mass[(size_t)row * w.chunks + tid] : 0;
     const u64 key = block_max64(mine, red);
@@ -563,7 +566,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
     const int row = blockIdx.y, c = blockIdx.x;
     if (c == 0 && threadIdx.x < sizeof(SampleInfo) / 4) ((uint32_t*)(w.info + row))[threadIdx.x] = 0;
     const RowPens r = row_pens(s, row);
-    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = temp > 0.0 ? 1.0 / temp : 1.0;
+    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = inverse(temp);
     FirstMax first;
     float least = INFINITY, a[LG_J][4];
     adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, r, c * LG_CH, lds, a);

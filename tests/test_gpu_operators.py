@@ -794,6 +794,25 @@ def test_sample_with_min_p_at_its_end(ctx, top):
             check_sample(ctx, Ask(rng, 4, V, u=rng.random(4), temp=1.0, min_p=p, **kw), x)
 
 
+def test_sample_at_infinite_temperature_and_parameters_that_are_no_numbers(ctx):
+    """All allowed tokens alike at temperature infinity, barred ones never; a top-p or min-p of NaN cuts nothing, a temperature
+    of NaN is greedy."""
+    rng = np.random.default_rng(37)
+    V = 9000
+    x = (rng.standard_normal((6, V)) * 3).astype(np.float32)
+    x[:, ::2] = -np.inf
+    u = rng.random(6)
+    for kw in (dict(), dict(top_k=5), dict(top_p=0.5), dict(min_p=0.5)):
+        for temp in (np.inf, np.finfo(np.float32).max):
+            ids = check_sample(ctx, Ask(rng, 6, V, u=u, temp=temp, masks=1, **kw), x)
+            assert (ids % 2 == 1).all()
+    plain = ctx.sample(dev(x), Ask(rng, 6, V, u=u, temp=1.0).device())
+    for kw in (dict(top_p=np.nan), dict(min_p=np.nan), dict(top_p=np.nan, min_p=np.nan, top_k=-5)):
+        got = ctx.sample(dev(x), Ask(rng, 6, V, u=u, temp=1.0, **kw).device())
+        assert np.array_equal(got[0].numpy(), plain[0].numpy())
+    assert np.array_equal(ctx.sample(dev(x), Ask(rng, 6, V, u=u, temp=np.nan, top_k=5).device())[0].numpy(), x.argmax(1))
+
+
 def test_the_largest_vocabulary_and_long_lists(ctx):
     """2^20 logits a row, odd ones beside; more than 2^16 entries in a row's lists, many of one token."""
     rng = np.random.default_rng(36)
