@@ -376,6 +376,7 @@ struct SampleInfo {
     u64 want;              // top-p without top-k: the weight to reach
     uint32_t floor, fixed; // min-p as a value's ordered bits; whether it is the cut
     uint32_t done[2];
+    float m, bins;         // RowDraw's (bins 0: no cut to find)
 };
 struct SampleWs {
     u64* best;        // [rows][chunks] ordered(a) << 32 | ~token; 0: nothing above -inf
@@ -778,6 +779,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
         info->above = (uint32_t)above;
         info->mass_above = mass_above;
         info->want = want;
+        info->m = d.m;
+        info->bins = d.bins;
     }
 }
 
@@ -814,7 +817,12 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t kmin, uint32_t kma
             u64 before = wave_scan64(sum) - sum;
             if (before < left && left <= before + sum) {
                 int e = 0;
-                while (before + v[e] < left) before += v[e++];
+#pragma unroll
+                for (int q = 0; q < 3; q++)   // no index at run time: the array stays in registers
+                    if (e == q && before + v[q] < left) {
+                        before += v[q];
+                        e = q + 1;
+                    }
                 sel[0] = prefix | ((uint32_t)(255 - 4 * lane - e) << sh);
                 sel[1] = left - before;
             }
@@ -828,10 +836,10 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t kmin, uint32_t kma
 
 __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, SampleWs w, int32_t* __restrict__ ids,
                                                      float* __restrict__ probs) {
-    __shared__ uint32_t keys[SM_CAND];
+    __shared__ __align__(16) uint32_t keys[SM_CAND];
     __shared__ uint8_t group[SM_CAND];   // the chunk that a value came from
-    __shared__ u64 gmass[LG_T], hist[256], red[4], found[2], wts[SM_SMALL], runs[LG_J][4];
-    __shared__ uint32_t tok[SM_SMALL];
+    __shared__ __align__(16) u64 wts[SM_SMALL], gmass[LG_T], hist[256], red[4], found[2], runs[LG_J][4];
+    __shared__ __align__(16) uint32_t tok[SM_SMALL];
     __shared__ uint32_t s_last, s_n, s_at;
     __shared__ double T[32];
     static_assert(SM_CHUNKS <= LG_T, "a thread a workgroup of the row");
@@ -841,11 +849,11 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     if (!ask.cut) return;
     const float* sr = w.s + row * w.lds;
     float v[LG_J][4];
-    scaled_runs(sr, V, g * LG_CH, v);   // in flight while the row's maximum is found
+    scaled_runs(sr, V, g * LG_CH, v);
     exp_table(T);
-    const RowDraw d = row_draw(w, row, ask, red);
-    if (d.key == 0) return;
     SampleInfo* info = w.info + row;
+    const RowDraw d{info->m, info->bins, 0};
+    if (d.bins == 0.0f) return;
     const int lo = info->lo, hi = info->hi;
     uint2* cand = w.cand + (size_t)row * SM_CAND;
     const uint32_t floor = info->floor;
@@ -908,10 +916,12 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
         __syncthreads();
         if (ask.k > 0) {
             uint32_t larger[2] = {0, 0};
-            for (uint32_t i = 0; i < n; i++) {
-                larger[0] += keys[i] > kv[0];
-                larger[1] += keys[i] > kv[1];
-            }
+            for (uint32_t i = 0; i < n; i += 8)   // past n: zeros
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    larger[0] += keys[i + e] > kv[0];
+                    larger[1] += keys[i + e] > kv[1];
+                }
             in[0] = in[0] && larger[0] < (uint32_t)ask.k;
             in[1] = in[1] && larger[1] < (uint32_t)ask.k;
         }
@@ -925,12 +935,14 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                 want = (u64)fmax(ceil(ask.top_p * (double)block_sum64((in[0] ? mv[0] : 0) + (in[1] ? mv[1] : 0), red)), 1.0);
             __syncthreads();
             u64 over[2] = {0, 0};
-            for (uint32_t i = 0; i < n; i++) {
-                const u64 x = wts[i];
-                const uint32_t kk = keys[i];
-                over[0] += kk > kv[0] ? x : 0;
-                over[1] += kk > kv[1] ? x : 0;
-            }
+            for (uint32_t i = 0; i < n; i += 8)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const u64 x = wts[i + e];
+                    const uint32_t kk = keys[i + e];
+                    over[0] += kk > kv[0] ? x : 0;
+                    over[1] += kk > kv[1] ? x : 0;
+                }
             in[0] = in[0] && over[0] < want;
             in[1] = in[1] && over[1] < want;
         }
@@ -945,12 +957,14 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
         const u64 target = target_of(s.u ? s.u[row] : 0.0, total);
         u64 before[2] = {0, 0};
         const uint32_t t0 = tok[tid], t1 = tok[tid + LG_T];
-        for (uint32_t i = 0; i < n; i++) {
-            const u64 x = wts[i];
-            const uint32_t tt = tok[i];
-            before[0] += tt < t0 ? x : 0;
-            before[1] += tt < t1 ? x : 0;
-        }
+        for (uint32_t i = 0; i < n; i += 8)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const u64 x = wts[i + e];
+                const uint32_t tt = tok[i + e];
+                before[0] += tt < t0 ? x : 0;
+                before[1] += tt < t1 ? x : 0;
+            }
 #pragma unroll
         for (int q = 0; q < 2; q++)
             if (before[q] <= target && target < before[q] + mv[q]) {
