@@ -784,7 +784,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
 }
 
 // The value (as ordered bits) at which the sum over the values from the top
-// first reaches `want`, 8 bits at a time below the bits that all keys (in
+// first reaches `want`, 9 bits at a time below the bits that all keys (in
 // [kmin, kmax]) share: `each` calls its argument for every value with its key
 // and what it adds. kmin (everything is kept) if they all sum to less.
 template <class E>
@@ -793,9 +793,10 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t kmin, uint32_t kma
     uint32_t prefix = 0;   // of key - kmin
     u64 left = want;
     const int bits = kmax > kmin ? 32 - __clz(kmax - kmin) : 0;
-    for (int sh = ((bits + 7) >> 3 << 3) - 8; sh >= 0; sh -= 8) {
+    for (int sh = (bits + 8) / 9 * 9 - 9; sh >= 0; sh -= 9) {
         __syncthreads();
         hist[tid] = 0;
+        hist[LG_T + tid] = 0;
         if (tid == 0) {
             sel[0] = prefix;
             sel[1] = left;
@@ -803,26 +804,26 @@ __device__ static inline uint32_t find_cut(u64 want, uint32_t kmin, uint32_t kma
         __syncthreads();
         each([&](uint32_t key, u64 adds) {
             const uint32_t k = key - kmin;
-            if (sh == 24 || (k >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(k >> sh) & 255u], adds);
+            if (sh == 27 || (k >> (sh + 9)) == (prefix >> (sh + 9))) atomicAdd(&hist[(k >> sh) & 511u], adds);
         });
         __syncthreads();
-        if (tid < 64) {   // lane l: digits 255 - 4l .. 252 - 4l
-            u64 v[4], sum = 0;
+        if (tid < 64) {   // lane l: digits 511 - 8l .. 504 - 8l
+            u64 v[8], sum = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[e] = hist[255 - 4 * lane - e];
+            for (int e = 0; e < 8; e++) {
+                v[e] = hist[511 - 8 * lane - e];
                 sum += v[e];
             }
             u64 before = wave_scan64(sum) - sum;
             if (before < left && left <= before + sum) {
                 int e = 0;
 #pragma unroll
-                for (int q = 0; q < 3; q++)   // no index at run time: the array stays in registers
+                for (int q = 0; q < 7; q++)   // no index at run time: the array stays in registers
                     if (e == q && before + v[q] < left) {
                         before += v[q];
                         e = q + 1;
                     }
-                sel[0] = prefix | ((uint32_t)(255 - 4 * lane - e) << sh);
+                sel[0] = prefix | ((uint32_t)(511 - 8 * lane - e) << sh);
                 sel[1] = left - before;
             }
         }
@@ -837,7 +838,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
                                                      float* __restrict__ probs) {
     __shared__ __align__(16) uint32_t keys[SM_CAND];
     __shared__ uint8_t group[SM_CAND];   // the chunk that a value came from
-    __shared__ __align__(16) u64 wts[SM_SMALL], gmass[LG_T], hist[256], red[4], found[2], runs[LG_J][4];
+    __shared__ __align__(16) u64 wts[SM_SMALL], gmass[LG_T], hist[2 * LG_T], red[4], found[2], runs[LG_J][4];
     __shared__ __align__(16) uint32_t tok[SM_SMALL];
     __shared__ uint32_t s_last, s_n, s_at;
     __shared__ double T[32];
