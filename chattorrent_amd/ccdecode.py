@@ -656,10 +656,12 @@ class Context:
             return DeviceArray(shape, dtype)
         torch = sys.modules["torch"]
         if given is None:
-            return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
+            if dtype == "float32" and shape == like.shape:   # half of torch.empty's 2 us; rows stay whole rows
+                return torch.empty_like(like, memory_format=torch.contiguous_format)
+            return like.new_empty(shape, dtype=getattr(torch, dtype))
         s = torch.cuda.ExternalStream(given, like.device) if given > 1 else torch.cuda.default_stream(like.device)
         with torch.cuda.stream(s):
-            return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
+            return like.new_empty(shape, dtype=getattr(torch, dtype))
 
     def _same_device(self, held):
         if held.device is not None and held.device != self.opts.device:
@@ -699,7 +701,9 @@ class Context:
             raise ValueError(f"q: rows of {width} values are not whole heads of {D}")
         if out is None:
             out = self._new(q, (rows, width), "float32", given)
-        op, ldo = self._rows(out, "out", rows, width)
+            op, ldo = out.data_ptr(), width
+        else:
+            op, ldo = self._rows(out, "out", rows, width)
         need = cache.workspace.get((rows, heads, budget))
         if need is None:
             need = self.lib.cc_attend_workspace(self.h, cache.ref, rows, heads, budget) if rows else 0
@@ -724,7 +728,9 @@ class Context:
         lp, ld = self._rows(logits, "logits", rows, V)
         if out is None:
             out = self._new(logits, (rows, V), "float32", given)
-        op, ldo = self._rows(out, "out", rows, V)
+            op, ldo = out.data_ptr(), V
+        else:
+            op, ldo = self._rows(out, "out", rows, V)
         st = self.lib.cc_logits_adjust(self.h, lp, ld, rows, V, sampling.ref, op, ldo, stream)
         if st:
             self._chk(st)

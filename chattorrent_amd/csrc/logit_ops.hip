@@ -203,8 +203,8 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 //   k_sample_scale    writes s to the workspace, with every chunk's largest and
 //                     smallest value: lists, masks and the division once;
 //   k_sample_mass     with the row's m known, a histogram of m - s in SM_BINS
-//                     bins (counts for top-k, weights for top-p) of every
-//                     chunk; the row's last workgroup to finish adds them and
+//                     bins (counts for top-k, weights for top-p), by chunk
+//                     and of the row; the row's last workgroup to finish
 //                     finds the bins that the cuts fall into. (A row
 //                     without a cut: the weights, and the last one draws.)
 //   k_sample_cut      the values of those bins are gathered; the row's last
@@ -365,9 +365,9 @@ __device__ static inline u64 block_max64(u64 v, u64* red) {
 }
 
 // The workspace of a call: per row and chunk the largest key and the weight;
-// with cuts also the smallest value and the histogram, and per row the scaled
-// logits, what the cuts found, two counters of finished workgroups and the
-// gathered values.
+// with cuts also the smallest value and the weights' histogram, and per row the
+// histograms, the scaled logits, what the cuts found, two counters of finished
+// workgroups and the gathered values.
 struct SampleInfo {
     int32_t lo, hi;        // the bins whose values are gathered
     uint32_t above;        // values in the bins before lo
