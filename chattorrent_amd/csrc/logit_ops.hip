@@ -864,6 +864,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
     uint2* cand = w.cand + (size_t)row * SM_CAND;
     const uint32_t floor = info->floor;
     const bool from_hist = ask.top_p < 1.0;   // the weights of the bins before lo, all above min-p's, are in the histogram
+    if (tid == 0) s_n = 0;
+    __syncthreads();   // T is there for every wave, and s_n
     u64 sum = 0;
     if (from_hist) {
         const u64* h = w.hmass + ((size_t)row * w.chunks + g) * SM_BINS;
@@ -880,8 +882,6 @@ __global__ __launch_bounds__(LG_T) void k_sample_cut(int V, SamplingDev s, Sampl
             if (b < lo && !from_hist) sum += whole_weight(q, d.m, T);
         }
     // the workgroup's place among the gathered values, then each thread's
-    if (tid == 0) s_n = 0;
-    __syncthreads();
     uint32_t mine = in ? atomicAdd(&s_n, (uint32_t)__popc(in)) : 0;
     __syncthreads();
     if (tid == 0 && s_n) s_at = atomicAdd(&info->n_cand, s_n);

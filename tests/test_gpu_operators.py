@@ -779,6 +779,33 @@ def test_sample_among_nearly_equal_logits(ctx, spread):
         check_sample(ctx, Ask(rng, rows, V, u=rng.random(rows), temp=1.0, **kw), x)
 
 
+@pytest.mark.parametrize("V", [9001, 49152, 151936])
+@pytest.mark.parametrize("kw", [
+    dict(top_k=700), dict(top_k=1000), dict(top_k=3000), dict(top_k=7000), dict(top_k=3000, min_p=0.05), dict(top_k=2000, min_p=1e-4)],
+    ids=lambda k: "-".join(f"{a}{b}" for a, b in k.items()))
+def test_sample_with_a_large_top_k_alone(ctx, V, kw):
+    """More values above the cut's bin than are gathered whole, and no top-p: the weights before the bin are summed by the
+    workgroups themselves. The draw over the whole range of u, so that a chunk's weight that is off shows in the token."""
+    rng = np.random.default_rng(V + len(kw))
+    rows = 16
+    x = (rng.standard_normal((rows, V)) * 2.5).astype(np.float32)
+    for temp in (1.0, 1.7):
+        check_sample(ctx, Ask(rng, rows, V, u=(np.arange(rows) + rng.random(rows)) / rows, temp=temp, **kw), x)
+
+
+def test_sample_with_the_cut_in_the_last_bin(ctx):
+    """Flat rows under a few higher values: the k-th largest lies in the last bin, and the weights before it count."""
+    rng = np.random.default_rng(38)
+    rows, V = 8, 20011
+    x = np.full((rows, V), -np.inf, np.float32)
+    for r in range(rows):
+        at = rng.choice(V, 3000, replace=False)
+        x[r, at] = rng.standard_normal(3000) * 1e-4
+        x[r, at[:200]] = rng.uniform(1.5, 2.0, 200)
+    for kw in (dict(top_k=900), dict(top_k=2500), dict(top_k=2500, min_p=0.01), dict(top_k=V - 1)):
+        check_sample(ctx, Ask(rng, rows, V, u=(np.arange(rows) + rng.random(rows)) / rows, temp=1.0, **kw), x)
+
+
 @pytest.mark.parametrize("top", [0.0, 1e-30, -1e-40, 1e-8, 2.0 ** 26, -3.4028234663852886e38])
 def test_sample_with_min_p_at_its_end(ctx, top):
     """min-p at and next to 1, where next to zero a great many f32 values share the largest weight, and where a step of f32 at the
