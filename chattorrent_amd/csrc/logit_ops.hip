@@ -28,13 +28,14 @@ __device__ static inline RowPens row_pens(const SamplingDev& s, int row) {
     r.pres = s.pres ? (double)s.pres[row] : 0.0;
     r.cap = (double)s.freq_cap;
     r.p0 = r.p1 = r.b0 = r.b1 = 0;
+    // within the lists whatever the offsets say, both ends: an end past them alone would have the loops' indices wrap
     if (s.pen_at) {
-        r.p0 = max(s.pen_at[row], 0);
-        r.p1 = min(s.pen_at[row + 1], s.n_pen);
+        r.p0 = min(max(s.pen_at[row], 0), s.n_pen);
+        r.p1 = min(max(s.pen_at[row + 1], 0), s.n_pen);
     }
     if (s.bias_at) {
-        r.b0 = max(s.bias_at[row], 0);
-        r.b1 = min(s.bias_at[row + 1], s.n_bias);
+        r.b0 = min(max(s.bias_at[row], 0), s.n_bias);
+        r.b1 = min(max(s.bias_at[row + 1], 0), s.n_bias);
     }
     r.mask = nullptr;
     if (s.mask) {
@@ -79,12 +80,12 @@ __device__ static inline void apply_lists(const SamplingDev& s, const RowPens& r
         __syncthreads();   // what was here is read
         for (int i = 4 * tid; i < LG_CH; i += 4 * LG_T) *(uint4*)(lds + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        for (int i = r.b0 + tid; i < r.b1; i += LG_T) {
+        for (uint32_t i = r.b0 + tid; i < (uint32_t)r.b1; i += LG_T) {
             const uint32_t at = (uint32_t)s.bias_ids[i] - first;
-            if (at < n) atomicMax(&lds[narrow ? at : LG_CH / 2 + at], (uint32_t)(i - r.b0 + 1));
+            if (at < n) atomicMax(&lds[narrow ? at : LG_CH / 2 + at], i - r.b0 + 1);
         }
         if (narrow && r.b0 < r.b1) __syncthreads();   // the largest of whole words, before counts come in above
-        for (int i = r.p0 + tid; i < r.p1; i += LG_T) {
+        for (uint32_t i = r.p0 + tid; i < (uint32_t)r.p1; i += LG_T) {
             const uint32_t at = (uint32_t)s.pen_ids[i] - first;
             const int c = s.pen_counts ? s.pen_counts[i] : 1;
             if (at < n && c > 0) atomicAdd(&lds[at], narrow ? 0x10000u : (uint32_t)c);

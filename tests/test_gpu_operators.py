@@ -856,6 +856,32 @@ def test_the_largest_vocabulary_and_long_lists(ctx):
             assert np.array_equal(got, ask.adjust(x).astype(np.float32), equal_nan=True)
 
 
+def test_list_offsets_outside_the_lists(ctx):
+    """Rows whose offsets lie before or past the lists, next to the ends of 32 bits, or run backwards: the entries within count."""
+    rng = np.random.default_rng(39)
+    V, top, low = 9001, 2**31 - 1, -2**31
+    pairs = [(top, top), (low, top), (top - 3, low), (7, 3), (low, 5), (20, top), (top - 200, top), (0, 40), (40, 40), (-1, 41)]
+    x = (rng.standard_normal((len(pairs), V)) * 2).astype(np.float32)
+    for pen in (True, False):
+        for r, (lo, hi) in enumerate(pairs):   # a row a call, beside one with entries of both kinds
+            ask = Ask(rng, 2, V, history=40, rep=1.3, freq=0.4, pres=0.25, biases=40)
+            n = {name: len(ask.a[name + "_ids"]) for name in ("pen", "bias")}
+            name = "pen" if pen else "bias"
+            ask.a[name + "_at"] = np.array([lo, hi, n[name]], np.int32)
+            other = "bias" if pen else "pen"
+            ask.a[other + "_at"] = np.array([0, n[other] // 2, n[other]], np.int32)
+            got = ctx.adjust_logits(dev(x[:2]), ask.device()).numpy()
+            for row in range(2):
+                ends = [min(max(int(e), 0), n[name]) for e in ask.a[name + "_at"][row:row + 2]]
+                one = Ask(rng, 1, V)
+                one.a = {k: v[row:row + 1] if k in ("rep", "freq", "pres") else v for k, v in ask.a.items()}
+                one.a[name + "_at"] = np.array([ends[0], max(ends)], np.int32)
+                one.a[other + "_at"] = ask.a[other + "_at"][row:row + 2]
+                with np.errstate(over="ignore", invalid="ignore"):
+                    want = one.adjust(x[row:row + 1])[0].astype(np.float32)
+                assert np.array_equal(got[row], want, equal_nan=True), (name, lo, hi, row)
+
+
 def test_sample_follows_its_distribution(ctx):
     """4096 draws of one row: each token's share within five standard deviations of its weight."""
     rng = np.random.default_rng(34)
