@@ -47,10 +47,10 @@ __device__ static inline RowPens row_pens(const SamplingDev& s, int row) {
 
 constexpr int LG_CH = 4096;
 
-__device__ static inline float adjust_one(float x, const SamplingDev& s, const RowPens& r, int cnt, int last) {
-    if (cnt <= 0 && last <= 0) return x;
+__device__ static inline float adjust_one(float x, const SamplingDev& s, const RowPens& r, uint32_t cnt, int last) {
+    if (cnt == 0 && last <= 0) return x;
     double v = (double)x;
-    if (cnt > 0) {
+    if (cnt != 0) {
         v = v > 0.0 ? v / r.rep : v * r.rep;
         v -= r.pres + fmin(r.freq * (double)cnt, r.cap);
     }
@@ -70,7 +70,8 @@ constexpr int LG_J = LG_CH / (4 * LG_T);
 // is gathered in LDS first (LG_CH words): its count in the upper half of its
 // word, its last bias entry + 1 in the lower. Where those do not fit (a row of
 // 2^16 entries, or counts of the caller's), each half of the chunk in turn
-// gets a word for either.
+// gets a word for either; a count that passes 32 bits stays at 2^32 - 1 (told by
+// the top bit of the bias word, which no entry's index reaches).
 __device__ static inline void apply_lists(const SamplingDev& s, const RowPens& r, int base, uint32_t* lds,
                                           float (&a)[LG_J][4]) {
     const int tid = threadIdx.x;
@@ -84,11 +85,13 @@ __device__ static inline void apply_lists(const SamplingDev& s, const RowPens& r
             const uint32_t at = (uint32_t)s.bias_ids[i] - first;
             if (at < n) atomicMax(&lds[narrow ? at : LG_CH / 2 + at], i - r.b0 + 1);
         }
-        if (narrow && r.b0 < r.b1) __syncthreads();   // the largest of whole words, before counts come in above
+        if (r.b0 < r.b1) __syncthreads();   // the largest of whole words, before counts and the top bit come in above
         for (uint32_t i = r.p0 + tid; i < (uint32_t)r.p1; i += LG_T) {
             const uint32_t at = (uint32_t)s.pen_ids[i] - first;
             const int c = s.pen_counts ? s.pen_counts[i] : 1;
-            if (at < n && c > 0) atomicAdd(&lds[at], narrow ? 0x10000u : (uint32_t)c);
+            if (at >= n || c <= 0) continue;
+            if (narrow) atomicAdd(&lds[at], 0x10000u);
+            else if (atomicAdd(&lds[at], (uint32_t)c) > 0xffffffffu - (uint32_t)c) atomicOr(&lds[LG_CH / 2 + at], 0x80000000u);
         }
         __syncthreads();
 #pragma unroll
@@ -100,10 +103,13 @@ __device__ static inline void apply_lists(const SamplingDev& s, const RowPens& r
                                    : *(const uint4*)(lds + LG_CH / 2 + i);
             const int up = narrow ? 16 : 0;
             if ((u.x | u.y | u.z | u.w | l.x | l.y | l.z | l.w) != 0) {   // few of the fours hold a listed token
-                a[j][0] = adjust_one(a[j][0], s, r, (int)(u.x >> up), (int)l.x);
-                a[j][1] = adjust_one(a[j][1], s, r, (int)(u.y >> up), (int)l.y);
-                a[j][2] = adjust_one(a[j][2], s, r, (int)(u.z >> up), (int)l.z);
-                a[j][3] = adjust_one(a[j][3], s, r, (int)(u.w >> up), (int)l.w);
+                auto one = [&](float& x, uint32_t cnt, uint32_t last) {
+                    x = adjust_one(x, s, r, (int)last < 0 ? 0xffffffffu : cnt >> up, (int)(last & 0x7fffffffu));
+                };
+                one(a[j][0], u.x, l.x);
+                one(a[j][1], u.y, l.y);
+                one(a[j][2], u.z, l.z);
+                one(a[j][3], u.w, l.w);
             }
         }
     }

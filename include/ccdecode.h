@@ -402,8 +402,8 @@ cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* job
  *              none); one token's frequency penalty is at most freq_cap
  *   pen_at [rows+1], pen_ids [n_pen], pen_counts [n_pen] or NULL: row r's
  *              history is the entries [pen_at[r], pen_at[r+1]); an entry counts
- *              pen_counts, or 1, and an id's entries add up (0 or below: no
- *              entry)
+ *              pen_counts, or 1, and an id's entries add up, to 2^32 - 1 at
+ *              most (0 or below: no entry)
  *   bias_at [rows+1], bias_ids, bias [n_bias]: added to the row's logits; of an
  *              id's entries the last counts
  *   mask [n_masks][mask_words], mask_of [rows]: bit t%32 of word t/32 allows

@@ -882,6 +882,30 @@ def test_list_offsets_outside_the_lists(ctx):
                 assert np.array_equal(got[row], want, equal_nan=True), (name, lo, hi, row)
 
 
+def test_counts_that_pass_32_bits(ctx):
+    """An id's counts add up past 2^31, to 2^32 - 1 at most, whatever their order and beside biases of the same ids."""
+    rng = np.random.default_rng(40)
+    V, top = 5000, 2**31 - 1
+    x = (rng.standard_normal((1, V)) * 2).astype(np.float32)
+    #           2^31          2^32 - 2      2^32 - 1          past it                two of 2^30      one and nothing
+    sums = {3: [top, 1], 4: [top, top], 2500: [top, top, 1], 4999: [top] * 5 + [7], 70: [2**30] * 2, 71: [1, -5, 0]}
+    ids = np.array([t for t, c in sums.items() for _ in c], np.int32)
+    counts = np.array([v for c in sums.values() for v in c], np.int32)
+    order = rng.permutation(len(ids))
+    for freq, biases in ((2.0 ** -33, False), (2.0 ** -33, True), (0.0, False)):
+        kw = dict(biases=3) if biases else {}
+        ask = Ask(rng, 1, V, rep=1.5, freq=freq, pres=0.25, **kw)
+        ask.a.update(pen_at=np.array([0, len(ids)], np.int32), pen_ids=ids[order], pen_counts=counts[order])
+        if biases:
+            ask.a["bias_ids"][:] = [4999, 3, 4]
+        got = ctx.adjust_logits(dev(x), ask.device()).numpy()[0]
+        held = {t: min(sum(v for v in c if v > 0), 2**32 - 1) for t, c in sums.items()}
+        ask.a.update(pen_at=np.array([0, len(held)]), pen_ids=np.array(list(held)), pen_counts=np.array(list(held.values())))
+        want = ask.adjust(x)[0]
+        with np.errstate(over="ignore", invalid="ignore"):
+            assert np.array_equal(got, want.astype(np.float32), equal_nan=True), (freq, biases)
+
+
 def test_sample_follows_its_distribution(ctx):
     """4096 draws of one row: each token's share within five standard deviations of its weight."""
     rng = np.random.default_rng(34)
