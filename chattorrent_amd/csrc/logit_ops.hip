@@ -192,7 +192,9 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 // With a the adjusted row (a NaN counts as -inf) and temp > 0:
 //   s = f32(a / temp) (a finite value stays finite), m = max s,
 //   w = exp(s - m) as a whole number of 2^-42, so that sums of weights are
-//   exact integers and do not depend on their order;
+//   exact integers and do not depend on their order (a row without cuts: by
+//   chunk, relative to the chunk's maximum; the chunks' sums then relative to m
+//   and whole numbers again);
 //   kept by top-k: s >= the k-th largest s (ties stay);
 //   kept by top-p: s >= the largest value t for which the kept weights of
 //   s >= t reach p of all kept weights (ties stay);
@@ -213,12 +215,16 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 //                     bins (counts for top-k, weights for top-p), by chunk
 //                     and of the row; the row's last workgroup to finish
 //                     finds the bins that the cuts fall into. (A row
-//                     without a cut: the weights, and the last one draws.)
+//                     with min-p alone: the weights, and the last one draws.)
 //   k_sample_cut      the values of those bins are gathered; the row's last
 //                     workgroup finds the cuts' exact values among them and
 //                     draws. Where everything up to the cut's bin is at most
 //                     SM_SMALL values, all of it is gathered, and each value
 //                     counts the larger ones; else 9 bits at a time.
+// A row of such a call that asks for no cut is drawn as in the other kind, from
+// the same whole numbers (k_sample_scale sums its chunks' weights, the first
+// workgroup of k_sample_mass picks), so its token and probability do not
+// depend on what its neighbours ask for.
 // A row whose cut falls among more than SM_CAND values (nearly equal logits) is
 // drawn by its last workgroup alone, in passes over the row.
 //
@@ -230,6 +236,7 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 constexpr int SM_BINS = 512, SM_CAND = 4096, SM_SMALL = 512, SM_CHUNKS = (1 << 20) / LG_CH;
 constexpr float SM_REACH = 32.0f;            // the histogram's last bin takes everything below m - 32
 constexpr double SM_ONE = 4398046511104.0;   // 2^42: a row of 2^20 tokens sums to at most 2^62
+constexpr double SM_LEAST = 1e-13;           // under half a 2^-42
 typedef unsigned long long u64;
 
 // 1 / temp, never 0: a barred token's -inf stays so at an infinite temperature.
@@ -298,12 +305,12 @@ __device__ static inline uint32_t ordered(float v) {
 __device__ static inline float unordered(uint32_t k) { return u2f((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
 // min-p as a cut of s: the ordered bits of the smallest value whose weight
-// reaches min_p (0: none is cut; a weight under 1e-13 counts as nothing anyhow).
+// reaches min_p (0: none is cut; a weight under SM_LEAST counts as nothing anyhow).
 // Mostly m + log(min_p) to a step; but next to zero an f32 step is so short
 // that millions of values share a weight (min_p 1 and m 0: all of the 10^9 from
 // -2^-54 up weigh 1), so the search's steps double and then halve: 64 at most.
 __device__ static inline uint32_t min_cut(float m, double min_p, const double* T) {
-    if (!(min_p > 1e-13)) return 0;
+    if (!(min_p > SM_LEAST)) return 0;
     if (m == INFINITY) return ordered(m);
     const uint32_t top = ordered(m), least = ordered((float)((double)m - 31.0)) - 1;   // it weighs nothing
     auto cut = [&](uint32_t k) { return k <= least || (k < top && weight(unordered(k), m, T) < min_p); };
@@ -407,7 +414,7 @@ struct SampleWs {
 
 struct RowAsk {
     double inv, top_p, min_p;
-    bool greedy, cut;
+    bool greedy, cut, plain;   // cut: by top-k or top-p; plain: by nothing
     int k;
     __device__ RowAsk(const SamplingDev& s, int row, int V) {
         const double temp = s.temp ? (double)s.temp[row] : 0.0;
@@ -420,6 +427,7 @@ struct RowAsk {
         min_p = s.min_p ? (double)s.min_p[row] : 0.0;
         if (min_p > 1.0) min_p = 1.0;   // the maximum itself stays
         cut = !greedy && (k > 0 || top_p < 1.0);
+        plain = !greedy && !cut && !(min_p > SM_LEAST);
     }
 };
 
@@ -489,6 +497,50 @@ __device__ static inline void draw_in_runs(const float (&v)[N][4], int base, u64
 }
 
 // ---- without cuts
+// The weight of a chunk of adjusted logits relative to its own maximum (best),
+// to every thread.
+__device__ static inline u64 chunk_weight(const float (&a)[LG_J][4], u64 best, double inv, const double* T, u64* red) {
+    const float m = scaled_logit(unordered((uint32_t)(best >> 32)), inv);
+    u64 sum = 0;
+#pragma unroll
+    for (int j = 0; j < LG_J; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += based_weight(scaled_logit(a[j][e], inv), (double)m, T);
+    return block_sum64(sum - LG_J * 4 * SM_BASE, red);
+}
+
+// The token of a row, from its chunks' maxima and weights (mine and local:
+// those of chunk threadIdx.x; key: the row's best). The chunks' weights
+// relative to the row's maximum m are theirs times exp(m_c - m), rounded to
+// whole numbers again. load(c, v): the scaled logits of chunk c.
+template <class L>
+__device__ static inline void pick_row(u64 key, u64 mine, u64 local, double inv, double u, const double* T, u64* red, u64* found,
+                                       float* s_m, u64 (&runs)[LG_J][4], int32_t* id, float* prob, L&& load) {
+    const float m = scaled_logit(unordered((uint32_t)(key >> 32)), inv);
+    const float mc = mine ? scaled_logit(unordered((uint32_t)(mine >> 32)), inv) : -INFINITY;
+    const double f = weight(mc, m, T);
+    const u64 mass = (u64)rint((double)local * f);
+    const u64 before = block_before64(mass, red);
+    const u64 total = red[0] + red[1] + red[2] + red[3];
+    const u64 target = target_of(u, total);
+    if (before <= target && target < before + mass) {
+        const u64 left = (u64)((double)(target - before) / f);
+        found[0] = threadIdx.x;
+        found[1] = left < local - 1 ? left : local - 1;
+        *s_m = mc;
+    }
+    __syncthreads();
+    const int c = (int)found[0];
+    const u64 left = found[1];
+    const float m_c = *s_m;
+    float v[LG_J][4];
+    load(c, v);
+    draw_in_runs(v, c * LG_CH, left, runs, [&](float x) { return whole_weight(x, m_c, T); }, [&](int t, float x) {
+        *id = t;
+        if (prob) *prob = (float)(weight(x, m, T) * SM_ONE / (double)total);
+    });
+}
+
 template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                          SampleWs w) {
@@ -506,23 +558,13 @@ __global__ __launch_bounds__(LG_T) void k_sample_weights(const float* __restrict
 #pragma unroll
         for (int e = 0; e < 4; e++) first.take(a[j][e], c * LG_CH + 4 * (LG_T * j + threadIdx.x) + e);
     const u64 best = block_max64(first.key(), red);
-    u64 sum = 0;
-    if (best && temp > 0.0) {
-        const float m = scaled_logit(unordered((uint32_t)(best >> 32)), inv);
-#pragma unroll
-        for (int j = 0; j < LG_J; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) sum += based_weight(scaled_logit(a[j][e], inv), (double)m, T);
-        sum = block_sum64(sum - LG_J * 4 * SM_BASE, red);
-    }
+    const u64 sum = best && temp > 0.0 ? chunk_weight(a, best, inv, T, red) : 0;
     if (threadIdx.x == 0) {
         w.best[(size_t)row * w.chunks + c] = best;
         w.mass[(size_t)row * w.chunks + c] = sum;
     }
 }
 
-// The chunks' weights relative to the row's maximum m are theirs times
-// exp(m_c - m), rounded to whole numbers again.
 template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                       SampleWs w, int32_t* __restrict__ ids, float* __restrict__ probs) {
@@ -543,33 +585,14 @@ __global__ __launch_bounds__(LG_T) void k_sample_pick(const float* __restrict__ 
         }
         return;
     }
-    const float m = scaled_logit(unordered((uint32_t)(key >> 32)), inv);
-    const float mc = mine ? scaled_logit(unordered((uint32_t)(mine >> 32)), inv) : -INFINITY;
-    const double f = weight(mc, m, T);
-    const u64 mass = (u64)rint((double)local * f);
-    const u64 before = block_before64(mass, red);
-    const u64 total = red[0] + red[1] + red[2] + red[3];
-    const u64 target = target_of(s.u ? s.u[row] : 0.0, total);
-    if (before <= target && target < before + mass) {
-        const u64 left = (u64)((double)(target - before) / f);
-        found[0] = tid;
-        found[1] = left < local - 1 ? left : local - 1;
-        s_m = mc;
-    }
-    __syncthreads();
-    const int c = (int)found[0];
-    const u64 left = found[1];
-    const float m_c = s_m;
-    float a[LG_J][4];
-    adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, lds, a);
+    pick_row(key, mine, local, inv, s.u ? s.u[row] : 0.0, T, red, found, &s_m, runs, ids + row, probs ? probs + row : nullptr,
+             [&](int c, float (&v)[LG_J][4]) {
+                 adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, row_pens(s, row), c * LG_CH, lds, v);
 #pragma unroll
-    for (int j = 0; j < LG_J; j++)
+                 for (int j = 0; j < LG_J; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) a[j][e] = scaled_logit(a[j][e], inv);
-    draw_in_runs(a, c * LG_CH, left, runs, [&](float v) { return whole_weight(v, m_c, T); }, [&](int t, float v) {
-        ids[row] = t;
-        if (probs) probs[row] = (float)(weight(v, m, T) * SM_ONE / (double)total);
-    });
+                     for (int e = 0; e < 4; e++) v[j][e] = scaled_logit(v[j][e], inv);
+             });
 }
 
 // ---- with cuts
@@ -577,8 +600,10 @@ template <bool VEC, bool LISTS>
 __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__ x, int64_t ldx, int V, SamplingDev s,
                                                        SampleWs w) {
     __shared__ __align__(16) uint32_t lds[LISTS ? LG_CH : 4];
+    __shared__ double T[32];
     __shared__ u64 red[4];
     const int row = blockIdx.y, c = blockIdx.x;
+    exp_table(T);
     if (c == 0) {   // the next launch adds to them
         if (threadIdx.x < sizeof(SampleInfo) / 4) ((uint32_t*)(w.info + row))[threadIdx.x] = 0;
         for (int b = threadIdx.x; b < SM_BINS; b += LG_T) {
@@ -587,7 +612,8 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
         }
     }
     const RowPens r = row_pens(s, row);
-    const double temp = s.temp ? (double)s.temp[row] : 0.0, inv = inverse(temp);
+    const RowAsk ask(s, row, V);
+    const double inv = ask.inv;
     FirstMax first;
     float least = INFINITY, a[LG_J][4];
     adjusted_chunk<VEC, LISTS>(x + row * ldx, V, s, r, c * LG_CH, lds, a);
@@ -610,6 +636,9 @@ __global__ __launch_bounds__(LG_T) void k_sample_scale(const float* __restrict__
         w.best[(size_t)row * w.chunks + c] = best;
         w.least[(size_t)row * w.chunks + c] = unordered((uint32_t)~low);
     }
+    if (!ask.plain) return;
+    const u64 sum = best ? chunk_weight(a, best, inv, T, red) : 0;
+    if (threadIdx.x == 0) w.mass[(size_t)row * w.chunks + c] = sum;
 }
 
 // N runs of a row's scaled logits, from token `base` on.
@@ -677,6 +706,7 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
     __shared__ u64 hmass[SM_BINS], red[4], found[2], runs[LG_J][4];
     __shared__ uint32_t hcount[SM_BINS], s_last;
     __shared__ double T[32];
+    __shared__ float s_m;
     const int row = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
     const float* sr = w.s + row * w.lds;
     float v[LG_J][4];
@@ -690,6 +720,14 @@ __global__ __launch_bounds__(LG_T) void k_sample_mass(int V, SamplingDev s, Samp
             ids[row] = d.key ? (int32_t)(0xffffffffu - (uint32_t)d.key) : -1;
             if (prob) *prob = d.key ? 1.0f : 0.0f;
         }
+        return;
+    }
+    if (ask.plain) {   // as in a call without cuts, from the scaled logits
+        if (g != 0) return;
+        const bool on = tid < w.chunks;
+        pick_row(d.key, on ? w.best[(size_t)row * w.chunks + tid] : 0, on ? w.mass[(size_t)row * w.chunks + tid] : 0, ask.inv,
+                 s.u ? s.u[row] : 0.0, T, red, found, &s_m, runs, ids + row, prob,
+                 [&](int c, float (&x)[LG_J][4]) { scaled_runs(sr, V, c * LG_CH, x); });
         return;
     }
     SampleInfo* info = w.info + row;

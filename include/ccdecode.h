@@ -450,9 +450,12 @@ cc_status cc_logits_adjust(cc_ctx* ctx, const float* logits, int64_t ld, int32_t
  * weight exp(s), and of those exp(s - max) >= min_p; equal values are kept or
  * cut together. The token is the first, in id order, at which the running sum
  * of the kept weights is above u times their sum. Weights are held to 2^-42 of
- * the largest one, their sums exactly. ids gets the token, probs (may be NULL)
- * the probability it was drawn with. Greedy: the first maximum of a, 1. A row
- * with nothing above -inf: -1, 0. `workspace`: cc_sample_workspace bytes
+ * the row's largest one and summed exactly; in a row without cuts, to 2^-42 of
+ * the largest among the same 4096 tokens, and each 4096 tokens' sum to 2^-42
+ * of the row's largest. A row's result does not depend on the call's other
+ * rows. ids gets the token, probs (may be NULL) the probability it was drawn
+ * with. Greedy: the first maximum of a, 1. A row with nothing above -inf:
+ * -1, 0. `workspace`: cc_sample_workspace bytes
  * (0: the shape would be refused), 16-byte aligned, of any contents; two calls
  * that may overlap need two. */
 size_t cc_sample_workspace(int32_t rows, int32_t vocab, const cc_sampling* sampling);

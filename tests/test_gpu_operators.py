@@ -744,6 +744,36 @@ def test_sample_rows_that_ask_for_different_things(ctx):
     check_sample(ctx, ask, x)
 
 
+@pytest.mark.parametrize("V,temp", [(33, 1.0), (4096, 0.6), (12345, 1.0), (151936, 1.8)])
+def test_sample_rows_do_not_hang_on_their_neighbours(ctx, V, temp):
+    """Each row's token and probability, bit for bit, in a call by itself and beside rows that ask for other cuts; u at the
+    borders between tokens, where the last bit of a sum tells."""
+    rng = np.random.default_rng(V)
+    rows = 96
+    x = np.repeat((rng.standard_normal((1, V)) * 2.5).astype(np.float32), rows, 0)
+    s = (x[0].astype(np.float64) / np.float64(np.float32(temp))).astype(np.float32).astype(np.float64)
+    run = np.cumsum(np.exp(s - s.max()))
+    likely = np.searchsorted(run, rng.random(rows) * run[-1])
+    u = np.minimum(run[np.minimum(likely, V - 1)] / run[-1], np.nextafter(1.0, 0.0))
+    dx = dev(x)
+
+    def draw(pick, u, **kw):
+        ids, probs = (a.numpy() for a in ctx.sample(dx, Ask(rng, rows, V, u=u, temp=temp, **kw).device()))
+        return ids[pick], probs[pick].view(np.uint32)
+
+    odd = np.arange(rows) % 2 == 1
+    off = dict(top_k=np.where(odd, 40, 0), top_p=np.where(odd, 0.9, 1.0), min_p=np.where(odd, 0.01, 0.0))
+    for name, alone in (("plain", {}), ("top_k", dict(top_k=np.full(rows, 50))), ("top_p", dict(top_p=np.full(rows, 0.95))),
+                        ("min_p", dict(min_p=np.full(rows, 0.001)))):
+        want = draw(~odd, u, **alone)
+        for others in ({"top_k": off["top_k"]}, {"top_p": off["top_p"]}, {"min_p": off["min_p"]}, off):
+            kw = dict(others)
+            for n, v in alone.items():      # what the even rows ask for, beside what the odd ones do
+                kw[n] = np.where(odd, kw.get(n, v), v)
+            got = draw(~odd, u, **kw)
+            assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1]), (name, sorted(others))
+
+
 def test_sample_ties_infinities_and_empty_rows(ctx):
     """Equal values are kept or cut together; +inf takes everything; the type's lowest value is a value; NaN is none; a row
     that the mask leaves nothing of gives -1 and 0."""
