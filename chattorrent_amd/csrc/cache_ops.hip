@@ -510,8 +510,9 @@ __device__ static inline void best_pages(const uint32_t* __restrict__ sc, int a,
 // in log2 units; S^T = K . Q^T with the query as an f16 pair; O^T += V^T .
 // (p * s) with p * s as an f16 pair; one page of codes in flight), but its
 // pages come from a list, and a page's V scales enter p * s relative to the
-// power of two below the largest of them, so that f16 holds them whatever the
-// values' magnitude (O is carried relative to the last page's). The waves'
+// power of two below the largest of their 32-channel group, so that f16 holds
+// them whatever the values' magnitude, also where it differs from group to
+// group (O's channels of a group are carried relative to the last page's). The waves'
 // parts meet in LDS, the workgroups' in the workspace: the last workgroup of a
 // (row, tile) to finish joins them in split order, whichever it is, so a row's
 // result does not depend on it.
@@ -635,7 +636,10 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     }
     float mrow = -INFINITY, lsum = 0.0f;
     bool shifted = true;   // p carries 2^PV_SHIFT_LOG2 until a running max leaves no room for it
-    int ev = -127, etop = -127;   // O is relative to 2^ev; the largest ev yet
+    // lane 16 j + .., entry s: of group 4 s + j, whose O is relative to 2^ev; the largest ev yet
+    int ev[SCL], etop[SCL];
+#pragma unroll
+    for (int s = 0; s < SCL; s++) ev[s] = etop[s] = -127;
     float4_t o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) o[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -661,7 +665,9 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
         const int p64 = 64 * __builtin_amdgcn_readlane(lp, i);
         const bool bad = (uint32_t)__builtin_amdgcn_readlane(pgv, i) >= (uint32_t)c.n_pages;
         const int last = bad ? -1 : pos;   // the last token that counts
-        uint32_t top = 0;
+        // a group's V scales are one row of 16 lanes: the exponent of the largest (all zero: as before), and every scale
+        // relative to it; O has room for values 2^60 times as large as this page's
+        int by[SCL];   // what brings O from the page before to this one's exponent
 #pragma unroll
         for (int s = 0; s < SCL; s++) {
             *(u32x4*)&ksl[256 * s + lane * 4] = kst[s];
@@ -671,17 +677,15 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
                 for (int e = 0; e < 4; e++)
                     if (t0 + e > last) vst[s][e] = 0u;
             }
+            uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < 4; e++) top = max(top, vst[s][e]);   // scales are not negative
-        }
-        // the largest V scale's exponent (all zero: as before), and every scale relative to it; O has room for values
-        // 2^60 times as large as this page's
-        const uint32_t mx = wave_max_u32(top);
-        const int en = max(mx ? min((int)(mx >> 23) - 127, 127) : ev, etop - 60);
-        etop = max(etop, en);
-        const float down = u2f((uint32_t)(en < 127 ? 127 - en : 1) << 23) * (en < 127 ? 1.0f : 0.5f);   // 2^-en
-#pragma unroll
-        for (int s = 0; s < SCL; s++) {
+            const uint32_t mx = row_max_u32(top);
+            const int en = max(mx ? min((int)(mx >> 23) - 127, 127) : ev[s], etop[s] - 60);
+            etop[s] = max(etop[s], en);
+            by[s] = ev[s] - en;
+            ev[s] = en;
+            const float down = u2f((uint32_t)(en < 127 ? 127 - en : 1) << 23) * (en < 127 ? 1.0f : 0.5f);   // 2^-en
             u32x4 v;
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = f2u(u2f(vst[s][e]) * down);
@@ -733,12 +737,15 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
         shifted = shifted && !drop;
         const float alpha = (mrow == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrow - mnew)) * shrink;
         lsum *= alpha;
-        const float alpha_o = ldexpf(alpha, ev - en);
-        ev = en;
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
+        for (int b = 0; b < NG; b++) {
+            const float alpha_o = ldexpf(alpha, __builtin_amdgcn_readlane(by[b >> 2], 16 * (b & 3)));
 #pragma unroll
-            for (int r = 0; r < 4; r++) o[dt][r] *= alpha_o;
+            for (int r = 0; r < 4; r++) {
+                o[2 * b][r] *= alpha_o;
+                o[2 * b + 1][r] *= alpha_o;
+            }
+        }
         const float msub = (mnew == -INFINITY ? 0.0f : mnew) - (shifted ? PV_SHIFT_LOG2 : 0.0f);
 #pragma unroll
         for (int tt = 0; tt < 4; tt++)
@@ -791,10 +798,12 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
     lsum += __shfl_xor(lsum, 16);
     lsum += __shfl_xor(lsum, 32);
     {
-        const float un = shifted ? PV_UNSHIFT : 1.0f, up = ldexpf(un, ev);
+        const float un = shifted ? PV_UNSHIFT : 1.0f;
         float* part = smem + wave * OW;   // its scale slices are this wave's own and done with
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) *(float4_t*)(part + l16 * D + dt * 16 + 4 * j4) = o[dt] * up;
+        for (int dt = 0; dt < DT; dt++)
+            *(float4_t*)(part + l16 * D + dt * 16 + 4 * j4) =
+                o[dt] * ldexpf(un, __builtin_amdgcn_readlane(ev[dt >> 3], 16 * ((dt >> 1) & 3)));
         if (j4 == 0) {
             part[16 * D + l16] = mrow;
             part[16 * D + 16 + l16] = lsum * un;

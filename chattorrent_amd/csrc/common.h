@@ -201,16 +201,14 @@ __device__ static inline bool pv_big(u32x4 v) {
 }
 
 
-// The largest of a wave's words as unsigned integers, in a scalar register:
-// within rows of 16 lanes by DPP, the four rows' by readlane.
-__device__ static inline uint32_t wave_max_u32(uint32_t x) {
+// The largest of the words of a row of 16 lanes as unsigned integers, in each
+// of them.
+__device__ static inline uint32_t row_max_u32(uint32_t x) {
     auto mx = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
-    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true));    // lane ^ 1
-    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));    // lane ^ 2
-    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));   // 7 - lane of the eight
-    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));   // 15 - lane of the row
-    return mx(mx((uint32_t)__builtin_amdgcn_readlane((int)x, 0), (uint32_t)__builtin_amdgcn_readlane((int)x, 16)),
-              mx((uint32_t)__builtin_amdgcn_readlane((int)x, 32), (uint32_t)__builtin_amdgcn_readlane((int)x, 48)));
+    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true));      // lane ^ 1
+    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));      // lane ^ 2
+    x = mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));     // 7 - lane of the eight
+    return mx(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));  // 15 - lane of the row
 }
 
 // Words that the workgroups of a launch leave for the one of them that

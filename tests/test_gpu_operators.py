@@ -495,6 +495,29 @@ def test_attend_queries_of_any_magnitude(ctx, D, size):
     assert (np.abs(got - want).max(1) <= attend_bound(D, vmax, smax)).all()
 
 
+@pytest.mark.parametrize("D,nkv,budget", [(64, 2, 12), (128, 1, 12), (128, 2, 5), (256, 1, 12)])
+def test_attend_values_whose_groups_differ_in_size(ctx, D, nkv, budget):
+    """V's 32-channel groups of magnitudes 2^-40 to 2^40 beside each other in a page, the same from page to page or changing
+    by 2^20: every channel to the bound of its own group's values."""
+    rng = np.random.default_rng(D + budget)
+    jobs = [(0, 64 * 12 - 20, 3)]
+    for wander in (0, 10):
+        ref = of_random_pages(rng, nkv, D, 12)
+        scale = ref.v.view(np.float32)[..., 16 * D:]      # [pages, kv heads, 64 tokens' scales by group]
+        for h in range(nkv):
+            for g, e in enumerate(rng.permutation(np.linspace(-40, 40, D // 32)).round()):
+                at = scale_index(1, D)[:, g]
+                scale[:, h, at] *= 2.0 ** (e + rng.integers(-wander, wander + 1, (12, 1)))
+        cache = ref.device()
+        q = rng.standard_normal((3, 3 * nkv * D)).astype(np.float32)
+        want, _, smax = ref.attend(jobs, q, 3 * nkv, budget, 1, 2)
+        got = ctx.attend_pages(cache, jobs, dev(q), budget).numpy()
+        for h in range(nkv):
+            vmax = np.max([np.abs(ref.exact_rows(1, page, h)).max(0) for page in ref.table[0]], 0).reshape(-1, 32).max(-1)
+            off = np.abs(got - want).reshape(3, nkv, 3, D // 32, 32)[:, h].max((1, 3))
+            assert (off <= attend_bound(D, vmax[None], smax[:, None])).all(), (wander, h, off / vmax)
+
+
 def test_attend_queries_that_are_no_numbers(ctx):
     """A head whose query holds NaN or infinity gives NaN; the other heads and rows what they give without it."""
     rng = np.random.default_rng(26)
