@@ -732,7 +732,7 @@ __global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_attend_pages(CacheDev c
         pm = fmaxf(pm, __shfl_xor(pm, 16));
         pm = fmaxf(pm, __shfl_xor(pm, 32));
         const float mnew = fmaxf(mrow, pm);
-        const bool drop = !(fabsf(mnew) < PV_MAX_SCORE);
+        const bool drop = !(fabsf(mnew) < PV_MAX_SCORE) && mnew != -INFINITY;   // -inf: nothing but masked tokens yet
         const float shrink = drop && shifted ? PV_UNSHIFT : 1.0f;
         shifted = shifted && !drop;
         const float alpha = (mrow == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrow - mnew)) * shrink;

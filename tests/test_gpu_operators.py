@@ -518,6 +518,29 @@ def test_attend_values_whose_groups_differ_in_size(ctx, D, nkv, budget):
             assert (off <= attend_bound(D, vmax[None], smax[:, None])).all(), (wander, h, off / vmax)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attend_a_page_outside_the_cache_changes_no_other_pages_bits(ctx, D):
+    """A page that is none adds nothing, wherever it stands: each of four waves walks two pages, the absent one before or after.
+    The tokens of most weight have no values, so that what is left hangs on the last bits of small weights."""
+    rng = np.random.default_rng(D)
+    ref = of_random_pages(rng, 4, D, 8)
+    pages = ref.table[0].copy()
+    there = pages[::2]
+    ref.table = np.array([[p for a in there for p in (-1, a)], [p for a in there for p in (a, -1)]], np.int32)
+    q = (rng.standard_normal((1, 4 * D)) * 5).astype(np.float32)
+    at = np.arange(64)[:, None]
+    for h in range(4):
+        x = rotate32(q[0].reshape(4, D)[h][None], ref.rope[511][None])[0]
+        for page in there:
+            score = ref.rows(0, page, h) @ x
+            heavy = at[score > np.median(score), 0]
+            ref.v[page, h, code_index(1, D)[heavy]] = 128
+    cache = ref.device(bounds=False)
+    rows = dev(np.repeat(q, 128, 0))      # a launch of 128 rows and 4 kv heads: one workgroup each
+    got = [ctx.attend_pages(cache, [(slot, 511, 1)] * 128, rows, 8).numpy() for slot in (0, 1)]
+    assert same_bits(got[0], got[1]) and got[0].any()
+
+
 def test_attend_queries_that_are_no_numbers(ctx):
     """A head whose query holds NaN or infinity gives NaN; the other heads and rows what they give without it."""
     rng = np.random.default_rng(26)
