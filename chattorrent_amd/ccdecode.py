@@ -163,25 +163,51 @@ def _hip():
     h.hipMalloc.argtypes = [C.POINTER(C.c_void_p), C.c_size_t]
     h.hipFree.argtypes = [C.c_void_p]
     h.hipMemcpy.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int]
+    h.hipGetDevice.argtypes = [C.POINTER(C.c_int)]
     return h
 
 
-class DeviceArray:
-    """A C-contiguous array in device memory, for callers without torch."""
+class _Gpu:
+    """GPU `device` is the thread's current one within; None: the one that is, as `device`."""
 
-    def __init__(self, shape, dtype):
+    def __init__(self, h, device=None):
+        self.h, self.device = h, device
+
+    def __enter__(self):
+        now = C.c_int()
+        if self.h.hipGetDevice(C.byref(now)):
+            raise RuntimeError("no current GPU")
+        if self.device is None:
+            self.device = now.value
+        self.before = now.value
+        if self.before != self.device and self.h.hipSetDevice(self.device):
+            raise RuntimeError(f"no GPU {self.device}")
+        return self
+
+    def __exit__(self, *exc):
+        if self.before != self.device:
+            self.h.hipSetDevice(self.before)
+
+
+class DeviceArray:
+    """A C-contiguous array in the memory of one GPU (`device`; None: the
+    thread's current one), for callers without torch."""
+
+    def __init__(self, shape, dtype, device=None):
         self.shape, self.dtype = tuple(int(n) for n in np.atleast_1d(shape)), np.dtype(dtype)
         self.nbytes = int(np.prod(self.shape)) * self.dtype.itemsize
         self._h, p = _hip(), C.c_void_p()
-        if self._h.hipMalloc(C.byref(p), max(self.nbytes, 16)):
-            raise MemoryError(f"no device memory for {self.nbytes} bytes")
+        with _Gpu(self._h, device) as gpu:
+            self.device = gpu.device
+            if self._h.hipMalloc(C.byref(p), max(self.nbytes, 16)):
+                raise MemoryError(f"no device memory for {self.nbytes} bytes")
         self._p = p.value
 
     @classmethod
-    def of(cls, a):
+    def of(cls, a, device=None):
         """A copy of a numpy array on the device."""
         a = np.ascontiguousarray(a)
-        out = cls(a.shape, a.dtype)
+        out = cls(a.shape, a.dtype, device)
         out.set(a)
         return out
 
@@ -198,8 +224,9 @@ class DeviceArray:
         return out
 
     def _copy(self, to, of, kind):
-        if self._h.hipDeviceSynchronize() or (self.nbytes and self._h.hipMemcpy(to, of, self.nbytes, kind)):
-            raise RuntimeError("a copy between host and device failed")
+        with _Gpu(self._h, self.device):
+            if self._h.hipDeviceSynchronize() or (self.nbytes and self._h.hipMemcpy(to, of, self.nbytes, kind)):
+                raise RuntimeError("a copy between host and device failed")
 
     def data_ptr(self):
         return self._p
@@ -216,6 +243,11 @@ class DeviceArray:
 def _is_torch(t):
     torch = sys.modules.get("torch")
     return torch is not None and isinstance(t, torch.Tensor)
+
+
+def _gpu_of(t):
+    """The GPU whose memory t is in (-1: a CPU tensor's); None where it does not say."""
+    return t.get_device() if _is_torch(t) else getattr(t, "device", None)
 
 
 _dtypes = {}   # a dtype object's name
@@ -244,9 +276,9 @@ class _Buffers:
         have = tuple(t.shape)
         if have != shape and (len(have) != len(shape) or any(w is not None and n != w for n, w in zip(have, shape))):
             raise ValueError(f"{name}: shape {have}, not {shape}")
-        if _is_torch(t):
-            device = t.get_device()
-            if device < 0 or not t.is_contiguous():
+        device = _gpu_of(t)
+        if device is not None:
+            if device < 0 or (_is_torch(t) and not t.is_contiguous()):
                 raise ValueError(f"{name}: a contiguous tensor on the GPU")
             if self.device is not None and device != self.device:
                 raise ValueError(f"{name}: on another GPU than the others")
@@ -303,7 +335,7 @@ class KVCache(_Buffers):
         self.c = CCache()
         ctx._chk(ctx.lib.cc_cache_of(ctx.h, layer, C.byref(self.c)))
         self.kept.append(ctx)
-        self.device = ctx.opts.device if _is_torch(bounds) else None
+        self.device = ctx.opts.device
         self.c.bounds = self.take(bounds, "bounds", ("uint8", "int8"),
                                   (self.c.n_pages, int(ctx.lib.cc_bounds_bytes(C.byref(self.c)))))
         self._done()
@@ -623,11 +655,11 @@ class Context:
     def _on(self, stream, t, out=None):
         """The stream of a call on `t`: the one given, else torch's current one, else the context's. (0 is
         torch's default stream where t is torch's.)"""
+        for x in (t,) if out is None else (t, out):
+            if _gpu_of(x) not in (None, self.opts.device):
+                raise ValueError(f"an array on {x.device}, not on the context's GPU ({self.opts.device})")
         if not _is_torch(t):
             return stream
-        for x in (t,) if out is None else (t, out):
-            if x.get_device() != self.opts.device:
-                raise ValueError(f"a tensor on {x.device}, not on the context's GPU ({self.opts.device})")
         if not _torch_first:
             raise RuntimeError("import torch before the library is loaded: they would hold two HIP runtimes")
         if stream is not None:
@@ -648,12 +680,11 @@ class Context:
         ld = t.stride(0)
         return t.data_ptr(), ld if rows > 1 else max(ld, shape[1])
 
-    @staticmethod
-    def _new(like, shape, dtype, given=None):
+    def _new(self, like, shape, dtype, given=None):
         """An array for a call on `like`. On a stream that was given, torch allocates for that stream: its memory goes to
         another tensor as soon as it is let go, which only the stream's own order makes safe."""
         if not _is_torch(like):
-            return DeviceArray(shape, dtype)
+            return DeviceArray(shape, dtype, self.opts.device)
         torch = sys.modules["torch"]
         if given is None:
             if dtype == "float32" and shape == like.shape:   # half of torch.empty's 2 us; rows stay whole rows
