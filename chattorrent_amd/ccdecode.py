@@ -154,7 +154,8 @@ class CCError(RuntimeError):
 
 
 # --- device buffers: the operators on the caller's own memory -------------------------
-# They take torch tensors (a call then runs on torch's current stream) or DeviceArrays.
+# They take torch tensors or DeviceArrays. A call whose k, q or logits are torch's runs on torch's current stream, else on the
+# context's; where a call on the one reads what a call on the other wrote, the caller orders them, or gives both one stream.
 
 def _hip():
     """The HIP runtime that the library itself uses."""
@@ -265,7 +266,7 @@ class _Buffers:
     """Buffers that one C struct points into: checked, kept alive, on one device."""
 
     def __init__(self):
-        self.kept, self.device = [], None
+        self.kept, self.device, self.torch = [], None, False
 
     def take(self, t, name, dtypes, shape, nullable=True):
         """The pointer of a contiguous device array of one of `dtypes` and of `shape` (None: any extent)."""
@@ -283,6 +284,7 @@ class _Buffers:
             if self.device is not None and device != self.device:
                 raise ValueError(f"{name}: on another GPU than the others")
             self.device = device
+        self.torch = self.torch or _is_torch(t)
         self.kept.append(t)
         return t.data_ptr()
 
@@ -652,13 +654,19 @@ class Context:
         return ids, probs
 
     # --- operators on the caller's device buffers --------------------------------------
-    def _on(self, stream, t, out=None):
+    def _on(self, stream, held, t, out=None):
         """The stream of a call on `t`: the one given, else torch's current one, else the context's. (0 is
-        torch's default stream where t is torch's.)"""
+        torch's default stream where t is torch's.) held: the call's KVCache or Sampling, which is on the context's GPU as
+        well."""
+        if held.device is not None and held.device != self.opts.device:
+            raise ValueError(f"buffers on GPU {held.device}, not on the context's ({self.opts.device})")
         for x in (t,) if out is None else (t, out):
             if _gpu_of(x) not in (None, self.opts.device):
                 raise ValueError(f"an array on {x.device}, not on the context's GPU ({self.opts.device})")
         if not _is_torch(t):
+            if stream is None and (held.torch or (out is not None and _is_torch(out))):
+                # what torch has queued for them is on its stream, what was queued for the others on the context's
+                raise ValueError("torch tensors beside arrays that are not torch's: the call's stream must be given")
             return stream
         if not _torch_first:
             raise RuntimeError("import torch before the library is loaded: they would hold two HIP runtimes")
@@ -694,16 +702,11 @@ class Context:
         with torch.cuda.stream(s):
             return like.new_empty(shape, dtype=getattr(torch, dtype))
 
-    def _same_device(self, held):
-        if held.device is not None and held.device != self.opts.device:
-            raise ValueError(f"buffers on GPU {held.device}, not on the context's ({self.opts.device})")
-
     def kv_append(self, cache, jobs, k, v, stream=None):
         """cc_kv_append: the jobs' rows (slot, past, n) of k (before RoPE) and v,
         f32 [rows, kv heads * D], into the cache's pages, and the key bounds of
         the pages they complete."""
-        self._same_device(cache)
-        stream = self._on(stream, k, v)
+        stream = self._on(stream, cache, k, v)
         a, at, n, rows = _job_rows(jobs)
         kp, ldk = self._rows(k, "k", rows, cache.width)
         vp, ldv = self._rows(v, "v", rows, cache.width)
@@ -713,8 +716,7 @@ class Context:
 
     def kv_bounds(self, cache, jobs, stream=None):
         """cc_kv_bounds: key bounds of the pages within the jobs' rows, from the cache."""
-        self._same_device(cache)
-        stream = self._on(stream, cache.kept[-1])
+        stream = self._on(stream, cache, cache.kept[-1])
         a, at, n, _ = _job_rows(jobs)
         self._chk(self.lib.cc_kv_bounds(self.h, cache.ref, at, n, stream))
 
@@ -722,8 +724,7 @@ class Context:
         """cc_attend_pages: attention of the jobs' rows, q f32 [rows, heads * D]
         before RoPE, over at most `budget` pages a row and kv head. Returns the
         rows' output (`out`, or a new array)."""
-        self._same_device(cache)
-        given, stream = stream, self._on(stream, q, out)
+        given, stream = stream, self._on(stream, cache, q, out)
         a, at, n, rows = _job_rows(jobs)
         qp, ldq = self._rows(q, "q", rows, None)
         D, width = cache.c.head_dim, int(q.shape[1])
@@ -753,8 +754,7 @@ class Context:
     def adjust_logits(self, logits, sampling, out=None, stream=None):
         """cc_logits_adjust: the rows with penalties, biases and masks, in `out`
         (logits itself, another array, or a new one)."""
-        self._same_device(sampling)
-        given, stream = stream, self._on(stream, logits, out)
+        given, stream = stream, self._on(stream, sampling, logits, out)
         rows, V = sampling.rows, sampling.vocab
         lp, ld = self._rows(logits, "logits", rows, V)
         if out is None:
@@ -770,8 +770,7 @@ class Context:
     def sample(self, logits, sampling, stream=None):
         """cc_sample: a token of each row of logits and the probability it was
         drawn with, int32 and f32 [rows]."""
-        self._same_device(sampling)
-        given, stream = stream, self._on(stream, logits)
+        given, stream = stream, self._on(stream, sampling, logits)
         rows, V = sampling.rows, sampling.vocab
         lp, ld = self._rows(logits, "logits", rows, V)
         ids, probs = self._new(logits, (rows,), "int32", given), self._new(logits, (rows,), "float32", given)

@@ -170,3 +170,52 @@ for g in (0, 1):
 out.append(hip.stand_in_launches().count(b"k_kv_append"))
 """)
     assert out == [4]
+
+
+TENSORS = """
+class Tensor(cc.DeviceArray):      # stands for torch's: on GPU 0, contiguous
+    def get_device(self):
+        return self.gpu
+    def is_contiguous(self):
+        return True
+def tensor(*shape, of=np.float32, gpu=0):
+    hip.hipSetDevice(0)
+    t = Tensor(shape, of)
+    t.gpu = gpu
+    return t
+cc._is_torch = lambda t: isinstance(t, Tensor)
+def outcome(call):
+    hip.stand_in_reset(-1)
+    try:
+        call()
+    except (ValueError, RuntimeError) as e:
+        return [str(e), hip.stand_in_launches().count(b"k_")]
+    return ["", hip.stand_in_launches().count(b"k_")]
+x, q, kv = on(0, 2, 100), on(0, 1, 256), on(0, 1, 128)
+s, c, job = cc.Sampling(2, 100), cache(*[0] * 5), [(0, 70, 1)]
+"""
+
+
+def test_tensors_beside_other_arrays_need_a_stream(host):
+    """The call's arrays are each ordered on the stream of their kind: a mixed call must say where it runs."""
+    out = host(TENSORS + """
+mixed = cc.Sampling(2, 100, temp=tensor(2), u=on(0, 2, of=np.float64))
+c2 = cc.KVCache(*[a for a in c.kept[:4]], 64, bounds=tensor(*c.kept[4].shape, of=np.uint8))
+calls = [lambda **kw: ctx[0].kv_append(c, job, kv, tensor(1, 128), **kw), lambda **kw: ctx[0].kv_append(c2, job, kv, kv, **kw),
+         lambda **kw: ctx[0].attend_pages(c, job, q, 3, out=tensor(1, 256), **kw), lambda **kw: ctx[0].attend_pages(c2, job, q, 3, **kw),
+         lambda **kw: ctx[0].adjust_logits(x, s, out=tensor(2, 100), **kw), lambda **kw: ctx[0].adjust_logits(x, mixed, **kw),
+         lambda **kw: ctx[0].sample(x, mixed, **kw)]
+out = [outcome(c) for c in calls] + [outcome(lambda: c(stream=0))[0] for c in calls]
+""")
+    assert all("stream must be given" in said and n == 0 for said, n in out[:7]), out
+    assert out[7:] == [""] * 7
+
+
+def test_tensors_on_the_cpu_are_refused_beside_device_arrays(host):
+    out = host(TENSORS + """
+cpu = lambda *a: tensor(*a, gpu=-1)
+out = [outcome(c) for c in (lambda: ctx[0].kv_append(c, job, kv, cpu(1, 128), stream=0), lambda: ctx[0].kv_append(c, job, cpu(1, 128), kv),
+                            lambda: ctx[0].attend_pages(c, job, q, 3, out=cpu(1, 256), stream=0),
+                            lambda: ctx[0].adjust_logits(x, s, out=cpu(2, 100), stream=0), lambda: ctx[0].sample(cpu(2, 100), s))]
+""")
+    assert all("not on the context's GPU" in said and n == 0 for said, n in out), out
