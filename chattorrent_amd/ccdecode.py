@@ -251,6 +251,12 @@ def _gpu_of(t):
     return t.get_device() if _is_torch(t) else getattr(t, "device", None)
 
 
+def _no_gradient(t):
+    """Refuses a tensor whose gradient would end at a call: the operators have no backward pass."""
+    if t.requires_grad and sys.modules["torch"].is_grad_enabled():
+        raise ValueError("a tensor that requires a gradient: none passes through a call (detach it, or call under no_grad)")
+
+
 _dtypes = {}   # a dtype object's name
 
 
@@ -284,7 +290,9 @@ class _Buffers:
             if self.device is not None and device != self.device:
                 raise ValueError(f"{name}: on another GPU than the others")
             self.device = device
-        self.torch = self.torch or _is_torch(t)
+        if _is_torch(t):
+            _no_gradient(t)
+            self.torch = True
         self.kept.append(t)
         return t.data_ptr()
 
@@ -663,6 +671,8 @@ class Context:
         for x in (t,) if out is None else (t, out):
             if _gpu_of(x) not in (None, self.opts.device):
                 raise ValueError(f"an array on {x.device}, not on the context's GPU ({self.opts.device})")
+            if _is_torch(x):
+                _no_gradient(x)
         if not _is_torch(t):
             if stream is None and (held.torch or (out is not None and _is_torch(out))):
                 # what torch has queued for them is on its stream, what was queued for the others on the context's

@@ -174,6 +174,7 @@ out.append(hip.stand_in_launches().count(b"k_kv_append"))
 
 TENSORS = """
 class Tensor(cc.DeviceArray):      # stands for torch's: on GPU 0, contiguous
+    requires_grad = False
     def get_device(self):
         return self.gpu
     def is_contiguous(self):
@@ -219,3 +220,25 @@ out = [outcome(c) for c in (lambda: ctx[0].kv_append(c, job, kv, cpu(1, 128), st
                             lambda: ctx[0].adjust_logits(x, s, out=cpu(2, 100), stream=0), lambda: ctx[0].sample(cpu(2, 100), s))]
 """)
     assert all("not on the context's GPU" in said and n == 0 for said, n in out), out
+
+
+def test_gradients_do_not_end_silently(host):
+    """A tensor that requires a gradient is refused in each place, except where gradients are off."""
+    out = host(TENSORS + """
+import types
+grad = [True]
+sys.modules["torch"] = types.SimpleNamespace(is_grad_enabled=lambda: grad[0])
+def learnt(*a, **kw):
+    t = tensor(*a, **kw)
+    t.requires_grad = True
+    return t
+calls = [lambda: ctx[0].kv_append(c, job, learnt(1, 128), kv), lambda: ctx[0].kv_append(c, job, kv, learnt(1, 128), stream=0),
+         lambda: ctx[0].attend_pages(c, job, learnt(1, 256), 3), lambda: ctx[0].attend_pages(c, job, q, 3, out=learnt(1, 256), stream=0),
+         lambda: ctx[0].adjust_logits(learnt(2, 100), s), lambda: ctx[0].adjust_logits(x, s, out=learnt(2, 100), stream=0),
+         lambda: ctx[0].sample(learnt(2, 100), s), lambda: cc.Sampling(2, 100, temp=learnt(2))]
+out = [outcome(c) for c in calls]
+grad[0] = False
+out += [outcome(c) for c in (calls[1], calls[3], calls[5], calls[7])]
+""")
+    assert all("gradient" in said and n == 0 for said, n in out[:8]), out
+    assert all(said == "" for said, n in out[8:]), out
