@@ -298,13 +298,22 @@ class _Buffers:
 
 
 class _HostArray:
-    """A wish of cc_sample_pass, in host memory and in the type that Sampling takes."""
+    """A wish of cc_sample_pass, in host memory and in the type that Sampling
+    takes; whole numbers as they are given, or refused (a mask's words may be
+    signed or not)."""
 
     def __init__(self, name, a):
         kind = {"u": np.float64, "mask": np.uint32}.get(name, np.float32)
         if name in ("top_k", "pen_at", "pen_ids", "pen_counts", "bias_at", "bias_ids", "mask_of"):
             kind = np.int32
-        self.a = np.ascontiguousarray(a, kind)
+        given = np.asarray(a)
+        if kind in (np.int32, np.uint32) and given.size:
+            low, high = np.min(given), np.max(given)      # NaN: in neither's range
+            if not (low >= -2**31 and high < (2**31 if kind is np.int32 else 2**32) and (given == np.trunc(given)).all()):
+                raise ValueError(f"{name}: whole numbers of 32 bits")
+            if kind is np.uint32:
+                given = given.astype(np.int64)
+        self.a = np.ascontiguousarray(given, kind)
         self.shape, self.dtype = self.a.shape, self.a.dtype
 
     def data_ptr(self):

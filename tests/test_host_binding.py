@@ -242,3 +242,23 @@ out += [outcome(c) for c in (calls[1], calls[3], calls[5], calls[7])]
 """)
     assert all("gradient" in said and n == 0 for said, n in out[:8]), out
     assert all(said == "" for said, n in out[8:]), out
+
+
+def test_wishes_that_are_no_32_bit_numbers(host):
+    """What does not fit is refused, not wrapped or cut; what fits keeps its bits."""
+    out = host("""
+bad = [("top_k", np.array([2**32 + 5])), ("top_k", [1.5]), ("top_k", [np.nan]), ("pen_at", [0, 2**31]), ("pen_ids", np.array([-2**40])),
+       ("mask_of", [np.inf]), ("bias_ids", np.array([2**63], np.uint64)), ("mask", np.array([[2**32]])), ("mask", [[0.5]])]
+out = []
+for name, a in bad:
+    try:
+        cc._HostArray(name, a)
+        out.append([name, str(a)])
+    except ValueError as e:
+        out += [] if name in str(e) else [str(e)]
+good = [("top_k", [3.0, -2**31, 2**31 - 1]), ("mask", np.array([[-1, 7]], np.int32)), ("mask", np.array([[2**32 - 1, 0]])), ("pen_ids", []),
+        ("mask", np.zeros((1, 2))), ("top_k", np.array([1, 2], np.uint8)), ("temp", [1, 0.5]), ("u", [0.1]), ("mask_of", [True])]
+out += [[a.tolist(), str(a.dtype)] for a in (cc._HostArray(n, v).a for n, v in good)]
+""")
+    assert out == [[[3, -2**31, 2**31 - 1], "int32"], [[[2**32 - 1, 7]], "uint32"], [[[2**32 - 1, 0]], "uint32"], [[], "int32"],
+                   [[[0, 0]], "uint32"], [[1, 2], "int32"], [[1.0, 0.5], "float32"], [[0.1], "float64"], [[1], "int32"]]
