@@ -394,7 +394,12 @@ cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* job
 
 /* What a call asks of each of its rows: device arrays [rows], or NULL where
  * none asks for it. The meaning is the reference's sampler's
- * (web/model/sampling.js:57-215) with two more cuts, biases and masks.
+ * (web/model/sampling.js:57-215) with two more cuts, biases and masks, but:
+ * an id that a list repeats is penalised once for its counts' sum (there once
+ * an entry); a count of 0 is no entry (there rep and pres apply); a row with
+ * no token left gives -1 (there its first or last token); and the draw's sums
+ * are of f64 weights as cc_sample says (there the walk adds their f32 copies,
+ * so a u within about 2^-23 of a border may fall to the other side).
  *   temp       0 or below: greedy
  *   top_k      0 or below, or vocab and more: off
  *   top_p      1 and more: off;  min_p  0: off (at most 1 counts)

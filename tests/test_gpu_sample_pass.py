@@ -1,6 +1,11 @@
 """cc_sample_pass: the tokens of a pass's own logits, drawn where they are,
 against the same logits read back and drawn in numpy in 64 bits, and against
 cc_sample over a copy of them."""
+import base64
+import json
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -8,6 +13,7 @@ from chattorrent_amd import configs
 from tests.test_gpu_operators import Ask, U32, dev
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 V = configs.SMOLLM2["vocab"]
 
 
@@ -82,3 +88,57 @@ def test_refusals(ctx):
         fresh.sample_pass(1)
     fresh.close()
     assert (ctx.sample_pass(2)[0] >= 0).all()
+
+
+HOST_DRAWS = """
+const { sampleFromLogitsRow } = require(process.argv[1]);
+const jobs = JSON.parse(require('fs').readFileSync(0, 'utf8'));
+console.log(JSON.stringify(jobs.map(j => {
+    const b = Buffer.from(j.row, 'base64');
+    const row = new Float32Array(b.buffer.slice(b.byteOffset, b.byteOffset + b.length));
+    return j.draws.map(d => sampleFromLogitsRow(row, d.opts, () => d.u));
+})));
+"""
+
+
+def test_the_hosts_sampler_draws_the_same_tokens(ctx):
+    """The same options through node/sampling.js over the rows read back and through cc_sample_pass: greedy, temperatures, top-k,
+    penalties of distinct ids with counts of 1 and more, bans (all parameters whole in f32). Where u is not within 2^-20 of a border: there the host's walk,
+    which adds weights rounded to f32 (2^-24 each, so 2^-24 of the sum behind a border and as much of the total), may differ."""
+    rng = np.random.default_rng(12)
+    rows = 8
+    x = feed(ctx, rng, [2] * rows, [1] * rows)
+    opts, u = [], []
+    for i in range(12):
+        for r in range(rows):
+            o = dict(temp=[0, 0.75, 1.0, 1.875][i % 4], topK=[0, 40, 200][i % 3])
+            if i % 2:
+                top = np.argsort(-x[r])[:20]
+                ids = np.unique(np.concatenate([rng.integers(0, V, 30), rng.choice(top, 10, replace=False)]))
+                o.update(pen=[[int(t), int(rng.integers(1, 9))] for t in ids], rep=1.25, freq=0.5, pres=0.25)
+                o["ban"] = [int(t) for t in rng.choice(top, 3, replace=False)]
+            opts.append(o)
+            u.append(float(rng.random()))
+    jobs = [dict(row=base64.b64encode(x[r].tobytes()).decode(), draws=[dict(opts=opts[i * rows + r], u=u[i * rows + r]) for i in range(12)])
+            for r in range(rows)]
+    told = subprocess.run(["node", "-e", HOST_DRAWS, os.path.join(ROOT, "chattorrent_amd", "node", "sampling.js")],
+                          input=json.dumps(jobs), capture_output=True, text=True, timeout=100)
+    assert told.returncode == 0, told.stderr
+    host, compared = json.loads(told.stdout), 0
+    for i in range(12):
+        mine = opts[i * rows:(i + 1) * rows]
+        kw = dict(temp=[o["temp"] for o in mine], top_k=[o["topK"] for o in mine], u=u[i * rows:(i + 1) * rows])
+        ask = Ask(rng, rows, V, **kw)
+        if i % 2:
+            flat = [e for o in mine for e in o["pen"]]
+            ask.a.update(rep=np.full(rows, 1.25, np.float32), freq=np.full(rows, 0.5, np.float32), pres=np.full(rows, 0.25, np.float32),
+                         pen_at=np.cumsum([0] + [len(o["pen"]) for o in mine]).astype(np.int32),
+                         pen_ids=np.array([e[0] for e in flat], np.int32), pen_counts=np.array([e[1] for e in flat], np.int32),
+                         bias_at=np.arange(0, 3 * rows + 1, 3, dtype=np.int32), bias=np.full(3 * rows, -np.inf, np.float32),
+                         bias_ids=np.array([t for o in mine for t in o["ban"]], np.int32))
+        ids, _ = ctx.sample_pass(rows, freq_cap=ask.cap, **ask.a)
+        for r, (t, p, near) in enumerate(ask.sample(x)):
+            if near > 2.0 ** -20:
+                compared += 1
+                assert ids[r] == host[r][i], (i, r, ids[r], host[r][i], t)
+    assert compared >= 80
