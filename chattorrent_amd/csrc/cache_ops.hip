@@ -29,7 +29,10 @@ __device__ static inline OpJob job_of(const OpJobs& jobs, int u) {
 // exchanges away) and a wave takes 512/D rows at a time. RoPE, amax, scale =
 // amax/127, inv = 1/scale, rint, clamp: the f32 steps of the pass's own store,
 // so the codes and scales are its bits. 4000 rows of 8 heads of 128 (42 MB)
-// take 15.5 us, 2.7 TB/s: rotation and quantisation, not memory; 32 rows 4.4 us.
+// take 15.5-16 us, 2.7 TB/s: half the rate of a copy. A wave of a whole page
+// walks its strides of rows one after another, and loads the next when the one
+// before is stored: a chain of four latencies. 32 rows take 4.4 us. Bounds
+// alone, of 16 chats of 16384 tokens (311 MB): 160 us, 1.9 TB/s, the same walk.
 //
 // Key bounds (a page's, made when its 64th row is stored): per channel the
 // largest and the smallest of the page's 64 dequantised keys, as codes against
@@ -518,8 +521,13 @@ __device__ static inline void best_pages(const uint32_t* __restrict__ sc, int a,
 // result does not depend on it.
 //
 // 32 rows, 8 kv heads of 128, 64 pages each (302 MB): 61 us, 4.9 TB/s, memory.
-// 128 rows, 4 heads of 256, 48 pages: 145 us, the issue of vector instructions
-// (codes unpacked, P split) at one wave a SIMD; two spill and take twice that.
+// 128 rows, 4 heads of 256, 48 pages: 149 us, one wave a SIMD. A page is some
+// 1490 vector instructions (codes unpacked, P split) and 128 MFMA, 24 pages a
+// SIMD 60-80 us of them; the rest is waiting that one wave does not cover. It
+// holds 256 registers and 144 in the accumulation file; two waves have 256 in
+// all each, where it spills and takes twice as long.
+// Rows of a prompt take a tile each as well: 512 rows at 8192 of 40 heads of
+// 128, 64 pages a row, 0.6 ms.
 // One row, 8 heads of 128, 32 pages: 14 us, a chain of choice (2.4 of it),
 // pages and two joins.
 template <int NG>

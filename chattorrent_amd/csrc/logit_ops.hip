@@ -225,12 +225,18 @@ hipError_t launch_logits_adjust(hipStream_t st, const float* x, int64_t ldx, int
 // the same whole numbers (k_sample_scale sums its chunks' weights, the first
 // workgroup of k_sample_mass picks), so its token and probability do not
 // depend on what its neighbours ask for.
-// A row whose cut falls among more than SM_CAND values (nearly equal logits) is
-// drawn by its last workgroup alone, in passes over the row.
+// A row with more than SM_CAND values in the bins from its cuts' lowest to their
+// highest is drawn by its last workgroup alone, in passes over the row. That is
+// where one finite value far below the others widens the bins to 1/16 (a ban of
+// -1e4 on logits with a spread of 0.5: 151936 of them with top-p take 1.7 ms
+// instead of 0.04, 32 such rows 1.9 instead of 0.06), and where top-k is large
+// and top-p cuts far above it (k 20000, p 0.5: 0.7-0.9 ms a row, 32 rows 1.3).
 //
-// 128 rows of 128256 without cuts: 27 + 8 us, bound by f64 issue (about 14
-// operations a weight; the logits' bytes alone take 13). 32 rows of 151936 with
-// top-p and min-p: 14.6 + 19.6 + 18.0 us, the weights' histogram in LDS, then
+// 128 rows of 128256 without cuts: 27 + 8 us, bound by the issue of vector
+// instructions: 877 for a lane's 16 logits, a third of them the f64 of the
+// weights; the rest follows the first maximum by token, applies masks and keeps
+// finite values finite (the logits' bytes alone take 13). 32 rows of 151936 with
+// top-p and min-p: 15.7 + 17.7 + 17.8 us, the weights' histogram in LDS, then
 // one workgroup a row that finds the cut (3 us) and draws (5). One row of 49152
 // with top-k: 7 + 7 + 9 us, a chain of loads and barriers.
 constexpr int SM_BINS = 512, SM_CAND = 4096, SM_SMALL = 512, SM_CHUNKS = (1 << 20) / LG_CH;

@@ -381,7 +381,11 @@ cc_status cc_kv_bounds(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, 
  * 32 channels) and a page's bounds (hi, lo, B), a query head's score is the
  *   sum over groups g of T_g * B_g * sum over d in g of max(c*hi, c*lo),
  * and the kv head's the largest over its query heads, rounded to f32.
- * out = softmax(q . k / sqrt(D)) v over the tokens read.
+ * out = softmax(q . k / sqrt(D)) v over the tokens read. How many workgroups
+ * share a row's pages follows from the rows of the call, so a row's last bits
+ * may differ between calls of few and of many rows; which pages it reads does
+ * not. An output value's error is relative to the largest |v| of its 32
+ * channels among the tokens read.
  * 0 <= sink, 1 <= recent, sink + recent <= budget. cache->bounds is needed
  * where a row sees more than `budget` pages: the pages before the row's last
  * `recent` have theirs. `workspace`: cc_attend_workspace bytes (for a
