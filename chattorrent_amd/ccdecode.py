@@ -30,7 +30,8 @@ EXPORTS = [
     "cc_stats_get", "cc_op_matmul_q8", "cc_op_store_kv", "cc_op_round_f16", "cc_op_topk", "cc_op_rmsnorm",
     "cc_op_attend", "cc_profile", "cc_profile_read", "cc_read_logits", "cc_mtp_draft", "cc_topk_noalloc",
     "cc_decode_steps", "cc_cache_of", "cc_bounds_bytes", "cc_kv_append", "cc_kv_bounds", "cc_attend_workspace",
-    "cc_attend_pages", "cc_logits_adjust", "cc_sample_workspace", "cc_sample", "cc_sample_pass",
+    "cc_attend_pages", "cc_kv_append_at", "cc_weigh_workspace", "cc_attend_weigh", "cc_evict_workspace", "cc_kv_evict",
+    "cc_logits_adjust", "cc_sample_workspace", "cc_sample", "cc_sample_pass",
 ]
 
 
@@ -68,6 +69,16 @@ class CCache(C.Structure):
     _fields_ = [("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("n_pages", C.c_int32),
                 ("max_pages", C.c_int32), ("slots", C.c_int32), ("rope_rows", C.c_int32), ("k", C.c_void_p),
                 ("v", C.c_void_p), ("bounds", C.c_void_p), ("page_table", C.c_void_p), ("rope", C.c_void_p)]
+
+
+class CPositions(C.Structure):
+    """cc_positions: the rows' positions on several axes (Positions builds it)."""
+    _fields_ = [("n_axes", C.c_int32), ("pos", C.c_void_p), ("axis_of", C.c_void_p)]
+
+
+class CMarks(C.Structure):
+    """cc_marks: the weights and token numbers of a cache's rows (Marks builds it)."""
+    _fields_ = [("weight", C.c_void_p), ("token", C.c_void_p)]
 
 
 class CSampling(C.Structure):
@@ -125,6 +136,11 @@ def load():
         "cc_kv_bounds": (i32, [P, P, P, i32, P]),
         "cc_attend_workspace": (size, [P, P, i32, i32, i32]),
         "cc_attend_pages": (i32, [P, P, P, i32, i32, i32, i32, i32, P, i64, P, i64, P, size, P]),
+        "cc_kv_append_at": (i32, [P, P, P, P, P, i32, P, P, i64, P, i64, P]),
+        "cc_weigh_workspace": (size, [P, P, P, i32, i32, i32]),
+        "cc_attend_weigh": (i32, [P, P, P, P, P, i32, i32, i32, C.c_float, P, i64, P, i64, P, size, P]),
+        "cc_evict_workspace": (size, [P, P, i32]),
+        "cc_kv_evict": (i32, [P, P, P, P, i32, i32, i32, P, size, P]),
         "cc_logits_adjust": (i32, [P, P, i64, i32, i32, P, P, i64, P]),
         "cc_sample_workspace": (size, [i32, i32, P]),
         "cc_sample": (i32, [P, P, i64, i32, i32, P, P, P, P, size, P]),
@@ -361,6 +377,55 @@ class KVCache(_Buffers):
         return self
 
 
+class Positions(_Buffers):
+    """The positions of a call's rows (cc_positions): pos int32 [rows, axes] in
+    device memory, 1 to 4 axes, and the axis that each pair of rotary channels
+    turns by, whole numbers [rot_dim/2] in host memory (None: the first)."""
+
+    def __init__(self, pos, axis_of=None):
+        super().__init__()
+        self.rows, self.axes = int(pos.shape[0]), int(pos.shape[1]) if len(pos.shape) == 2 else 0
+        self.pairs = None
+        a = None
+        if axis_of is not None:
+            a = np.asarray(axis_of)
+            if a.ndim != 1 or (a.size and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() >= max(self.axes, 1))):
+                raise ValueError(f"axis_of: whole numbers of 0 to {self.axes - 1}, one of each pair")
+            a = np.ascontiguousarray(a, np.uint8)
+            self.pairs = len(a)
+            self.kept.append(a)
+        self.c = CPositions(n_axes=self.axes, pos=self.take(pos, "pos", ("int32",), (None, None), False),
+                            axis_of=None if a is None else a.ctypes.data)
+        self.ref = C.byref(self.c)
+
+    def fit(self, cache, rows):
+        if rows != self.rows:
+            raise ValueError(f"pos: {self.rows} rows, the call has {rows}")
+        if self.pairs is not None and 2 * self.pairs != cache.c.rot_dim:
+            raise ValueError(f"axis_of: {self.pairs} pairs, the cache rotates {cache.c.rot_dim // 2}")
+        return self.ref
+
+
+class Marks(_Buffers):
+    """The marks of a cache's rows (cc_marks), [pages, kv heads, 64] each in
+    device memory: weight f32, the attention that a row has gathered, and token
+    int32, its token's number in the chat."""
+
+    def __init__(self, weight, token):
+        super().__init__()
+        self.shape = tuple(weight.shape)
+        if len(self.shape) != 3 or self.shape[2] != 64:
+            raise ValueError(f"weight: [pages, kv heads, 64], not {self.shape}")
+        self.c = CMarks(weight=self.take(weight, "weight", ("float32",), self.shape, False),
+                        token=self.take(token, "token", ("int32",), self.shape, False))
+        self.ref = C.byref(self.c)
+
+    def fit(self, cache):
+        if self.shape[:2] != (cache.c.n_pages, cache.c.n_kv_heads):
+            raise ValueError(f"marks of {self.shape[:2]} blocks, the cache has {(cache.c.n_pages, cache.c.n_kv_heads)}")
+        return self.ref
+
+
 class Sampling(_Buffers):
     """What the rows of a call ask for (cc_sampling): device arrays, None where
     no row asks for it. temp, top_p, min_p, rep, freq, pres f32 [rows]; top_k
@@ -396,20 +461,26 @@ class Sampling(_Buffers):
         self.ref, self.workspace = C.byref(self.c), None
 
 
-def _job_rows(jobs):
-    """(slot, past, n) of each job as int32 [jobs, 3], its address, and the rows they hold."""
-    a = np.asarray(jobs)
+def _int32s(a, name, width=None):
+    """`a` as a contiguous int32 array [n], or [n, the names of `width`], and its address."""
+    a = np.asarray(a)
     if a.dtype != np.int32:
         if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
-            raise ValueError("jobs: 32-bit integers (slot, past, n)")
+            raise ValueError(f"{name}: 32-bit integers {width or ''}".rstrip())
         a = a.astype(np.int32)
-    if a.ndim != 2 or a.shape[1] != 3:
-        raise ValueError("jobs: one (slot, past, n) each")
+    if a.ndim != (2 if width else 1) or (width and a.shape[1] != width.count(",") + 1):
+        raise ValueError(f"{name}: one {width or 'number'} each")
     if not a.flags.c_contiguous:
         a = np.ascontiguousarray(a)
+    return a, a.__array_interface__["data"][0]
+
+
+def _job_rows(jobs):
+    """(slot, past, n) of each job as int32 [jobs, 3], its address, and the rows they hold."""
+    a, at = _int32s(jobs, "jobs", "(slot, past, n)")
     n = len(a)
     rows = int(a[0, 2]) if n == 1 else int(np.add.reduce(a[:, 2], dtype=np.int64))
-    return a, a.__array_interface__["data"][0], n, rows
+    return a, at, n, rows
 
 
 def layer_kinds(d):
@@ -769,6 +840,82 @@ class Context:
         if st:
             self._chk(st)
         return out
+
+    def _beside(self, stream, cache, t, *others):
+        """Positions and marks beside a call's rows t: on the context's GPU, and where torch's meet arrays that are not, on a
+        stream that was given (_on's reason)."""
+        for x in others:
+            if x is None:
+                continue
+            if x.device is not None and x.device != self.opts.device:
+                raise ValueError(f"buffers on GPU {x.device}, not on the context's ({self.opts.device})")
+            if x.torch and stream is None and not _is_torch(t):
+                raise ValueError("torch tensors beside arrays that are not torch's: the call's stream must be given")
+
+    def kv_append_at(self, cache, jobs, k, v, positions=None, marks=None, first=None, stream=None):
+        """cc_kv_append_at: kv_append's rows, k rotated to `positions`
+        (Positions; None: the rows' indices). marks (Marks): the rows' weights
+        become 0, their tokens first[job] and on (`first` None: past)."""
+        stream = self._on(stream, cache, k, v)
+        self._beside(stream, cache, k, positions, marks)
+        a, at, n, rows = _job_rows(jobs)
+        kp, ldk = self._rows(k, "k", rows, cache.width)
+        vp, ldv = self._rows(v, "v", rows, cache.width)
+        fa, fp = (None, None) if first is None else _int32s(first, "first")
+        if fa is not None and len(fa) != n:
+            raise ValueError(f"first: {len(fa)} numbers for {n} jobs")
+        st = self.lib.cc_kv_append_at(self.h, cache.ref, None if positions is None else positions.fit(cache, rows),
+                                      None if marks is None else marks.fit(cache), at, n, fp, kp, ldk, vp, ldv, stream)
+        if st:
+            self._chk(st)
+
+    def attend_weigh(self, cache, jobs, q, positions=None, marks=None, observe=None, fade=1.0, out=None, stream=None):
+        """cc_attend_weigh: attention of the jobs' rows, q f32 [rows, heads * D]
+        before RoPE, at `positions` (Positions; None: their indices), over all
+        rows of their slots up to their own. marks (Marks): the slots' weights
+        become fade times what they were, plus what each row receives from a
+        job's last `observe` rows (None: all). Returns the rows' output (`out`,
+        or a new array)."""
+        given, stream = stream, self._on(stream, cache, q, out)
+        self._beside(stream, cache, q, positions, marks)
+        a, at, n, rows = _job_rows(jobs)
+        qp, ldq = self._rows(q, "q", rows, None)
+        D, width = cache.c.head_dim, int(q.shape[1])
+        heads = width // D
+        if heads * D != width:
+            raise ValueError(f"q: rows of {width} values are not whole heads of {D}")
+        pr = None if positions is None else positions.fit(cache, rows)
+        mr = None if marks is None else marks.fit(cache)
+        observe = 0 if marks is None else 2**31 - 1 if observe is None else int(observe)
+        if out is None:
+            out = self._new(q, (rows, width), "float32", given)
+            op, ldo = out.data_ptr(), width
+        else:
+            op, ldo = self._rows(out, "out", rows, width)
+        need = self.lib.cc_weigh_workspace(self.h, cache.ref, at, n, heads, observe)
+        if not need:
+            raise CCError(CC_EARG, self.lib.cc_last_error(self.h).decode())
+        ws = self._new(q, (need,), "uint8", given)
+        st = self.lib.cc_attend_weigh(self.h, cache.ref, pr, mr, at, n, heads, observe, fade, qp, ldq, op, ldo,
+                                      ws.data_ptr(), need, stream)
+        if st:
+            self._chk(st)
+        return out
+
+    def kv_evict(self, cache, marks, jobs, sink=0, recent=0, stream=None):
+        """cc_kv_evict: of each job's (slot, rows, keep, seen) rows every kv head
+        keeps `keep`: those of the chat's first `sink` and latest `recent` of
+        its `seen` tokens, then those with the largest weight."""
+        like = marks.kept[0]
+        given, stream = stream, self._on(stream, cache, like)
+        self._beside(stream, cache, like, marks)
+        a, at = _int32s(jobs, "jobs", "(slot, rows, keep, seen)")
+        mr = marks.fit(cache)
+        need = self.lib.cc_evict_workspace(cache.ref, at, len(a))
+        ws = self._new(like, (need,), "uint8", given) if need else None
+        st = self.lib.cc_kv_evict(self.h, cache.ref, mr, at, len(a), sink, recent, ws.data_ptr() if need else None, need, stream)
+        if st:
+            self._chk(st)
 
     def adjust_logits(self, logits, sampling, out=None, stream=None):
         """cc_logits_adjust: the rows with penalties, biases and masks, in `out`

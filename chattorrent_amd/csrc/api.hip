@@ -2269,21 +2269,24 @@ cc_status cache_dev(cc_ctx* ctx, const cc_cache* c, CacheDev& d) {
     d.rot = c->rot_dim;
     d.n_pages = c->n_pages;
     d.max_pages = c->max_pages;
+    d.rope_rows = c->rope_rows;
     d.blk = 64 * d.D + 64 * d.ng * 4;
     d.bblk = (int)cc_bounds_bytes(c);
     return CC_OK;
 }
 
-cc_status check_rows(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t njobs, int64_t* rows, bool once) {
+// placed: the rows' positions are given, and need not lie within the rope table.
+cc_status check_rows(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t njobs, int64_t* rows, bool once,
+                     bool placed = false) {
     if (!jobs || njobs < 1) return fail(ctx, CC_EARG, "jobs: at least one");
-    const int64_t cap = std::min((int64_t)c->max_pages * 64, (int64_t)c->rope_rows);
+    const int64_t cap = placed ? (int64_t)c->max_pages * 64 : std::min((int64_t)c->max_pages * 64, (int64_t)c->rope_rows);
     std::vector<bool> seen(once ? (size_t)c->slots : 0, false);
     *rows = 0;
     for (int j = 0; j < njobs; j++) {
         const cc_rows& r = jobs[j];
         if (r.slot < 0 || r.slot >= c->slots || r.past < 0 || r.n < 1 || (int64_t)r.past + r.n > cap)
             return fail(ctx, CC_EARG, "job " + std::to_string(j) + ": slot within the cache, past >= 0, n >= 1 and past + n at most " +
-                                          std::to_string(cap) + " (the slot's pages and the rope table)");
+                                          std::to_string(cap) + (placed ? " (the slot's pages)" : " (the slot's pages and the rope table)"));
         if (once) {
             if (seen[r.slot]) return fail(ctx, CC_EARG, "slot " + std::to_string(r.slot) + " twice in one call");
             seen[r.slot] = true;
@@ -2385,6 +2388,162 @@ cc_status attend_shape(cc_ctx* ctx, const cc_cache* c, int64_t rows, int32_t n_h
         return fail(ctx, CC_EARG, "attend: at most 1024 tiles of 16 query heads of a kv head");
     if (budget < 1) return fail(ctx, CC_EARG, "budget must be at least one page");
     return CC_OK;
+}
+
+cc_status axes_dev(cc_ctx* ctx, const cc_cache* c, const cc_positions* at, AxesDev& d) {
+    if (!at) return CC_OK;
+    if (at->n_axes < 1 || at->n_axes > 4) return fail(ctx, CC_EARG, "positions: 1 .. 4 axes");
+    if (!at->pos || !is_aligned(at->pos, 4)) return fail(ctx, CC_EARG, "positions: pos must be set, 4-byte aligned");
+    d.pos = at->pos;
+    d.n = at->n_axes;
+    for (int j = 0; at->axis_of && j < c->rot_dim / 2; j++) {
+        if (at->axis_of[j] >= at->n_axes) return fail(ctx, CC_EARG, "positions: axis_of[" + std::to_string(j) + "] is not below n_axes");
+        d.of[j >> 4] |= (uint32_t)at->axis_of[j] << (2 * (j & 15));
+    }
+    return CC_OK;
+}
+
+cc_status marks_dev(cc_ctx* ctx, const cc_marks* m, MarksDev& d) {
+    if (!m) return CC_OK;
+    if (!m->weight || !m->token || !is_aligned(m->weight, 16) || !is_aligned(m->token, 16))
+        return fail(ctx, CC_EARG, "marks: weight and token must be set, 16-byte aligned");
+    d.weight = m->weight;
+    d.token = m->token;
+    return CC_OK;
+}
+
+// A call of cc_attend_weigh as launches: jobs of at most 16 columns (rows *
+// query heads of a kv head) and the others apart, and a job of many rows in
+// pieces of its rows. f(jobs, plan, few) launches; the result is the workspace
+// that the largest launch takes. `per`, the pages of an attention workgroup, is
+// such that a launch has some `want` workgroups, and no job over 128 splits.
+constexpr int WEIGH_ROWS = 4096;              // rows of a piece, of up to 2048 heads
+constexpr int64_t WEIGH_UNITS = 1 << 20, WEIGH_PAGES = 1 << 24;   // of a launch with several jobs
+int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+template <class F>
+size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t njobs, int n_heads, int observe, bool weigh,
+                  F&& f) {
+    const int G = n_heads / c->n_kv_heads, D = c->head_dim;
+    const int64_t nkv = c->n_kv_heads;
+    size_t most = 0;
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    for (int pass = 0; pass < 2; pass++) {
+        const bool few = pass == 0;
+        WeighJobs b;
+        auto flush = [&]() {
+            if (!b.n) return true;
+            WeighPlan p;
+            p.group = G;
+            p.subs = 1;
+            p.weigh = weigh;
+            int64_t work = 0;
+            int longest = 0;
+            for (int j = 0; j < b.n; j++) {
+                const int pages = (b.j[j].past + b.j[j].n - 1) / 64 + 1, tiles = ceil_div(b.j[j].n * G, 16);
+                work += nkv * tiles * pages;
+                longest = std::max(longest, pages);
+                if (few) p.score_cols = std::max(p.score_cols, b.j[j].n * G);
+            }
+            const int64_t want = 4 * (int64_t)ctx->ncu;
+            int64_t per = std::max<int64_t>({4, ceil_div64(work, want), ceil_div(longest, 128)});
+            p.per = (int)std::min<int64_t>(256, per);
+            int64_t units = 0, joins = 0, pages_ = 0;
+            for (int j = 0; j < b.n; j++) {
+                WeighJob& w = b.j[j];
+                const int pages = (w.past + w.n - 1) / 64 + 1, tiles = ceil_div(w.n * G, 16);
+                w.unit0 = (int)units;
+                w.join0 = (int)joins;
+                w.page0 = (int)pages_;
+                units += nkv * tiles * ceil_div(pages, p.per);
+                joins += nkv * tiles;
+                pages_ += nkv * ceil_div(pages, 8) * 8;
+            }
+            b.units = (int)units;
+            b.joins = (int)joins;
+            b.pages = weigh ? (int)pages_ : 0;
+            if (!weigh) p.score_cols = 0;
+            p.ml = 0;
+            p.parts = up((size_t)units * 16 * 8);
+            p.scores = p.parts + up((size_t)units * 16 * D * 4);
+            p.q = p.scores + up(few ? (size_t)b.pages * p.score_cols * 256 : 0);
+            p.qs = p.q + up(few ? 0 : (size_t)joins * 16 * D * 4);
+            p.bytes = p.qs + up(few ? 0 : (size_t)joins * 64);
+            most = std::max(most, p.bytes);
+            const bool ok = f(b, p, few);
+            b.n = 0;
+            return ok;
+        };
+        int64_t row0 = 0, units = 0, pages = 0;
+        const int most_rows = std::min(WEIGH_ROWS, (1 << 23) / n_heads);
+        for (int j = 0; j < njobs; j++) {
+            const cc_rows& r = jobs[j];
+            const bool is_few = (int64_t)r.n * G <= 16;
+            if (is_few == few) {
+                int fresh = 0;
+                for (int i = 0; i < r.n;) {
+                    const int n = std::min(r.n - i, most_rows), seen = (r.past + i + n - 1) / 64 + 1;
+                    const int64_t u = nkv * ceil_div64((int64_t)n * G, 16) * std::min(128, seen), pg = nkv * (seen + 8);
+                    // (the pieces of a job add to the same weights: each in a launch of its own)
+                    if (b.n == WEIGH_JOBS || i > 0 || (b.n && (units + u > WEIGH_UNITS || pages + pg > WEIGH_PAGES))) {
+                        if (!flush()) return most;
+                        units = pages = 0;
+                    }
+                    units += u;
+                    pages += pg;
+                    const int count0 = (int)std::max<int64_t>(0, std::min<int64_t>(n, (int64_t)r.n - observe - i));
+                    b.j[b.n++] = WeighJob{r.slot, r.past + i, n, (int32_t)(row0 + i), count0, fresh, 0, 0, 0};
+                    if (count0 < n) fresh = r.past + i + n;
+                    i += n;
+                }
+            }
+            row0 += r.n;
+        }
+        if (!flush()) return most;
+    }
+    return most;
+}
+
+cc_status check_keeps(cc_ctx* ctx, const cc_cache* c, const cc_keep* jobs, int32_t njobs) {
+    if (!jobs || njobs < 1) return fail(ctx, CC_EARG, "jobs: at least one");
+    std::vector<bool> seen((size_t)c->slots, false);
+    for (int j = 0; j < njobs; j++) {
+        const cc_keep& k = jobs[j];
+        if (k.slot < 0 || k.slot >= c->slots || k.rows < 0 || (int64_t)k.rows > (int64_t)c->max_pages * 64 || k.keep < 1 || k.seen < 0)
+            return fail(ctx, CC_EARG, "job " + std::to_string(j) + ": slot within the cache, rows 0 .. " +
+                                          std::to_string((int64_t)c->max_pages * 64) + ", keep >= 1 and seen >= 0");
+        if (seen[k.slot]) return fail(ctx, CC_EARG, "slot " + std::to_string(k.slot) + " twice in one call");
+        seen[k.slot] = true;
+    }
+    return CC_OK;
+}
+
+// The jobs of cc_kv_evict that have rows to give up, in launches whose lists of
+// moves each have a place of their own. f(jobs, most rows) launches.
+template <class F>
+size_t each_evict(const cc_cache* c, const cc_keep* jobs, int32_t njobs, F&& f) {
+    size_t most = 0;
+    EvictJobs b;
+    int64_t words = 0;
+    int max_rows = 0;
+    auto flush = [&]() {
+        const bool ok = !b.n || f(b, max_rows);
+        b.n = b.room = max_rows = 0;
+        words = 0;
+        return ok;
+    };
+    for (int j = 0; j < njobs; j++) {
+        const cc_keep& k = jobs[j];
+        if (k.rows <= k.keep) continue;
+        const int room = std::min(k.rows - k.keep, k.keep);
+        if ((b.n == EVICT_JOBS || (int64_t)(b.n + 1) * c->n_kv_heads > 65535) && !flush()) return most;
+        b.j[b.n++] = EvictJob{k.slot, k.rows, k.keep, k.seen, room, words};
+        b.room = std::max(b.room, room);
+        max_rows = std::max(max_rows, k.rows);
+        if (room > EVICT_HERE) words += (int64_t)c->n_kv_heads * (2 * (int64_t)room + 2);
+        most = std::max(most, (size_t)words * 4);
+    }
+    flush();
+    return most;
 }
 
 cc_status sampling_dev(cc_ctx* ctx, const cc_sampling* s, int64_t vocab, SamplingDev& d) {
@@ -2538,6 +2697,131 @@ cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* job
             p.recent = recent;
             return launch_attend_pages(s, c, b, p, q, ldq, out, ldo, (uint8_t*)workspace);
         }));
+    });
+}
+
+cc_status cc_kv_append_at(cc_ctx* ctx, const cc_cache* cache, const cc_positions* at, const cc_marks* marks,
+                          const cc_rows* jobs, int32_t njobs, const int32_t* first, const float* k, int64_t ldk,
+                          const float* v, int64_t ldv, void* stream) {
+    if (!ctx) return CC_EARG;
+    if (!cache || !k || !v) return fail(ctx, CC_EARG, "append: cache, k and v must be set");
+    return guarded(ctx, [&]() -> cc_status {
+        CacheDev c;
+        AppendAt a;
+        cc_status st = cache_dev(ctx, cache, c);
+        if (st == CC_OK) st = axes_dev(ctx, cache, at, a.axes);
+        if (st == CC_OK) st = marks_dev(ctx, marks, a.marks);
+        if (st != CC_OK) return st;
+        int64_t rows = 0;
+        st = check_rows(ctx, cache, jobs, njobs, &rows, true, at != nullptr);
+        if (st != CC_OK) return st;
+        for (int j = 0; first && j < njobs; j++)
+            if (first[j] < 0 || (int64_t)first[j] + jobs[j].n > INT32_MAX)
+                return fail(ctx, CC_EARG, "append: token numbers (first + n) from 0 to 2^31 - 1");
+        const int64_t width = (int64_t)c.nKV * c.D;
+        if (ldk < width || ldv < width) return fail(ctx, CC_EARG, "append: ldk and ldv are at least n_kv_heads * head_dim");
+        if (rows > (1 << 30)) return fail(ctx, CC_EARG, "append: too many rows in one call");
+        const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+        int next = 0;   // every job has work, so a launch's jobs are the call's next ones
+        return launched(ctx, "append", each_batch(jobs, njobs, OP_BLOCKS / 4,
+            [](const cc_rows& r) { return (int64_t)(r.past + r.n - 1) / 64 - r.past / 64 + 1; },
+            [&](const OpJobs& b) {
+                for (int j = 0; j < b.n; j++, next++) a.first[j] = first ? first[next] : jobs[next].past;
+                return launch_kv_append_at(s, c, b, a, k, ldk, v, ldv);
+            }));
+    });
+}
+
+size_t cc_weigh_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
+                          int32_t observe) {
+    if (!ctx || !cache) return 0;
+    try {
+        CacheDev c;
+        int64_t rows = 0;
+        if (cache_dev(ctx, cache, c) != CC_OK || check_rows(ctx, cache, jobs, njobs, &rows, true, true) != CC_OK ||
+            attend_shape(ctx, cache, rows, n_heads, 1) != CC_OK)
+            return 0;
+        if (observe < 0) {
+            (void)fail(ctx, CC_EARG, "weigh: observe must not be negative");
+            return 0;
+        }
+        return each_weigh(ctx, cache, jobs, njobs, n_heads, observe, observe > 0,
+                          [](const WeighJobs&, const WeighPlan&, bool) { return true; });
+    } catch (...) {
+        return 0;
+    }
+}
+
+cc_status cc_attend_weigh(cc_ctx* ctx, const cc_cache* cache, const cc_positions* at, const cc_marks* marks,
+                          const cc_rows* jobs, int32_t njobs, int32_t n_heads, int32_t observe, float fade, const float* q,
+                          int64_t ldq, float* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!ctx) return CC_EARG;
+    if (!cache || !q || !out) return fail(ctx, CC_EARG, "weigh: cache, q and out must be set");
+    return guarded(ctx, [&]() -> cc_status {
+        CacheDev c;
+        AxesDev axes;
+        MarksDev m;
+        cc_status st = cache_dev(ctx, cache, c);
+        if (st == CC_OK) st = axes_dev(ctx, cache, at, axes);
+        if (st == CC_OK) st = marks_dev(ctx, marks, m);
+        if (st != CC_OK) return st;
+        int64_t rows = 0;
+        st = check_rows(ctx, cache, jobs, njobs, &rows, true, at != nullptr);
+        if (st == CC_OK) st = attend_shape(ctx, cache, rows, n_heads, 1);
+        if (st != CC_OK) return st;
+        if (observe < 0) return fail(ctx, CC_EARG, "weigh: observe must not be negative");
+        if (!(fade >= 0.0f && fade <= 1.0f)) return fail(ctx, CC_EARG, "weigh: fade is 0 .. 1");
+        const int64_t width = (int64_t)n_heads * c.D;
+        if (ldq < width || ldo < width) return fail(ctx, CC_EARG, "weigh: ldq and ldo are at least n_heads * head_dim");
+        if (rows_meet(q, ldq, out, ldo, rows, width)) return fail(ctx, CC_EARG, "weigh: out must not share memory with q");
+        const bool weigh = m.weight && observe > 0;
+        const size_t need = each_weigh(ctx, cache, jobs, njobs, n_heads, observe, weigh,
+                                       [](const WeighJobs&, const WeighPlan&, bool) { return true; });
+        if (!workspace || workspace_bytes < need || !is_aligned(workspace, 16))
+            return fail(ctx, CC_EARG, "weigh: a workspace of " + std::to_string(need) + " bytes, 16-byte aligned");
+        const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+        hipError_t e = hipSuccess;
+        each_weigh(ctx, cache, jobs, njobs, n_heads, observe, weigh, [&](const WeighJobs& b, const WeighPlan& plan, bool few) {
+            WeighPlan p = plan;
+            p.fade = fade;
+            e = launch_weigh(s, c, b, p, few, axes, m, q, ldq, out, ldo, (uint8_t*)workspace);
+            return e == hipSuccess;
+        });
+        return launched(ctx, "weigh", e);
+    });
+}
+
+size_t cc_evict_workspace(const cc_cache* cache, const cc_keep* jobs, int32_t njobs) {
+    if (!cache || !jobs || cache->n_kv_heads < 1 || cache->n_kv_heads > 1024) return 0;
+    try {
+        return each_evict(cache, jobs, njobs, [](const EvictJobs&, int) { return true; });
+    } catch (...) {
+        return 0;
+    }
+}
+
+cc_status cc_kv_evict(cc_ctx* ctx, const cc_cache* cache, const cc_marks* marks, const cc_keep* jobs, int32_t njobs,
+                      int32_t sink, int32_t recent, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!ctx) return CC_EARG;
+    if (!cache || !marks) return fail(ctx, CC_EARG, "evict: cache and marks must be set");
+    return guarded(ctx, [&]() -> cc_status {
+        CacheDev c;
+        MarksDev m;
+        cc_status st = cache_dev(ctx, cache, c);
+        if (st == CC_OK) st = marks_dev(ctx, marks, m);
+        if (st == CC_OK) st = check_keeps(ctx, cache, jobs, njobs);
+        if (st != CC_OK) return st;
+        if (sink < 0 || recent < 0) return fail(ctx, CC_EARG, "evict: sink and recent must not be negative");
+        const size_t need = cc_evict_workspace(cache, jobs, njobs);
+        if (need && (!workspace || workspace_bytes < need || !is_aligned(workspace, 16)))
+            return fail(ctx, CC_EARG, "evict: a workspace of " + std::to_string(need) + " bytes, 16-byte aligned");
+        const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
+        hipError_t e = hipSuccess;
+        each_evict(cache, jobs, njobs, [&](const EvictJobs& b, int max_rows) {
+            e = launch_evict(s, c, b, max_rows, m, sink, recent, (uint8_t*)workspace);
+            return e == hipSuccess;
+        });
+        return launched(ctx, "evict", e);
     });
 }
 

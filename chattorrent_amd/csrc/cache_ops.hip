@@ -2,23 +2,8 @@
 // with the key bounds of the pages they complete, and attention over the pages
 // that a cheap score selects. The cache is laid out as the pass lays its own
 // out (common.h, KV geometry), so they run on a context's cache as well.
-#include "common.h"
-#include "ops.h"
+#include "cache_dev.h"
 #include <algorithm>
-
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
-
-// The job that holds unit u (uniform: u comes from the block's index).
-__device__ static inline OpJob job_of(const OpJobs& jobs, int u) {
-    int lo = 0, hi = jobs.n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (jobs.j[mid].first <= u) lo = mid;
-        else hi = mid;
-    }
-    return jobs.j[lo];
-}
 
 // ================================================================= append ===
 // Rows of keys and values into their pages, and key bounds.
@@ -49,50 +34,17 @@ __device__ static inline void bound_code(float mx, float mn, float B, int8_t& hi
     lo = (int8_t)(int)fminf(fmaxf(floorf(mn / B), -127.0f), 127.0f);
 }
 
-// Channels d0 .. d0 + 7 of one head of a row x, rotated with the position's
-// (cos, sin) pairs cs: the f32 steps of rope_cs (rot 0: as they are). vec: x
-// is 16-byte aligned at groups of 4 channels, as is cs, and RoPE's halves are
-// whole groups of 8.
-__device__ static inline void rotated8(const float* __restrict__ x, int d0, const float* __restrict__ cs, int rot,
-                                       bool vec, float (&r)[8]) {
-    const int half = rot >> 1;
-    if (vec) {
-        const float4 a = *(const float4*)(x + d0), b = *(const float4*)(x + d0 + 4);
-        r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
-        r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
-        if (d0 < rot) {
-            const bool low = d0 < half;
-            const float* y = x + d0 + (low ? half : -half);
-            const float4 ya = *(const float4*)y, yb = *(const float4*)(y + 4);
-            const float o[8] = {ya.x, ya.y, ya.z, ya.w, yb.x, yb.y, yb.z, yb.w};
-            const float4* t = (const float4*)(cs + 2 * (d0 - (low ? 0 : half)));
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float4 c = t[e >> 1];
-                r[e] = low ? r[e] * c.x - o[e] * c.y : r[e] * c.x + o[e] * c.y;
-                r[e + 1] = low ? r[e + 1] * c.z - o[e + 1] * c.w : r[e + 1] * c.z + o[e + 1] * c.w;
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const int d = d0 + e;
-        r[e] = x[d];
-        if (d < rot) {
-            const float* t = cs + 2 * (d < half ? d : d - half);
-            const float o = x[d < half ? d + half : d - half];
-            r[e] = d < half ? r[e] * t[0] - o * t[1] : r[e] * t[0] + o * t[1];
-        }
-    }
-}
-
-template <int D, bool VEC>
-__global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, const float* __restrict__ k, int64_t ldk,
-                                                   const float* __restrict__ v, int64_t ldv, int only) {
+//
+// AT: the rows' positions are not their indices but given, each pair of
+// channels turning by its own axis's (AxesDev), and each row gets its mark: no
+// weight yet, and its token's number.
+template <int D, bool VEC, bool AT>
+__device__ static inline void append_rows(const CacheDev& c, const OpJobs& jobs, const float* __restrict__ k, int64_t ldk,
+                                          const float* __restrict__ v, int64_t ldv, int only, const AppendAt* at) {
     constexpr int G8 = D / 8, RPW = 64 / G8, NG = D / 32;
     __shared__ float red[2][4][D];
-    const OpJob jb = job_of(jobs, blockIdx.x);
+    const int ji = job_at(jobs, blockIdx.x);
+    const OpJob jb = jobs.j[ji];
     const int head = blockIdx.y, which = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // bounds alone (`only`): the job's whole pages, each with 64 rows that were there before
@@ -101,6 +53,11 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
     const uint32_t page = c.page_table[(size_t)jb.slot * c.max_pages + p];
     if (page >= (uint32_t)c.n_pages) return;
     uint8_t* blk = (which ? c.v : c.k) + ((size_t)page * c.nKV + head) * c.blk;
+    if (AT && which == 0 && at->marks.weight && (int)threadIdx.x >= s0 && (int)threadIdx.x < s1) {
+        const size_t m = ((size_t)page * c.nKV + head) * 64 + threadIdx.x;
+        at->marks.weight[m] = 0.0f;
+        at->marks.token[m] = at->first[ji] + 64 * p + (int)threadIdx.x - jb.past;
+    }
     const int g = lane & (G8 - 1), rr = lane / G8;
     const bool bounds = which == 0 && c.bounds != nullptr && s1 == 64;
     float mx[8], mn[8];
@@ -159,7 +116,9 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
         const bool live = s < s1;
         const int pos = 64 * p + (live ? s : s0);
         float r[8];
-        rotated8(src + (jb.row0 + pos - jb.past) * ld, 8 * g, c.rope + (size_t)pos * c.rot, which == 0 ? c.rot : 0, VEC, r);
+        const int64_t row = jb.row0 + pos - jb.past;
+        if (AT && which == 0 && at->axes.pos) rotated8_at(src + row * ld, 8 * g, c, at->axes, row, VEC, r);
+        else rotated8(src + row * ld, 8 * g, c.rope + (size_t)pos * c.rot, which == 0 ? c.rot : 0, VEC, r);
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(r[e]));
@@ -227,21 +186,50 @@ __global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, cons
     if ((g & 3) == 0) *(float*)(b + c.nKV * 2 * D + (head * NG + (g >> 2)) * 4) = B;
 }
 
+template <int D, bool VEC>
+__global__ __launch_bounds__(256) void k_kv_append(CacheDev c, OpJobs jobs, const float* __restrict__ k, int64_t ldk,
+                                                   const float* __restrict__ v, int64_t ldv, int only) {
+    append_rows<D, VEC, false>(c, jobs, k, ldk, v, ldv, only, nullptr);
+}
+template <int D, bool VEC>
+__global__ __launch_bounds__(256) void k_kv_append_at(CacheDev c, OpJobs jobs, const float* __restrict__ k, int64_t ldk,
+                                                      const float* __restrict__ v, int64_t ldv, AppendAt at) {
+    append_rows<D, VEC, true>(c, jobs, k, ldk, v, ldv, 0, &at);
+}
+
 template <int D>
 static hipError_t append_d(hipStream_t st, dim3 grid, bool vec, const CacheDev& c, const OpJobs& jobs, const float* k,
                            int64_t ldk, const float* v, int64_t ldv, int only) {
     return op_launch(vec ? k_kv_append<D, true> : k_kv_append<D, false>, grid, dim3(256), st, c, jobs, k, ldk, v, ldv, only);
 }
 
-static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+static bool append_vec(const CacheDev& c, const float* k, int64_t ldk, const float* v, int64_t ldv) {
+    return aligned16(k) && aligned16(v) && aligned16(c.rope) && ldk % 4 == 0 && ldv % 4 == 0 && c.rot % 16 == 0;
+}
 
 hipError_t launch_kv_append(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const float* k, int64_t ldk,
                             const float* v, int64_t ldv) {
-    const bool vec = aligned16(k) && aligned16(v) && aligned16(c.rope) && ldk % 4 == 0 && ldv % 4 == 0 && c.rot % 16 == 0;
+    const bool vec = append_vec(c, k, ldk, v, ldv);
     const dim3 grid(jobs.units, c.nKV, 2);
     if (c.D == 64) return append_d<64>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
     if (c.D == 128) return append_d<128>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
     return append_d<256>(st, grid, vec, c, jobs, k, ldk, v, ldv, 0);
+}
+
+template <int D>
+static hipError_t append_at_d(hipStream_t st, dim3 grid, bool vec, const CacheDev& c, const OpJobs& jobs, const AppendAt& at,
+                              const float* k, int64_t ldk, const float* v, int64_t ldv) {
+    return op_launch(vec ? k_kv_append_at<D, true> : k_kv_append_at<D, false>, grid, dim3(256), st, c, jobs, k, ldk, v, ldv,
+                     at);
+}
+
+hipError_t launch_kv_append_at(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AppendAt& at, const float* k,
+                               int64_t ldk, const float* v, int64_t ldv) {
+    const bool vec = append_vec(c, k, ldk, v, ldv);
+    const dim3 grid(jobs.units, c.nKV, 2);
+    if (c.D == 64) return append_at_d<64>(st, grid, vec, c, jobs, at, k, ldk, v, ldv);
+    if (c.D == 128) return append_at_d<128>(st, grid, vec, c, jobs, at, k, ldk, v, ldv);
+    return append_at_d<256>(st, grid, vec, c, jobs, at, k, ldk, v, ldv);
 }
 
 hipError_t launch_kv_bounds(hipStream_t st, const CacheDev& c, const OpJobs& jobs) {
@@ -252,30 +240,6 @@ hipError_t launch_kv_bounds(hipStream_t st, const CacheDev& c, const OpJobs& job
 }
 
 // ========================================================== selected pages ===
-// Order-preserving bits of an f32.
-__device__ static inline uint32_t order_bits(float v) {
-    const uint32_t b = f2u(v);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-
-// A workgroup's unit of work: part `part` of a row and head. Workgroups go
-// round the eight XCDs in launch order, each with its own L2, so an XCD gets
-// a run of the units in (head, row, part) order: the rows of a job, which
-// read the same bounds and many of the same pages, meet in one L2. row < 0: none.
-struct OpWork {
-    int row, head, part;
-};
-__device__ static inline OpWork op_work(int rows, int heads, int parts) {
-    const int per = (int)gridDim.x >> 3, w = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
-    OpWork o{-1, 0, 0};
-    if (w >= rows * heads * parts) return o;
-    o.part = w % parts;
-    o.row = (w / parts) % rows;
-    o.head = w / parts / rows;
-    return o;
-}
-static int op_blocks(int64_t units) { return (int)((units + 7) / 8 * 8); }
-
 // The score of a page for a row and kv head: an upper bound, in 8 bits, of
 // q . k over the page's keys, the largest over the head's query heads:
 //   sum_b T_b * B_b * (sum_{d in b} qc > 0 ? qc * hi : qc * lo),

@@ -34,7 +34,7 @@ struct CacheDev {
     uint8_t* bounds = nullptr;
     const uint32_t* page_table = nullptr;
     const float* rope = nullptr;
-    int nKV = 0, D = 0, ng = 0, rot = 0, n_pages = 0, max_pages = 0, blk = 0, bblk = 0;
+    int nKV = 0, D = 0, ng = 0, rot = 0, n_pages = 0, max_pages = 0, blk = 0, bblk = 0, rope_rows = 0;
 };
 
 // A launch's jobs, by value in its kernel arguments (no table to upload, and a
@@ -49,9 +49,30 @@ struct OpJobs {
     OpJob j[OP_JOBS];
 };
 
+// cc_positions: positions [rows][n] on n axes (null: a row's index in the
+// cache), and the axis of pair j, two bits each.
+struct AxesDev {
+    const int32_t* pos = nullptr;
+    int32_t n = 1;
+    uint32_t of[8] = {};
+};
+// cc_marks: of each (page, kv head) block's 64 rows.
+struct MarksDev {
+    float* weight = nullptr;
+    int32_t* token = nullptr;
+};
+// What cc_kv_append_at adds; first: the number of each job's first token.
+struct AppendAt {
+    AxesDev axes;
+    MarksDev marks;
+    int32_t first[OP_JOBS];
+};
+
 // units: pages that the jobs' rows touch.
 hipError_t launch_kv_append(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const float* k, int64_t ldk,
                             const float* v, int64_t ldv);
+hipError_t launch_kv_append_at(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AppendAt& at, const float* k,
+                               int64_t ldk, const float* v, int64_t ldv);
 // units: pages that lie in the jobs' rows as a whole.
 hipError_t launch_kv_bounds(hipStream_t st, const CacheDev& c, const OpJobs& jobs);
 
@@ -71,6 +92,48 @@ struct AttendPlan {
 // units: rows.
 hipError_t launch_attend_pages(hipStream_t st, const CacheDev& c, const OpJobs& jobs, const AttendPlan& p,
                                const float* q, int64_t ldq, float* out, int64_t ldo, uint8_t* ws);
+
+// How cc_attend_weigh lays a launch out. A job's columns are its (row, query
+// head of a kv head) pairs, row by row. A unit of attention is a tile of 16 *
+// subs columns of a (job, kv head) over `per` pages; its parts lie in the
+// workspace as [unit][sub] pieces of 16 columns.
+constexpr int WEIGH_JOBS = 64;
+struct WeighJob {
+    int32_t slot, past, n, row0;
+    int32_t count0;   // the first row that counts
+    int32_t fresh;    // the first of the slot's rows whose weights fade in this launch
+    int32_t unit0, join0, page0;   // its first attention unit, output join and (kv head, page)
+};
+struct WeighJobs {
+    int n = 0, units = 0, joins = 0, pages = 0;
+    WeighJob j[WEIGH_JOBS];
+};
+struct WeighPlan {
+    int group = 0, per = 1, subs = 1, score_cols = 0;
+    bool vec = false, weigh = false;
+    float fade = 1.0f;
+    size_t ml = 0, parts = 0, scores = 0, q = 0, qs = 0, bytes = 0;   // offsets into the workspace, and its size
+};
+constexpr int WEIGH_JOIN = 256;   // floats of a unit's output that a workgroup joins
+// few: each job has at most 16 columns.
+hipError_t launch_weigh(hipStream_t st, const CacheDev& c, const WeighJobs& jobs, const WeighPlan& p, bool few,
+                        const AxesDev& axes, const MarksDev& marks, const float* q, int64_t ldq, float* out, int64_t ldo,
+                        uint8_t* ws);
+
+// cc_keep; its list of moves lies in the workspace from moves0 on, for each kv
+// head `room` of them behind a count.
+struct EvictJob {
+    int32_t slot, rows, keep, seen, room;
+    int64_t moves0;
+};
+constexpr int EVICT_JOBS = 96;
+struct EvictJobs {
+    int n = 0, room = 0;   // room: the largest of the jobs
+    EvictJob j[EVICT_JOBS];
+};
+constexpr int EVICT_HERE = 64;   // moves that the workgroup which selects makes itself
+hipError_t launch_evict(hipStream_t st, const CacheDev& c, const EvictJobs& jobs, int max_rows, const MarksDev& marks,
+                        int sink, int recent, uint8_t* ws);
 
 // -------------------------------------------------------- logits, sampling ---
 // cc_sampling with its pointers typed; null: that part is off.

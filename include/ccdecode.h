@@ -396,6 +396,82 @@ cc_status cc_attend_pages(cc_ctx* ctx, const cc_cache* cache, const cc_rows* job
                           int32_t budget, int32_t sink, int32_t recent, const float* q, int64_t ldq, float* out,
                           int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
 
+/* A cache held within a bound: rows whose positions are not their indices,
+ * what attention gives each row of the cache, and giving up the rows that get
+ * the least.
+ *
+ * Positions of the rows of a call, `pos` [rows][n_axes] in device memory, on 1
+ * to 4 axes (time, height and width of an image's patches; text has the same
+ * position on each). Pair j of rotary channels turns by axis axis_of[j]
+ * (rot_dim/2 bytes of HOST memory, read during the call; NULL: the first axis).
+ * A position outside the rope table is taken as the table's nearest. */
+typedef struct cc_positions {
+    int32_t n_axes;
+    const int32_t* pos;
+    const uint8_t* axis_of;
+} cc_positions;
+
+/* The marks of a cache's rows, [n_pages][n_kv_heads][64] each, 16-byte aligned:
+ * the attention weight that a row has gathered, and its token's number in the
+ * chat (0 is the chat's first token). */
+typedef struct cc_marks {
+    float* weight;
+    int32_t* token;
+} cc_marks;
+
+/* cc_kv_append at positions `at` (NULL: each row's index, as there) instead of
+ * the rows' indices: row past + i of a slot may hold any token. Where marks is
+ * given the rows' weights become 0 and their tokens first[j] + i (`first`: host
+ * memory, one of each job; NULL: past). The key bounds of pages that a call
+ * completes are made as there. */
+cc_status cc_kv_append_at(cc_ctx* ctx, const cc_cache* cache, const cc_positions* at, const cc_marks* marks,
+                          const cc_rows* jobs, int32_t njobs, const int32_t* first, const float* k, int64_t ldk,
+                          const float* v, int64_t ldv, void* stream);
+
+/* Attention of the jobs' rows, at positions `at` (NULL: their indices), over
+ * all rows of their slot up to their own: row i of a job sees the rows 0 ..
+ * past + i. q, out, n_heads as in cc_attend_pages. Where marks is given and
+ * observe > 0, the weights w of the slot's rows r = 0 .. past + n - 1 become
+ *   fade * w[r] + the sum over the job's last `observe` rows i that see r, and
+ *   over the query heads of the kv head, of softmax(q_i . k / sqrt(D))[r]
+ * (0 <= fade <= 1; 0: what was there does not matter). One job a slot. The
+ * order of the sums follows from the call's jobs alone: the same call gives the
+ * same bits. A row that sees no row (its pages are outside the cache) gives 0
+ * and adds nothing. An output value's error is relative to the largest finite
+ * |v| of its 32 channels among the rows that the job sees; a row that sees one
+ * that is no finite number has NaN in these 32 channels. `workspace`: cc_weigh_workspace bytes for
+ * the same jobs (0: the call would be refused), 16-byte aligned, of any
+ * contents; two calls that may overlap need two. */
+size_t cc_weigh_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
+                          int32_t observe);
+cc_status cc_attend_weigh(cc_ctx* ctx, const cc_cache* cache, const cc_positions* at, const cc_marks* marks,
+                          const cc_rows* jobs, int32_t njobs, int32_t n_heads, int32_t observe, float fade, const float* q,
+                          int64_t ldq, float* out, int64_t ldo, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Of a slot's `rows` rows each kv head is to keep `keep`, and the slot's chat
+ * has seen `seen` tokens. Host memory, read during the call. */
+typedef struct cc_keep {
+    int32_t slot, rows, keep, seen;
+} cc_keep;
+
+/* Gives up rows - keep rows of each kv head of the jobs' slots (none where rows
+ * <= keep). Kept are the rows whose token is among the chat's first `sink`
+ * (token < sink) or latest `recent` (token >= seen - recent; where these are
+ * more than `keep`, the lower rows of them), then those with the largest
+ * weight, ties to the lower row; a weight that is no number, and a
+ * row whose page is outside the cache, counts least. The rows below `keep` that
+ * stay, stay where they are; in row order, the i-th row from `keep` on that
+ * stays moves to the i-th row below `keep` that goes, with its codes, scales
+ * and marks, and rows from `keep` on are left as they were. So a slot's kv heads
+ * hold different tokens in its rows 0 .. keep - 1, in no order; the pages behind
+ * them are the caller's again. Key bounds are not touched (cc_kv_bounds makes
+ * them anew). 1 <= keep, sink >= 0, recent >= 0; one job a slot. `workspace`:
+ * cc_evict_workspace bytes (may be 0 even for a call that is not refused), as
+ * above. */
+size_t cc_evict_workspace(const cc_cache* cache, const cc_keep* jobs, int32_t njobs);
+cc_status cc_kv_evict(cc_ctx* ctx, const cc_cache* cache, const cc_marks* marks, const cc_keep* jobs, int32_t njobs,
+                      int32_t sink, int32_t recent, void* workspace, size_t workspace_bytes, void* stream);
+
 /* What a call asks of each of its rows: device arrays [rows], or NULL where
  * none asks for it. The meaning is the reference's sampler's
  * (web/model/sampling.js:57-215) with two more cuts, biases and masks, but:
