@@ -2412,14 +2412,45 @@ cc_status marks_dev(cc_ctx* ctx, const cc_marks* m, MarksDev& d) {
     return CC_OK;
 }
 
-// A call of cc_attend_weigh as launches: jobs of at most 16 columns (rows *
-// query heads of a kv head) and the others apart, and a job of many rows in
-// pieces of its rows. f(jobs, plan, few) launches; the result is the workspace
-// that the largest launch takes. `per`, the pages of an attention workgroup, is
-// such that a launch has some `want` workgroups, and no job over 128 splits.
+// A call of cc_attend_weigh as launches: jobs of each kind (WeighKind) apart,
+// and a job of many rows in pieces of its rows. f(jobs, plan, kind) launches;
+// the result is the workspace that the largest launch takes.
 constexpr int WEIGH_ROWS = 4096;              // rows of a piece, of up to 2048 heads
 constexpr int64_t WEIGH_UNITS = 1 << 20, WEIGH_PAGES = 1 << 24;   // of a launch with several jobs
 int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The pages of an attention workgroup. Up to 64 columns: such that there are
+// some eight workgroups for each compute unit. More: the cut of the longest job
+// with the least time, counted in pages that a compute unit, which holds one
+// workgroup, does after another, with two pages' time to begin with.
+int weigh_per(int ncu, const WeighJobs& b, const WeighPlan& p, int64_t nkv, WeighKind kind) {
+    int longest = 0;
+    int64_t work = 0;
+    for (int j = 0; j < b.n; j++) {
+        const int pages = (b.j[j].past + b.j[j].n - 1) / 64 + 1;
+        longest = std::max(longest, pages);
+        work += nkv * ceil_div(b.j[j].n * p.group, 16 * p.subs) * pages;
+    }
+    const int least = std::max(ceil_div(longest, 128), 1);
+    if (kind != WEIGH_WIDE) return (int)std::min<int64_t>(256, std::max<int64_t>({2, ceil_div64(work, 8 * (int64_t)ncu), least}));
+    const int64_t slots = ncu;
+    int best = 0;
+    int64_t cost = 0;
+    for (int cuts = 1; cuts <= 32; cuts++) {
+        const int per = std::min(256, std::max(ceil_div(longest, cuts), least));
+        int64_t units = 0;
+        for (int j = 0; j < b.n; j++)
+            units += nkv * ceil_div(b.j[j].n * p.group, 16 * p.subs) * ceil_div((b.j[j].past + b.j[j].n - 1) / 64 + 1, per);
+        const int64_t t = ceil_div64(units, slots) * (per + 2);
+        if (!best || t < cost) {
+            best = per;
+            cost = t;
+        }
+        if (per == least) break;
+    }
+    return best;
+}
+
 template <class F>
 size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t njobs, int n_heads, int observe, bool weigh,
                   F&& f) {
@@ -2427,49 +2458,49 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
     const int64_t nkv = c->n_kv_heads;
     size_t most = 0;
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    for (int pass = 0; pass < 2; pass++) {
-        const bool few = pass == 0;
+    for (WeighKind kind : {WEIGH_FEW, WEIGH_NARROW, WEIGH_WIDE}) {
+        const int subs = kind == WEIGH_FEW ? 1 : kind == WEIGH_NARROW ? 4 : 8 * weigh_wave_subs(D);
         WeighJobs b;
         auto flush = [&]() {
             if (!b.n) return true;
             WeighPlan p;
             p.group = G;
-            p.subs = 1;
+            p.subs = kind == WEIGH_WIDE ? subs : 1;
+            for (int j = 0; j < b.n && kind == WEIGH_NARROW; j++) p.subs = std::max(p.subs, ceil_div(b.j[j].n * G, 16));
             p.weigh = weigh;
-            int64_t work = 0;
-            int longest = 0;
-            for (int j = 0; j < b.n; j++) {
-                const int pages = (b.j[j].past + b.j[j].n - 1) / 64 + 1, tiles = ceil_div(b.j[j].n * G, 16);
-                work += nkv * tiles * pages;
-                longest = std::max(longest, pages);
-                if (few) p.score_cols = std::max(p.score_cols, b.j[j].n * G);
-            }
-            const int64_t want = 4 * (int64_t)ctx->ncu;
-            int64_t per = std::max<int64_t>({4, ceil_div64(work, want), ceil_div(longest, 128)});
-            p.per = (int)std::min<int64_t>(256, per);
+            for (int j = 0; j < b.n && kind != WEIGH_WIDE && weigh; j++) p.score_cols = std::max(p.score_cols, b.j[j].n * G);
+            p.per = weigh_per(ctx->ncu, b, p, nkv, kind);
             int64_t units = 0, joins = 0, pages_ = 0;
             for (int j = 0; j < b.n; j++) {
                 WeighJob& w = b.j[j];
-                const int pages = (w.past + w.n - 1) / 64 + 1, tiles = ceil_div(w.n * G, 16);
+                const int pages = (w.past + w.n - 1) / 64 + 1, tiles = ceil_div(w.n * G, 16 * p.subs);
                 w.unit0 = (int)units;
                 w.join0 = (int)joins;
                 w.page0 = (int)pages_;
                 units += nkv * tiles * ceil_div(pages, p.per);
-                joins += nkv * tiles;
+                joins += nkv * tiles * p.subs;
                 pages_ += nkv * ceil_div(pages, 8) * 8;
             }
             b.units = (int)units;
             b.joins = (int)joins;
-            b.pages = weigh ? (int)pages_ : 0;
-            if (!weigh) p.score_cols = 0;
-            p.ml = 0;
-            p.parts = up((size_t)units * 16 * 8);
-            p.scores = p.parts + up((size_t)units * 16 * D * 4);
-            p.q = p.scores + up(few ? (size_t)b.pages * p.score_cols * 256 : 0);
-            p.qs = p.q + up(few ? 0 : (size_t)joins * 16 * D * 4);
-            p.bytes = p.qs + up(few ? 0 : (size_t)joins * 64);
+            b.pages = weigh || kind == WEIGH_WIDE ? (int)pages_ : 0;
+            const bool pairs = kind == WEIGH_WIDE;
+            size_t at = 256;   // (offset 0: there is none)
+            auto take = [&](bool some, size_t bytes) {
+                const size_t here = some ? at : 0;
+                if (some) at += up(bytes);
+                return here;
+            };
+            p.ml = take(true, (size_t)units * p.subs * 16 * 8);
+            p.parts = take(true, (size_t)units * p.subs * 16 * D * 4);
+            p.scores = take(p.score_cols > 0, (size_t)b.pages * p.score_cols * 256);
+            p.q = take(true, (size_t)joins * 16 * D * 4);
+            p.qs = take(true, (size_t)joins * 64);
+            p.exps = take(pairs, (size_t)b.pages * 16);
+            p.tot = take(kind == WEIGH_WIDE && weigh, (size_t)joins * 128);
+            p.bytes = at;
             most = std::max(most, p.bytes);
-            const bool ok = f(b, p, few);
+            const bool ok = f(b, p, kind);
             b.n = 0;
             return ok;
         };
@@ -2477,12 +2508,12 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
         const int most_rows = std::min(WEIGH_ROWS, (1 << 23) / n_heads);
         for (int j = 0; j < njobs; j++) {
             const cc_rows& r = jobs[j];
-            const bool is_few = (int64_t)r.n * G <= 16;
-            if (is_few == few) {
+            const int64_t cols = (int64_t)r.n * G;
+            if (kind == (cols <= 16 ? WEIGH_FEW : cols <= 64 ? WEIGH_NARROW : WEIGH_WIDE)) {
                 int fresh = 0;
                 for (int i = 0; i < r.n;) {
                     const int n = std::min(r.n - i, most_rows), seen = (r.past + i + n - 1) / 64 + 1;
-                    const int64_t u = nkv * ceil_div64((int64_t)n * G, 16) * std::min(128, seen), pg = nkv * (seen + 8);
+                    const int64_t u = nkv * ceil_div64((int64_t)n * G, 16 * subs) * std::min(128, seen), pg = nkv * (seen + 8);
                     // (the pieces of a job add to the same weights: each in a launch of its own)
                     if (b.n == WEIGH_JOBS || i > 0 || (b.n && (units + u > WEIGH_UNITS || pages + pg > WEIGH_PAGES))) {
                         if (!flush()) return most;
@@ -2746,7 +2777,7 @@ size_t cc_weigh_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* job
             return 0;
         }
         return each_weigh(ctx, cache, jobs, njobs, n_heads, observe, observe > 0,
-                          [](const WeighJobs&, const WeighPlan&, bool) { return true; });
+                          [](const WeighJobs&, const WeighPlan&, WeighKind) { return true; });
     } catch (...) {
         return 0;
     }
@@ -2776,15 +2807,15 @@ cc_status cc_attend_weigh(cc_ctx* ctx, const cc_cache* cache, const cc_positions
         if (rows_meet(q, ldq, out, ldo, rows, width)) return fail(ctx, CC_EARG, "weigh: out must not share memory with q");
         const bool weigh = m.weight && observe > 0;
         const size_t need = each_weigh(ctx, cache, jobs, njobs, n_heads, observe, weigh,
-                                       [](const WeighJobs&, const WeighPlan&, bool) { return true; });
+                                       [](const WeighJobs&, const WeighPlan&, WeighKind) { return true; });
         if (!workspace || workspace_bytes < need || !is_aligned(workspace, 16))
             return fail(ctx, CC_EARG, "weigh: a workspace of " + std::to_string(need) + " bytes, 16-byte aligned");
         const hipStream_t s = stream ? (hipStream_t)stream : ctx->stream;
         hipError_t e = hipSuccess;
-        each_weigh(ctx, cache, jobs, njobs, n_heads, observe, weigh, [&](const WeighJobs& b, const WeighPlan& plan, bool few) {
+        each_weigh(ctx, cache, jobs, njobs, n_heads, observe, weigh, [&](const WeighJobs& b, const WeighPlan& plan, WeighKind kind) {
             WeighPlan p = plan;
             p.fade = fade;
-            e = launch_weigh(s, c, b, p, few, axes, m, q, ldq, out, ldo, (uint8_t*)workspace);
+            e = launch_weigh(s, c, b, p, kind, axes, m, q, ldq, out, ldo, (uint8_t*)workspace);
             return e == hipSuccess;
         });
         return launched(ctx, "weigh", e);

@@ -9,12 +9,40 @@
 // the rows that a query row sees, out = sum p v / l, and a cache row's weight
 // grows by the sum of p / l over query rows and heads.
 //
-// M need not be the largest score, only near it: it is the largest rounded up
-// to a whole number. So what brings sums from one M to another is a power of
-// two, exactly, and p can be formed 2^14 times as large, in one rounding, for
-// the f16 pairs that enter the P.V product (p to 2^-24 of 2^14 there).
-constexpr float P_SHIFT = 14.0f, P_UNSHIFT = 1.0f / 16384.0f;
+// M need not be the largest score, only near it. It is a whole number, so what
+// brings sums from one M to another is a power of two, exactly, and it stays as
+// it is while no score passes it by more than P_ROOM; then it is the largest
+// score rounded up. p is formed 2^P_SHIFT times as large, in one rounding, at
+// most 2^14, for the f16 pairs that enter the P.V product.
+typedef float4_t float4_a4 __attribute__((aligned(4)));
+constexpr float P_SHIFT = 6.0f, P_ROOM = 8.0f, P_UNSHIFT = 1.0f / 64.0f;
 constexpr float M_LARGE = 1048576.0f;   // beyond: the score is rounded before M is taken off, or the largest may miss it
+
+// The largest of a lane's value and those of the lanes 16, 32 and 48 away.
+__device__ static inline float rows_max(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+    x = fmaxf(u2f(a[0]), u2f(a[1]));
+    a = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+    return fmaxf(u2f(a[0]), u2f(a[1]));
+}
+__device__ static inline uint32_t rows_max(uint32_t x) {
+    auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+    a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(a[0], a[1]);
+}
+// Two values as f16 pairs (split_hilo2's), the remainder in one v_fma_mix each:
+// x - (float)hi, exact.
+__device__ static inline void split_mix2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    asm("" : "+v"(x0), "+v"(x1));
+    const f2_t x = {x0, x1};
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, half2_t));
+    f2_t r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(hi), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(hi), "v"(x1));
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, half2_t));
+}
 
 __device__ static inline float pow2_diff(float a, float b) {   // 2^(a - b) of whole numbers, 0 where a is -inf
     return a == -INFINITY ? 0.0f : ldexpf(1.0f, (int)fmaxf(a - b, -300.0f));
@@ -55,8 +83,13 @@ __device__ static inline bool weigh_unit(const WeighJobs& jobs, const WeighPlan&
     w.tiles = weigh_tiles(w.jb, p);
     w.splits = (w.pages + p.per - 1) / p.per;
     const int r = u - w.jb.unit0;
-    w.split = r % w.splits;
-    w.tile = r / w.splits % w.tiles;
+    if (p.subs > 1) {   // tiles that read the same pages run together
+        w.tile = r % w.tiles;
+        w.split = r / w.tiles % w.splits;
+    } else {
+        w.split = r % w.splits;
+        w.tile = r / w.splits % w.tiles;
+    }
     w.head = r / w.splits / w.tiles;
     return true;
 }
@@ -79,406 +112,41 @@ __device__ static inline float score_scale(int D, int eq) {
     return 1.4426950408889634f / sqrtf((float)D) * u2f((uint32_t)(127 + eq) << 23);
 }
 
-// Attention of a tile of 16 columns over `per` pages, split over four waves. A
-// wave walks its pages as attention over selected pages does (cache_ops.hip):
-// S^T = K . Q^T with the query as an f16 pair, O^T += V^T . (p * s) with p * s
-// as an f16 pair and V scales relative to their page and group's largest power
-// of two; one page of codes in flight. Where p.score_cols is set the scores
-// stay in the workspace, [page][column][64] f32, for k_weigh_finish: 4 bytes a
-// column and token beside the 2 * (D + D/8) that a token's K and V take.
-template <int NG>
-__global__ __launch_bounds__(256, NG > 4 ? 1 : 2) void k_weigh(CacheDev c, WeighJobs jobs, WeighPlan p, AxesDev axes,
-                                                               const float* __restrict__ q, int64_t ldq,
-                                                               float* __restrict__ out, int64_t ldo,
-                                                               uint8_t* __restrict__ ws) {
-    constexpr int D = 32 * NG, DT = D / 16, SCL = NG > 4 ? NG / 4 : 1;
-    constexpr int OW = 16 * D + 32;   // floats of a wave's part: O [16][D], M [16], l [16]
-    __shared__ __align__(16) float smem[4 * OW];
-    WeighUnit w;
-    if (!weigh_unit(jobs, p, w)) return;
-    const WeighJob& jb = w.jb;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j4 = lane >> 4, l16 = lane & 15;
-    const int col0 = w.tile * 16, gt = min(16, jb.n * p.group - col0);
-    const int e0 = w.split * p.per, e1 = min(e0 + p.per, w.pages);
-    const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
-    // this wave's pages, an index a lane (per <= 256)
-    const int n = e1 - e0, w0 = e0 + (n * wave) / 4, nw = e0 + (n * (wave + 1)) / 4 - w0;
-    const uint32_t pgv = lane < nw ? pt[w0 + lane] : 0u;
-    for (int i = tid; i < gt * (D / 8); i += 256) {
-        const int h = i / (D / 8), d0 = 8 * (i & (D / 8 - 1));
-        float r[8];
-        query8(c, axes, jb, p, w.head, col0 + h, d0, q, ldq, r);
-        *(float4*)&smem[h * D + d0] = make_float4(r[0], r[1], r[2], r[3]);
-        *(float4*)&smem[h * D + d0 + 4] = make_float4(r[4], r[5], r[6], r[7]);
-    }
-    __syncthreads();
-    float qmax = 0.0f;
-    const bool live = l16 < gt;
+// 8 codes (biased) times a scale each, as an f16 pair: u * s - 128 * s is (u -
+// 128) * s in one rounding. The scales are in 2^7 .. 2^8 where they are largest,
+// so a value is below 2^15, and keeps 22 bits down to 2^-18 of that.
+__device__ static inline void code_pair(uint32_t lo4, uint32_t hi4, const float (&s)[8], u32x4& hi, u32x4& lo) {
 #pragma unroll
-    for (int i = 0; i < 8 * NG; i += 4) {
-        const float4 f = *(const float4*)&smem[l16 * D + 32 * (i >> 3) + 8 * j4 + (i & 4)];
-        if (live) qmax = fmaxf(qmax, fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))));
-    }
-    qmax = fmaxf(qmax, __shfl_xor(qmax, 16));
-    qmax = fmaxf(qmax, __shfl_xor(qmax, 32));
-    const int eq = query_exponent(qmax);
-    const float qdown = u2f((uint32_t)(127 - eq) << 23);
-    half8_t qh[NG], ql[NG];
-#pragma unroll
-    for (int g = 0; g < NG; g++)
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            const float4 f = *(const float4*)&smem[l16 * D + 32 * g + 8 * j4 + e];
-            const float x[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                _Float16 hi, lo;
-                split_hilo(live ? x[i] * qdown : 0.0f, hi, lo);
-                qh[g][e + i] = hi;
-                ql[g][e + i] = lo;
-            }
-        }
-    __syncthreads();   // every wave has its query: the space is free
-    float* ksl = smem + wave * OW;
-    float* vsl = ksl + 256 * SCL;
-    const float sscale = score_scale(D, eq);
-    // the last cache row that the lane's column sees, and the tile's first and last column
-    const int first_last = jb.past + col0 / p.group, last_last = jb.past + (col0 + gt - 1) / p.group;
-    const int my_last = live ? jb.past + (col0 + l16) / p.group : last_last;
-    const bool store = p.score_cols > 0 && live && col0 + l16 >= jb.count0 * p.group;
-    float* score_at = (float*)(ws + p.scores) +
-                      (((size_t)jb.page0 + (size_t)w.head * page_room(w.pages)) * p.score_cols + l16) * 64 + 4 * j4;
-    const size_t pstride = (size_t)c.nKV * c.blk, hoff = (size_t)w.head * c.blk;
-    auto page_rsrc = [&](const uint8_t* pool, int i) {
-        const uint32_t pg = __builtin_amdgcn_readlane(pgv, i);
-        const bool ok = pg < (uint32_t)c.n_pages;   // an index outside the cache: the page reads as zero, and is masked
-        return __builtin_amdgcn_make_buffer_rsrc((void*)(pool + (ok ? (size_t)pg * pstride + hoff : 0)), 0,
-                                                 ok ? c.blk : 0, 0x00020000);
-    };
-    const int vk = l16 * D + (D / 4) * j4, vv = j4 * D * 16 + l16 * 16;
-    int vso[SCL];
-#pragma unroll
-    for (int s = 0; s < SCL; s++) {
-        const int e = 256 * s + lane * 4, b = e >> 6, jb4 = (e >> 4) & 3;
-        vso[s] = e < 64 * NG ? 4 * ((jb4 * NG + b) * 16 + (e & 15)) : c.blk;   // D = 64: the upper lanes read zero
-    }
-    float M = -INFINITY, lsum = 0.0f;
-    // lane 16 j + .., entry s: of group 4 s + j, whose O is relative to 2^ev; the largest ev yet
-    int ev[SCL], etop[SCL];
-#pragma unroll
-    for (int s = 0; s < SCL; s++) ev[s] = etop[s] = -127;
-    float4_t o[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++) o[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
-    u32x4 kc[4][NG / 2], vc[DT], kst[SCL], vst[SCL];
-    auto load_k = [&](__amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv) {
-#pragma unroll
-        for (int s = 0; s < SCL; s++) {
-            kst[s] = __builtin_amdgcn_raw_buffer_load_b128(rk, lane * 16, 64 * D + 1024 * s, 0);
-            vst[s] = __builtin_amdgcn_raw_buffer_load_b128(rv, vso[s], 64 * D, 0);
-        }
-#pragma unroll
-        for (int tt = 0; tt < 4; tt++)
-#pragma unroll
-            for (int s = 0; s < NG / 2; s++)
-                kc[tt][s] = __builtin_amdgcn_raw_buffer_load_b128(rk, vk, tt * 16 * D + 16 * s, 0);
-    };
-    auto load_v = [&](__amdgpu_buffer_rsrc_t rv) {
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) vc[dt] = __builtin_amdgcn_raw_buffer_load_b128(rv, vv, dt * 256, 0);
-    };
-    auto page = [&](int i) {
-        const int in = i + 1 < nw ? i + 1 : i;
-        const int p64 = 64 * (w0 + i);
-        const bool bad = (uint32_t)__builtin_amdgcn_readlane(pgv, i) >= (uint32_t)c.n_pages;
-        const int last = bad ? -1 : my_last;                // the last row that counts for the lane's column
-        const int any_last = bad ? -1 : last_last;          // .. for one of them
-        const bool edge = bad || p64 + 63 > first_last;     // a row that not every column sees
-        int by[SCL];   // what brings O from the page before to this one's exponent
-#pragma unroll
-        for (int s = 0; s < SCL; s++) {
-            *(u32x4*)&ksl[256 * s + lane * 4] = kst[s];
-            if (edge) {   // rows past the tile's: whatever scale lies there, NaN too, goes in as zero
-                const int t0 = p64 + 16 * (lane & 3) + 4 * (((256 * s + lane * 4) >> 4) & 3);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (t0 + e > any_last) vst[s][e] = 0u;
-            }
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) top = max(top, finite_bits(vst[s][e]));
-            const uint32_t mx = row_max_u32(top);
-            const int en = max(mx ? min((int)(mx >> 23) - 127, 127) : ev[s], etop[s] - 60);
-            etop[s] = max(etop[s], en);
-            by[s] = ev[s] - en;
-            ev[s] = en;
-            const float down = u2f((uint32_t)(en < 127 ? 127 - en : 1) << 23) * (en < 127 ? 1.0f : 0.5f);   // 2^-en
-            u32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = f2u(u2f(vst[s][e]) * down);
-            *(u32x4*)&vsl[256 * s + lane * 4] = v;
-        }
-        float pr[4][4];
-        float pm = -INFINITY;
-#pragma unroll
-        for (int tt = 0; tt < 4; tt++) {
-            float ks[4 * NG];
-#pragma unroll
-            for (int s = 0; s < NG; s++) {
-                const float4 f = *(const float4*)&ksl[(tt * 16 + 4 * j4) * NG + 4 * s];
-                ks[4 * s] = f.x; ks[4 * s + 1] = f.y; ks[4 * s + 2] = f.z; ks[4 * s + 3] = f.w;
-            }
-            float4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const u32x4 kw = kc[tt][g >> 1];
-                const half8_t kf = (g & 1) ? dequant8_biased(kw[2], kw[3]) : dequant8_biased(kw[0], kw[1]);
-                float4_t pp = {0.f, 0.f, 0.f, 0.f};
-                pp = mfma16x16x32(kf, qh[g], pp);
-                pp = mfma16x16x32(kf, ql[g], pp);
-#pragma unroll
-                for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(ks[r * NG + g], pp[r], acc[r]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) pr[tt][r] = acc[r];
-        }
-        if (edge) {
-#pragma unroll
-            for (int tt = 0; tt < 4; tt++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (p64 + tt * 16 + 4 * j4 + r > last) pr[tt][r] = -INFINITY;
-        }
-        if (store) {
-#pragma unroll
-            for (int tt = 0; tt < 4; tt++)
-                *(float4_t*)(score_at + (size_t)(w0 + i) * p.score_cols * 64 + 16 * tt) =
-                    float4_t{pr[tt][0], pr[tt][1], pr[tt][2], pr[tt][3]} * sscale;
-        }
-#pragma unroll
-        for (int tt = 0; tt < 4; tt++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) pm = fmaxf(pm, pr[tt][r]);
-        const auto rvn = page_rsrc(c.v, in);
-        load_k(page_rsrc(c.k, in), rvn);
-        __builtin_amdgcn_sched_barrier(0);
-        pm = fmaxf(pm, __shfl_xor(pm, 16));
-        pm = fmaxf(pm, __shfl_xor(pm, 32));
-        const float Mn = fmaxf(M, ceilf(pm * sscale));
-        const float alpha = pow2_diff(M, Mn);
-        lsum *= alpha;
-#pragma unroll
-        for (int b = 0; b < NG; b++) {
-            const float alpha_o = ldexpf(alpha, __builtin_amdgcn_readlane(by[b >> 2], 16 * (b & 3)));
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                o[2 * b][r] *= alpha_o;
-                o[2 * b + 1][r] *= alpha_o;
-            }
-        }
-        const float base = P_SHIFT - (Mn == -INFINITY ? 0.0f : Mn);
-        const bool large = __any(!(fabsf(base) < M_LARGE));
-#pragma unroll
-        for (int tt = 0; tt < 4; tt++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float t = __builtin_fmaf(pr[tt][r], sscale, base);
-                if (large) t = pr[tt][r] * sscale - (Mn == -INFINITY ? 0.0f : Mn) + P_SHIFT;
-                const float e = __builtin_amdgcn_exp2f(t);
-                pr[tt][r] = e;
-                lsum += e;
-            }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int b = 0; b < NG; b++) {
-            float sv[16];
-#pragma unroll
-            for (int s = 0; s < 4; s++) {
-                const float4 f = *(const float4*)&vsl[b * 64 + 16 * j4 + 4 * s];
-                sv[4 * s] = f.x; sv[4 * s + 1] = f.y; sv[4 * s + 2] = f.z; sv[4 * s + 3] = f.w;
-            }
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-                u32x4 phw, plw;
-#pragma unroll
-                for (int ii = 0; ii < 8; ii += 2) {
-                    const int tt = 2 * ks + (ii >> 2), r = ii & 3;
-                    float x0 = pr[tt][r] * sv[4 * tt + r], x1 = pr[tt][r + 1] * sv[4 * tt + r + 1];
-                    if (edge) {   // a row that this column does not see, whose scale is no finite number
-                        if (p64 + tt * 16 + 4 * j4 + r > last) x0 = 0.0f;
-                        if (p64 + tt * 16 + 4 * j4 + r + 1 > last) x1 = 0.0f;
-                    }
-                    uint32_t h, l;
-                    split_hilo2(x0, x1, h, l);
-                    phw[ii >> 1] = h;
-                    plw[ii >> 1] = l;
-                }
-                const half8_t ph = __builtin_bit_cast(half8_t, phw), pl = __builtin_bit_cast(half8_t, plw);
-#pragma unroll
-                for (int dd = 0; dd < 2; dd++) {
-                    const int dt = 2 * b + dd;
-                    const u32x4 vw = vc[dt];
-                    const half8_t vf = ks ? dequant8_biased(vw[2], vw[3]) : dequant8_biased(vw[0], vw[1]);
-                    o[dt] = mfma16x16x32(vf, ph, o[dt]);
-                    o[dt] = mfma16x16x32(vf, pl, o[dt]);
-                }
-            }
-        }
-        M = Mn;
-        load_v(rvn);
-    };
-    if (nw > 0) {
-        const auto rv = page_rsrc(c.v, 0);
-        load_k(page_rsrc(c.k, 0), rv);
-        load_v(rv);
-        for (int i = 0; i < nw; i++) page(i);
-    }
-    lsum += __shfl_xor(lsum, 16);
-    lsum += __shfl_xor(lsum, 32);
-    {
-        float* part = smem + wave * OW;   // its scale slices are this wave's own and done with
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-            *(float4_t*)(part + l16 * D + dt * 16 + 4 * j4) =
-                o[dt] * ldexpf(P_UNSHIFT, __builtin_amdgcn_readlane(ev[dt >> 3], 16 * ((dt >> 1) & 3)));
-        if (j4 == 0) {
-            part[16 * D + l16] = M;
-            part[16 * D + 16 + l16] = lsum * P_UNSHIFT;
-        }
-    }
-    __syncthreads();
-    // the four waves' parts, two channels a thread
-    const size_t unit = (size_t)jb.unit0 + ((size_t)w.head * w.tiles + w.tile) * w.splits + w.split;
-    float* mine = (float*)(ws + p.parts) + unit * 16 * D;
-    float2* ml = (float2*)(ws + p.ml) + unit * 16;
-    for (int i = tid; i < gt * (D / 2); i += 256) {
-        const int h = i / (D / 2), d = 2 * (i & (D / 2 - 1));
-        float m = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < 4; v++) m = fmaxf(m, smem[v * OW + 16 * D + h]);
-        float l = 0.0f, x = 0.0f, y = 0.0f;
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-            const float* part = smem + v * OW;
-            const float f = pow2_diff(part[16 * D + h], m);
-            const float2 xy = *(const float2*)(part + h * D + d);
-            l = __builtin_fmaf(part[16 * D + 16 + h], f, l);
-            x = __builtin_fmaf(xy.x, f, x);
-            y = __builtin_fmaf(xy.y, f, y);
-        }
-        if (w.splits == 1) {
-            const int col = col0 + h;
-            float* dst = out + ((int64_t)jb.row0 + col / p.group) * ldo + (size_t)(w.head * p.group + col % p.group) * D + d;
-            dst[0] = l != 0.0f ? x / l : 0.0f;
-            dst[1] = l != 0.0f ? y / l : 0.0f;
-        } else {
-            *(float2*)(mine + (size_t)h * D + d) = make_float2(x, y);
-        }
-        if (d == 0) ml[h] = make_float2(m, l);
+    for (int e = 0; e < 8; e += 2) {
+        const uint32_t w = e < 4 ? lo4 : hi4;
+        const float x = __builtin_fmaf((float)((w >> (8 * (e & 3))) & 0xffu), s[e], -128.0f * s[e]);
+        const float y = __builtin_fmaf((float)((w >> (8 * (e & 3) + 8)) & 0xffu), s[e + 1], -128.0f * s[e + 1]);
+        uint32_t h, l;
+        split_mix2(x, y, h, l);
+        hi[e >> 1] = h;
+        lo[e >> 1] = l;
     }
 }
-
-// M and 1/l of a column over its unit's splits (0 where it sees nothing), the
-// splits' sums in their order; at: the first split's (M, l), `stride` from one
-// split to the next.
-__device__ static inline float2 column_total(const float2* __restrict__ at, int splits, int stride) {
-    float m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < splits; s++) {
-        const float2 v = at[(size_t)s * stride];
-        const float mn = fmaxf(m, v.x);
-        l = l * pow2_diff(m, mn) + v.y * pow2_diff(v.x, mn);
-        m = mn;
-    }
-    return make_float2(m, l != 0.0f ? 1.0f / l : 0.0f);
+__device__ static inline void code_pair(uint32_t lo4, uint32_t hi4, float s, half8_t& hi, half8_t& lo) {
+    const float sv[8] = {s, s, s, s, s, s, s, s};
+    u32x4 h, l;
+    code_pair(lo4, hi4, sv, h, l);
+    hi = __builtin_bit_cast(half8_t, h);
+    lo = __builtin_bit_cast(half8_t, l);
 }
+// The exponent of the largest of scales (bits), within what the pair's scale
+// can be: times pair_down(e) a scale is at most 2^8.
+__device__ static inline int pair_exponent(uint32_t top) { return max((int)(top >> 23) - 127, -112); }
+__device__ static inline float pair_down(int e) { return u2f((uint32_t)(134 - e) << 23); }
 
-// After k_weigh: joins the splits' outputs (the first jobs.joins workgroups,
-// WEIGH_JOIN floats of a 16-column piece each, its splits dealt to four waves),
-// and, from the stored scores, adds up the weights of FINISH_PAGES pages of a
-// (job, kv head) a workgroup, a token a lane.
-template <int NG>
-__global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs, WeighPlan p, MarksDev marks,
-                                                      float* __restrict__ out, int64_t ldo, const uint8_t* __restrict__ ws) {
-    constexpr int D = 32 * NG, CH = 16 * D / WEIGH_JOIN;   // chunks of a 16-column piece
-    __shared__ __align__(16) float red[4][WEIGH_JOIN];
-    __shared__ float2 total[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float2* ml = (const float2*)(ws + p.ml);
-    if ((int)blockIdx.x < jobs.joins * CH) {
-        const int piece = (int)blockIdx.x / CH, ch = (int)blockIdx.x % CH;
-        const WeighJob jb = jobs.j[weigh_job_at(jobs, piece, &WeighJob::join0)];
-        const int tiles = weigh_tiles(jb, p), splits = (weigh_pages(jb) + p.per - 1) / p.per;
-        if (splits == 1) return;   // the attention kernel wrote them
-        const int r = piece - jb.join0, sub = r % p.subs, tile = r / p.subs % tiles, head = r / p.subs / tiles;
-        const int col0 = (tile * p.subs + sub) * 16, gt = min(16, jb.n * p.group - col0);
-        const int h = (ch * WEIGH_JOIN + lane * 4) / D, d = (ch * WEIGH_JOIN + lane * 4) % D;
-        if (ch * WEIGH_JOIN / D >= gt) return;
-        const size_t unit = (size_t)jb.unit0 + ((size_t)head * tiles + tile) * splits;
-        const float2* at = ml + (unit * p.subs + sub) * 16 + h;
-        const float* part = (const float*)(ws + p.parts) + (unit * p.subs + sub) * 16 * D + ch * WEIGH_JOIN + lane * 4;
-        float m = -INFINITY, l = 0.0f;
-        float4_t x = {0.f, 0.f, 0.f, 0.f};
-        if (h < gt) {
-#pragma unroll 4
-            for (int s = wave; s < splits; s += 4) {
-                const float2 v = at[(size_t)s * p.subs * 16];
-                const float4_t y = *(const float4_t*)(part + (size_t)s * p.subs * 16 * D);
-                const float mn = fmaxf(m, v.x), fa = pow2_diff(m, mn), fb = pow2_diff(v.x, mn);
-                l = l * fa + v.y * fb;
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = x[e] * fa + y[e] * fb;
-                m = mn;
-            }
-        }
-        __shared__ float2 wml[4][64];
-        wml[wave][lane] = make_float2(m, l);
-        *(float4_t*)&red[wave][lane * 4] = x;
-        __syncthreads();
-        if (wave || h >= gt) return;
-        for (int v = 1; v < 4; v++) {
-            const float2 o = wml[v][lane];
-            const float4_t y = *(const float4_t*)&red[v][lane * 4];
-            const float mn = fmaxf(m, o.x), fa = pow2_diff(m, mn), fb = pow2_diff(o.x, mn);
-            l = l * fa + o.y * fb;
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = x[e] * fa + y[e] * fb;
-            m = mn;
-        }
-        const int col = col0 + h;
-        float* dst = out + ((int64_t)jb.row0 + col / p.group) * ldo + (size_t)(head * p.group + col % p.group) * D + d;
-#pragma unroll
-        for (int e = 0; e < 4; e++) dst[e] = l != 0.0f ? x[e] / l : 0.0f;
-        return;
-    }
-    const int u = ((int)blockIdx.x - jobs.joins * CH) * FINISH_PAGES;
-    const WeighJob jb = jobs.j[weigh_job_at(jobs, u, &WeighJob::page0)];
-    const int pages = weigh_pages(jb), room = page_room(pages);
-    const int head = (u - jb.page0) / room, p0 = (u - jb.page0) % room;
-    const int splits = (pages + p.per - 1) / p.per;
-    const int c0 = jb.count0 * p.group, cols = jb.n * p.group;
-    const size_t unit = (size_t)jb.unit0 + (size_t)head * splits;
-    if (tid < cols) total[tid] = column_total(ml + unit * 16 + tid, splits, 16);
-    __syncthreads();
-    for (int i = wave; i < FINISH_PAGES && p0 + i < pages; i += 4) {
-        const int pg = p0 + i;
-        const uint32_t id = c.page_table[(size_t)jb.slot * c.max_pages + pg];
-        if (id >= (uint32_t)c.n_pages || 64 * pg + lane >= jb.past + jb.n) continue;
-        float* wt = marks.weight + ((size_t)id * c.nKV + head) * 64 + lane;
-        const float* s = (const float*)(ws + p.scores) + ((size_t)jb.page0 + (size_t)head * room + pg) * p.score_cols * 64 + lane;
-        const float before = p.fade == 0.0f && 64 * pg + lane >= jb.fresh ? 0.0f : *wt;
-        float got = 0.0f;
-        for (int col = c0; col < cols; col++) {
-            const float2 t = total[col];
-            const float x = __builtin_amdgcn_exp2f(s[(size_t)col * 64] - (t.x == -INFINITY ? 0.0f : t.x));
-            got = __builtin_fmaf(x, t.y, got);
-        }
-        *wt = __builtin_fmaf(before, 64 * pg + lane >= jb.fresh ? p.fade : 1.0f, got);
-    }
-}
-
-// The queries of many columns, rotated once, as the matrix products take them:
-// a piece of 16 columns is [hi, lo][NG][64 lanes] of 8 f16, and its scale for
-// the scores 16 f32.
+// Of a page's scales, for the f16 pairs below: 16 bytes, the exponents of each
+// group's largest V scale, of the largest K scale at PAIR_K, and at PAIR_BAD
+// whether a V scale is no finite number.
+constexpr int PAIR_K = 8, PAIR_BAD = 9;
+// What comes before attention: the queries, rotated once, as the matrix
+// products take them (a piece of 16 columns is [hi, lo][NG][64 lanes] of 8 f16,
+// and its scale for the scores 16 f32), then, for k_weigh_many, the exponents
+// of the jobs' pages, a wave each.
 template <int NG>
 __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs, WeighPlan p, AxesDev axes,
                                                      const float* __restrict__ q, int64_t ldq, uint8_t* __restrict__ ws) {
@@ -486,6 +154,40 @@ __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs,
     __shared__ __align__(16) float x[16 * D];
     __shared__ int s_eq[16];
     const int tid = threadIdx.x, piece = blockIdx.x;
+    if (piece >= jobs.joins) {
+        const int lane = tid & 63, u = (piece - jobs.joins) * 4 + (tid >> 6);
+        const WeighJob jb = jobs.j[weigh_job_at(jobs, u, &WeighJob::page0)];
+        const int pages = weigh_pages(jb), room = page_room(pages), head = (u - jb.page0) / room, pg = (u - jb.page0) % room;
+        if (pg >= pages) return;
+        const uint32_t id = c.page_table[(size_t)jb.slot * c.max_pages + pg];
+        if (id >= (uint32_t)c.n_pages) return;
+        const int held = jb.past + jb.n - 64 * pg;   // of the page's rows
+        const size_t at = ((size_t)id * c.nKV + head) * c.blk + 64 * D;
+        const uint32_t *ks = (const uint32_t*)(c.k + at), *vs = (const uint32_t*)(c.v + at);
+        const int vt = 16 * ((lane & 15) >> 2) + 4 * (lane >> 4) + (lane & 3);   // the row of V's entry `lane`
+        uint32_t top = 0;
+        bool bad = false;
+        uint8_t* to = ws + p.exps + (size_t)u * 16;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            if (lane < held) top = max(top, finite_bits(ks[lane * NG + g]));
+            uint32_t v = vt < held ? vs[((lane >> 4) * NG + g) * 16 + (lane & 15)] : 0u;
+            bad = bad || v >= 0x7f800000u;
+            v = row_max_u32(finite_bits(v));
+            v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+            v = max(v, (uint32_t)__shfl_xor((int)v, 32));
+            if (lane == 0) to[g] = (uint8_t)(int8_t)pair_exponent(v);
+        }
+        top = row_max_u32(top);
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+        bad = __any(bad);
+        if (lane == 0) {
+            to[PAIR_K] = (uint8_t)(int8_t)pair_exponent(top);
+            to[PAIR_BAD] = bad;
+        }
+        return;
+    }
     const WeighJob jb = jobs.j[weigh_job_at(jobs, piece, &WeighJob::join0)];
     const int per_head = weigh_tiles(jb, p) * p.subs, r = piece - jb.join0, head = r / per_head;
     const int col0 = r % per_head * 16, gt = max(0, min(16, jb.n * p.group - col0));
@@ -524,21 +226,745 @@ __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs,
     }
 }
 
-// 8 codes times a scale, in 2^7 .. 2^15 where they are largest, as an f16 pair.
-__device__ static inline void code_pair(uint32_t lo4, uint32_t hi4, float scale, half8_t& hi, half8_t& lo) {
+// Attention of up to 16 * CT columns over `per` pages, a page at a time by the
+// whole workgroup: of S^T = K . Q^T each of the four waves makes a page's 16
+// rows, of O^T += V^T . P^T a quarter of the channels, and P meets in LDS. So a
+// wave loads and unpacks a quarter of the page's codes, straight into the
+// registers that the matrix products read, and no code is unpacked twice. Keys
+// are whole numbers in f16, scaled in f32 behind each group's product; values
+// are f16 pairs relative to the largest scale so far of their group; queries
+// and P are f16 pairs as well. While a page is at its second product the next
+// one's codes are on their way.
+// A page takes one barrier: each wave forms its P with the M it has, and the
+// waves see each other's largest scores with each other's P. Where one of those
+// passes M by more than P_ROOM, every wave forms its P anew from a new M.
+//
+// Where p.score_cols is set the scores stay in the workspace, [page][column][64]
+// f32, for k_weigh_finish: 4 bytes a column and token beside the 2 * (D + D/8)
+// that a token's K and V take.
+template <int NG, int CT>
+__global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs jobs, WeighPlan p, float* __restrict__ out,
+                                                       int64_t ldo, uint8_t* __restrict__ ws) {
+    constexpr int D = 32 * NG, DW = D / 64, GW = DW > 1 ? DW / 2 : 1;   // of a wave: 16-channel pieces, groups
+    constexpr int PB = 2 * 2 * CT * 64;   // P of a page: [hi, lo][2][CT][64] fragments
+    __shared__ u32x4 qf[CT][2][NG][64];
+    __shared__ u32x4 pbuf[2 * PB];
+    __shared__ float tops[2][4][CT][16];
+    __shared__ float s_sc[CT][16];
+    __shared__ __align__(16) float ksl[4][NG][16], vsl[4][GW][64];   // each wave's own scales
+    __shared__ uint32_t ids[256];
+    WeighUnit w;
+    if (!weigh_unit(jobs, p, w)) return;
+    const WeighJob& jb = w.jb;
+    const int tid = threadIdx.x, lane = tid & 63, j4 = lane >> 4, l16 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cols = jb.n * p.group;
+    const int e0 = w.split * p.per, e1 = min(e0 + p.per, w.pages);
+    const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
+
+    // a page's codes and scales on their way
+    constexpr int SK = NG > 4 ? 2 : 1;   // scales a lane: K's of (row, group) e = SK * lane + ..; V's of entry e % 64 of group e / 64
+    u32x4 kr[NG / 2], vr[DW];
+    uint32_t ksr[SK], vsr[SK];
+    const int ke0 = (SK * lane) % (16 * NG), ve0 = (SK * lane) % (64 * GW);
+    auto rsrc = [&](const uint8_t* pool, uint32_t id) {
+        const bool ok = id < (uint32_t)c.n_pages;   // an index outside the cache reads as zero, and is masked
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(pool + (ok ? ((size_t)id * c.nKV + w.head) * c.blk : 0)), 0,
+                                                 ok ? c.blk : 0, 0x00020000);
+    };
+    auto load_k = [&](uint32_t id) {
+        const auto r = rsrc(c.k, id);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float x = (float)((int)(((e < 4 ? lo4 : hi4) >> (8 * (e & 3))) & 0xffu) - 128) * scale;
-        _Float16 a, b;
-        split_hilo(x, a, b);
-        hi[e] = a;
-        lo[e] = b;
+        for (int i = 0; i < NG / 2; i++)
+            kr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (16 * wave + l16) * D + (D / 4) * j4 + 16 * i, 0, 0);
+#pragma unroll
+        for (int i = 0; i < SK; i++) ksr[i] = __builtin_amdgcn_raw_buffer_load_b32(r, 64 * D + (16 * wave * NG + ke0 + i) * 4, 0, 0);
+    };
+    auto load_v = [&](uint32_t id) {
+        const auto r = rsrc(c.v, id);
+#pragma unroll
+        for (int i = 0; i < DW; i++)
+            vr[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (j4 * D + (wave * DW + i) * 16 + l16) * 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < SK; i++) {
+            const int e = ve0 + i, g = (wave * DW) / 2 + (e >> 6);
+            vsr[i] = __builtin_amdgcn_raw_buffer_load_b32(r, 64 * D + (((e >> 4 & 3) * NG + g) * 16 + (e & 15)) * 4, 0, 0);
+        }
+    };
+    const uint32_t my_id = pt[min(e0 + tid, e1 - 1)];
+    uint32_t id = __builtin_amdgcn_readfirstlane(pt[e0]);
+    ids[tid] = my_id;
+    load_k(id);
+    load_v(id);
+
+    const size_t piece0 = (size_t)jb.join0 + (size_t)w.head * p.subs;
+    {
+        const u32x4* of = (const u32x4*)(ws + p.q) + piece0 * 2 * NG * 64;
+        u32x4* to = &qf[0][0][0][0];
+#pragma unroll
+        for (int i = 0; i < CT * NG / 2; i++) to[256 * i + tid] = of[256 * i + tid];
+        if (tid < 16 * CT) s_sc[tid >> 4][tid & 15] = ((const float*)(ws + p.qs))[piece0 * 16 + tid];
+    }
+    __syncthreads();
+    float sc[CT], M[CT], lsum[CT];
+    int my_last[CT];
+    float4_t o[DW][CT];
+    bool store[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int col = 16 * ct + l16;
+        sc[ct] = s_sc[ct][l16];
+        M[ct] = -INFINITY;
+        lsum[ct] = 0.0f;
+        my_last[ct] = jb.past + min(col, cols - 1) / p.group;
+        store[ct] = p.score_cols > 0 && col < cols && col >= jb.count0 * p.group;
+#pragma unroll
+        for (int i = 0; i < DW; i++) o[i][ct] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    int ev[GW];   // O of a group's channels is relative to 2^(ev - 7)
+#pragma unroll
+    for (int g = 0; g < GW; g++) ev[g] = -112;
+    float* score_at = (float*)(ws + p.scores) +
+                      (((size_t)jb.page0 + (size_t)w.head * page_room(w.pages) + e0) * p.score_cols + l16) * 64 + 16 * wave + 4 * j4;
+    for (int e = e0; e < e1; e++) {
+        const int b = (e - e0) & 1, r0 = 64 * e + 16 * wave + 4 * j4;   // the lane's first row of S
+        const bool ok = id < (uint32_t)c.n_pages;
+        const uint32_t next = __builtin_amdgcn_readfirstlane(ids[min(e + 1, e1 - 1) - e0]);
+        const bool edge = !ok || 64 * e + 63 > jb.past;    // a row that not every column sees
+        float4_t s[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) s[ct] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < SK; i++) ksl[wave][(ke0 + i) % NG][(ke0 + i) / NG] = u2f(ksr[i]);
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const float4_t ks = *(const float4_t*)&ksl[wave][g][4 * j4];
+            const u32x4 kw = kr[g >> 1];
+            const half8_t kf = (g & 1) ? dequant8_biased(kw[2], kw[3]) : dequant8_biased(kw[0], kw[1]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                float4_t pp = {0.f, 0.f, 0.f, 0.f};
+                pp = mfma16x16x32(kf, __builtin_bit_cast(half8_t, qf[ct][0][g][lane]), pp);
+                pp = mfma16x16x32(kf, __builtin_bit_cast(half8_t, qf[ct][1][g][lane]), pp);
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[ct][r] = __builtin_fmaf(ks[r], pp[r], s[ct][r]);
+            }
+            if (CT * NG >= 16 && (g & 1)) __builtin_amdgcn_sched_barrier(0);   // no more query fragments ahead than fit
+        }
+        load_k(next);
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            if (edge) {
+                const int last = ok ? my_last[ct] : -1;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (r0 + r > last) s[ct][r] = -INFINITY;
+            }
+            s[ct] = s[ct] * sc[ct];
+            if (store[ct]) *(float4_t*)(score_at + ((size_t)(e - e0) * p.score_cols + 16 * ct) * 64) = s[ct];
+            const float m = rows_max(fmaxf(fmaxf(s[ct][0], s[ct][1]), fmaxf(s[ct][2], s[ct][3])));
+            if (j4 == 0) tops[b][wave][ct][l16] = m;
+        }
+        float sum[CT];
+        uint2* pw = (uint2*)(pbuf + b * PB);
+        auto form = [&]() {   // P of the wave's rows, relative to M
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const float m = M[ct] == -INFINITY ? 0.0f : M[ct];
+                float pr[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) pr[r] = __builtin_amdgcn_exp2f(s[ct][r] - m + P_SHIFT);
+                sum[ct] = (pr[0] + pr[1]) + (pr[2] + pr[3]);
+                uint2 h, l;
+                split_mix2(pr[0], pr[1], h.x, l.x);
+                split_mix2(pr[2], pr[3], h.y, l.y);
+                pw[(((0 * 2 + (wave >> 1)) * CT + ct) * 64 + lane) * 2 + (wave & 1)] = h;
+                pw[(((1 * 2 + (wave >> 1)) * CT + ct) * 64 + lane) * 2 + (wave & 1)] = l;
+            }
+        };
+        form();
+        __syncthreads();
+        bool over = false;
+        float Mn[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            const float m = fmaxf(fmaxf(tops[b][0][ct][l16], tops[b][1][ct][l16]), fmaxf(tops[b][2][ct][l16], tops[b][3][ct][l16]));
+            const bool mine = M[ct] == -INFINITY ? m > -INFINITY : m > M[ct] + P_ROOM;
+            Mn[ct] = mine ? ceilf(m) : M[ct];
+            over = over || mine;
+        }
+        if (__any(over)) {   // the same in every wave
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const float alpha = pow2_diff(M[ct], Mn[ct]);
+                lsum[ct] *= alpha;
+#pragma unroll
+                for (int i = 0; i < DW; i++) o[i][ct] = o[i][ct] * alpha;
+                M[ct] = Mn[ct];
+            }
+            form();
+            __syncthreads();
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) lsum[ct] += sum[ct];
+        // V's scales, relative to the largest so far of their group
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < SK; i++) {
+            const int v = ve0 + i, row = 64 * e + 16 * (v >> 2 & 3) + 4 * (v >> 4 & 3) + (v & 3);
+            if (row >= jb.past + jb.n) vsr[i] = 0u;
+            bad = bad || vsr[i] >= 0x7f800000u;
+            vsr[i] = finite_bits(vsr[i]);
+        }
+        uint32_t most = row_max_u32(max(vsr[0], vsr[SK - 1]));   // (a row of 16 lanes is of one group)
+        if (GW == 1) most = rows_max(most);
+        else most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+#pragma unroll
+        for (int g = 0; g < GW; g++) {
+            const int en = max(ev[g], pair_exponent(__builtin_amdgcn_readlane(most, 32 * g)));
+            if (en != ev[g]) {
+                const float f = ldexpf(1.0f, max(ev[g] - en, -300));
+#pragma unroll
+                for (int i = 0; i < DW; i++)
+                    if ((DW > 1 ? i >> 1 : 0) == g)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) o[i][ct] = o[i][ct] * f;
+                ev[g] = en;
+            }
+        }
+        const float down = pair_down(GW > 1 && lane >= 32 ? ev[GW - 1] : ev[0]);
+#pragma unroll
+        for (int i = 0; i < SK; i++) vsl[wave][(ve0 + i) >> 6][(ve0 + i) & 63] = u2f(vsr[i]) * down;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            half8_t ph[CT], pl[CT];
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                ph[ct] = __builtin_bit_cast(half8_t, pbuf[b * PB + (0 * 2 + ks) * CT * 64 + ct * 64 + lane]);
+                pl[ct] = __builtin_bit_cast(half8_t, pbuf[b * PB + (1 * 2 + ks) * CT * 64 + ct * 64 + lane]);
+            }
+#pragma unroll
+            for (int i = 0; i < DW; i++) {
+                const float* at = &vsl[wave][DW > 1 ? i >> 1 : 0][16 * j4 + 8 * ks];
+                const float4_t sa = *(const float4_t*)at, sb = *(const float4_t*)(at + 4);
+                const float s8[8] = {sa[0], sa[1], sa[2], sa[3], sb[0], sb[1], sb[2], sb[3]};
+                u32x4 h, l;
+                code_pair(vr[i][2 * ks], vr[i][2 * ks + 1], s8, h, l);
+                const half8_t vh = __builtin_bit_cast(half8_t, h), vl = __builtin_bit_cast(half8_t, l);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    o[i][ct] = mfma16x16x32(vh, ph[ct], o[i][ct]);
+                    o[i][ct] = mfma16x16x32(vl, ph[ct], o[i][ct]);
+                    o[i][ct] = mfma16x16x32(vh, pl[ct], o[i][ct]);
+                }
+                if (CT * NG >= 16 && (i & 1)) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        load_v(next);
+        if (ok && __any(bad)) {   // a scale that is no finite number: NaN for the columns that see it
+            const uint32_t* vs = (const uint32_t*)(c.v + ((size_t)id * c.nKV + w.head) * c.blk + 64 * D);
+#pragma unroll
+            for (int g = 0; g < GW; g++)
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    int any = 0;
+                    for (int i = 0; i < 16; i++)   // entry i: row 16 * (i / 4) + 4 * j4 + i % 4
+                        any |= 64 * e + 16 * (i >> 2) + 4 * j4 + (i & 3) <= my_last[ct] &&
+                               vs[(j4 * NG + (wave * DW) / 2 + g) * 16 + i] >= 0x7f800000u;
+                    any |= __shfl_xor(any, 16);
+                    any |= __shfl_xor(any, 32);
+                    if (any) {
+#pragma unroll
+                        for (int i = 0; i < DW; i++)
+                            if ((DW > 1 ? i >> 1 : 0) == g)
+#pragma unroll
+                                for (int r = 0; r < 4; r++) o[i][ct][r] = NAN;
+                    }
+                }
+        }
+        id = next;
+    }
+    // l: a lane's rows, a wave's, the four waves'
+    __syncthreads();
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        float l = lsum[ct] + __shfl_xor(lsum[ct], 16);
+        l += __shfl_xor(l, 32);
+        if (j4 == 0) tops[0][wave][ct][l16] = l;
+    }
+    __syncthreads();
+    const size_t unit = (size_t)jb.unit0 + (size_t)w.head * w.splits + w.split;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int col = 16 * ct + l16;
+        if (col >= cols) continue;
+        const float l = ((tops[0][0][ct][l16] + tops[0][1][ct][l16]) + (tops[0][2][ct][l16] + tops[0][3][ct][l16])) * P_UNSHIFT;
+        if (wave == 0 && j4 == 0) ((float2*)(ws + p.ml))[(unit * p.subs + ct) * 16 + l16] = make_float2(M[ct], l);
+        float* part = (float*)(ws + p.parts) + ((unit * p.subs + ct) * 16 + l16) * D + wave * (D / 4) + 4 * j4;
+        float* dst = out + ((int64_t)jb.row0 + col / p.group) * ldo + (size_t)(w.head * p.group + col % p.group) * D + wave * (D / 4) + 4 * j4;
+#pragma unroll
+        for (int i = 0; i < DW; i++) {
+            float4_t y = o[i][ct] * ldexpf(P_UNSHIFT, ev[DW > 1 ? i >> 1 : 0] - 7);
+            if (w.splits == 1) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) y[r] = l != 0.0f ? y[r] / l : 0.0f;
+                *(float4_a4*)(dst + 16 * i) = y;
+            } else {
+                *(float4_t*)(part + 16 * i) = y;
+            }
+        }
     }
 }
-// The exponent of the largest of a page's scales (bits), within what the pair's
-// scale can be: 2^-pair_down(e) brings a scale to 2^7 .. 2^8.
-__device__ static inline int pair_exponent(uint32_t top) { return max((int)(top >> 23) - 127, -112); }
-__device__ static inline float pair_down(int e) { return u2f((uint32_t)(134 - e) << 23); }
+
+// M and 1/l of a column over its unit's splits (0 where it sees nothing), the
+// splits' sums in their order; at: the first split's (M, l), `stride` from one
+// split to the next.
+__device__ static inline float2 column_total(const float2* __restrict__ at, int splits, int stride) {
+    float m = -INFINITY, l = 0.0f;
+    for (int s = 0; s < splits; s++) {
+        const float2 v = at[(size_t)s * stride];
+        const float mn = fmaxf(m, v.x);
+        l = l * pow2_diff(m, mn) + v.y * pow2_diff(v.x, mn);
+        m = mn;
+    }
+    return make_float2(m, l != 0.0f ? 1.0f / l : 0.0f);
+}
+
+// After k_weigh: joins the splits' outputs (the first jobs.joins workgroups,
+// WEIGH_JOIN floats of a 16-column piece each, its splits dealt to four waves),
+// and, from the stored scores, adds up the weights of FINISH_PAGES pages of a
+// (job, kv head) a workgroup, a token a lane.
+template <int NG>
+__global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs, WeighPlan p, MarksDev marks,
+                                                      float* __restrict__ out, int64_t ldo, uint8_t* __restrict__ ws) {
+    constexpr int D = 32 * NG, CH = 16 * D / WEIGH_JOIN;   // chunks of a 16-column piece
+    __shared__ __align__(16) float red[4][WEIGH_JOIN];
+    __shared__ float2 total[64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float2* ml = (const float2*)(ws + p.ml);
+    if ((int)blockIdx.x < jobs.joins * CH) {
+        const int piece = (int)blockIdx.x / CH, ch = (int)blockIdx.x % CH;
+        const WeighJob jb = jobs.j[weigh_job_at(jobs, piece, &WeighJob::join0)];
+        const int tiles = weigh_tiles(jb, p), splits = (weigh_pages(jb) + p.per - 1) / p.per;
+        if (splits == 1) return;   // the attention kernel wrote them
+        const int r = piece - jb.join0, sub = r % p.subs, tile = r / p.subs % tiles, head = r / p.subs / tiles;
+        const int col0 = (tile * p.subs + sub) * 16, gt = min(16, jb.n * p.group - col0);
+        const int h = (ch * WEIGH_JOIN + lane * 4) / D, d = (ch * WEIGH_JOIN + lane * 4) % D;
+        if (ch * WEIGH_JOIN / D >= gt) return;
+        const size_t unit = (size_t)jb.unit0 + ((size_t)head * tiles + tile) * splits;
+        const float2* at = ml + (unit * p.subs + sub) * 16 + h;
+        const float* part = (const float*)(ws + p.parts) + (unit * p.subs + sub) * 16 * D + ch * WEIGH_JOIN + lane * 4;
+        float m = -INFINITY, l = 0.0f;
+        float4_t x = {0.f, 0.f, 0.f, 0.f};
+        if (h < gt) {
+#pragma unroll 4
+            for (int s = wave; s < splits; s += 4) {
+                const float2 v = at[(size_t)s * p.subs * 16];
+                const float4_t y = *(const float4_t*)(part + (size_t)s * p.subs * 16 * D);
+                if (v.x == -INFINITY && v.y == 0.0f) continue;   // nothing seen: there is no part
+                const float mn = fmaxf(m, v.x), fa = pow2_diff(m, mn), fb = pow2_diff(v.x, mn);
+                l = l * fa + v.y * fb;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = x[e] * fa + y[e] * fb;
+                m = mn;
+            }
+        }
+        __shared__ float2 wml[4][64];
+        wml[wave][lane] = make_float2(m, l);
+        *(float4_t*)&red[wave][lane * 4] = x;
+        __syncthreads();
+        if (wave || h >= gt) return;
+        for (int v = 1; v < 4; v++) {
+            const float2 o = wml[v][lane];
+            const float4_t y = *(const float4_t*)&red[v][lane * 4];
+            const float mn = fmaxf(m, o.x), fa = pow2_diff(m, mn), fb = pow2_diff(o.x, mn);
+            l = l * fa + o.y * fb;
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = x[e] * fa + y[e] * fb;
+            m = mn;
+        }
+        const int col = col0 + h;
+        float* dst = out + ((int64_t)jb.row0 + col / p.group) * ldo + (size_t)(head * p.group + col % p.group) * D + d;
+#pragma unroll
+        for (int e = 0; e < 4; e++) dst[e] = l != 0.0f ? x[e] / l : 0.0f;
+        if (p.tot && d == 0) ((float2*)(ws + p.tot))[(size_t)piece * 16 + h] = make_float2(m, l != 0.0f ? 1.0f / l : 0.0f);
+        return;
+    }
+    const int u = ((int)blockIdx.x - jobs.joins * CH) * FINISH_PAGES;
+    const WeighJob jb = jobs.j[weigh_job_at(jobs, u, &WeighJob::page0)];
+    const int pages = weigh_pages(jb), room = page_room(pages);
+    const int head = (u - jb.page0) / room, p0 = (u - jb.page0) % room;
+    const int splits = (pages + p.per - 1) / p.per;
+    const int c0 = jb.count0 * p.group, cols = jb.n * p.group;
+    const size_t unit = (size_t)jb.unit0 + (size_t)head * splits;   // one tile a (job, kv head)
+    if (tid < cols) total[tid] = column_total(ml + unit * p.subs * 16 + tid, splits, p.subs * 16);
+    __syncthreads();
+    for (int i = wave; i < FINISH_PAGES && p0 + i < pages; i += 4) {
+        const int pg = p0 + i;
+        const uint32_t id = c.page_table[(size_t)jb.slot * c.max_pages + pg];
+        if (id >= (uint32_t)c.n_pages || 64 * pg + lane >= jb.past + jb.n) continue;
+        float* wt = marks.weight + ((size_t)id * c.nKV + head) * 64 + lane;
+        const float* s = (const float*)(ws + p.scores) + ((size_t)jb.page0 + (size_t)head * room + pg) * p.score_cols * 64 + lane;
+        const float before = p.fade == 0.0f && 64 * pg + lane >= jb.fresh ? 0.0f : *wt;
+        float got = 0.0f;
+        for (int col = c0; col < cols; col++) {
+            const float2 t = total[col];
+            const float x = __builtin_amdgcn_exp2f(s[(size_t)col * 64] - (t.x == -INFINITY ? 0.0f : t.x));
+            got = __builtin_fmaf(x, t.y, got);
+        }
+        *wt = __builtin_fmaf(before, 64 * pg + lane >= jb.fresh ? p.fade : 1.0f, got);
+    }
+}
+
+// Attention of a tile of 16 * CT columns for each of W waves over `per` pages.
+// The workgroup unpacks a step of TOK rows once for all its columns, K and V as
+// f16 pairs relative to the page's largest scales (V: the largest so far), in
+// the order in which the matrix products read them: a fragment is 64 lanes of
+// 16 bytes. Each product is then three: hi * hi, lo * hi and hi * lo, into one
+// f32 sum, and nothing is scaled in between (a pair's two halves hold 22 bits).
+// While a step is computed the next one is unpacked into the other buffer and
+// the one after it is loaded.
+template <int NG, int CT, int W, int TOK>
+__global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs jobs, WeighPlan p, float* __restrict__ out,
+                                                          int64_t ldo, uint8_t* __restrict__ ws) {
+    constexpr int D = 32 * NG, DT = D / 16, TT = TOK / 16, KS = TOK / 32, HALVES = 64 / TOK;
+    constexpr int NK = TT * NG / 2, NV = DT, NKW = (NK + W - 1) / W, NVW = (NV + W - 1) / W;   // unpacking, in pieces of a wave
+    __shared__ u32x4 kbuf[2][2][TT][NG][64];
+    __shared__ u32x4 vbuf[2][2][KS][DT][64];
+    __shared__ uint32_t ids[256];
+    __shared__ u32x4 exps[256];
+    WeighUnit w;
+    if (!weigh_unit(jobs, p, w)) return;
+    const WeighJob& jb = w.jb;
+    const int tid = threadIdx.x, lane = tid & 63, j4 = lane >> 4, l16 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cols = jb.n * p.group, tcol = w.tile * 16 * p.subs, tile_end = min(tcol + 16 * p.subs, cols);
+    const int tile_pages = (jb.past + (tile_end - 1) / p.group) / 64 + 1;
+    const int e0 = w.split * p.per, e1 = min(e0 + p.per, tile_pages);
+    const size_t unit = (size_t)jb.unit0 + ((size_t)w.head * w.tiles + w.tile) * w.splits + w.split;
+    float2* ml = (float2*)(ws + p.ml) + unit * p.subs * 16;
+    if (e0 >= e1) {   // the tile ends before these pages
+        if (tid < 16 * p.subs) ml[tid] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+    const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
+    {   // the pages and their scales' exponents
+        const u32x4* ex = (const u32x4*)(ws + p.exps) + (size_t)jb.page0 + (size_t)w.head * page_room(w.pages) + e0;
+        for (int i = tid; i < e1 - e0; i += 64 * W) {
+            ids[i] = pt[e0 + i];
+            exps[i] = ex[i];
+        }
+    }
+    const int held = jb.past + jb.n, steps = (e1 - e0) * HALVES;
+    // byte i of a page's exponents (NG <= 8)
+    struct Exps {
+        uint32_t w[3];
+        __device__ int at(int i) const { return (int)(int8_t)(w[i >> 2] >> (8 * (i & 3))); }
+    };
+    auto exps_of = [&](int pg) {
+        const u32x4 x = exps[pg];
+        return Exps{{(uint32_t)__builtin_amdgcn_readfirstlane(x[0]), (uint32_t)__builtin_amdgcn_readfirstlane(x[1]),
+                     (uint32_t)__builtin_amdgcn_readfirstlane(x[2])}};
+    };
+    // the wave's queries
+    const int wcol = tcol + wave * CT * 16;
+    const bool busy = wcol < cols;
+    const size_t piece0 = (size_t)jb.join0 + ((size_t)w.head * w.tiles + w.tile) * p.subs + wave * CT;
+    half8_t qh[CT][NG], ql[CT][NG];
+    float sc[CT];
+    int my_last[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const u32x4* qf = (const u32x4*)(ws + p.q) + (piece0 + ct) * 2 * NG * 64 + lane;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            qh[ct][g] = __builtin_bit_cast(half8_t, qf[g * 64]);
+            ql[ct][g] = __builtin_bit_cast(half8_t, qf[(NG + g) * 64]);
+        }
+        sc[ct] = ((const float*)(ws + p.qs))[(piece0 + ct) * 16 + l16];
+        my_last[ct] = jb.past + min(wcol + 16 * ct + l16, cols - 1) / p.group;
+    }
+    const int first_last = jb.past + wcol / p.group;   // the least of the wave's columns'
+    __syncthreads();
+
+    // a step's codes and scales on their way: pieces of 16 rows x 64 channels of K, of 16 channels x TOK rows of V
+    u32x4 kr[NKW], vr[NVW], vsr[NVW][TOK / 16];
+    uint2 ksr[NKW];
+    const int at_k = l16 * D + (D / 4) * j4, at_ks = l16 * NG * 4, at_v = (j4 * D + l16) * 16, at_vs = j4 * NG * 64;
+    auto load = [&](int st) {
+        const uint32_t id = __builtin_amdgcn_readfirstlane(ids[st / HALVES]);
+        const int half = st % HALVES;
+        const bool ok = id < (uint32_t)c.n_pages;   // an index outside the cache reads as zero, and is masked
+        const size_t at = ok ? ((size_t)id * c.nKV + w.head) * c.blk : 0;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc((void*)(c.k + at), 0, ok ? c.blk : 0, 0x00020000);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc((void*)(c.v + at), 0, ok ? c.blk : 0, 0x00020000);
+#pragma unroll
+        for (int k = 0; k < NKW; k++) {
+            const int task = wave + W * k, t = half * TOK + 16 * (task / (NG / 2)), gp = task % (NG / 2);
+            if (NK % W && task >= NK) break;
+            kr[k] = __builtin_amdgcn_raw_buffer_load_b128(rk, at_k, t * D + 16 * gp, 0);
+            const auto s2 = __builtin_amdgcn_raw_buffer_load_b64(rk, at_ks, 64 * D + (t * NG + 2 * gp) * 4, 0);
+            ksr[k] = make_uint2(s2[0], s2[1]);
+        }
+#pragma unroll
+        for (int k = 0; k < NVW; k++) {
+            const int dt = wave + W * k;
+            if (NV % W && dt >= NV) break;
+            if (TOK == 64) vr[k] = __builtin_amdgcn_raw_buffer_load_b128(rv, at_v, dt * 256, 0);
+            else {
+                const auto x = __builtin_amdgcn_raw_buffer_load_b64(rv, at_v, dt * 256 + 8 * half, 0);
+                vr[k][0] = x[0];
+                vr[k][1] = x[1];
+            }
+#pragma unroll
+            for (int i = 0; i < TOK / 16; i++)
+                vsr[k][i] = __builtin_amdgcn_raw_buffer_load_b128(rv, at_vs, 64 * D + (dt >> 1) * 64 + 32 * half + 16 * i, 0);
+        }
+    };
+    int etask[NVW];   // the largest V exponent so far of the pieces' groups
+#pragma unroll
+    for (int k = 0; k < NVW; k++) etask[k] = -112;
+    auto unpack = [&](int st) {
+        const int b = st & 1, half = st % HALVES, pg = st / HALVES;
+        const int r0 = (e0 + pg) * 64 + half * TOK;   // the step's first row
+        const Exps ex = exps_of(pg);
+        const bool ok = __builtin_amdgcn_readfirstlane(ids[pg]) < (uint32_t)c.n_pages;
+        const float kdown = ok ? pair_down(ex.at(PAIR_K)) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < NKW; k++) {
+            const int task = wave + W * k, tt = task / (NG / 2), gp = task % (NG / 2);
+            if (NK % W && task >= NK) break;
+            float s0 = u2f(ksr[k].x) * kdown, s1 = u2f(ksr[k].y) * kdown;
+            if (r0 + TOK > held && r0 + 16 * tt + l16 >= held) s0 = s1 = 0.0f;
+            half8_t h, l;
+            code_pair(kr[k][0], kr[k][1], s0, h, l);
+            kbuf[b][0][tt][2 * gp][lane] = __builtin_bit_cast(u32x4, h);
+            kbuf[b][1][tt][2 * gp][lane] = __builtin_bit_cast(u32x4, l);
+            code_pair(kr[k][2], kr[k][3], s1, h, l);
+            kbuf[b][0][tt][2 * gp + 1][lane] = __builtin_bit_cast(u32x4, h);
+            kbuf[b][1][tt][2 * gp + 1][lane] = __builtin_bit_cast(u32x4, l);
+        }
+#pragma unroll
+        for (int k = 0; k < NVW; k++) {
+            const int dt = wave + W * k;
+            if (NV % W && dt >= NV) break;
+            const int g = dt >> 1;
+            if (ok) etask[k] = max(etask[k], (int)(int8_t)((g >= 4 ? ex.w[1] : ex.w[0]) >> (8 * (g & 3))));
+            const float down = pair_down(etask[k]);
+            float s[TOK / 4];
+#pragma unroll
+            for (int i = 0; i < TOK / 4; i++) s[i] = u2f(vsr[k][i >> 2][i & 3]) * down;
+            if (ok && ex.at(PAIR_BAD)) {
+#pragma unroll
+                for (int i = 0; i < TOK / 4; i++) s[i] = u2f(finite_bits(vsr[k][i >> 2][i & 3])) * down;
+            }
+            if (r0 + TOK > held) {
+#pragma unroll
+                for (int i = 0; i < TOK / 4; i++)   // entry i: row 16 * (i / 4) + 4 * j4 + i % 4
+                    if (r0 + 16 * (i >> 2) + 4 * j4 + (i & 3) >= held) s[i] = 0.0f;
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const float s8[8] = {s[8 * ks], s[8 * ks + 1], s[8 * ks + 2], s[8 * ks + 3],
+                                     s[8 * ks + 4], s[8 * ks + 5], s[8 * ks + 6], s[8 * ks + 7]};
+                u32x4 h, l;
+                code_pair(vr[k][2 * ks], vr[k][2 * ks + 1], s8, h, l);
+                vbuf[b][0][ks][dt][lane] = h;
+                vbuf[b][1][ks][dt][lane] = l;
+            }
+        }
+    };
+
+    float M[CT], lsum[CT], base[CT];
+    bool large = false;   // an M so large that a score is rounded before M is taken off
+    int ev[NG];   // O of a group's channels is relative to 2^(ev - 7)
+    float4_t o[CT][DT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        M[ct] = -INFINITY;
+        lsum[ct] = 0.0f;
+        base[ct] = P_SHIFT;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) o[ct][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int g = 0; g < NG; g++) ev[g] = -112;
+    auto compute = [&](int st) {
+        const int b = st & 1, half = st % HALVES, pg = st / HALVES;
+        const int r0 = (e0 + pg) * 64 + half * TOK;
+        const Exps ex = exps_of(pg);
+        const bool ok = __builtin_amdgcn_readfirstlane(ids[pg]) < (uint32_t)c.n_pages;
+        const int ke = ok ? ex.at(PAIR_K) : 0;
+        float4_t acc[CT][TT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) acc[ct][tt] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) {
+                const half8_t kh = __builtin_bit_cast(half8_t, kbuf[b][0][tt][g][lane]);
+                const half8_t kl = __builtin_bit_cast(half8_t, kbuf[b][1][tt][g][lane]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    acc[ct][tt] = mfma16x16x32(kh, qh[ct][g], acc[ct][tt]);
+                    acc[ct][tt] = mfma16x16x32(kl, qh[ct][g], acc[ct][tt]);
+                    acc[ct][tt] = mfma16x16x32(kh, ql[ct][g], acc[ct][tt]);
+                }
+            }
+        const bool edge = !ok || r0 + TOK - 1 > first_last;
+        half8_t ph[CT][KS], pl[CT][KS];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            const int last = ok ? my_last[ct] : -1;
+            const float scp = ldexpf(sc[ct], ke - 7);
+            if (edge) {
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (r0 + 16 * tt + 4 * j4 + r > last) acc[ct][tt][r] = -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++)
+                top = fmaxf(fmaxf(top, fmaxf(acc[ct][tt][0], acc[ct][tt][1])), fmaxf(acc[ct][tt][2], acc[ct][tt][3]));
+            top *= scp;
+            if (__any(top > M[ct] + P_ROOM)) {   // (M -inf: the first score of a column)
+                top = rows_max(top);
+                const float Mn = top > M[ct] + P_ROOM ? ceilf(top) : M[ct];
+                const float alpha = pow2_diff(M[ct], Mn);
+                M[ct] = Mn;
+                lsum[ct] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[ct][dt] = o[ct][dt] * alpha;
+                base[ct] = P_SHIFT - (Mn == -INFINITY ? 0.0f : Mn);
+                large = __any(large || !(fabsf(base[ct]) < M_LARGE));
+            }
+            if (large) {
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[ct][tt][r] = __builtin_amdgcn_exp2f(acc[ct][tt][r] * scp - (M[ct] == -INFINITY ? 0.0f : M[ct]) + P_SHIFT);
+            } else {
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[ct][tt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[ct][tt][r], scp, base[ct]));
+            }
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++) lsum[ct] += (acc[ct][tt][0] + acc[ct][tt][1]) + (acc[ct][tt][2] + acc[ct][tt][3]);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                u32x4 h4, l4;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    uint32_t h, l;
+                    split_mix2(acc[ct][2 * ks + (i >> 2)][i & 3], acc[ct][2 * ks + (i >> 2)][(i & 3) + 1], h, l);
+                    h4[i >> 1] = h;
+                    l4[i >> 1] = l;
+                }
+                ph[ct][ks] = __builtin_bit_cast(half8_t, h4);
+                pl[ct][ks] = __builtin_bit_cast(half8_t, l4);
+            }
+        }
+        int grown[NG];
+        bool grew = false;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const int en = ok ? max(ev[g], ex.at(g)) : ev[g];
+            grown[g] = ev[g] - en;
+            grew = grew || grown[g];
+            ev[g] = en;
+        }
+        if (grew) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[ct][dt] = o[ct][dt] * ldexpf(1.0f, max(grown[dt >> 1], -300));
+        }
+        if (ok && ex.at(PAIR_BAD)) {   // a V scale that is no finite number: NaN for the columns that see it
+            const size_t at = ((size_t)__builtin_amdgcn_readfirstlane(ids[pg]) * c.nKV + w.head) * c.blk + 64 * D;
+            const uint32_t* vs = (const uint32_t*)(c.v + at);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    bool bad = false;
+                    for (int i = 0; i < TOK / 4; i++) {
+                        const int row = r0 + 16 * (i >> 2) + 4 * j4 + (i & 3);
+                        if (row <= my_last[ct] && row < held && vs[(j4 * NG + g) * 16 + 8 * half * (TOK == 32) + i] >= 0x7f800000u) bad = true;
+                    }
+                    int any = bad;
+                    any |= __shfl_xor(any, 16);
+                    any |= __shfl_xor(any, 32);
+                    if (any) {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) o[ct][2 * g][r] = o[ct][2 * g + 1][r] = NAN;
+                    }
+                }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const half8_t vh = __builtin_bit_cast(half8_t, vbuf[b][0][ks][dt][lane]);
+                const half8_t vl = __builtin_bit_cast(half8_t, vbuf[b][1][ks][dt][lane]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    o[ct][dt] = mfma16x16x32(vh, ph[ct][ks], o[ct][dt]);
+                    o[ct][dt] = mfma16x16x32(vl, ph[ct][ks], o[ct][dt]);
+                    o[ct][dt] = mfma16x16x32(vh, pl[ct][ks], o[ct][dt]);
+                }
+            }
+    };
+    load(0);
+    unpack(0);
+    if (steps > 1) load(1);
+    __syncthreads();
+    // half of the waves unpack before they compute and half after, so that a SIMD's two are not at their matrix products,
+    // nor at the rest, at the same time
+    const bool early = wave < W / 2;
+    for (int st = 0; st < steps; st++) {
+        auto ahead = [&]() {
+            if (st + 1 < steps) unpack(st + 1);
+            if (st + 2 < steps) load(st + 2);
+        };
+        if (early) ahead();
+        if (busy) compute(st);
+        if (!early) ahead();
+        __syncthreads();
+    }
+    if (!busy) return;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        lsum[ct] += __shfl_xor(lsum[ct], 16);
+        lsum[ct] += __shfl_xor(lsum[ct], 32);
+        const float l = lsum[ct] * P_UNSHIFT;
+        const int col = wcol + 16 * ct + l16;
+        if (col >= cols) continue;
+        const int sub = wave * CT + ct;
+        if (j4 == 0) {
+            ml[sub * 16 + l16] = make_float2(M[ct], l);
+            if (p.tot && w.splits == 1)
+                ((float2*)(ws + p.tot))[(piece0 + ct) * 16 + l16] = make_float2(M[ct], l != 0.0f ? 1.0f / l : 0.0f);
+        }
+        float* part = (float*)(ws + p.parts) + ((unit * p.subs + sub) * 16 + l16) * D + 4 * j4;
+        float* dst = out + ((int64_t)jb.row0 + col / p.group) * ldo + (size_t)(w.head * p.group + col % p.group) * D + 4 * j4;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+            float4_t x = o[ct][dt] * ldexpf(P_UNSHIFT, ev[dt >> 1] - 7);
+            if (w.splits == 1) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[r] = l != 0.0f ? x[r] / l : 0.0f;
+                *(float4_a4*)(dst + 16 * dt) = x;
+            } else {
+                *(float4_t*)(part + 16 * dt) = x;
+            }
+        }
+    }
+}
 
 // The weights from many columns: q . k again, with the columns' M and l known.
 // A wave holds the keys of 16 * TT rows of the cache as f16 pairs in registers
@@ -562,21 +988,16 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
     const int held = jb.past + jb.n;
     const uint8_t* blk = c.k + ((size_t)id * c.nKV + head) * c.blk;
     half8_t kh[TT][NG], kl[TT][NG];
-    int e;
+    const int e = (int8_t)ws[p.exps + (size_t)(jb.page0 + head * room + pg) * 16 + PAIR_K];
     {
         float sc[TT][NG];
-        uint32_t top = 0;
 #pragma unroll
         for (int tt = 0; tt < TT; tt++) {
             const int r = r0 + 16 * tt + l16;
             const float* at = (const float*)(blk + 64 * D) + (r & 63) * NG;
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                sc[tt][g] = r < held ? at[g] : 0.0f;
-                top = max(top, finite_bits(f2u(sc[tt][g])));
-            }
+            for (int g = 0; g < NG; g++) sc[tt][g] = r < held ? at[g] : 0.0f;
         }
-        e = pair_exponent(row_max_u32(top));
         const float down = pair_down(e);
 #pragma unroll
         for (int tt = 0; tt < TT; tt++)
@@ -587,7 +1008,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
                 code_pair(w[2], w[3], sc[tt][g + 1] * down, kh[tt][g + 1], kl[tt][g + 1]);
             }
     }
-    const int splits = (pages + p.per - 1) / p.per, tiles = weigh_tiles(jb, p);
+    const int tiles = weigh_tiles(jb, p);
     const int c0 = jb.count0 * p.group, cols = jb.n * p.group;
     const int from = max(c0, max(0, r0 - jb.past) * p.group);   // the first column that sees one of the wave's rows
     float4_t got[TT];
@@ -610,9 +1031,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
             }
         }
         const int col = t16 * 16 + l16;
-        const float2 t = column_total((const float2*)(ws + p.ml) +
-                                          (((size_t)jb.unit0 + ((size_t)head * tiles + t16 / p.subs) * splits) * p.subs + t16 % p.subs) * 16 + l16,
-                                      splits, p.subs * 16);
+        const float2 t = col < cols ? ((const float2*)(ws + p.tot))[piece * 16 + l16] : make_float2(-INFINITY, 0.0f);
         const float sc = ldexpf(((const float*)(ws + p.qs))[piece * 16 + l16], e - 7);
         const float base = t.x == -INFINITY ? 0.0f : -t.x;
         const bool large = __any(!(fabsf(base) < M_LARGE));
@@ -623,7 +1042,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 float a = __builtin_fmaf(acc[tt][r], sc, base);
-                if (large && a > 0.0f) a = 0.0f;   // its rounding alone can be above M
+                if (large && a > P_ROOM) a = P_ROOM;   // its rounding alone can be above that
                 const float x = __builtin_amdgcn_exp2f(a) * t.y;
                 got[tt][r] += edge && r0 + 16 * tt + 4 * j4 + r > last ? 0.0f : x;
             }
@@ -648,34 +1067,43 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
 }
 
 template <int NG>
-static hipError_t weigh_ng(hipStream_t st, const CacheDev& c, const WeighJobs& jobs, const WeighPlan& p, bool few,
+static hipError_t weigh_ng(hipStream_t st, const CacheDev& c, const WeighJobs& jobs, const WeighPlan& p, WeighKind kind,
                            const AxesDev& axes, const MarksDev& marks, const float* q, int64_t ldq, float* out, int64_t ldo,
                            uint8_t* ws) {
     constexpr int D = 32 * NG, CH = 16 * D / WEIGH_JOIN, PER_PAGE = NG > 4 ? 2 : 1;
-    hipError_t e = hipSuccess;
-    if (!few && p.weigh) e = op_launch(k_weigh_query<NG>, dim3(jobs.joins), dim3(256), st, c, jobs, p, axes, q, ldq, ws);
-    if (e == hipSuccess)
-        e = op_launch(k_weigh<NG>, dim3(op_blocks(jobs.units)), dim3(256), st, c, jobs, p, axes, q, ldq, out, ldo, ws);
+    const dim3 units(op_blocks(jobs.units));
+    const int before = jobs.joins + (kind == WEIGH_WIDE ? jobs.pages / 4 : 0);
+    hipError_t e = op_launch(k_weigh_query<NG>, dim3(before), dim3(256), st, c, jobs, p, axes, q, ldq, ws);
+    if (e != hipSuccess) return e;
+    auto page = [&](auto k) { return op_launch(k, units, dim3(256), st, c, jobs, p, out, ldo, ws); };
+    if (kind != WEIGH_WIDE) {
+        if (p.subs == 1) e = page(k_weigh_page<NG, 1>);
+        else if (p.subs == 2) e = page(k_weigh_page<NG, 2>);
+        else if (p.subs == 3) e = page(k_weigh_page<NG, 3>);
+        else e = page(k_weigh_page<NG, 4>);
+    } else {
+        e = op_launch(k_weigh_many<NG, (NG > 4 ? 1 : 2), 8, (NG > 2 ? 32 : 64)>, units, dim3(512), st, c, jobs, p, out, ldo, ws);
+    }
     bool split = false;
     for (int j = 0; j < jobs.n; j++) split = split || weigh_pages(jobs.j[j]) > p.per;
     WeighJobs finish = jobs;
     if (!split) finish.joins = 0;
-    const int blocks = finish.joins * CH + (few && p.weigh ? jobs.pages / FINISH_PAGES : 0);
+    const int blocks = finish.joins * CH + (kind != WEIGH_WIDE && p.weigh ? jobs.pages / FINISH_PAGES : 0);
     if (e == hipSuccess && blocks)
         e = op_launch(k_weigh_finish<NG>, dim3(blocks), dim3(256), st, c, finish, p, marks, out, ldo, ws);
-    if (e == hipSuccess && !few && p.weigh)
+    if (e == hipSuccess && kind == WEIGH_WIDE && p.weigh)
         e = op_launch(k_weigh_sums<NG>, dim3(jobs.pages * PER_PAGE / 4), dim3(256), st, c, jobs, p, marks, ws);
     return e;
 }
 
-hipError_t launch_weigh(hipStream_t st, const CacheDev& c, const WeighJobs& jobs, const WeighPlan& plan, bool few,
+hipError_t launch_weigh(hipStream_t st, const CacheDev& c, const WeighJobs& jobs, const WeighPlan& plan, WeighKind kind,
                         const AxesDev& axes, const MarksDev& marks, const float* q, int64_t ldq, float* out, int64_t ldo,
                         uint8_t* ws) {
     WeighPlan p = plan;
     p.vec = aligned16(q) && aligned16(c.rope) && ldq % 4 == 0 && c.rot % 16 == 0;
-    if (c.ng == 2) return weigh_ng<2>(st, c, jobs, p, few, axes, marks, q, ldq, out, ldo, ws);
-    if (c.ng == 4) return weigh_ng<4>(st, c, jobs, p, few, axes, marks, q, ldq, out, ldo, ws);
-    return weigh_ng<8>(st, c, jobs, p, few, axes, marks, q, ldq, out, ldo, ws);
+    if (c.ng == 2) return weigh_ng<2>(st, c, jobs, p, kind, axes, marks, q, ldq, out, ldo, ws);
+    if (c.ng == 4) return weigh_ng<4>(st, c, jobs, p, kind, axes, marks, q, ldq, out, ldo, ws);
+    return weigh_ng<8>(st, c, jobs, p, kind, axes, marks, q, ldq, out, ldo, ws);
 }
 
 // ================================================================== evict ===

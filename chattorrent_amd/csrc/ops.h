@@ -112,11 +112,15 @@ struct WeighPlan {
     int group = 0, per = 1, subs = 1, score_cols = 0;
     bool vec = false, weigh = false;
     float fade = 1.0f;
-    size_t ml = 0, parts = 0, scores = 0, q = 0, qs = 0, bytes = 0;   // offsets into the workspace, and its size
+    size_t ml = 0, parts = 0, scores = 0, q = 0, qs = 0, exps = 0, tot = 0, bytes = 0;   // offsets into the workspace, its size
 };
 constexpr int WEIGH_JOIN = 256;   // floats of a unit's output that a workgroup joins
-// few: each job has at most 16 columns.
-hipError_t launch_weigh(hipStream_t st, const CacheDev& c, const WeighJobs& jobs, const WeighPlan& p, bool few,
+// By a job's columns: at most 16; up to 64 (a launch's jobs take as many
+// 16-column pieces as the largest of them); more, for eight waves of
+// weigh_wave_subs(D) pieces each.
+enum WeighKind { WEIGH_FEW, WEIGH_NARROW, WEIGH_WIDE };
+inline int weigh_wave_subs(int D) { return D > 128 ? 1 : 2; }
+hipError_t launch_weigh(hipStream_t st, const CacheDev& c, const WeighJobs& jobs, const WeighPlan& p, WeighKind kind,
                         const AxesDev& axes, const MarksDev& marks, const float* q, int64_t ldq, float* out, int64_t ldo,
                         uint8_t* ws);
 

@@ -13,8 +13,8 @@ import test_host_binding as two
 import test_host_operators as one
 
 MORE = """
-NAMES = ("k_kv_append_at", "k_weigh_query", "k_weigh_finish", "k_weigh_sums", "k_weigh_many", "k_weigh", "k_evict_select",
-         "k_evict_move")
+NAMES = ("k_kv_append_at", "k_weigh_query", "k_weigh_page", "k_weigh_many", "k_weigh_finish", "k_weigh_sums",
+         "k_evict_select", "k_evict_move")
 def launched():
     return [next(k for k in NAMES if k in n) for n in hip.stand_in_launches().decode().split() if any(k in n for k in NAMES)]
 
@@ -185,11 +185,12 @@ out["stale"] = [weigh(c, (0, 100, 60), **big), append_at(c, (0, 0, 1)), evict(c,
 hip.hipGetLastError()
 """)
     assert out["append"] == ["k_kv_append_at"] and out["many"] == ["k_kv_append_at"] * 3
-    assert out["token"] == ["k_weigh"] == out["off"] and out["weighed"] == ["k_weigh", "k_weigh_finish"]
+    page = ["k_weigh_query", "k_weigh_page"]
+    assert out["token"] == page == out["off"] and out["weighed"] == page + ["k_weigh_finish"]
     assert out["chunk"][0] == "k_weigh_query" and out["chunk"][-1] == "k_weigh_sums"
     assert "k_weigh_sums" not in out["alone"] and "k_weigh_finish" not in out["token"]
-    assert out["both"][:2] == ["k_weigh", "k_weigh_finish"] and out["both"][-1] == "k_weigh_sums"
-    assert out["jobs"].count("k_weigh") == 3 and out["pieces"].count("k_weigh_sums") == 3
+    assert out["both"][:3] == page + ["k_weigh_finish"] and out["both"][-1] == "k_weigh_sums"
+    assert out["jobs"].count("k_weigh_page") == 3 and out["pieces"].count("k_weigh_sums") == 3
     assert out["none"] == [] and out["one"] == ["k_evict_select"] and out["lot"] == ["k_evict_select", "k_evict_move"]
     assert out["jobs_"] == ["k_evict_select", "k_evict_move"] * 3
     assert out["failed"] == [[8, 0, k + 1] for k in range(3)] + [[8, 0, 1], [8, 0, 2], [8, 0, 1]]
