@@ -2419,8 +2419,10 @@ constexpr int WEIGH_ROWS = 4096;              // rows of a piece, of up to 2048 
 constexpr int64_t WEIGH_UNITS = 1 << 20, WEIGH_PAGES = 1 << 24;   // of a launch with several jobs
 int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The pages of an attention workgroup. Up to 64 columns: such that there are
-// some eight workgroups for each compute unit. More: the cut of the longest job
+// The pages of an attention workgroup. Up to 16 columns: such that there are
+// some eight workgroups for each compute unit (32 chats, heads of 128: 127 us;
+// four 151, two 147); up to 64, two (16 x 8 verify rows, heads of 256: 74 us;
+// four 84, eight 103). More: the cut of the longest job
 // with the least time, counted in pages that a compute unit, which holds one
 // workgroup, does after another, with two pages' time to begin with.
 int weigh_per(int ncu, const WeighJobs& b, const WeighPlan& p, int64_t nkv, WeighKind kind) {
@@ -2432,7 +2434,8 @@ int weigh_per(int ncu, const WeighJobs& b, const WeighPlan& p, int64_t nkv, Weig
         work += nkv * ceil_div(b.j[j].n * p.group, 16 * p.subs) * pages;
     }
     const int least = std::max(ceil_div(longest, 128), 1);
-    if (kind != WEIGH_WIDE) return (int)std::min<int64_t>(256, std::max<int64_t>({2, ceil_div64(work, 8 * (int64_t)ncu), least}));
+    if (kind != WEIGH_WIDE)
+        return (int)std::min<int64_t>(256, std::max<int64_t>({2, ceil_div64(work, (kind == WEIGH_FEW ? 8 : 2) * (int64_t)ncu), least}));
     const int64_t slots = ncu;
     int best = 0;
     int64_t cost = 0;
@@ -2447,6 +2450,29 @@ int weigh_per(int ncu, const WeighJobs& b, const WeighPlan& p, int64_t nkv, Weig
             cost = t;
         }
         if (per == least) break;
+    }
+    return best;
+}
+
+// The chunks of the counting columns that k_weigh_sums takes apart: the cut with
+// the least time, in 16-column pieces that a compute unit, which holds two
+// workgroups, does after another, with eight pieces' time to begin with.
+int weigh_chunks(int ncu, const WeighJobs& b, const WeighPlan& p, int64_t nkv, int D) {
+    int64_t groups = 0;
+    int most = 1;
+    for (int j = 0; j < b.n; j++) {
+        if (b.j[j].count0 >= b.j[j].n) continue;
+        groups += nkv * ceil_div(ceil_div(b.j[j].past + b.j[j].n, 64), D > 128 ? 2 : 4);
+        most = std::max(most, ceil_div(b.j[j].n * p.group, 16) - b.j[j].count0 * p.group / 16);
+    }
+    int best = 1;
+    int64_t cost = 0;
+    for (int k = 1; k <= std::min(most, 16); k++) {
+        const int64_t t = ceil_div64(groups * k, 2 * (int64_t)ncu) * (ceil_div(most, k) + 8);
+        if (!cost || t < cost) {
+            best = k;
+            cost = t;
+        }
     }
     return best;
 }
@@ -2497,7 +2523,9 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
             p.q = take(true, (size_t)joins * 16 * D * 4);
             p.qs = take(true, (size_t)joins * 64);
             p.exps = take(pairs, (size_t)b.pages * 16);
-            p.tot = take(kind == WEIGH_WIDE && weigh, (size_t)joins * 128);
+            p.tot = take(pairs && weigh, (size_t)joins * 128);
+            if (pairs && weigh) p.chunks = weigh_chunks(ctx->ncu, b, p, nkv, D);
+            p.lines = take(p.chunks > 1, (size_t)p.chunks * b.pages * 256);
             p.bytes = at;
             most = std::max(most, p.bytes);
             const bool ok = f(b, p, kind);

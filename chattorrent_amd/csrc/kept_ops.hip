@@ -516,78 +516,84 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
     }
 }
 
-// M and 1/l of a column over its unit's splits (0 where it sees nothing), the
-// splits' sums in their order; at: the first split's (M, l), `stride` from one
-// split to the next.
-__device__ static inline float2 column_total(const float2* __restrict__ at, int splits, int stride) {
+// M and l of a column over a unit's splits, dealt to the lane's row of 16
+// (lane / 16 of four): at is the column's first (M, l), `stride` from one split
+// to the next. Then over the four rows, in a fixed order.
+__device__ static inline float2 column_total(const float2* __restrict__ at, int splits, int stride, int row) {
     float m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < splits; s++) {
-        const float2 v = at[(size_t)s * stride];
-        const float mn = fmaxf(m, v.x);
-        l = l * pow2_diff(m, mn) + v.y * pow2_diff(v.x, mn);
+    for (int s0 = row; s0 < splits; s0 += 32) {
+        float2 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = s0 + 4 * i < splits ? at[(size_t)(s0 + 4 * i) * stride] : make_float2(-INFINITY, 0.0f);
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < 8; i++) mn = fmaxf(mn, v[i].x);
+        l *= pow2_diff(m, mn);
+#pragma unroll
+        for (int i = 0; i < 8; i++) l = __builtin_fmaf(v[i].y, pow2_diff(v[i].x, mn), l);
         m = mn;
     }
-    return make_float2(m, l != 0.0f ? 1.0f / l : 0.0f);
+    const float mx = rows_max(m);
+    l *= pow2_diff(m, mx);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    return make_float2(mx, l);
 }
 
-// After k_weigh: joins the splits' outputs (the first jobs.joins workgroups,
-// WEIGH_JOIN floats of a 16-column piece each, its splits dealt to four waves),
+// After k_weigh_page: joins the splits' outputs (the first workgroups, a
+// WEIGH_JOIN floats of a 16-column piece each, its splits dealt to four waves)
 // and, from the stored scores, adds up the weights of FINISH_PAGES pages of a
-// (job, kv head) a workgroup, a token a lane.
+// (job, kv head) a workgroup, a row a lane.
 template <int NG>
 __global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs, WeighPlan p, MarksDev marks,
-                                                      float* __restrict__ out, int64_t ldo, uint8_t* __restrict__ ws) {
+                                                      float* __restrict__ out, int64_t ldo, const uint8_t* __restrict__ ws) {
     constexpr int D = 32 * NG, CH = 16 * D / WEIGH_JOIN;   // chunks of a 16-column piece
-    __shared__ __align__(16) float red[4][WEIGH_JOIN];
+    __shared__ __align__(16) float4_t red[4][64];
     __shared__ float2 total[64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float2* ml = (const float2*)(ws + p.ml);
     if ((int)blockIdx.x < jobs.joins * CH) {
         const int piece = (int)blockIdx.x / CH, ch = (int)blockIdx.x % CH;
         const WeighJob jb = jobs.j[weigh_job_at(jobs, piece, &WeighJob::join0)];
-        const int tiles = weigh_tiles(jb, p), splits = (weigh_pages(jb) + p.per - 1) / p.per;
+        const int splits = (weigh_pages(jb) + p.per - 1) / p.per;
         if (splits == 1) return;   // the attention kernel wrote them
-        const int r = piece - jb.join0, sub = r % p.subs, tile = r / p.subs % tiles, head = r / p.subs / tiles;
-        const int col0 = (tile * p.subs + sub) * 16, gt = min(16, jb.n * p.group - col0);
+        const int r = piece - jb.join0, sub = r % p.subs, head = r / p.subs;
+        const int gt = min(16, jb.n * p.group - sub * 16);
         const int h = (ch * WEIGH_JOIN + lane * 4) / D, d = (ch * WEIGH_JOIN + lane * 4) % D;
         if (ch * WEIGH_JOIN / D >= gt) return;
-        const size_t unit = (size_t)jb.unit0 + ((size_t)head * tiles + tile) * splits;
-        const float2* at = ml + (unit * p.subs + sub) * 16 + h;
-        const float* part = (const float*)(ws + p.parts) + (unit * p.subs + sub) * 16 * D + ch * WEIGH_JOIN + lane * 4;
-        float m = -INFINITY, l = 0.0f;
-        float4_t x = {0.f, 0.f, 0.f, 0.f};
-        if (h < gt) {
-#pragma unroll 4
-            for (int s = wave; s < splits; s += 4) {
-                const float2 v = at[(size_t)s * p.subs * 16];
-                const float4_t y = *(const float4_t*)(part + (size_t)s * p.subs * 16 * D);
-                if (v.x == -INFINITY && v.y == 0.0f) continue;   // nothing seen: there is no part
-                const float mn = fmaxf(m, v.x), fa = pow2_diff(m, mn), fb = pow2_diff(v.x, mn);
-                l = l * fa + v.y * fb;
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = x[e] * fa + y[e] * fb;
-                m = mn;
-            }
+        const size_t unit = (size_t)jb.unit0 + (size_t)head * splits;
+        if (wave == 0) {   // every column's M and l
+            const float2 t = column_total(ml + (unit * p.subs + sub) * 16 + (lane & 15), splits, p.subs * 16, lane >> 4);
+            if (lane < 16) total[lane] = t;
         }
-        __shared__ float2 wml[4][64];
-        wml[wave][lane] = make_float2(m, l);
-        *(float4_t*)&red[wave][lane * 4] = x;
+        __syncthreads();
+        const float2* at = ml + (unit * p.subs + sub) * 16 + h;
+        const float4_t* part = (const float4_t*)(ws + p.parts) + ((unit * p.subs + sub) * 16 * D + ch * WEIGH_JOIN) / 4 + lane;
+        const float m = total[h].x;
+        float4_t x = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = wave; s0 < splits; s0 += 16) {
+            float4_t y[4];
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int s = min(s0 + 4 * i, splits - 1);
+                v[i] = at[(size_t)s * p.subs * 16];
+                y[i] = part[(size_t)s * p.subs * 4 * D];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (s0 + 4 * i < splits && !(v[i].x == -INFINITY && v[i].y == 0.0f)) x += y[i] * pow2_diff(v[i].x, m);
+        }
+        red[wave][lane] = x;
         __syncthreads();
         if (wave || h >= gt) return;
-        for (int v = 1; v < 4; v++) {
-            const float2 o = wml[v][lane];
-            const float4_t y = *(const float4_t*)&red[v][lane * 4];
-            const float mn = fmaxf(m, o.x), fa = pow2_diff(m, mn), fb = pow2_diff(o.x, mn);
-            l = l * fa + o.y * fb;
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = x[e] * fa + y[e] * fb;
-            m = mn;
-        }
-        const int col = col0 + h;
+        x = (x + red[1][lane]) + (red[2][lane] + red[3][lane]);
+        const float l = total[h].y;
+        const int col = sub * 16 + h;
         float* dst = out + ((int64_t)jb.row0 + col / p.group) * ldo + (size_t)(head * p.group + col % p.group) * D + d;
 #pragma unroll
-        for (int e = 0; e < 4; e++) dst[e] = l != 0.0f ? x[e] / l : 0.0f;
-        if (p.tot && d == 0) ((float2*)(ws + p.tot))[(size_t)piece * 16 + h] = make_float2(m, l != 0.0f ? 1.0f / l : 0.0f);
+        for (int e = 0; e < 4; e++) x[e] = l != 0.0f ? x[e] / l : 0.0f;
+        *(float4_a4*)dst = x;
         return;
     }
     const int u = ((int)blockIdx.x - jobs.joins * CH) * FINISH_PAGES;
@@ -597,23 +603,76 @@ __global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs
     const int splits = (pages + p.per - 1) / p.per;
     const int c0 = jb.count0 * p.group, cols = jb.n * p.group;
     const size_t unit = (size_t)jb.unit0 + (size_t)head * splits;   // one tile a (job, kv head)
-    if (tid < cols) total[tid] = column_total(ml + unit * p.subs * 16 + tid, splits, p.subs * 16);
+    if (wave < p.subs && 16 * wave < cols) {
+        const int col = 16 * wave + (lane & 15);
+        const float2 t = column_total(ml + unit * p.subs * 16 + col, splits, p.subs * 16, lane >> 4);
+        if (lane < 16) total[col] = make_float2(t.x == -INFINITY ? 0.0f : t.x, t.y != 0.0f ? 1.0f / t.y : 0.0f);
+    }
     __syncthreads();
     for (int i = wave; i < FINISH_PAGES && p0 + i < pages; i += 4) {
-        const int pg = p0 + i;
+        const int pg = p0 + i, row = 64 * pg + lane;
         const uint32_t id = c.page_table[(size_t)jb.slot * c.max_pages + pg];
-        if (id >= (uint32_t)c.n_pages || 64 * pg + lane >= jb.past + jb.n) continue;
+        if (id >= (uint32_t)c.n_pages || row >= jb.past + jb.n) continue;
         float* wt = marks.weight + ((size_t)id * c.nKV + head) * 64 + lane;
         const float* s = (const float*)(ws + p.scores) + ((size_t)jb.page0 + (size_t)head * room + pg) * p.score_cols * 64 + lane;
-        const float before = p.fade == 0.0f && 64 * pg + lane >= jb.fresh ? 0.0f : *wt;
+        const float before = p.fade == 0.0f && row >= jb.fresh ? 0.0f : *wt;
         float got = 0.0f;
-        for (int col = c0; col < cols; col++) {
-            const float2 t = total[col];
-            const float x = __builtin_amdgcn_exp2f(s[(size_t)col * 64] - (t.x == -INFINITY ? 0.0f : t.x));
-            got = __builtin_fmaf(x, t.y, got);
+        for (int col = c0; col < cols; col += 8) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = s[(size_t)min(col + e, cols - 1) * 64];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float2 t = total[min(col + e, cols - 1)];
+                if (col + e < cols) got = __builtin_fmaf(__builtin_amdgcn_exp2f(x[e] - t.x), t.y, got);
+            }
         }
-        *wt = __builtin_fmaf(before, 64 * pg + lane >= jb.fresh ? p.fade : 1.0f, got);
+        *wt = __builtin_fmaf(before, row >= jb.fresh ? p.fade : 1.0f, got);   // (weigh_add, the load ahead)
     }
+}
+
+// After k_weigh_many, where a tile's pages were split: joins the outputs of
+// 1024 / D columns of a piece a workgroup, 4 channels a thread, and leaves the
+// columns' M and 1/l.
+template <int NG>
+__global__ __launch_bounds__(256) void k_weigh_join(WeighJobs jobs, WeighPlan p, float* __restrict__ out, int64_t ldo,
+                                                    uint8_t* __restrict__ ws) {
+    constexpr int D = 32 * NG, CH = D / 64;
+    const int piece = (int)blockIdx.x / CH, i = ((int)blockIdx.x % CH) * 256 + (int)threadIdx.x, h = 4 * i / D, d = 4 * i % D;
+    const WeighJob jb = jobs.j[weigh_job_at(jobs, piece, &WeighJob::join0)];
+    const int tiles = weigh_tiles(jb, p), splits = (weigh_pages(jb) + p.per - 1) / p.per;
+    if (splits == 1) return;   // the attention kernel wrote them
+    const int r = piece - jb.join0, sub = r % p.subs, tile = r / p.subs % tiles, head = r / p.subs / tiles;
+    const int col = (tile * p.subs + sub) * 16 + h;
+    if (col >= jb.n * p.group) return;
+    const size_t unit = (size_t)jb.unit0 + ((size_t)head * tiles + tile) * splits;
+    const float2* at = (const float2*)(ws + p.ml) + (unit * p.subs + sub) * 16 + h;
+    const float4_t* part = (const float4_t*)(ws + p.parts) + (unit * p.subs + sub) * 4 * D + i;
+    float m = -INFINITY, l = 0.0f;
+    float4_t x = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < splits; s0 += 4) {
+        float4_t y[4];
+        float2 v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int s = min(s0 + e, splits - 1);
+            v[e] = at[(size_t)s * p.subs * 16];
+            y[e] = part[(size_t)s * p.subs * 4 * D];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (s0 + e >= splits || (v[e].x == -INFINITY && v[e].y == 0.0f)) continue;   // nothing seen: there is no part
+            const float mn = fmaxf(m, v[e].x), fa = pow2_diff(m, mn), fb = pow2_diff(v[e].x, mn);
+            l = l * fa + v[e].y * fb;
+            x = x * fa + y[e] * fb;
+            m = mn;
+        }
+    }
+    float* dst = out + ((int64_t)jb.row0 + col / p.group) * ldo + (size_t)(head * p.group + col % p.group) * D + d;
+    if (p.tot && d == 0) ((float2*)(ws + p.tot))[(size_t)piece * 16 + h] = make_float2(m, l != 0.0f ? 1.0f / l : 0.0f);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = l != 0.0f ? x[e] / l : 0.0f;
+    *(float4_a4*)dst = x;
 }
 
 // Attention of a tile of 16 * CT columns for each of W waves over `per` pages.
@@ -968,85 +1027,119 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
 
 // The weights from many columns: q . k again, with the columns' M and l known.
 // A wave holds the keys of 16 * TT rows of the cache as f16 pairs in registers
-// and walks the columns, 16 at a time; a lane adds up its 4 * TT rows' p / l,
-// and 16 lanes meet at the end, in a fixed order.
+// and walks the columns of its chunk, a piece of 16 at a time, which its
+// workgroup's four waves share through LDS; a lane adds up its 4 * TT rows' p /
+// l, and 16 lanes meet at the end, in a fixed order. With one chunk the result
+// goes to the marks, else to the chunk's line in the workspace (k_weigh_add).
+__device__ static inline void weigh_add(float* at, const WeighPlan& p, bool fades, float got) {
+    const float before = fades && p.fade == 0.0f ? 0.0f : *at;
+    *at = __builtin_fmaf(before, fades ? p.fade : 1.0f, got);
+}
 template <int NG>
 __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs jobs, WeighPlan p, MarksDev marks,
-                                                       const uint8_t* __restrict__ ws) {
-    constexpr int D = 32 * NG, TT = NG > 4 ? 2 : 4, PER_PAGE = 4 / TT;
+                                                       uint8_t* __restrict__ ws) {
+    constexpr int D = 32 * NG, TT = NG > 4 ? 2 : 4, PER_PAGE = 4 / TT, NQ = NG / 2;   // NQ: 16 bytes a thread of a piece
+    __shared__ u32x4 qs[2][2 * NG * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j4 = lane >> 4, l16 = lane & 15;
     constexpr int WGS = FINISH_PAGES * PER_PAGE / 4;   // workgroups of FINISH_PAGES pages
     const int u = (int)blockIdx.x / WGS * FINISH_PAGES;
     const WeighJob jb = jobs.j[weigh_job_at(jobs, u, &WeighJob::page0)];
     if (jb.count0 >= jb.n) return;   // a piece of a job before the rows that count
     const int pages = weigh_pages(jb), room = page_room(pages), head = (u - jb.page0) / room;
-    const int part = (u - jb.page0) % room * PER_PAGE + (int)blockIdx.x % WGS * 4 + wave;   // 16 * TT rows each
-    const int pg = part / PER_PAGE, r0 = part * 16 * TT;     // the first of the wave's rows
-    if (pg >= pages) return;
-    const uint32_t id = c.page_table[(size_t)jb.slot * c.max_pages + pg];
-    if (id >= (uint32_t)c.n_pages) return;
-    const int held = jb.past + jb.n;
-    const uint8_t* blk = c.k + ((size_t)id * c.nKV + head) * c.blk;
-    half8_t kh[TT][NG], kl[TT][NG];
-    const int e = (int8_t)ws[p.exps + (size_t)(jb.page0 + head * room + pg) * 16 + PAIR_K];
-    {
-        float sc[TT][NG];
+    const int part0 = (u - jb.page0) % room * PER_PAGE + (int)blockIdx.x % WGS * 4;   // the workgroup's first: 16 * TT rows each
+    if (part0 / PER_PAGE >= pages) return;
+    const int part = part0 + wave, pg = part / PER_PAGE, r0 = part * 16 * TT;     // the first of the wave's rows
+    const uint32_t id = pg < pages ? c.page_table[(size_t)jb.slot * c.max_pages + pg] : 0xffffffffu;
+    const bool busy = id < (uint32_t)c.n_pages;
+    const int held = jb.past + jb.n, tiles = weigh_tiles(jb, p);
+    const int c0 = jb.count0 * p.group, cols = jb.n * p.group;
+    // the chunk's pieces, from the first whose columns see one of the workgroup's rows
+    const int t0 = c0 / 16, t1 = (cols + 15) / 16, step = (t1 - t0 + p.chunks - 1) / p.chunks;
+    const int to = min(t0 + ((int)blockIdx.y + 1) * step, t1);
+    const int from = max(t0 + (int)blockIdx.y * step, max(c0, max(0, part0 * 16 * TT - jb.past) * p.group) / 16);
+    const int my_from = busy ? max(0, r0 - jb.past) * p.group / 16 : to;
+    const size_t piece0 = (size_t)jb.join0 + (size_t)head * tiles * p.subs;
+    float4_t got[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; tt++) got[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
+    u32x4 qn[NQ];
+    float2 tn;
+    float scn;
+    auto load = [&](int t16) {
+        const u32x4* of = (const u32x4*)(ws + p.q) + (piece0 + t16) * 2 * NG * 64;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) qn[i] = of[256 * i + tid];
+        const int col = t16 * 16 + l16;
+        tn = col < cols ? ((const float2*)(ws + p.tot))[(piece0 + t16) * 16 + l16] : make_float2(-INFINITY, 0.0f);
+        scn = ((const float*)(ws + p.qs))[(piece0 + t16) * 16 + l16];
+    };
+    if (from < to) {
+        load(from);
+        half8_t kh[TT][NG], kl[TT][NG];
+        // (a wave without a page goes through page 0's keys, for nothing)
+        const uint8_t* blk = c.k + ((size_t)(busy ? id : 0u) * c.nKV + head) * c.blk;
+        const int e = busy ? (int8_t)ws[p.exps + (size_t)(jb.page0 + head * room + pg) * 16 + PAIR_K] : 0;
+        const float down = pair_down(e);
 #pragma unroll
         for (int tt = 0; tt < TT; tt++) {
             const int r = r0 + 16 * tt + l16;
             const float* at = (const float*)(blk + 64 * D) + (r & 63) * NG;
 #pragma unroll
-            for (int g = 0; g < NG; g++) sc[tt][g] = r < held ? at[g] : 0.0f;
-        }
-        const float down = pair_down(e);
-#pragma unroll
-        for (int tt = 0; tt < TT; tt++)
-#pragma unroll
             for (int g = 0; g < NG; g += 2) {
-                const u32x4 w = *(const u32x4*)(blk + (size_t)((r0 & 63) + 16 * tt + l16) * D + (D / 4) * j4 + 8 * g);
-                code_pair(w[0], w[1], sc[tt][g] * down, kh[tt][g], kl[tt][g]);
-                code_pair(w[2], w[3], sc[tt][g + 1] * down, kh[tt][g + 1], kl[tt][g + 1]);
-            }
-    }
-    const int tiles = weigh_tiles(jb, p);
-    const int c0 = jb.count0 * p.group, cols = jb.n * p.group;
-    const int from = max(c0, max(0, r0 - jb.past) * p.group);   // the first column that sees one of the wave's rows
-    float4_t got[TT];
-#pragma unroll
-    for (int tt = 0; tt < TT; tt++) got[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
-    for (int t16 = from / 16; t16 * 16 < cols; t16++) {
-        const size_t piece = (size_t)jb.join0 + (size_t)head * tiles * p.subs + t16;
-        const u32x4* qf = (const u32x4*)(ws + p.q) + piece * 2 * NG * 64 + lane;
-        float4_t acc[TT];
-#pragma unroll
-        for (int tt = 0; tt < TT; tt++) acc[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            const half8_t qh = __builtin_bit_cast(half8_t, qf[g * 64]), ql = __builtin_bit_cast(half8_t, qf[(NG + g) * 64]);
-#pragma unroll
-            for (int tt = 0; tt < TT; tt++) {
-                acc[tt] = mfma16x16x32(kh[tt][g], qh, acc[tt]);
-                acc[tt] = mfma16x16x32(kl[tt][g], qh, acc[tt]);
-                acc[tt] = mfma16x16x32(kh[tt][g], ql, acc[tt]);
+                const u32x4 w = *(const u32x4*)(blk + (size_t)(r & 63) * D + (D / 4) * j4 + 8 * g);
+                const float2 sc = *(const float2*)(at + g);
+                code_pair(w[0], w[1], r < held ? sc.x * down : 0.0f, kh[tt][g], kl[tt][g]);
+                code_pair(w[2], w[3], r < held ? sc.y * down : 0.0f, kh[tt][g + 1], kl[tt][g + 1]);
             }
         }
-        const int col = t16 * 16 + l16;
-        const float2 t = col < cols ? ((const float2*)(ws + p.tot))[piece * 16 + l16] : make_float2(-INFINITY, 0.0f);
-        const float sc = ldexpf(((const float*)(ws + p.qs))[piece * 16 + l16], e - 7);
-        const float base = t.x == -INFINITY ? 0.0f : -t.x;
-        const bool large = __any(!(fabsf(base) < M_LARGE));
-        const int last = col >= c0 && col < cols ? jb.past + col / p.group : -1;
-        const bool edge = t16 * 16 < c0 || t16 * 16 + 16 > cols || jb.past + t16 * 16 / p.group < r0 + 16 * TT - 1;
+        for (int t16 = from; t16 < to; t16++) {
+            const int b = t16 & 1;
 #pragma unroll
-        for (int tt = 0; tt < TT; tt++)
+            for (int i = 0; i < NQ; i++) qs[b][256 * i + tid] = qn[i];
+            const float2 t = tn;
+            const float sc = ldexpf(scn, e - 7);
+            __syncthreads();   // (a piece's place is written again two pieces on, past the next barrier)
+            if (t16 + 1 < to) load(t16 + 1);
+            if (t16 < my_from) continue;
+            float4_t acc[TT];
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float a = __builtin_fmaf(acc[tt][r], sc, base);
-                if (large && a > P_ROOM) a = P_ROOM;   // its rounding alone can be above that
-                const float x = __builtin_amdgcn_exp2f(a) * t.y;
-                got[tt][r] += edge && r0 + 16 * tt + 4 * j4 + r > last ? 0.0f : x;
+            for (int tt = 0; tt < TT; tt++) acc[tt] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const half8_t qh = __builtin_bit_cast(half8_t, qs[b][g * 64 + lane]);
+                const half8_t ql = __builtin_bit_cast(half8_t, qs[b][(NG + g) * 64 + lane]);
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++) acc[tt] = mfma16x16x32(kh[tt][g], qh, acc[tt]);
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++) acc[tt] = mfma16x16x32(kl[tt][g], qh, acc[tt]);
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++) acc[tt] = mfma16x16x32(kh[tt][g], ql, acc[tt]);
             }
+            const float base = t.x == -INFINITY ? 0.0f : -t.x;
+            const bool large = __any(!(fabsf(base) < M_LARGE));
+            const bool edge = t16 * 16 < c0 || t16 * 16 + 16 > cols || jb.past + t16 * 16 / p.group < r0 + 16 * TT - 1;
+            if (!large && !edge) {
+#pragma unroll
+                for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        got[tt][r] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(acc[tt][r], sc, base)), t.y, got[tt][r]);
+                continue;
+            }
+            const int col = t16 * 16 + l16, last = col >= c0 && col < cols ? jb.past + col / p.group : -1;
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float a = __builtin_fmaf(acc[tt][r], sc, base);
+                    if (large && a > P_ROOM) a = P_ROOM;   // its rounding alone can be above that
+                    const bool sees = r0 + 16 * tt + 4 * j4 + r <= last;
+                    const float x = __builtin_amdgcn_exp2f(a);
+                    got[tt][r] = __builtin_fmaf(sees ? x : 0.0f, sees ? t.y : 0.0f, got[tt][r]);
+                }
+        }
     }
+    if (!busy) return;
 #pragma unroll
     for (int tt = 0; tt < TT; tt++)
 #pragma unroll
@@ -1054,16 +1147,35 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
             for (int o = 1; o < 16; o <<= 1) got[tt][r] += __shfl_xor(got[tt][r], o);
     if (l16) return;
     float* wt = marks.weight + ((size_t)id * c.nKV + head) * 64;
+    float4_t* line = (float4_t*)(ws + p.lines) + (((size_t)blockIdx.y * jobs.pages + jb.page0 + head * room + pg) * 64 + (r0 & 63) + 4 * j4) / 4;
 #pragma unroll
-    for (int tt = 0; tt < TT; tt++)
+    for (int tt = 0; tt < TT; tt++) {
+        if (p.chunks > 1) {
+            line[4 * tt] = got[tt];
+            continue;
+        }
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int row = r0 + 16 * tt + 4 * j4 + r;
-            if (row >= held) continue;
-            const bool fades = row >= jb.fresh;
-            const float before = fades && p.fade == 0.0f ? 0.0f : wt[row & 63];
-            wt[row & 63] = __builtin_fmaf(before, fades ? p.fade : 1.0f, got[tt][r]);
+            if (row < held) weigh_add(&wt[row & 63], p, row >= jb.fresh, got[tt][r]);
         }
+    }
+}
+
+// The chunks' lines, added in their order.
+__global__ __launch_bounds__(256) static void k_weigh_add(CacheDev c, WeighJobs jobs, WeighPlan p, MarksDev marks,
+                                                          const uint8_t* __restrict__ ws) {
+    const int u = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const WeighJob jb = jobs.j[weigh_job_at(jobs, u, &WeighJob::page0)];
+    const int pages = weigh_pages(jb), room = page_room(pages), head = (u - jb.page0) / room, pg = (u - jb.page0) % room;
+    if (jb.count0 >= jb.n || pg >= pages || 64 * pg + lane >= jb.past + jb.n) return;
+    const uint32_t id = c.page_table[(size_t)jb.slot * c.max_pages + pg];
+    if (id >= (uint32_t)c.n_pages) return;
+    const float* line = (const float*)(ws + p.lines) + (size_t)u * 64 + lane;
+    float got = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < p.chunks; i++) got += line[(size_t)i * jobs.pages * 64];
+    weigh_add(marks.weight + ((size_t)id * c.nKV + head) * 64 + lane, p, 64 * pg + lane >= jb.fresh, got);
 }
 
 template <int NG>
@@ -1086,13 +1198,19 @@ static hipError_t weigh_ng(hipStream_t st, const CacheDev& c, const WeighJobs& j
     }
     bool split = false;
     for (int j = 0; j < jobs.n; j++) split = split || weigh_pages(jobs.j[j]) > p.per;
-    WeighJobs finish = jobs;
-    if (!split) finish.joins = 0;
-    const int blocks = finish.joins * CH + (kind != WEIGH_WIDE && p.weigh ? jobs.pages / FINISH_PAGES : 0);
-    if (e == hipSuccess && blocks)
-        e = op_launch(k_weigh_finish<NG>, dim3(blocks), dim3(256), st, c, finish, p, marks, out, ldo, ws);
-    if (e == hipSuccess && kind == WEIGH_WIDE && p.weigh)
-        e = op_launch(k_weigh_sums<NG>, dim3(jobs.pages * PER_PAGE / 4), dim3(256), st, c, jobs, p, marks, ws);
+    if (kind != WEIGH_WIDE) {
+        WeighJobs finish = jobs;
+        if (!split) finish.joins = 0;
+        const int blocks = finish.joins * CH + (p.weigh ? jobs.pages / FINISH_PAGES : 0);
+        if (e == hipSuccess && blocks)
+            e = op_launch(k_weigh_finish<NG>, dim3(blocks), dim3(256), st, c, finish, p, marks, out, ldo, ws);
+        return e;
+    }
+    if (e == hipSuccess && split) e = op_launch(k_weigh_join<NG>, dim3(jobs.joins * (D / 64)), dim3(256), st, jobs, p, out, ldo, ws);
+    if (e == hipSuccess && p.weigh)
+        e = op_launch(k_weigh_sums<NG>, dim3(jobs.pages * PER_PAGE / 4, p.chunks), dim3(256), st, c, jobs, p, marks, ws);
+    if (e == hipSuccess && p.weigh && p.chunks > 1)
+        e = op_launch(k_weigh_add, dim3(jobs.pages / 4), dim3(256), st, c, jobs, p, marks, ws);
     return e;
 }
 

@@ -110,9 +110,10 @@ struct WeighJobs {
 };
 struct WeighPlan {
     int group = 0, per = 1, subs = 1, score_cols = 0;
+    int chunks = 1;   // of the columns whose weights k_weigh_sums adds up
     bool vec = false, weigh = false;
     float fade = 1.0f;
-    size_t ml = 0, parts = 0, scores = 0, q = 0, qs = 0, exps = 0, tot = 0, bytes = 0;   // offsets into the workspace, its size
+    size_t ml = 0, parts = 0, scores = 0, q = 0, qs = 0, exps = 0, tot = 0, lines = 0, bytes = 0;   // offsets into the workspace, its size
 };
 constexpr int WEIGH_JOIN = 256;   // floats of a unit's output that a workgroup joins
 // By a job's columns: at most 16; up to 64 (a launch's jobs take as many

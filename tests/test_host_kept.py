@@ -13,7 +13,7 @@ import test_host_binding as two
 import test_host_operators as one
 
 MORE = """
-NAMES = ("k_kv_append_at", "k_weigh_query", "k_weigh_page", "k_weigh_many", "k_weigh_finish", "k_weigh_sums",
+NAMES = ("k_kv_append_at", "k_weigh_query", "k_weigh_page", "k_weigh_many", "k_weigh_finish", "k_weigh_join", "k_weigh_sums", "k_weigh_add",
          "k_evict_select", "k_evict_move")
 def launched():
     return [next(k for k in NAMES if k in n) for n in hip.stand_in_launches().decode().split() if any(k in n for k in NAMES)]
@@ -187,9 +187,10 @@ hip.hipGetLastError()
     assert out["append"] == ["k_kv_append_at"] and out["many"] == ["k_kv_append_at"] * 3
     page = ["k_weigh_query", "k_weigh_page"]
     assert out["token"] == page == out["off"] and out["weighed"] == page + ["k_weigh_finish"]
-    assert out["chunk"][0] == "k_weigh_query" and out["chunk"][-1] == "k_weigh_sums"
+    many = ["k_weigh_query", "k_weigh_many", "k_weigh_join", "k_weigh_sums", "k_weigh_add"]
+    assert [k for k in many if k in out["chunk"]] == out["chunk"] and "k_weigh_sums" in out["chunk"]
     assert "k_weigh_sums" not in out["alone"] and "k_weigh_finish" not in out["token"]
-    assert out["both"][:3] == page + ["k_weigh_finish"] and out["both"][-1] == "k_weigh_sums"
+    assert out["both"][:3] == page + ["k_weigh_finish"] and out["both"][3:] == out["chunk"]
     assert out["jobs"].count("k_weigh_page") == 3 and out["pieces"].count("k_weigh_sums") == 3
     assert out["none"] == [] and out["one"] == ["k_evict_select"] and out["lot"] == ["k_evict_select", "k_evict_move"]
     assert out["jobs_"] == ["k_evict_select", "k_evict_move"] * 3
