@@ -2586,7 +2586,7 @@ size_t each_evict(const cc_cache* c, const cc_keep* jobs, int32_t njobs, F&& f) 
     int max_rows = 0;
     auto flush = [&]() {
         const bool ok = !b.n || f(b, max_rows);
-        b.n = b.room = max_rows = 0;
+        b.n = b.room = b.keep = max_rows = 0;
         words = 0;
         return ok;
     };
@@ -2598,7 +2598,10 @@ size_t each_evict(const cc_cache* c, const cc_keep* jobs, int32_t njobs, F&& f) 
         b.j[b.n++] = EvictJob{k.slot, k.rows, k.keep, k.seen, room, words};
         b.room = std::max(b.room, room);
         max_rows = std::max(max_rows, k.rows);
-        if (room > EVICT_HERE) words += (int64_t)c->n_kv_heads * (2 * (int64_t)room + 2);
+        if (room > EVICT_HERE) {
+            b.keep = std::max(b.keep, k.keep);
+            words += (int64_t)c->n_kv_heads * (int64_t)evict_list_words(b.j[b.n - 1]);
+        }
         most = std::max(most, (size_t)words * 4);
     }
     flush();

@@ -1233,44 +1233,91 @@ __device__ static inline uint32_t keep_key(float weight, int token, int sink, in
     return weight != weight ? 0u : order_bits(weight + 0.0f);
 }
 
-// One row's codes, scales and marks to another row of the same slot and kv
-// head, by a wave.
-template <int NG>
-__device__ static inline void move_row(const CacheDev& c, const MarksDev& marks, const uint32_t* pt, int head, int of, int to,
-                                       int lane) {
-    constexpr int D = 32 * NG;
-    const uint32_t pf = pt[of >> 6], ptt = pt[to >> 6];
-    if (pf >= (uint32_t)c.n_pages || ptt >= (uint32_t)c.n_pages) return;
-    const size_t bf = (size_t)pf * c.nKV + head, bt = (size_t)ptt * c.nKV + head;
-    const int s = of & 63, t = to & 63;
-    const uint8_t *kf = c.k + bf * c.blk, *vf = c.v + bf * c.blk;
-    uint8_t *kt = c.k + bt * c.blk, *vt = c.v + bt * c.blk;
-    if (lane < D / 4) *(uint32_t*)(kt + t * D + 4 * lane) = *(const uint32_t*)(kf + s * D + 4 * lane);
+// Where a move's two rows lie: their (page, kv head) blocks in the cache and
+// their places in them. of_row < 0: none.
+struct EvictMove {
+    uint32_t of, to;
+    int of_row, to_row;
+};
+
+// The codes, scales and marks of N rows at a time, by a wave: all N are loaded
+// before the first is stored (one after another a row waits for its page, its
+// codes and the row before it: 370 us for 32 prompts instead of 115).
+template <int NG, int N>
+__device__ static inline void move_rows(const CacheDev& c, const MarksDev& marks, const EvictMove* moves, int lane) {
+    constexpr int D = 32 * NG, VB = D / 64;
+    uint32_t kc[N], ks[N], vs[N], mk[N];
+    uint8_t vc[N][VB];
+    const int kl = min(lane, D / 4 - 1), gl = min(lane, NG - 1);
+    const uint32_t* mark = lane & 1 ? (const uint32_t*)marks.token : (const uint32_t*)marks.weight;
 #pragma unroll
-    for (int i = 0; i < D / 64; i++) vt[vcode_at(lane + 64 * i, t, D)] = vf[vcode_at(lane + 64 * i, s, D)];
-    if (lane < NG) {
-        *(uint32_t*)(kt + 64 * D + 4 * (t * NG + lane)) = *(const uint32_t*)(kf + 64 * D + 4 * (s * NG + lane));
-        *(uint32_t*)(vt + 64 * D + 4 * vscale_at(lane, t, NG)) = *(const uint32_t*)(vf + 64 * D + 4 * vscale_at(lane, s, NG));
+    for (int i = 0; i < N; i++) {
+        const EvictMove m = moves[i];
+        const int row = max(m.of_row, 0);
+        const uint8_t *k = c.k + (size_t)m.of * c.blk, *v = c.v + (size_t)m.of * c.blk;
+        kc[i] = *(const uint32_t*)(k + row * D + 4 * kl);
+        ks[i] = *(const uint32_t*)(k + 64 * D + 4 * (row * NG + gl));
+        vs[i] = *(const uint32_t*)(v + 64 * D + 4 * vscale_at(gl, row, NG));
+        mk[i] = mark[(size_t)m.of * 64 + row];
+#pragma unroll
+        for (int e = 0; e < VB; e++) vc[i][e] = v[vcode_at(lane + 64 * e, row, D)];
     }
-    if (lane == 32) marks.weight[bt * 64 + t] = marks.weight[bf * 64 + s];
-    if (lane == 33) marks.token[bt * 64 + t] = marks.token[bf * 64 + s];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const EvictMove m = moves[i];
+        if (m.of_row < 0) continue;
+        uint8_t *k = c.k + (size_t)m.to * c.blk, *v = c.v + (size_t)m.to * c.blk;
+        if (lane < D / 4) *(uint32_t*)(k + m.to_row * D + 4 * lane) = kc[i];
+        if (lane < NG) {
+            *(uint32_t*)(k + 64 * D + 4 * (m.to_row * NG + lane)) = ks[i];
+            *(uint32_t*)(v + 64 * D + 4 * vscale_at(lane, m.to_row, NG)) = vs[i];
+        }
+        if (lane < 2) (lane ? (uint32_t*)marks.token : (uint32_t*)marks.weight)[(size_t)m.to * 64 + m.to_row] = mk[i];
+#pragma unroll
+        for (int e = 0; e < VB; e++) v[vcode_at(lane + 64 * e, m.to_row, D)] = vc[i][e];
+    }
 }
+constexpr EvictMove NO_MOVE{0u, 0u, -1, -1};
+__device__ static inline EvictMove move_at(const CacheDev& c, const uint32_t* pt, int head, int of, int to) {
+    const uint32_t pf = pt[of >> 6], pg = pt[to >> 6];
+    if (pf >= (uint32_t)c.n_pages || pg >= (uint32_t)c.n_pages) return NO_MOVE;
+    return EvictMove{pf * (uint32_t)c.nKV + (uint32_t)head, pg * (uint32_t)c.nKV + (uint32_t)head, of & 63, to & 63};
+}
+
+// Sums of the lanes up to each, in six steps of the vector unit.
+__device__ static inline uint32_t wave_running(uint32_t x) {
+#define ADD_DPP(ctrl, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false)
+    ADD_DPP(0x111, 0xf);   // row_shr 1, 2, 4, 8
+    ADD_DPP(0x112, 0xf);
+    ADD_DPP(0x114, 0xf);
+    ADD_DPP(0x118, 0xf);
+    ADD_DPP(0x142, 0xa);   // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+    ADD_DPP(0x143, 0xc);
+#undef ADD_DPP
+    return x;
+}
+
+// A (job, kv head)'s list: the first move to each page below `keep`, their
+// number, then (of, to) pairs.
+__host__ __device__ static inline int evict_first(const EvictJob& j) { return ((j.keep + 63) / 64 + 2) & ~1; }
+__device__ static inline int64_t evict_words(const EvictJob& j) { return evict_first(j) + 2 * (int64_t)j.room; }
 
 // A workgroup of 1024 finds the rows that one (job, kv head) keeps. A thread
 // holds a run of rows' keys (REG of them in registers; 0: as many as it takes,
-// read again for each pass); the keep-th largest key comes from three passes
-// over 11, 11 and 10 bits from the top with a histogram in LDS, and of its
-// equals the lower rows stay. The rows below `keep` that go and the rows from
-// `keep` on that stay are as many, and the i-th of the one takes the place of
-// the i-th of the other: `of` and `to` lists in the workspace, or up to
-// EVICT_HERE moves made here.
+// read again for each pass); the keep-th largest key comes from up to three
+// passes over 11, 11 and 10 bits from the top with a histogram in LDS, the last
+// one that where a digit's rows all stay; of its equals the lower rows stay.
+// The rows below `keep` that go and the rows from `keep` on that stay are as
+// many, and the i-th of the one takes the place of the i-th of the other: a
+// list of them in the workspace, or up to EVICT_HERE moves made here.
 template <int NG, int REG>
 __global__ __launch_bounds__(1024) void k_evict_select(CacheDev c, EvictJobs jobs, MarksDev marks, int sink, int recent,
                                                        uint8_t* __restrict__ ws) {
-    __shared__ uint32_t hist[2048];
-    __shared__ uint32_t wsum[2][16];
-    __shared__ uint32_t s_sel[2];
+    __shared__ uint32_t hist[3][2048];
+    __shared__ uint32_t wsum[2][2][16];
+    __shared__ uint32_t s_sel[3];
     __shared__ int here_of[EVICT_HERE], here_to[EVICT_HERE];
+    __shared__ EvictMove moves[EVICT_HERE];
     const EvictJob jb = jobs.j[blockIdx.x / c.nKV];
     const int head = (int)blockIdx.x % c.nKV;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -1289,18 +1336,19 @@ __global__ __launch_bounds__(1024) void k_evict_select(CacheDev c, EvictJobs job
         const uint32_t pg = i0 < i1 ? pt[i0 >> 6] : 0xffffffffu;
         const bool ok = pg < (uint32_t)c.n_pages;
         const size_t m = ok ? ((size_t)pg * c.nKV + head) * 64 + (i0 & 63) : 0;
+        float4 w[REG / 4 + 1];
+        int4 k[REG / 4 + 1];
 #pragma unroll
-        for (int e = 0; e < REG; e += 4) {
-            float4 w = {0.f, 0.f, 0.f, 0.f};
-            int4 k = {0, 0, 0, 0};
-            if (ok) {
-                w = *(const float4*)(marks.weight + m + e);
-                k = *(const int4*)(marks.token + m + e);
-            }
-            reg[e] = ok ? keep_key(w.x, k.x, sink, latest) : 0u;
-            reg[e + 1] = ok ? keep_key(w.y, k.y, sink, latest) : 0u;
-            reg[e + 2] = ok ? keep_key(w.z, k.z, sink, latest) : 0u;
-            reg[e + 3] = ok ? keep_key(w.w, k.w, sink, latest) : 0u;
+        for (int e = 0; e < REG / 4; e++) {
+            w[e] = ok ? *(const float4*)(marks.weight + m + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            k[e] = ok ? *(const int4*)(marks.token + m + 4 * e) : make_int4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < REG / 4; e++) {
+            reg[4 * e] = ok ? keep_key(w[e].x, k[e].x, sink, latest) : 0u;
+            reg[4 * e + 1] = ok ? keep_key(w[e].y, k[e].y, sink, latest) : 0u;
+            reg[4 * e + 2] = ok ? keep_key(w[e].z, k[e].z, sink, latest) : 0u;
+            reg[4 * e + 3] = ok ? keep_key(w[e].w, k[e].w, sink, latest) : 0u;
         }
     }
     auto each = [&](auto&& f) {
@@ -1312,61 +1360,54 @@ __global__ __launch_bounds__(1024) void k_evict_select(CacheDev c, EvictJobs job
             for (int i = i0; i < i1; i++) f(i, key_at(i));
         }
     };
-    // what the threads before this one have of a and b
-    auto before = [&](uint32_t& a, uint32_t& b) {
-        uint32_t x = a, y = b;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t u = __shfl_up(x, o), v = __shfl_up(y, o);
-            if (lane >= o) {
-                x += u;
-                y += v;
-            }
-        }
-        if (lane == 63) {
-            wsum[0][wave] = x;
-            wsum[1][wave] = y;
-        }
+    // what the threads before this one have of a, and all of them together; `turn` alternates from call to call
+    auto before = [&](uint32_t a, int turn, int which, uint32_t& all) {
+        const uint32_t x = wave_running(a);
+        if (lane == 63) wsum[turn][which][wave] = x;
         __syncthreads();
-        x -= a;
-        y -= b;
-        for (int w = 0; w < wave; w++) {
-            x += wsum[0][w];
-            y += wsum[1][w];
-        }
-        __syncthreads();
-        a = x;
-        b = y;
+        const uint32_t w = lane < 16 ? wsum[turn][which][lane] : 0u;
+        const uint32_t r = wave_running(w);
+        all = __builtin_amdgcn_readlane(r, 15);
+        return x - a + (wave ? __builtin_amdgcn_readlane(r, wave - 1) : 0u);
     };
-    uint32_t prefix = 0, left = (uint32_t)jb.keep;
+#pragma unroll
+    for (int i = 0; i < 6; i++) ((uint32_t*)hist)[1024 * i + t] = 0;
+    __syncthreads();
+    uint32_t prefix = 0, left = (uint32_t)jb.keep, all = 0;
+    bool every = false;   // every row with prefix's digits stays
 #pragma unroll
     for (int ps = 0; ps < 3; ps++) {
         const int sh = ps == 0 ? 21 : ps == 1 ? 10 : 0, bits = ps == 2 ? 10 : 11;
         const uint32_t mask = (1u << bits) - 1;
-        hist[t] = hist[t + 1024] = 0;
-        __syncthreads();
+        if (every) break;   // uniform
         each([&](int, uint32_t k) {
-            if (ps == 0 || k >> (sh + bits) % 32 == prefix >> (sh + bits) % 32) atomicAdd(&hist[(k >> sh) & mask], 1u);
+            if (ps == 0 || k >> (sh + bits) % 32 == prefix >> (sh + bits) % 32) atomicAdd(&hist[ps][(k >> sh) & mask], 1u);
         });
         __syncthreads();
         // thread t: the digits 2047 - 2t and 2046 - 2t, from the largest down
-        const uint32_t n0 = hist[2047 - 2 * t], n1 = hist[2046 - 2 * t];
-        uint32_t b0 = n0 + n1, none = 0;
-        before(b0, none);
-        if (b0 < left && left <= b0 + n0 + n1) {
-            const bool first = left <= b0 + n0;
+        const uint2 n = *(const uint2*)&hist[ps][2046 - 2 * t];
+        const uint32_t b0 = before(n.x + n.y, ps & 1, 0, all);
+        if (b0 < left && left <= b0 + n.x + n.y) {
+            const bool first = left <= b0 + n.y;
             s_sel[0] = prefix | (uint32_t)(2047 - 2 * t - (first ? 0 : 1)) << sh;
-            s_sel[1] = left - b0 - (first ? 0 : n0);
+            s_sel[1] = left - b0 - (first ? 0 : n.y);
+            s_sel[2] = first ? n.y : n.x;
         }
         __syncthreads();
         prefix = s_sel[0];
         left = s_sel[1];
+        every = s_sel[2] == left;
     }
-    // prefix: the keep-th largest key; `left` of the rows that have it stay
-    uint32_t eq = 0, none = 0;
-    each([&](int, uint32_t k) { eq += k == prefix; });
-    before(eq, none);
-    uint32_t to = 0, of = 0, be = eq;
+    // every: the keys from `prefix` on stay; else `left` of those equal to it, and all above
+    uint32_t eq = 0, be = 0;
+    if (!every) {
+        each([&](int, uint32_t k) { eq += k == prefix; });
+        be = before(eq, 1, 0, all);
+    }
+    uint32_t to = 0, of = 0;
+    const uint32_t be0 = be;
     auto kept = [&](uint32_t k) {
+        if (every) return k >= prefix;
         const bool same = k == prefix, in = k > prefix || (same && be < left);
         be += same;
         return in;
@@ -1376,50 +1417,129 @@ __global__ __launch_bounds__(1024) void k_evict_select(CacheDev c, EvictJobs job
         to += i < jb.keep && !in;
         of += i >= jb.keep && in;
     });
-    const uint32_t mine = of;
-    before(to, of);
-    be = eq;
+    uint32_t moved = 0;
+    to = before(to, 0, 0, all);
+    of = before(of, 0, 1, moved);
+    be = be0;
     const bool here = jb.room <= EVICT_HERE;
-    int32_t* list = (int32_t*)ws + jb.moves0 + (int64_t)head * (2 * jb.room + 2);   // count, -, (of, to) pairs
-    if (t == 1023) {
-        const uint32_t n = min(of + mine, (uint32_t)jb.room);
-        if (here) s_sel[0] = n;
-        else list[0] = (int32_t)n;
-    }
+    int32_t* list = (int32_t*)ws + jb.moves0 + (int64_t)head * evict_words(jb);
+    int32_t* pairs = list + evict_first(jb);
+    const int n = (int)min(moved, (uint32_t)jb.room);   // (within `room` unless another stream writes the marks meanwhile)
+    if (!here && t == 0) list[(jb.keep + 63) >> 6] = n;
     each([&](int i, uint32_t k) {
         const bool in = kept(k);
-        if (i < jb.keep && !in) {   // (within `room` unless another stream writes the marks meanwhile)
+        if (!here && i < jb.keep && (i & 63) == 0) list[i >> 6] = (int32_t)min(to, (uint32_t)n);
+        if (i < jb.keep && !in) {
             if (here && to < EVICT_HERE) here_to[to] = i;
-            if (!here && to < (uint32_t)jb.room) list[2 + 2 * to + 1] = i;
+            if (!here && to < (uint32_t)jb.room) pairs[2 * to + 1] = i;
             to++;
         } else if (i >= jb.keep && in) {
             if (here && of < EVICT_HERE) here_of[of] = i;
-            if (!here && of < (uint32_t)jb.room) list[2 + 2 * of] = i;
+            if (!here && of < (uint32_t)jb.room) pairs[2 * of] = i;
             of++;
         }
     });
     if (!here) return;
     __syncthreads();
-    const int n = (int)s_sel[0];
-    for (int i = wave; i < n; i += 16) move_row<NG>(c, marks, pt, head, here_of[i], here_to[i], lane);
+    if (t < EVICT_HERE) moves[t] = t < n ? move_at(c, pt, head, here_of[t], here_to[t]) : NO_MOVE;
+    __syncthreads();
+    if (4 * wave < n) move_rows<NG, 4>(c, marks, moves + 4 * wave, lane);   // 16 waves: EVICT_HERE
 }
+static_assert(EVICT_HERE == 64, "four moves for each of k_evict_select's sixteen waves");
 
 // The moves of the lists: rows from `keep` on to rows below it, so no row is
-// both read and written. A workgroup takes EVICT_MOVES of a (job, kv head)'s.
-constexpr int EVICT_MOVES = 32;
+// both read and written. A workgroup takes those to the rows of one (page, kv
+// head). Where they are EVICT_PAGE or more, a thread takes a channel's 16 rows
+// of V, whose codes lie beside each other, and puts the new ones into the 16
+// bytes that it read; fewer are stored byte by byte.
+constexpr int EVICT_PAGE = 8;
 template <int NG>
 __global__ __launch_bounds__(256) void k_evict_move(CacheDev c, EvictJobs jobs, MarksDev marks,
                                                     const uint8_t* __restrict__ ws) {
+    constexpr int D = 32 * NG, DI = D / 64, SI = (NG + 3) / 4;   // 16 bytes of K or V a thread; scales
+    __shared__ EvictMove moves[64];
+    __shared__ int move_to[64];   // the move to a row of the page
     const EvictJob jb = jobs.j[blockIdx.y / c.nKV];
-    const int head = (int)blockIdx.y % c.nKV, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (jb.room <= EVICT_HERE) return;
-    const int32_t* list = (const int32_t*)ws + jb.moves0 + (int64_t)head * (2 * jb.room + 2);
-    const int i0 = (int)blockIdx.x * EVICT_MOVES, n = min(list[0] - i0, EVICT_MOVES);
+    const int head = (int)blockIdx.y % c.nKV, tid = threadIdx.x, pg = blockIdx.x;
+    if (jb.room <= EVICT_HERE || 64 * pg >= jb.keep) return;
+    const int32_t* list = (const int32_t*)ws + jb.moves0 + (int64_t)head * evict_words(jb);
+    const int32_t* pairs = list + evict_first(jb);
+    const int first = list[pg], n = list[pg + 1] - first;
+    if (n <= 0) return;
     const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
-    for (int i = wave; i < n; i += 4) {
-        const int2 m = *(const int2*)(list + 2 + 2 * (i0 + i));
-        move_row<NG>(c, marks, pt, head, m.x, m.y, lane);
+    if (tid < 64) {
+        move_to[tid] = -1;
+        if (tid < n) {   // (the 64 lanes of a wave)
+            const int2 m = *(const int2*)(pairs + 2 * (first + tid));
+            moves[tid] = move_at(c, pt, head, m.x, m.y);
+            if (moves[tid].of_row >= 0) move_to[m.y & 63] = tid;
+        }
     }
+    __syncthreads();
+    u32x4 kc[DI];
+    uint32_t ks[SI], vs[SI], mark = 0;
+#pragma unroll
+    for (int e = 0; e < DI; e++) {
+        const int i = 256 * e + tid, ch = i % (D / 16);
+        const EvictMove m = moves[min(i / (D / 16), n - 1)];
+        kc[e] = *(const u32x4*)(c.k + (size_t)m.of * c.blk + max(m.of_row, 0) * D + 16 * ch);
+    }
+#pragma unroll
+    for (int e = 0; e < SI; e++) {
+        const int i = 256 * e + tid, g = i % NG;
+        const EvictMove m = moves[min(i / NG, n - 1)];
+        const size_t at = (size_t)m.of * c.blk + 64 * D;
+        ks[e] = *(const uint32_t*)(c.k + at + 4 * (max(m.of_row, 0) * NG + g));
+        vs[e] = *(const uint32_t*)(c.v + at + 4 * vscale_at(g, max(m.of_row, 0), NG));
+    }
+    uint32_t* mark_of = tid & 1 ? (uint32_t*)marks.token : (uint32_t*)marks.weight;
+    if (tid < 2 * n) mark = mark_of[(size_t)moves[tid >> 1].of * 64 + max(moves[tid >> 1].of_row, 0)];
+    if (n >= EVICT_PAGE) {
+        const uint32_t page = pt[pg];
+        if (page < (uint32_t)c.n_pages) {
+            u32x4* to = (u32x4*)(c.v + ((size_t)page * c.nKV + head) * c.blk);
+#pragma unroll
+            for (int e = 0; e < DI; e++) {
+                const int i = 256 * e + tid, j4 = __builtin_amdgcn_readfirstlane(i / D), d = i % D;   // a wave's rows: 16 of the page
+                u32x4 w = to[i];
+                uint32_t b[16];
+#pragma unroll
+                for (int u = 0; u < 16; u++) {
+                    const int at = __builtin_amdgcn_readfirstlane(move_to[16 * (u >> 2) + 4 * j4 + (u & 3)]);
+                    b[u] = 0x100u;
+                    if (at >= 0) b[u] = c.v[(size_t)moves[at].of * c.blk + vcode_at(d, moves[at].of_row, D)];
+                }
+#pragma unroll
+                for (int u = 0; u < 16; u++) {
+                    const uint32_t sh = 8 * (u & 3);
+                    if (b[u] < 0x100u) w[u >> 2] = (w[u >> 2] & ~(0xffu << sh)) | b[u] << sh;
+                }
+                to[i] = w;
+            }
+        }
+    } else {
+        for (int i = tid; i < n * D; i += 256) {
+            const EvictMove m = moves[i / D];
+            if (m.of_row >= 0)
+                c.v[(size_t)m.to * c.blk + vcode_at(i % D, m.to_row, D)] = c.v[(size_t)m.of * c.blk + vcode_at(i % D, m.of_row, D)];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < DI; e++) {
+        const int i = 256 * e + tid, ch = i % (D / 16);
+        const EvictMove m = moves[min(i / (D / 16), n - 1)];
+        if (i < n * (D / 16) && m.of_row >= 0) *(u32x4*)(c.k + (size_t)m.to * c.blk + m.to_row * D + 16 * ch) = kc[e];
+    }
+#pragma unroll
+    for (int e = 0; e < SI; e++) {
+        const int i = 256 * e + tid, g = i % NG;
+        const EvictMove m = moves[min(i / NG, n - 1)];
+        if (i >= n * NG || m.of_row < 0) continue;
+        const size_t at = (size_t)m.to * c.blk + 64 * D;
+        *(uint32_t*)(c.k + at + 4 * (m.to_row * NG + g)) = ks[e];
+        *(uint32_t*)(c.v + at + 4 * vscale_at(g, m.to_row, NG)) = vs[e];
+    }
+    if (tid < 2 * n && moves[tid >> 1].of_row >= 0) mark_of[(size_t)moves[tid >> 1].to * 64 + moves[tid >> 1].to_row] = mark;
 }
 
 template <int NG>
@@ -1432,10 +1552,11 @@ static hipError_t evict_ng(hipStream_t st, const CacheDev& c, const EvictJobs& j
     else if (max_rows <= 16384) e = op_launch(k_evict_select<NG, 16>, grid, dim3(1024), st, c, jobs, marks, sink, recent, ws);
     else e = op_launch(k_evict_select<NG, 0>, grid, dim3(1024), st, c, jobs, marks, sink, recent, ws);
     if (e == hipSuccess && jobs.room > EVICT_HERE)
-        e = op_launch(k_evict_move<NG>, dim3((jobs.room + EVICT_MOVES - 1) / EVICT_MOVES, jobs.n * c.nKV), dim3(256), st, c,
-                      jobs, marks, ws);
+        e = op_launch(k_evict_move<NG>, dim3((jobs.keep + 63) / 64, jobs.n * c.nKV), dim3(256), st, c, jobs, marks, ws);
     return e;
 }
+
+size_t evict_list_words(const EvictJob& j) { return evict_first(j) + 2 * (size_t)j.room; }
 
 hipError_t launch_evict(hipStream_t st, const CacheDev& c, const EvictJobs& jobs, int max_rows, const MarksDev& marks,
                         int sink, int recent, uint8_t* ws) {

@@ -125,18 +125,19 @@ hipError_t launch_weigh(hipStream_t st, const CacheDev& c, const WeighJobs& jobs
                         const AxesDev& axes, const MarksDev& marks, const float* q, int64_t ldq, float* out, int64_t ldo,
                         uint8_t* ws);
 
-// cc_keep; its list of moves lies in the workspace from moves0 on, for each kv
-// head `room` of them behind a count.
+// cc_keep; its lists of moves (evict_words each) lie in the workspace from word
+// moves0 on, one for each kv head, where it may have more than EVICT_HERE.
 struct EvictJob {
     int32_t slot, rows, keep, seen, room;
     int64_t moves0;
 };
 constexpr int EVICT_JOBS = 96;
 struct EvictJobs {
-    int n = 0, room = 0;   // room: the largest of the jobs
+    int n = 0, room = 0, keep = 0;   // room, keep: the largest of the jobs with lists
     EvictJob j[EVICT_JOBS];
 };
 constexpr int EVICT_HERE = 64;   // moves that the workgroup which selects makes itself
+size_t evict_list_words(const EvictJob& j);
 hipError_t launch_evict(hipStream_t st, const CacheDev& c, const EvictJobs& jobs, int max_rows, const MarksDev& marks,
                         int sink, int recent, uint8_t* ws);
 

@@ -136,7 +136,9 @@ no("marks", evict(c, (0, 10, 5, 10), m=marks(weight=f + 8)))
 no("negative", evict(c, (0, 10, 5, 10), sink=-1))
 no("negative", evict(c, (0, 10, 5, 10), recent=-1))
 no("workspace", evict(c, (0, 400, 200, 400), ws=None))
-no("workspace", evict(c, (0, 400, 200, 400), n=2 * 4 * 402 - 4))
+need = ctx.lib.cc_evict_workspace(C.byref(c), *jobs((0, 400, 200, 400)))
+no("workspace", evict(c, (0, 400, 200, 400), n=need - 4))
+out.append(["", 5 if need >= 2 * 4 * 2 * 200 else 0, str(need)])
 no("workspace", evict(c, (0, 400, 200, 400), ws=f + 4))
 for field, bad in (("head_dim", 96), ("rot_dim", 0), ("n_kv_heads", 0), ("n_kv_heads", 2000), ("max_pages", 32769),
                    ("n_pages", 0), ("slots", 0), ("rope_rows", 0), ("k", None), ("page_table", None), ("rope", None), ("v", c.v + 8)):
