@@ -1316,7 +1316,7 @@ __global__ __launch_bounds__(1024) void k_evict_select(CacheDev c, EvictJobs job
     __shared__ uint32_t hist[3][2048];
     __shared__ uint32_t wsum[2][2][16];
     __shared__ uint32_t s_sel[3];
-    __shared__ int here_of[EVICT_HERE], here_to[EVICT_HERE];
+    __shared__ int here_rows[2 * EVICT_HERE];   // (of, to) pairs
     __shared__ EvictMove moves[EVICT_HERE];
     const EvictJob jb = jobs.j[blockIdx.x / c.nKV];
     const int head = (int)blockIdx.x % c.nKV;
@@ -1413,9 +1413,9 @@ __global__ __launch_bounds__(1024) void k_evict_select(CacheDev c, EvictJobs job
         return in;
     };
     each([&](int i, uint32_t k) {
-        const bool in = kept(k);
-        to += i < jb.keep && !in;
-        of += i >= jb.keep && in;
+        const bool in = kept(k), below = i < jb.keep;
+        to += below && !in;
+        of += !below && in;
     });
     uint32_t moved = 0;
     to = before(to, 0, 0, all);
@@ -1429,19 +1429,18 @@ __global__ __launch_bounds__(1024) void k_evict_select(CacheDev c, EvictJobs job
     each([&](int i, uint32_t k) {
         const bool in = kept(k);
         if (!here && i < jb.keep && (i & 63) == 0) list[i >> 6] = (int32_t)min(to, (uint32_t)n);
-        if (i < jb.keep && !in) {
-            if (here && to < EVICT_HERE) here_to[to] = i;
-            if (!here && to < (uint32_t)jb.room) pairs[2 * to + 1] = i;
-            to++;
-        } else if (i >= jb.keep && in) {
-            if (here && of < EVICT_HERE) here_of[of] = i;
-            if (!here && of < (uint32_t)jb.room) pairs[2 * of] = i;
-            of++;
+        const bool below = i < jb.keep, goes = below != in;
+        const uint32_t at = below ? to : of;
+        if (goes && at < (uint32_t)n) {
+            if (here) here_rows[2 * at + below] = i;
+            else pairs[2 * at + below] = i;
         }
+        to += below && goes;
+        of += !below && goes;
     });
     if (!here) return;
     __syncthreads();
-    if (t < EVICT_HERE) moves[t] = t < n ? move_at(c, pt, head, here_of[t], here_to[t]) : NO_MOVE;
+    if (t < EVICT_HERE) moves[t] = t < n ? move_at(c, pt, head, here_rows[2 * t], here_rows[2 * t + 1]) : NO_MOVE;
     __syncthreads();
     if (4 * wave < n) move_rows<NG, 4>(c, marks, moves + 4 * wave, lane);   // 16 waves: EVICT_HERE
 }
