@@ -351,7 +351,6 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
             }
             if (CT * NG >= 16 && (g & 1)) __builtin_amdgcn_sched_barrier(0);   // no more query fragments ahead than fit
         }
-        load_k(next);
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             if (edge) {
@@ -365,6 +364,10 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
             const float m = rows_max(fmaxf(fmaxf(s[ct][0], s[ct][1]), fmaxf(s[ct][2], s[ct][3])));
             if (j4 == 0) tops[b][wave][ct][l16] = m;
         }
+        // (behind the stores: loads and stores are waited for in the order in which they were issued, and what waits for V
+        // then waits for none of these)
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(next);
         float sum[CT];
         uint2* pw = (uint2*)(pbuf + b * PB);
         auto form = [&]() {   // P of the wave's rows, relative to M
