@@ -246,7 +246,10 @@ template <int NG, int CT>
 __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs jobs, WeighPlan p, float* __restrict__ out,
                                                        int64_t ldo, uint8_t* __restrict__ ws) {
     constexpr int D = 32 * NG, DW = D / 64, GW = DW > 1 ? DW / 2 : 1;   // of a wave: 16-channel pieces, groups
-    constexpr int PB = 2 * 2 * CT * 64;   // P of a page: [hi, lo][2][CT][64] fragments
+    // Where V's scales go. Into P, which is then split for each group (48 vector instructions a lane, group and 16 columns) and
+    // multiplies whole numbers, one instruction a code and two products; or into V, as f16 pairs, 5.5 a code and three.
+    constexpr bool PS = NG > 2 ? CT <= 3 : CT == 1;
+    constexpr int PB = 4 * CT * 64;   // P of a page: PS: f32 [CT][4][64] of a lane's rows; else fragments [hi, lo][2][CT][64]
     __shared__ u32x4 qf[CT][2][NG][64];
     __shared__ u32x4 pbuf[2 * PB];
     __shared__ float tops[2][4][CT][16];
@@ -321,7 +324,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
 #pragma unroll
         for (int i = 0; i < DW; i++) o[i][ct] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    int ev[GW];   // O of a group's channels is relative to 2^(ev - 7)
+    int ev[GW];   // O of a group's channels is relative to 2^ev, or 2^(ev - 7) of pairs
 #pragma unroll
     for (int g = 0; g < GW; g++) ev[g] = -112;
     float* score_at = (float*)(ws + p.scores) +
@@ -360,10 +363,11 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
                     if (r0 + r > last) s[ct][r] = -INFINITY;
             }
             s[ct] = s[ct] * sc[ct];
-            if (store[ct]) *(float4_t*)(score_at + ((size_t)(e - e0) * p.score_cols + 16 * ct) * 64) = s[ct];
+            if (store[ct]) *(float4_t*)(score_at + 16 * ct * 64) = s[ct];
             const float m = rows_max(fmaxf(fmaxf(s[ct][0], s[ct][1]), fmaxf(s[ct][2], s[ct][3])));
             if (j4 == 0) tops[b][wave][ct][l16] = m;
         }
+        score_at += p.score_cols * 64;
         // (behind the stores: loads and stores are waited for in the order in which they were issued, and what waits for V
         // then waits for none of these)
         __builtin_amdgcn_sched_barrier(0);
@@ -378,6 +382,10 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
 #pragma unroll
                 for (int r = 0; r < 4; r++) pr[r] = __builtin_amdgcn_exp2f(s[ct][r] - m + P_SHIFT);
                 sum[ct] = (pr[0] + pr[1]) + (pr[2] + pr[3]);
+                if (PS) {
+                    ((float4_t*)pbuf)[b * PB + (ct * 4 + wave) * 64 + lane] = float4_t{pr[0], pr[1], pr[2], pr[3]};
+                    continue;
+                }
                 uint2 h, l;
                 split_mix2(pr[0], pr[1], h.x, l.x);
                 split_mix2(pr[2], pr[3], h.y, l.y);
@@ -435,11 +443,54 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
                 ev[g] = en;
             }
         }
-        const float down = pair_down(GW > 1 && lane >= 32 ? ev[GW - 1] : ev[0]);
+        const float down = pair_down(GW > 1 && lane >= 32 ? ev[GW - 1] : ev[0]) * (PS ? 1.0f / 128.0f : 1.0f);
 #pragma unroll
         for (int i = 0; i < SK; i++) vsl[wave][(ve0 + i) >> 6][(ve0 + i) & 63] = u2f(vsr[i]) * down;
+        auto scales8 = [&](int g, int ks, float (&s8)[8]) {   // of the lane's rows 16 * (2 ks + i / 4) + 4 * j4 + i % 4
+            const float4_t sa = *(const float4_t*)&vsl[wave][g][16 * j4 + 8 * ks], sb = *(const float4_t*)&vsl[wave][g][16 * j4 + 8 * ks + 4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s8[i] = sa[i];
+                s8[4 + i] = sb[i];
+            }
+        };
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
+            if (PS) {
+                float4_t pa[CT], pb[CT];
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) {
+                    pa[ct] = ((const float4_t*)pbuf)[b * PB + (ct * 4 + 2 * ks) * 64 + lane];
+                    pb[ct] = ((const float4_t*)pbuf)[b * PB + (ct * 4 + 2 * ks + 1) * 64 + lane];
+                }
+#pragma unroll
+                for (int g = 0; g < GW; g++) {
+                    float s8[8];
+                    scales8(g, ks, s8);
+                    half8_t vf[2];
+#pragma unroll
+                    for (int i = 0; i < (DW > 1 ? 2 : 1); i++) vf[i] = dequant8_biased(vr[2 * g + i][2 * ks], vr[2 * g + i][2 * ks + 1]);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        u32x4 h4, l4;
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            const float4_t pv = i < 4 ? pa[ct] : pb[ct];
+                            uint32_t h, l;
+                            split_mix2(pv[i & 3] * s8[i], pv[(i & 3) + 1] * s8[i + 1], h, l);
+                            h4[i >> 1] = h;
+                            l4[i >> 1] = l;
+                        }
+                        const half8_t ph = __builtin_bit_cast(half8_t, h4), pl = __builtin_bit_cast(half8_t, l4);
+#pragma unroll
+                        for (int i = 0; i < (DW > 1 ? 2 : 1); i++) {
+                            o[2 * g + i][ct] = mfma16x16x32(vf[i], ph, o[2 * g + i][ct]);
+                            o[2 * g + i][ct] = mfma16x16x32(vf[i], pl, o[2 * g + i][ct]);
+                        }
+                    }
+                }
+                continue;
+            }
             half8_t ph[CT], pl[CT];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
@@ -448,9 +499,8 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
             }
 #pragma unroll
             for (int i = 0; i < DW; i++) {
-                const float* at = &vsl[wave][DW > 1 ? i >> 1 : 0][16 * j4 + 8 * ks];
-                const float4_t sa = *(const float4_t*)at, sb = *(const float4_t*)(at + 4);
-                const float s8[8] = {sa[0], sa[1], sa[2], sa[3], sb[0], sb[1], sb[2], sb[3]};
+                float s8[8];
+                scales8(DW > 1 ? i >> 1 : 0, ks, s8);
                 u32x4 h, l;
                 code_pair(vr[i][2 * ks], vr[i][2 * ks + 1], s8, h, l);
                 const half8_t vh = __builtin_bit_cast(half8_t, h), vl = __builtin_bit_cast(half8_t, l);
@@ -507,7 +557,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
         float* dst = out + ((int64_t)jb.row0 + col / p.group) * ldo + (size_t)(w.head * p.group + col % p.group) * D + wave * (D / 4) + 4 * j4;
 #pragma unroll
         for (int i = 0; i < DW; i++) {
-            float4_t y = o[i][ct] * ldexpf(P_UNSHIFT, ev[DW > 1 ? i >> 1 : 0] - 7);
+            float4_t y = o[i][ct] * ldexpf(P_UNSHIFT, ev[DW > 1 ? i >> 1 : 0] - (PS ? 0 : 7));
             if (w.splits == 1) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) y[r] = l != 0.0f ? y[r] / l : 0.0f;
