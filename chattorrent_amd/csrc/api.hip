@@ -2505,7 +2505,7 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
                 w.page0 = (int)pages_;
                 units += nkv * tiles * ceil_div(pages, p.per);
                 joins += nkv * tiles * p.subs;
-                pages_ += nkv * ceil_div(pages, 8) * 8;
+                pages_ += nkv * ceil_div(pages, FINISH_PAGES) * FINISH_PAGES;
             }
             b.units = (int)units;
             b.joins = (int)joins;
@@ -2541,7 +2541,7 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
                 int fresh = 0;
                 for (int i = 0; i < r.n;) {
                     const int n = std::min(r.n - i, most_rows), seen = (r.past + i + n - 1) / 64 + 1;
-                    const int64_t u = nkv * ceil_div64((int64_t)n * G, 16 * subs) * std::min(128, seen), pg = nkv * (seen + 8);
+                    const int64_t u = nkv * ceil_div64((int64_t)n * G, 16 * subs) * std::min(128, seen), pg = nkv * (seen + FINISH_PAGES);
                     // (the pieces of a job add to the same weights: each in a launch of its own)
                     if (b.n == WEIGH_JOBS || i > 0 || (b.n && (units + u > WEIGH_UNITS || pages + pg > WEIGH_PAGES))) {
                         if (!flush()) return most;

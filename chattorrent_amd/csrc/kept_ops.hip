@@ -48,8 +48,6 @@ __device__ static inline float pow2_diff(float a, float b) {   // 2^(a - b) of w
     return a == -INFINITY ? 0.0f : ldexpf(1.0f, (int)fmaxf(a - b, -300.0f));
 }
 
-constexpr int FINISH_PAGES = 8;
-
 // A scale's bits, which order as it does (none is negative); 0 of one that is
 // no finite number: the others' precision does not hang on it.
 __device__ static inline uint32_t finite_bits(uint32_t b) { return b < 0x7f800000u ? b : 0u; }
@@ -656,34 +654,47 @@ __global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs
     const int splits = (pages + p.per - 1) / p.per;
     const int c0 = jb.count0 * p.group, cols = jb.n * p.group;
     const size_t unit = (size_t)jb.unit0 + (size_t)head * splits;   // one tile a (job, kv head)
+    // a wave's pages: what does not hang on the columns' totals is loaded before them
+    constexpr int WP = FINISH_PAGES / 4;
+    const float* s0 = (const float*)(ws + p.scores) + ((size_t)jb.page0 + (size_t)head * room + p0 + wave) * p.score_cols * 64 + lane;
+    float x[WP][8], before[WP];
+    float* wt[WP];
+#pragma unroll
+    for (int i = 0; i < WP; i++) {
+        const int pg = p0 + wave + 4 * i, row = 64 * pg + lane;
+        const uint32_t id = pg < pages ? c.page_table[(size_t)jb.slot * c.max_pages + pg] : 0xffffffffu;
+        const bool there = id < (uint32_t)c.n_pages && row < jb.past + jb.n;
+        wt[i] = there ? marks.weight + ((size_t)id * c.nKV + head) * 64 + lane : nullptr;
+        before[i] = there && !(p.fade == 0.0f && row >= jb.fresh) ? *wt[i] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[i][e] = there ? s0[(size_t)(4 * i * p.score_cols + min(c0 + e, cols - 1)) * 64] : 0.0f;
+    }
     if (wave < p.subs && 16 * wave < cols) {
         const int col = 16 * wave + (lane & 15);
         const float2 t = column_total(ml + unit * p.subs * 16 + col, splits, p.subs * 16, lane >> 4);
         if (lane < 16) total[col] = make_float2(t.x == -INFINITY ? 0.0f : t.x, t.y != 0.0f ? 1.0f / t.y : 0.0f);
     }
     __syncthreads();
-    for (int i = wave; i < FINISH_PAGES && p0 + i < pages; i += 4) {
-        const int pg = p0 + i, row = 64 * pg + lane;
-        const uint32_t id = c.page_table[(size_t)jb.slot * c.max_pages + pg];
-        if (id >= (uint32_t)c.n_pages || row >= jb.past + jb.n) continue;
-        float* wt = marks.weight + ((size_t)id * c.nKV + head) * 64 + lane;
-        const float* s = (const float*)(ws + p.scores) + ((size_t)jb.page0 + (size_t)head * room + pg) * p.score_cols * 64 + lane;
-        const float before = p.fade == 0.0f && row >= jb.fresh ? 0.0f : *wt;
+#pragma unroll
+    for (int i = 0; i < WP; i++) {
+        if (!wt[i]) continue;
         float got = 0.0f;
-        for (int col = c0; col < cols; col += 8) {
-            float x[8];
+        auto add = [&](float x1, int col) {
+            const float2 t = total[min(col, cols - 1)];
+            if (col < cols) got = __builtin_fmaf(__builtin_amdgcn_exp2f(x1 - t.x), t.y, got);
+        };
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = s[(size_t)min(col + e, cols - 1) * 64];
+        for (int e = 0; e < 8; e++) add(x[i][e], c0 + e);
+        for (int col = c0 + 8; col < cols; col += 20) {
+            float y[20];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float2 t = total[min(col + e, cols - 1)];
-                if (col + e < cols) got = __builtin_fmaf(__builtin_amdgcn_exp2f(x[e] - t.x), t.y, got);
-            }
+            for (int e = 0; e < 20; e++) y[e] = s0[(size_t)(4 * i * p.score_cols + min(col + e, cols - 1)) * 64];
+#pragma unroll
+            for (int e = 0; e < 20; e++) add(y[e], col + e);
         }
-        *wt = __builtin_fmaf(before, row >= jb.fresh ? p.fade : 1.0f, got);   // (weigh_add, the load ahead)
+        *wt[i] = __builtin_fmaf(before[i], 64 * (p0 + wave + 4 * i) + lane >= jb.fresh ? p.fade : 1.0f, got);   // weigh_add's sum
     }
 }
-
 // After k_weigh_many, where a tile's pages were split: joins the outputs of
 // 1024 / D columns of a piece a workgroup, 4 channels a thread, and leaves the
 // columns' M and 1/l.

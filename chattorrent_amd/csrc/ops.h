@@ -115,6 +115,7 @@ struct WeighPlan {
     float fade = 1.0f;
     size_t ml = 0, parts = 0, scores = 0, q = 0, qs = 0, exps = 0, tot = 0, lines = 0, bytes = 0;   // offsets into the workspace, its size
 };
+constexpr int FINISH_PAGES = 8;   // pages of a workgroup that adds up weights; a (job, kv head)'s are counted in whole ones
 constexpr int WEIGH_JOIN = 256;   // floats of a unit's output that a workgroup joins
 // By a job's columns: at most 16; up to 64 (a launch's jobs take as many
 // 16-column pieces as the largest of them); more, for eight waves of
