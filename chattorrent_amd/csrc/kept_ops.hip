@@ -932,9 +932,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
                     acc[ct][tt] = mfma16x16x32(kh, qh[ct][g], acc[ct][tt]);
-                    acc[ct][tt] = mfma16x16x32(kl, qh[ct][g], acc[ct][tt]);
-                    acc[ct][tt] = mfma16x16x32(kh, ql[ct][g], acc[ct][tt]);
                 }
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) acc[ct][tt] = mfma16x16x32(kl, qh[ct][g], acc[ct][tt]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) acc[ct][tt] = mfma16x16x32(kh, ql[ct][g], acc[ct][tt]);
             }
         const bool edge = !ok || r0 + TOK - 1 > first_last;
         half8_t ph[CT][KS], pl[CT][KS];
@@ -1037,9 +1039,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
                     o[ct][dt] = mfma16x16x32(vh, ph[ct][ks], o[ct][dt]);
-                    o[ct][dt] = mfma16x16x32(vl, ph[ct][ks], o[ct][dt]);
-                    o[ct][dt] = mfma16x16x32(vh, pl[ct][ks], o[ct][dt]);
                 }
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) o[ct][dt] = mfma16x16x32(vl, ph[ct][ks], o[ct][dt]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) o[ct][dt] = mfma16x16x32(vh, pl[ct][ks], o[ct][dt]);
             }
     };
     load(0);
