@@ -739,6 +739,18 @@ __global__ __launch_bounds__(256) void k_weigh_join(WeighJobs jobs, WeighPlan p,
     *(float4_a4*)dst = x;
 }
 
+// Schedules a block of N groups of P matrix products, each group behind two LDS
+// reads of its operands, so that the reads are three groups ahead. (ID: one a block.)
+template <int N, int P, int ID>
+__device__ static inline void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, ID);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, P, ID);
+        if (i + 3 < N) __builtin_amdgcn_sched_group_barrier(0x100, 2, ID);
+    }
+}
+
 // Attention of a tile of 16 * CT columns for each of W waves over `per` pages.
 // The workgroup unpacks a step of TOK rows once for all its columns, K and V as
 // f16 pairs relative to the page's largest scales (V: the largest so far), in
@@ -938,6 +950,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) acc[ct][tt] = mfma16x16x32(kh, ql[ct][g], acc[ct][tt]);
             }
+        reads_ahead<NG * TT, 3 * CT, 0>();
         const bool edge = !ok || r0 + TOK - 1 > first_last;
         half8_t ph[CT][KS], pl[CT][KS];
 #pragma unroll
@@ -1045,6 +1058,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) o[ct][dt] = mfma16x16x32(vh, pl[ct][ks], o[ct][dt]);
             }
+        reads_ahead<KS * DT, 3 * CT, 1>();
     };
     load(0);
     unpack(0);
@@ -1531,7 +1545,7 @@ __global__ __launch_bounds__(256) void k_evict_move(CacheDev c, EvictJobs jobs, 
     if (jb.room <= EVICT_HERE || 64 * pg >= jb.keep) return;
     const int32_t* list = (const int32_t*)ws + jb.moves0 + (int64_t)head * evict_words(jb);
     const int32_t* pairs = list + evict_first(jb);
-    const int first = list[pg], n = list[pg + 1] - first;
+    const int first = list[pg], n = min(list[pg + 1] - first, 64);
     if (n <= 0) return;
     const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
     if (tid < 64) {
