@@ -2417,6 +2417,7 @@ cc_status marks_dev(cc_ctx* ctx, const cc_marks* m, MarksDev& d) {
 // the result is the workspace that the largest launch takes.
 constexpr int WEIGH_ROWS = 4096;              // rows of a piece, of up to 2048 heads
 constexpr int64_t WEIGH_UNITS = 1 << 20, WEIGH_PAGES = 1 << 24;   // of a launch with several jobs
+constexpr int64_t WEIGH_BYTES = 1 << 30;      // of such a launch's scores, or queries and split outputs: more jobs use the same memory again
 int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The pages of an attention workgroup. Up to 16 columns: such that there are
@@ -2497,12 +2498,14 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
             for (int j = 0; j < b.n && kind != WEIGH_WIDE && weigh; j++) p.score_cols = std::max(p.score_cols, b.j[j].n * G);
             p.per = weigh_per(ctx->ncu, b, p, nkv, kind);
             int64_t units = 0, joins = 0, pages_ = 0;
+            bool split = false;   // a job's pages are more than a workgroup's
             for (int j = 0; j < b.n; j++) {
                 WeighJob& w = b.j[j];
                 const int pages = (w.past + w.n - 1) / 64 + 1, tiles = ceil_div(w.n * G, 16 * p.subs);
                 w.unit0 = (int)units;
                 w.join0 = (int)joins;
                 w.page0 = (int)pages_;
+                split = split || pages > p.per;
                 units += nkv * tiles * ceil_div(pages, p.per);
                 joins += nkv * tiles * p.subs;
                 pages_ += nkv * ceil_div(pages, FINISH_PAGES) * FINISH_PAGES;
@@ -2518,7 +2521,7 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
                 return here;
             };
             p.ml = take(true, (size_t)units * p.subs * 16 * 8);
-            p.parts = take(true, (size_t)units * p.subs * 16 * D * 4);
+            p.parts = take(split, (size_t)units * p.subs * 16 * D * 4);
             p.scores = take(p.score_cols > 0, (size_t)b.pages * p.score_cols * 256);
             p.q = take(true, (size_t)joins * 16 * D * 4);
             p.qs = take(true, (size_t)joins * 64);
@@ -2532,7 +2535,7 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
             b.n = 0;
             return ok;
         };
-        int64_t row0 = 0, units = 0, pages = 0;
+        int64_t row0 = 0, units = 0, pages = 0, bytes = 0;
         const int most_rows = std::min(WEIGH_ROWS, (1 << 23) / n_heads);
         for (int j = 0; j < njobs; j++) {
             const cc_rows& r = jobs[j];
@@ -2542,13 +2545,17 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
                 for (int i = 0; i < r.n;) {
                     const int n = std::min(r.n - i, most_rows), seen = (r.past + i + n - 1) / 64 + 1;
                     const int64_t u = nkv * ceil_div64((int64_t)n * G, 16 * subs) * std::min(128, seen), pg = nkv * (seen + FINISH_PAGES);
+                    const int64_t held = kind == WEIGH_WIDE ? nkv * ceil_div64((int64_t)n * G, 16 * subs) * subs * 64 * D * (2 + 2 * ceil_div(seen, 256))
+                                                            : pg * 16 * subs * 256;
                     // (the pieces of a job add to the same weights: each in a launch of its own)
-                    if (b.n == WEIGH_JOBS || i > 0 || (b.n && (units + u > WEIGH_UNITS || pages + pg > WEIGH_PAGES))) {
+                    if (b.n == WEIGH_JOBS || i > 0 ||
+                        (b.n && (units + u > WEIGH_UNITS || pages + pg > WEIGH_PAGES || bytes + held > WEIGH_BYTES))) {
                         if (!flush()) return most;
-                        units = pages = 0;
+                        units = pages = bytes = 0;
                     }
                     units += u;
                     pages += pg;
+                    bytes += held;
                     const int count0 = (int)std::max<int64_t>(0, std::min<int64_t>(n, (int64_t)r.n - observe - i));
                     b.j[b.n++] = WeighJob{r.slot, r.past + i, n, (int32_t)(row0 + i), count0, fresh, 0, 0, 0};
                     if (count0 < n) fresh = r.past + i + n;
@@ -2592,7 +2599,7 @@ size_t each_evict(const cc_cache* c, const cc_keep* jobs, int32_t njobs, F&& f) 
     };
     for (int j = 0; j < njobs; j++) {
         const cc_keep& k = jobs[j];
-        if (k.rows <= k.keep) continue;
+        if (k.rows <= k.keep || k.keep < 1 || (int64_t)k.rows > (int64_t)c->max_pages * 64) continue;
         const int room = std::min(k.rows - k.keep, k.keep);
         if ((b.n == EVICT_JOBS || (int64_t)(b.n + 1) * c->n_kv_heads > 65535) && !flush()) return most;
         b.j[b.n++] = EvictJob{k.slot, k.rows, k.keep, k.seen, room, words};

@@ -434,14 +434,15 @@ cc_status cc_kv_append_at(cc_ctx* ctx, const cc_cache* cache, const cc_positions
  * observe > 0, the weights w of the slot's rows r = 0 .. past + n - 1 become
  *   fade * w[r] + the sum over the job's last `observe` rows i that see r, and
  *   over the query heads of the kv head, of softmax(q_i . k / sqrt(D))[r]
- * (0 <= fade <= 1; 0: what was there does not matter). One job a slot. The
- * order of the sums follows from the call's jobs alone: the same call gives the
- * same bits. A row that sees no row (its pages are outside the cache) gives 0
- * and adds nothing. An output value's error is relative to the largest finite
- * |v| of its 32 channels among the rows that the job sees; a row that sees one
- * that is no finite number has NaN in these 32 channels. `workspace`: cc_weigh_workspace bytes for
- * the same jobs (0: the call would be refused), 16-byte aligned, of any
- * contents; two calls that may overlap need two. */
+ * (0 <= fade <= 1; 0: what was there does not matter). One job a slot, and no
+ * page in two of the call's slots (its marks are one page's). The order of the
+ * sums follows from the call's jobs alone: the same call gives the same bits. A
+ * row that sees no row (its pages are outside the cache) gives 0 and adds
+ * nothing. An output value's error is relative to the largest finite |v| of its
+ * 32 channels among the rows that the job sees; a row that sees one that is no
+ * finite number has NaN in these 32 channels. `workspace`: cc_weigh_workspace
+ * bytes for the same jobs (0: the call would be refused), 16-byte aligned, of
+ * any contents; two calls that may overlap need two. */
 size_t cc_weigh_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
                           int32_t observe);
 cc_status cc_attend_weigh(cc_ctx* ctx, const cc_cache* cache, const cc_positions* at, const cc_marks* marks,
@@ -465,7 +466,8 @@ typedef struct cc_keep {
  * and marks, and rows from `keep` on are left as they were. So a slot's kv heads
  * hold different tokens in its rows 0 .. keep - 1, in no order; the pages behind
  * them are the caller's again. Key bounds are not touched (cc_kv_bounds makes
- * them anew). 1 <= keep, sink >= 0, recent >= 0; one job a slot. `workspace`:
+ * them anew). 1 <= keep, sink >= 0, recent >= 0; one job a slot, and no page that
+ * another slot reads (its rows are written over). `workspace`:
  * cc_evict_workspace bytes (may be 0 even for a call that is not refused), as
  * above. */
 size_t cc_evict_workspace(const cc_cache* cache, const cc_keep* jobs, int32_t njobs);

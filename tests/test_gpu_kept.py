@@ -3,12 +3,14 @@ cc_kv_evict) against plain implementations in numpy, in 64 bits, through the C
 ABI, at the sizes and masks where they can go wrong; their use on streams, in
 captured graphs and at addresses past 32 bits; and a run of them together."""
 import math
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 
 from chattorrent_amd import configs
-from test_gpu_operators import Plain, Strided, code_index, dev, hip, quantise, same_bits, scale_index  # noqa: F401
+from test_gpu_operators import ROOT, Plain, Strided, code_index, dev, hip, quantise, same_bits, scale_index  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 U32 = 2.0 ** -24      # half a step of f32, relative to the value
@@ -658,3 +660,158 @@ def test_rows_past_4_gib(ctx):
         ctx.kv_evict(cache, m, [(0, 380, 200, 380)], sink=1, recent=4)
         got.append(outs + [ctx.attend_weigh(cache, [(0, 199, 1)], q[0], marks=m).numpy()])
     assert all(same_bits(a, b) for a, b in zip(*got))
+
+
+# ------------------------------------------------------ what nothing above asks ---
+
+@pytest.mark.parametrize("heads,nkv,D,rot,axes,jobs,observe,fade", [
+    (8, 1, 64, 2, 1, [(0, 127, 2), (1, 0, 2)], None, 1.0),              # 16 columns
+    (17, 1, 64, 6, 4, [(0, 128, 1), (1, 200, 1)], None, 1.0),           # 17
+    (8, 1, 128, 10, 2, [(0, 57, 8), (1, 121, 6)], 5, 0.5),              # 64, and 48: up to 64 columns, some that do not count
+    (13, 1, 128, 128, 1, [(0, 190, 5)], 1, 1.0),                        # 65
+    (64, 1, 64, 64, 2, [(0, 66, 1), (1, 190, 1)], None, 0.0),
+    (1, 1, 256, 14, 3, [(0, 0, 64), (1, 63, 65)], 17, 1.0),             # as many rows of one head
+    (130, 1, 64, 64, 1, [(0, 90, 5)], 3, 0.25),                         # tiles that end inside a row's heads
+    (7, 1, 256, 2, 4, [(0, 61, 75)], 50, 0.0),
+    (4, 4, 64, 64, 1, [(0, 3, 300)], 299, 0.5),                         # all but one row count
+])
+def test_weigh_at_the_borders_of_the_variants(ctx, heads, nkv, D, rot, axes, jobs, observe, fade):
+    rng = np.random.default_rng(heads + D + rot)
+    lengths = [0] * (1 + max(j[0] for j in jobs))
+    for s, past, n in jobs:
+        lengths[s] = past + n
+    check_weigh(ctx, filled(rng, nkv, D, rot, lengths), jobs, heads, axes, observe=observe, fade=fade)
+
+
+@pytest.mark.parametrize("D,heads,n", [(64, 2, 300), (128, 1, 300), (256, 2, 100)])
+def test_weigh_many_tiles_over_several_splits(ctx, D, heads, n):
+    """Tiles of a chunk that end before the slot's last pages, beside a shorter chunk."""
+    rng = np.random.default_rng(D + n)
+    c = filled(rng, 1, D, D, [2000 + n, 170], rope_rows=2500)
+    check_weigh(ctx, c, [(0, 2000, n), (1, 40, 130)], heads, 1, observe=n // 2, size=2.0)
+
+
+def test_weigh_slots_whose_pages_are_in_any_order(ctx):
+    """Pages in falling order, between others' and with a slot that is not asked."""
+    rng = np.random.default_rng(3)
+    c = filled(rng, 2, 128, 128, [300, 310, 290], spare=4)
+    moved = rng.permutation(len(c.k))
+    for a in (c.k, c.v, c.weight, c.token):
+        a[:] = a[np.argsort(moved)]
+    c.table = moved[c.table].astype(c.table.dtype)[:, :]
+    check_weigh(ctx, c, [(2, 250, 40), (0, 299, 1)], 6, 3)
+
+
+def test_a_contexts_own_cache_kept(ctx):
+    """The cache that the pass fills, with marks beside it: weighed as attend_pages reads it, and given up by weight."""
+    from chattorrent_amd.ccdecode import Context, DeviceArray, KVCache, Marks
+    d = configs.with_layers(configs.SMOLLM2, 1)
+    c = Context(d, n_max=1024, t_max=8, slots=1)
+    try:
+        c.fill_random_kv(0, 900, 3, 1)
+        rng = np.random.default_rng(9)
+        q = rng.standard_normal((4, d["n_heads"] * d["head_dim"])).astype(np.float32)
+        want = c.op_attend(0, 0, q, 890)
+        cache = KVCache.of_context(c, 0)
+        shape = cache.c.n_pages, cache.c.n_kv_heads, 64
+        marks = Marks(dev(np.full(shape, 7, np.float32)), dev(np.tile(np.arange(64, dtype=np.int32), shape[:2] + (1,))))
+        got = c.attend_weigh(cache, [(0, 890, 4)], dev(q), marks=marks, fade=0.0).numpy()
+        assert np.abs(got - want).max() <= 2e-5 * np.abs(want).max() * 2
+        weight = marks.kept[0].numpy()
+        rows = weight != 7
+        assert rows.sum() == 894 * shape[1]
+        each = np.where(rows, weight, 0).sum((0, 2))       # the four rows' probabilities, of each head of a group
+        assert np.abs(each - 4 * d["n_heads"] / shape[1]).max() <= 4 * 9 * 2.0 ** -14
+        c.kv_evict(cache, marks, [(0, 894, 500, 894)])
+        few = c.attend_weigh(cache, [(0, 499, 1)], dev(q[3:])).numpy()
+        assert np.isfinite(few).all()
+        table, left = np.asarray(c.pages(0))[:15], marks.kept[0].numpy()
+        for h in range(shape[1]):
+            before, after = (a[table, h].reshape(-1) for a in (weight, left))
+            assert np.array_equal(np.sort(after[:500]), np.sort(before[:894])[-500:])
+    finally:
+        c.close()
+
+
+TORCH_KEPT = """
+import numpy as np, torch
+from chattorrent_amd import ccdecode as cc, configs
+ctx = cc.Context(configs.with_layers(configs.SMOLLM2, 1), n_max=256, t_max=8, slots=2)
+nkv, D, heads, pages = 2, 128, 6, 6
+def fresh():
+    blk = 64 * D + 64 * (D // 32) * 4
+    pools = [torch.full((pages, nkv, blk), 128, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").reshape(2, 3)
+    ang = torch.arange(192, device="cuda")[:, None] * torch.logspace(0, -4, D // 2, device="cuda")
+    rope = torch.stack([ang.cos(), ang.sin()], -1).contiguous()
+    marks = cc.Marks(torch.zeros(pages, nkv, 64, device="cuda"), torch.zeros(pages, nkv, 64, dtype=torch.int32, device="cuda"))
+    return cc.KVCache(*pools, table, rope, D), marks
+torch.manual_seed(1)
+jobs, n = [(0, 0, 150), (1, 0, 70)], 220
+k, v = (torch.randn(n, nkv * D + 8, device="cuda")[:, :nkv * D] for _ in range(2))
+q = torch.randn(n, heads * D, device="cuda")
+at = cc.Positions(torch.randint(0, 192, (n, 3), dtype=torch.int32, device="cuda"), np.arange(D // 2) % 3)
+def run(stream):
+    cache, marks = fresh()
+    torch.cuda.synchronize()
+    ctx.kv_append_at(cache, jobs, k, v, at, marks=marks, stream=stream)
+    out = ctx.attend_weigh(cache, jobs, q, at, marks=marks, stream=stream)
+    ctx.kv_evict(cache, marks, [(0, 150, 64, 150)], sink=1, recent=4, stream=stream)
+    torch.cuda.synchronize()
+    return [out.clone(), *(t.clone() for t in marks.kept)]
+want = run(None)
+side = torch.cuda.Stream()
+with torch.cuda.stream(side):
+    within = run(None)
+for got in (within, run(side.cuda_stream), run(0)):
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+assert torch.isfinite(want[0]).all() and abs(float(want[1][3:].sum()) - 70 * heads) < 0.1
+print("held")
+"""
+
+
+def test_torch_tensors_on_torchs_streams(gpu):
+    r = subprocess.run([sys.executable, "-c", TORCH_KEPT], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True,
+                       timeout=110)
+    assert r.returncode == 0 and r.stdout.strip().endswith("held"), r.stdout
+
+
+def test_two_graphs_with_workspaces_of_their_own(ctx, hip):
+    """Two captured steps, each with its own workspaces, replayed at the same time: each gives the eager step's bits."""
+    import ctypes as C
+    from chattorrent_amd.ccdecode import DeviceArray
+    L, h, held = ctx.lib, ctx.h, []
+    for seed in (51, 52):
+        args, reset, state = two_chats(ctx, seed)
+        want = step(ctx, *args).numpy()
+        after = state()
+        cache, marks, jobs, first, keeps, k, v, q, at = args
+        ja, ka, fa = np.array(jobs, np.int32), np.array(keeps, np.int32), np.array(first, np.int32)
+        out = DeviceArray(want.shape, np.float32)
+        nw, ne = L.cc_weigh_workspace(h, cache.ref, ja.ctypes.data, 2, 6, 1000), L.cc_evict_workspace(cache.ref, ka.ctypes.data, 2)
+        ws, we = DeviceArray(nw, np.uint8), DeviceArray(max(ne, 16), np.uint8)
+        st, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+        hip.check(hip.h.hipStreamCreate(C.byref(st)))
+        hip.check(hip.h.hipStreamBeginCapture(st, 2))
+        code = [L.cc_kv_append_at(h, cache.ref, at.ref, marks.ref, ja.ctypes.data, 2, fa.ctypes.data, k.data_ptr(), 256,
+                                  v.data_ptr(), 256, st),
+                L.cc_attend_weigh(h, cache.ref, at.ref, marks.ref, ja.ctypes.data, 2, 6, 1000, C.c_float(0.9), q.data_ptr(), 768,
+                                  out.data_ptr(), 768, ws.data_ptr(), nw, st),
+                L.cc_kv_evict(h, cache.ref, marks.ref, ka.ctypes.data, 2, 1, 8, we.data_ptr(), ne, st)]
+        hip.check(hip.h.hipStreamEndCapture(st, C.byref(graph)))
+        assert code == [0] * 3, L.cc_last_error(h)
+        hip.check(hip.h.hipGraphInstantiate(C.byref(exe), graph, None, None, 0))
+        held.append((st, graph, exe, args, reset, state, out, want, after, (ws, we)))
+    for _ in range(3):
+        for g in held:
+            g[4]()
+        for g in held:
+            hip.check(hip.h.hipGraphLaunch(g[2], g[0]))
+        for g in held:
+            hip.check(hip.h.hipStreamSynchronize(g[0]))
+        for st, graph, exe, args, reset, state, out, want, after, _ in held:
+            assert same_bits(out.numpy(), want) and all(np.array_equal(a, b) for a, b in zip(state(), after))
+    for st, graph, exe, *_ in held:
+        hip.h.hipGraphExecDestroy(exe)
+        hip.h.hipGraphDestroy(graph)
+        hip.check(hip.h.hipStreamDestroy(st))

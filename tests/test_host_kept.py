@@ -248,3 +248,21 @@ out.append([hip.stand_in_launches().count(b"k_") >= 4, ""])
 """)
     for ok, said in out:
         assert ok, said
+
+
+def test_the_memory_of_a_launch(host):
+    """What a launch with several jobs holds in memory stays near 1 GiB: more jobs use the memory again in further
+    launches. What a call asks for evict's lists hangs on no job that it would refuse."""
+    out = host("""
+c = cache(nkv=8, slots=64, per=512)
+verify, token, chunk = ([(s, 32000, n) for s in range(64)] for n in (8, 1, 600))
+out = dict(one=[room(c, j[0], heads=64) for j in (verify, token, chunk)], all=[room(c, *j, heads=64) for j in (verify, token, chunk)])
+hip.stand_in_reset(-1)
+assert weigh(c, *verify, heads=64, o=f + (1 << 40), ws=f, n=1 << 40) == 0, why()     # nothing runs
+out["launches"] = launched().count("k_weigh_page")
+out["evict"] = [ctx.lib.cc_evict_workspace(C.byref(c), *jobs(j)) for j in ((0, 100, -5, 100), (0, 2**31 - 1, 2**31 - 2, 0), (0, 100, 0, 1))]
+""")
+    scores = 8 * 504 * 64 * 256
+    assert out["one"][0] > scores and out["launches"] > 1
+    assert all(n < (1 << 30) * 1.25 for n in out["all"]) and all(a >= b for a, b in zip(out["all"], out["one"]))
+    assert out["evict"] == [0, 0, 0]
