@@ -2523,8 +2523,8 @@ size_t each_weigh(cc_ctx* ctx, const cc_cache* c, const cc_rows* jobs, int32_t n
             p.ml = take(true, (size_t)units * p.subs * 16 * 8);
             p.parts = take(split, (size_t)units * p.subs * 16 * D * 4);
             p.scores = take(p.score_cols > 0, (size_t)b.pages * p.score_cols * 256);
-            p.q = take(true, (size_t)joins * 16 * D * 4);
-            p.qs = take(true, (size_t)joins * 64);
+            p.q = take(kind != WEIGH_FEW, (size_t)joins * 16 * D * 4);
+            p.qs = take(kind != WEIGH_FEW, (size_t)joins * 64);
             p.exps = take(pairs, (size_t)b.pages * 16);
             p.tot = take(pairs && weigh, (size_t)joins * 128);
             if (pairs && weigh) p.chunks = weigh_chunks(ctx->ncu, b, p, nkv, D);

@@ -141,10 +141,54 @@ __device__ static inline float pair_down(int e) { return u2f((uint32_t)(134 - e)
 // group's largest V scale, of the largest K scale at PAIR_K, and at PAIR_BAD
 // whether a V scale is no finite number.
 constexpr int PAIR_K = 8, PAIR_BAD = 9;
-// What comes before attention: the queries, rotated once, as the matrix
-// products take them (a piece of 16 columns is [hi, lo][NG][64 lanes] of 8 f16,
-// and its scale for the scores 16 f32), then, for k_weigh_many, the exponents
-// of the jobs' pages, a wave each.
+// A piece of 16 columns' queries, rotated, by 256 threads, and their scales for
+// the scores: f32 in x, 8 channels d0 of column h at query_at. Ends past a
+// barrier.
+template <int NG>
+__device__ static inline int query_at(int h, int d0) { return h * 32 * NG + (d0 ^ 8 * (h & (4 * NG - 1))); }
+template <int NG>
+__device__ static inline void rotate_piece(const CacheDev& c, const AxesDev& axes, const WeighJob& jb, const WeighPlan& p, int head,
+                                           int col0, const float* __restrict__ q, int64_t ldq, float* x, int* eq, float* sc) {
+    constexpr int D = 32 * NG;
+    const int tid = threadIdx.x, gt = min(16, jb.n * p.group - col0);
+    for (int i = tid; i < 16 * (D / 8); i += 256) {
+        const int h = i / (D / 8), d0 = 8 * (i & (D / 8 - 1)), at = query_at<NG>(h, d0);
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (h < gt) query8(c, axes, jb, p, head, col0 + h, d0, q, ldq, v);
+        *(float4*)&x[at] = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)&x[at + 4] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    __syncthreads();
+    // 16 threads a column
+    float m = 0.0f;
+    for (int d = tid & 15; d < D; d += 16) m = fmaxf(m, fabsf(x[(tid >> 4) * D + d]));
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((tid & 15) == 0) {
+        eq[tid >> 4] = query_exponent(m);
+        sc[tid >> 4] = score_scale(D, query_exponent(m));
+    }
+    __syncthreads();
+}
+// Of these, what lane `lane` feeds the matrix products of group g.
+template <int NG>
+__device__ static inline void query_pair(const float* x, const int* eq, int g, int lane, u32x4& hi, u32x4& lo) {
+    const int h = lane & 15, at = query_at<NG>(h, 32 * g + 8 * (lane >> 4));
+    const float down = u2f((uint32_t)(127 - eq[h]) << 23);
+    const float4_t a = *(const float4_t*)&x[at] * down, b = *(const float4_t*)&x[at + 4] * down;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float4_t v = e < 2 ? a : b;
+        uint32_t h2, l2;
+        split_mix2(v[2 * (e & 1)], v[2 * (e & 1) + 1], h2, l2);
+        hi[e] = h2;
+        lo[e] = l2;
+    }
+}
+
+// What comes before attention of more than 16 columns: the queries, rotated
+// once, as the matrix products take them (a piece of 16 columns is [hi, lo]
+// [NG][64 lanes] of 8 f16, and its scale for the scores 16 f32), then, for
+// k_weigh_many, the exponents of the jobs' pages, a wave each.
 template <int NG>
 __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs, WeighPlan p, AxesDev axes,
                                                      const float* __restrict__ q, int64_t ldq, uint8_t* __restrict__ ws) {
@@ -187,40 +231,14 @@ __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs,
         return;
     }
     const WeighJob jb = jobs.j[weigh_job_at(jobs, piece, &WeighJob::join0)];
-    const int per_head = weigh_tiles(jb, p) * p.subs, r = piece - jb.join0, head = r / per_head;
-    const int col0 = r % per_head * 16, gt = max(0, min(16, jb.n * p.group - col0));
-    for (int i = tid; i < 16 * (D / 8); i += 256) {
-        const int h = i / (D / 8), d0 = 8 * (i & (D / 8 - 1));
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (h < gt) query8(c, axes, jb, p, head, col0 + h, d0, q, ldq, v);
-        *(float4*)&x[h * D + d0] = make_float4(v[0], v[1], v[2], v[3]);
-        *(float4*)&x[h * D + d0 + 4] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-    __syncthreads();
-    {   // 16 threads a column
-        float m = 0.0f;
-        for (int d = tid & 15; d < D; d += 16) m = fmaxf(m, fabsf(x[(tid >> 4) * D + d]));
-        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        if ((tid & 15) == 0) {
-            s_eq[tid >> 4] = query_exponent(m);
-            ((float*)(ws + p.qs))[(size_t)piece * 16 + (tid >> 4)] = score_scale(D, query_exponent(m));
-        }
-    }
-    __syncthreads();
+    const int per_head = weigh_tiles(jb, p) * p.subs, r = piece - jb.join0;
+    rotate_piece<NG>(c, axes, jb, p, r / per_head, r % per_head * 16, q, ldq, x, s_eq, (float*)(ws + p.qs) + (size_t)piece * 16);
     u32x4* to = (u32x4*)(ws + p.q) + (size_t)piece * 2 * NG * 64;
     for (int i = tid; i < NG * 64; i += 256) {
-        const int lane = i & 63, g = i >> 6, h = lane & 15;
-        const float down = u2f((uint32_t)(127 - s_eq[h]) << 23);
-        half8_t hi, lo;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            _Float16 a, b;
-            split_hilo(x[h * D + 32 * g + 8 * (lane >> 4) + e] * down, a, b);
-            hi[e] = a;
-            lo[e] = b;
-        }
-        to[i] = __builtin_bit_cast(u32x4, hi);
-        to[NG * 64 + i] = __builtin_bit_cast(u32x4, lo);
+        u32x4 hi, lo;
+        query_pair<NG>(x, s_eq, i >> 6, i & 63, hi, lo);
+        to[i] = hi;
+        to[NG * 64 + i] = lo;
     }
 }
 
@@ -241,7 +259,8 @@ __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs,
 // f32, for k_weigh_finish: 4 bytes a column and token beside the 2 * (D + D/8)
 // that a token's K and V take.
 template <int NG, int CT>
-__global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs jobs, WeighPlan p, float* __restrict__ out,
+__global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs jobs, WeighPlan p, AxesDev axes,
+                                                       const float* __restrict__ q, int64_t ldq, float* __restrict__ out,
                                                        int64_t ldo, uint8_t* __restrict__ ws) {
     constexpr int D = 32 * NG, DW = D / 64, GW = DW > 1 ? DW / 2 : 1;   // of a wave: 16-channel pieces, groups
     // Where V's scales go. Into P, which is then split for each group (48 vector instructions a lane, group and 16 columns) and
@@ -298,8 +317,25 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
     load_k(id);
     load_v(id);
 
-    const size_t piece0 = (size_t)jb.join0 + (size_t)w.head * p.subs;
-    {
+    if (CT == 1) {   // the queries rotated here: a launch less, for some 2 us of every workgroup's time
+        __shared__ int s_eq[16];
+        float* x = (float*)&qf[0][0][0][0];   // as many bytes as their pairs take
+        rotate_piece<NG>(c, axes, jb, p, w.head, 0, q, ldq, x, s_eq, s_sc[0]);
+        constexpr int N = (NG + 3) / 4;
+        u32x4 hi[N], lo[N];
+        const bool mine = NG >= 4 || wave < NG;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (mine) query_pair<NG>(x, s_eq, 4 * i + wave, lane, hi[i], lo[i]);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (mine) {
+                qf[0][0][4 * i + wave][lane] = hi[i];
+                qf[0][1][4 * i + wave][lane] = lo[i];
+            }
+    } else {
+        const size_t piece0 = (size_t)jb.join0 + (size_t)w.head * p.subs;
         const u32x4* of = (const u32x4*)(ws + p.q) + piece0 * 2 * NG * 64;
         u32x4* to = &qf[0][0][0][0];
 #pragma unroll
@@ -1266,10 +1302,13 @@ static hipError_t weigh_ng(hipStream_t st, const CacheDev& c, const WeighJobs& j
                            uint8_t* ws) {
     constexpr int D = 32 * NG, CH = 16 * D / WEIGH_JOIN, PER_PAGE = NG > 4 ? 2 : 1;
     const dim3 units(op_blocks(jobs.units));
-    const int before = jobs.joins + (kind == WEIGH_WIDE ? jobs.pages / 4 : 0);
-    hipError_t e = op_launch(k_weigh_query<NG>, dim3(before), dim3(256), st, c, jobs, p, axes, q, ldq, ws);
-    if (e != hipSuccess) return e;
-    auto page = [&](auto k) { return op_launch(k, units, dim3(256), st, c, jobs, p, out, ldo, ws); };
+    hipError_t e = hipSuccess;
+    if (kind != WEIGH_FEW) {
+        const int before = jobs.joins + (kind == WEIGH_WIDE ? jobs.pages / 4 : 0);
+        e = op_launch(k_weigh_query<NG>, dim3(before), dim3(256), st, c, jobs, p, axes, q, ldq, ws);
+        if (e != hipSuccess) return e;
+    }
+    auto page = [&](auto k) { return op_launch(k, units, dim3(256), st, c, jobs, p, axes, q, ldq, out, ldo, ws); };
     if (kind != WEIGH_WIDE) {
         if (p.subs == 1) e = page(k_weigh_page<NG, 1>);
         else if (p.subs == 2) e = page(k_weigh_page<NG, 2>);

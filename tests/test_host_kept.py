@@ -187,12 +187,12 @@ out["stale"] = [weigh(c, (0, 100, 60), **big), append_at(c, (0, 0, 1)), evict(c,
 hip.hipGetLastError()
 """)
     assert out["append"] == ["k_kv_append_at"] and out["many"] == ["k_kv_append_at"] * 3
-    page = ["k_weigh_query", "k_weigh_page"]
+    page = ["k_weigh_page"]      # which rotates up to 16 columns itself
     assert out["token"] == page == out["off"] and out["weighed"] == page + ["k_weigh_finish"]
     many = ["k_weigh_query", "k_weigh_many", "k_weigh_join", "k_weigh_sums", "k_weigh_add"]
     assert [k for k in many if k in out["chunk"]] == out["chunk"] and "k_weigh_sums" in out["chunk"]
     assert "k_weigh_sums" not in out["alone"] and "k_weigh_finish" not in out["token"]
-    assert out["both"][:3] == page + ["k_weigh_finish"] and out["both"][3:] == out["chunk"]
+    assert out["both"][:2] == page + ["k_weigh_finish"] and out["both"][2:] == out["chunk"]
     assert out["jobs"].count("k_weigh_page") == 3 and out["pieces"].count("k_weigh_sums") == 3
     assert out["none"] == [] and out["one"] == ["k_evict_select"] and out["lot"] == ["k_evict_select", "k_evict_move"]
     assert out["jobs_"] == ["k_evict_select", "k_evict_move"] * 3
