@@ -2421,11 +2421,15 @@ constexpr int64_t WEIGH_BYTES = 1 << 30;      // of such a launch's scores, or q
 int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The pages of an attention workgroup. Up to 16 columns: such that there are
-// some eight workgroups for each compute unit (32 chats, heads of 128: 127 us;
-// four 151, two 147); up to 64, two (16 x 8 verify rows, heads of 256: 74 us;
-// four 84, eight 103). More: the cut of the longest job
-// with the least time, counted in pages that a compute unit, which holds one
-// workgroup, does after another, with two pages' time to begin with.
+// some eight workgroups for each compute unit (32 chats, heads of 128: 126 us;
+// twelve 129, four 146, two 140), but at least four to six pages, so that the
+// joins of up to 192 pages take one batch of 32 splits' loads (one chat of 141
+// pages, with the joins: 5 pages 16.6 us, 2 20.1, 3 17.5, 6 17.6, 8 20.3; 7
+// chats of up to 244: 6 30.6 us, 2 36.9, 4 34.6, 8 30.5). Up to 64 columns, two
+// workgroups (16 x 8 verify rows, heads of 256: 68 us; one 106, three 86, four
+// 79, eight 94). More: the cut of the longest job with the least time, counted
+// in pages that a compute unit, which holds one workgroup, does after another,
+// with two pages' time to begin with.
 int weigh_per(int ncu, const WeighJobs& b, const WeighPlan& p, int64_t nkv, WeighKind kind) {
     int longest = 0;
     int64_t work = 0;
@@ -2435,8 +2439,11 @@ int weigh_per(int ncu, const WeighJobs& b, const WeighPlan& p, int64_t nkv, Weig
         work += nkv * ceil_div(b.j[j].n * p.group, 16 * p.subs) * pages;
     }
     const int least = std::max(ceil_div(longest, 128), 1);
-    if (kind != WEIGH_WIDE)
-        return (int)std::min<int64_t>(256, std::max<int64_t>({2, ceil_div64(work, (kind == WEIGH_FEW ? 8 : 2) * (int64_t)ncu), least}));
+    if (kind != WEIGH_WIDE) {
+        const bool few = kind == WEIGH_FEW;
+        const int some = few ? std::max(4, std::min(6, ceil_div(longest, 32))) : 2;
+        return (int)std::min<int64_t>(256, std::max<int64_t>({some, ceil_div64(work, (few ? 8 : 2) * (int64_t)ncu), least}));
+    }
     const int64_t slots = ncu;
     int best = 0;
     int64_t cost = 0;

@@ -145,7 +145,7 @@ constexpr int PAIR_K = 8, PAIR_BAD = 9;
 // the scores: f32 in x, 8 channels d0 of column h at query_at. Ends past a
 // barrier.
 template <int NG>
-__device__ static inline int query_at(int h, int d0) { return h * 32 * NG + (d0 ^ 8 * (h & (4 * NG - 1))); }
+__device__ static inline int query_at(int h, int d0) { return h * 32 * NG + (d0 ^ 8 * (h & (NG == 2 ? 7 : 15))); }
 template <int NG>
 __device__ static inline void rotate_piece(const CacheDev& c, const AxesDev& axes, const WeighJob& jb, const WeighPlan& p, int head,
                                            int col0, const float* __restrict__ q, int64_t ldq, float* x, int* eq, float* sc) {
@@ -188,7 +188,11 @@ __device__ static inline void query_pair(const float* x, const int* eq, int g, i
 // What comes before attention of more than 16 columns: the queries, rotated
 // once, as the matrix products take them (a piece of 16 columns is [hi, lo]
 // [NG][64 lanes] of 8 f16, and its scale for the scores 16 f32), then, for
-// k_weigh_many, the exponents of the jobs' pages, a wave each.
+// k_weigh_many, the exponents of the jobs' pages, a wave each. Bound by its
+// chain of loads (job, position, rope table, query): 8 us for 16 x 8 verify
+// rows of 24 heads of 256, 8.5 for 512 rows of 32 heads of 128. (In k_weigh_page,
+// which does it itself for up to 16 columns, the verify rows' three pieces in
+// every workgroup took 13 us more than here.)
 template <int NG>
 __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs, WeighPlan p, AxesDev axes,
                                                      const float* __restrict__ q, int64_t ldq, uint8_t* __restrict__ ws) {
@@ -258,6 +262,12 @@ __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs,
 // Where p.score_cols is set the scores stay in the workspace, [page][column][64]
 // f32, for k_weigh_finish: 4 bytes a column and token beside the 2 * (D + D/8)
 // that a token's K and V take.
+//
+// 32 chats of 2048 .. 16384 tokens, 5 heads of 128 a kv head: 127 us, 0.5 TB of
+// K, V and scores at 4.5 TB/s (a copy: 5.0). One chat of 9000: 12, a chain of
+// the query's loads and five pages a workgroup. 16 chats x 8 verify rows
+// (48 columns), heads of 256: 69 us, 2.6 TB/s: vector instructions (codes to
+// f16, P times V's scales as pairs, exp2) and waiting at 8 waves a CU.
 template <int NG, int CT>
 __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs jobs, WeighPlan p, AxesDev axes,
                                                        const float* __restrict__ q, int64_t ldq, float* __restrict__ out,
@@ -630,7 +640,10 @@ __device__ static inline float2 column_total(const float2* __restrict__ at, int 
 // After k_weigh_page: joins the splits' outputs (the first workgroups, a
 // WEIGH_JOIN floats of a 16-column piece each, its splits dealt to four waves)
 // and, from the stored scores, adds up the weights of FINISH_PAGES pages of a
-// (job, kv head) a workgroup, a row a lane.
+// (job, kv head) a workgroup, a row a lane. Loads in sequence (the columns' M and
+// l; scores, ahead of these) and one exp2 a score: 4.5 us for one chat, 21 for 32
+// chats (37 MB of scores, still in the last-level cache), 22 for verify rows. 4
+// and 16 pages a workgroup were slower.
 template <int NG>
 __global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs, WeighPlan p, MarksDev marks,
                                                       float* __restrict__ out, int64_t ldo, const uint8_t* __restrict__ ws) {
@@ -731,9 +744,12 @@ __global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs
         *wt[i] = __builtin_fmaf(before[i], 64 * (p0 + wave + 4 * i) + lane >= jb.fresh ? p.fade : 1.0f, got);   // weigh_add's sum
     }
 }
+
 // After k_weigh_many, where a tile's pages were split: joins the outputs of
 // 1024 / D columns of a piece a workgroup, 4 channels a thread, and leaves the
-// columns' M and 1/l.
+// columns' M and 1/l. 512 rows of 40 heads of 128: 8.6 us, the parts read and
+// the output written (three splits: 42 MB) at 4.9 TB/s, from the last-level
+// cache.
 template <int NG>
 __global__ __launch_bounds__(256) void k_weigh_join(WeighJobs jobs, WeighPlan p, float* __restrict__ out, int64_t ldo,
                                                     uint8_t* __restrict__ ws) {
@@ -795,6 +811,14 @@ __device__ static inline void reads_ahead() {
 // f32 sum, and nothing is scaled in between (a pair's two halves hold 22 bits).
 // While a step is computed the next one is unpacked into the other buffer and
 // the one after it is loaded.
+// Bound by the matrix units and what stands between their products: 512 rows of
+// 40 heads of 128 at 8192 take 258 us, 0.27 TFLOP with three products for one
+// (1.04 PFLOP/s; a large f16 matmul of random values: 1.25), 32 heads at 4000
+// 114 us.
+// The matrix units are busy 45-50% of the time and the vector unit about as
+// long, for the exp2s and pairs of P, with little of either beside the other.
+// Steps of 64 rows, wave priorities and unpacking between the products were
+// slower (300 us the last).
 template <int NG, int CT, int W, int TOK>
 __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs jobs, WeighPlan p, float* __restrict__ out,
                                                           int64_t ldo, uint8_t* __restrict__ ws) {
@@ -1149,6 +1173,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
 // workgroup's four waves share through LDS; a lane adds up its 4 * TT rows' p /
 // l, and 16 lanes meet at the end, in a fixed order. With one chunk the result
 // goes to the marks, else to the chunk's line in the workspace (k_weigh_add).
+// Three products as above: all 512 rows of 40 heads at 8192 counting 138 us
+// (0.96 PFLOP/s), the last 64 of 512 rows of 32 heads at 4000 17. (Scores kept
+// from the attention would be 0.7 GB of the former, written and read: 275 us.)
 __device__ static inline void weigh_add(float* at, const WeighPlan& p, bool fades, float got) {
     const float before = fades && p.fade == 0.0f ? 0.0f : *at;
     *at = __builtin_fmaf(before, fades ? p.fade : 1.0f, got);
@@ -1280,7 +1307,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
     }
 }
 
-// The chunks' lines, added in their order.
+// The chunks' lines, added in their order: 5 us, a launch's time.
 __global__ __launch_bounds__(256) static void k_weigh_add(CacheDev c, WeighJobs jobs, WeighPlan p, MarksDev marks,
                                                           const uint8_t* __restrict__ ws) {
     const int u = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -1363,7 +1390,8 @@ struct EvictMove {
 
 // The codes, scales and marks of N rows at a time, by a wave: all N are loaded
 // before the first is stored (one after another a row waits for its page, its
-// codes and the row before it: 370 us for 32 prompts instead of 115).
+// codes and the row before it). For the few moves of one workgroup; where a page
+// gets many, k_evict_move.
 template <int NG, int N>
 __device__ static inline void move_rows(const CacheDev& c, const MarksDev& marks, const EvictMove* moves, int lane) {
     constexpr int D = 32 * NG, VB = D / 64;
@@ -1431,6 +1459,10 @@ __device__ static inline int64_t evict_words(const EvictJob& j) { return evict_f
 // The rows below `keep` that go and the rows from `keep` on that stay are as
 // many, and the i-th of the one takes the place of the i-th of the other: a
 // list of them in the workspace, or up to EVICT_HERE moves made here.
+// A chain of the keys' load, the passes' barriers and the list or the moves: 6
+// us where one of 1025 rows goes, 20 where 32 chats of 4160 give up 64 each (9 of
+// it before the moves), 16 for 16001 rows of one, 18 for 32 prompts of 2048 ..
+// 16384.
 template <int NG, int REG>
 __global__ __launch_bounds__(1024) void k_evict_select(CacheDev c, EvictJobs jobs, MarksDev marks, int sink, int recent,
                                                        uint8_t* __restrict__ ws) {
@@ -1572,6 +1604,10 @@ static_assert(EVICT_HERE == 64, "four moves for each of k_evict_select's sixteen
 // head). Where they are EVICT_PAGE or more, a thread takes a channel's 16 rows
 // of V, whose codes lie beside each other, and puts the new ones into the 16
 // bytes that it read; fewer are stored byte by byte.
+// Bound by V's layout: a token's D codes lie in D/8 lines of 128 bytes, one in
+// every 16 bytes, so a scattered row of V costs these lines, not D bytes. 32
+// prompts (8 kv heads of 128) cut to 2048 rows: 122 us, 0.53 GB of lines at 4.3
+// TB/s where the rows alone are 0.25 GB; one prompt of 4 heads of 256: 14 us.
 constexpr int EVICT_PAGE = 8;
 template <int NG>
 __global__ __launch_bounds__(256) void k_evict_move(CacheDev c, EvictJobs jobs, MarksDev marks,

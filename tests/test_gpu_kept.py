@@ -691,6 +691,14 @@ def test_weigh_many_tiles_over_several_splits(ctx, D, heads, n):
     check_weigh(ctx, c, [(0, 2000, n), (1, 40, 130)], heads, 1, observe=n // 2, size=2.0)
 
 
+def test_weigh_more_splits_than_one_batch_of_loads(ctx):
+    """196 pages: 33 splits for a token, 98 for 40 columns."""
+    rng = np.random.default_rng(4)
+    c = filled(rng, 1, 64, 64, [12500], rope_rows=700)
+    check_weigh(ctx, c, [(0, 12499, 1)], 2, size=0.5)
+    check_weigh(ctx, c, [(0, 12480, 20)], 2, size=0.5, observe=3, fade=0.5)
+
+
 def test_weigh_slots_whose_pages_are_in_any_order(ctx):
     """Pages in falling order, between others' and with a slot that is not asked."""
     rng = np.random.default_rng(3)
