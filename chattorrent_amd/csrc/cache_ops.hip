@@ -37,7 +37,10 @@ __device__ static inline void bound_code(float mx, float mn, float B, int8_t& hi
 //
 // AT: the rows' positions are not their indices but given, each pair of
 // channels turning by its own axis's (AxesDev), and each row gets its mark: no
-// weight yet, and its token's number.
+// weight yet, and its token's number. The walk is the same, and so is its time:
+// 4000 rows of 8 x 128 beside 3 chats' 15.6 us, 2 x 1024 rows of 4 x 256 beside
+// 30 chats' 15.0, one row 3.8. (Five workgroups for a page's K and V, a quarter
+// of K's rows each: 17.3 for the first.)
 template <int D, bool VEC, bool AT>
 __device__ static inline void append_rows(const CacheDev& c, const OpJobs& jobs, const float* __restrict__ k, int64_t ldk,
                                           const float* __restrict__ v, int64_t ldv, int only, const AppendAt* at) {

@@ -459,17 +459,18 @@ typedef struct cc_keep {
  * <= keep). Kept are the rows whose token is among the chat's first `sink`
  * (token < sink) or latest `recent` (token >= seen - recent; where these are
  * more than `keep`, the lower rows of them), then those with the largest
- * weight, ties to the lower row; a weight that is no number, and a
- * row whose page is outside the cache, counts least. The rows below `keep` that
- * stay, stay where they are; in row order, the i-th row from `keep` on that
- * stays moves to the i-th row below `keep` that goes, with its codes, scales
- * and marks, and rows from `keep` on are left as they were. So a slot's kv heads
- * hold different tokens in its rows 0 .. keep - 1, in no order; the pages behind
- * them are the caller's again. Key bounds are not touched (cc_kv_bounds makes
- * them anew). 1 <= keep, sink >= 0, recent >= 0; one job a slot, and no page that
- * another slot reads (its rows are written over). `workspace`:
- * cc_evict_workspace bytes (may be 0 even for a call that is not refused), as
- * above. */
+ * weight, ties to the lower row; a weight that is no number, and a row whose
+ * page is outside the cache, counts least. The rows below `keep` that stay,
+ * stay where they are; in row order, the i-th row from `keep` on that stays
+ * moves to the i-th row below `keep` that goes, with its codes, scales and
+ * marks, and rows from `keep` on are left as they were. So a slot's kv heads
+ * hold different tokens in its rows 0 .. keep - 1, in no order; the pages
+ * behind them are the caller's again, and cc_kv_append and cc_attend_pages,
+ * which take a row's index for its position, no longer fit the slot. Key bounds
+ * are not touched (cc_kv_bounds makes them anew). 1 <= keep, sink >= 0, recent
+ * >= 0; one job a slot, and no page that another slot reads (its rows are
+ * written over). `workspace`: cc_evict_workspace bytes (may be 0 even for a
+ * call that is not refused), as above. */
 size_t cc_evict_workspace(const cc_cache* cache, const cc_keep* jobs, int32_t njobs);
 cc_status cc_kv_evict(cc_ctx* ctx, const cc_cache* cache, const cc_marks* marks, const cc_keep* jobs, int32_t njobs,
                       int32_t sink, int32_t recent, void* workspace, size_t workspace_bytes, void* stream);
