@@ -475,6 +475,11 @@ def _int32s(a, name, width=None):
     return a, a.__array_interface__["data"][0]
 
 
+def _count(n):
+    """A number of rows or tokens as int32: none has more than that holds, and a negative one stays negative."""
+    return max(-1, min(int(n), 2**31 - 1))
+
+
 def _job_rows(jobs):
     """(slot, past, n) of each job as int32 [jobs, 3], its address, and the rows they hold."""
     a, at = _int32s(jobs, "jobs", "(slot, past, n)")
@@ -886,7 +891,7 @@ class Context:
             raise ValueError(f"q: rows of {width} values are not whole heads of {D}")
         pr = None if positions is None else positions.fit(cache, rows)
         mr = None if marks is None else marks.fit(cache)
-        observe = 0 if marks is None else 2**31 - 1 if observe is None else int(observe)
+        observe = 0 if marks is None else _count(2**31 if observe is None else observe)
         if out is None:
             out = self._new(q, (rows, width), "float32", given)
             op, ldo = out.data_ptr(), width
@@ -913,7 +918,8 @@ class Context:
         mr = marks.fit(cache)
         need = self.lib.cc_evict_workspace(cache.ref, at, len(a))
         ws = self._new(like, (need,), "uint8", given) if need else None
-        st = self.lib.cc_kv_evict(self.h, cache.ref, mr, at, len(a), sink, recent, ws.data_ptr() if need else None, need, stream)
+        st = self.lib.cc_kv_evict(self.h, cache.ref, mr, at, len(a), _count(sink), _count(recent),
+                                  ws.data_ptr() if need else None, need, stream)
         if st:
             self._chk(st)
 

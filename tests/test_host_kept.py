@@ -250,6 +250,33 @@ out.append([hip.stand_in_launches().count(b"k_") >= 4, ""])
         assert ok, said
 
 
+def test_the_bindings_numbers_past_32_bits(gpus):
+    """A count that 32 bits do not hold means all of the rows, a negative one is refused, however far below 0."""
+    out = gpus("""
+out = []
+c = cache(0, 0, 0, 0, 0)
+q = on(0, 3, 256)
+m = cc.Marks(on(0, 4, 2, 64), on(0, 4, 2, 64, of=np.int32))
+for observe in (3, 1 << 32, 1 << 40):
+    hip.stand_in_reset(-1)
+    ctx[0].attend_weigh(c, [(0, 5, 3)], q, marks=m, observe=observe)
+    out.append([b"k_weigh_finish" in hip.stand_in_launches(), str(observe)])
+def no(call):
+    try:
+        call()
+    except cc.CCError as e:
+        out.append(["negative" in str(e), str(e)])
+    else:
+        out.append([False, "taken"])
+no(lambda: ctx[0].attend_weigh(c, [(0, 5, 3)], q, marks=m, observe=-(1 << 32)))
+no(lambda: ctx[0].kv_evict(c, m, [(0, 65, 64, 65)], sink=-(1 << 32)))
+no(lambda: ctx[0].kv_evict(c, m, [(0, 65, 64, 65)], recent=-(1 << 40)))
+ctx[0].kv_evict(c, m, [(0, 65, 64, 65)], sink=1 << 32, recent=1 << 40)
+""")
+    for ok, said in out:
+        assert ok, said
+
+
 def test_the_memory_of_a_launch(host):
     """What a launch with several jobs holds in memory stays near 1 GiB: more jobs use the memory again in further
     launches. What a call asks for evict's lists hangs on no job that it would refuse."""
