@@ -136,6 +136,14 @@ __device__ static inline void code_pair(uint32_t lo4, uint32_t hi4, float s, hal
 // can be: times pair_down(e) a scale is at most 2^8.
 __device__ static inline int pair_exponent(uint32_t top) { return max((int)(top >> 23) - 127, -112); }
 __device__ static inline float pair_down(int e) { return u2f((uint32_t)(134 - e) << 23); }
+// What a sum of a page's products of pairs takes to be a score: sc (score_scale)
+// and the 2^7 that the keys were brought to. It stays a normal number, so that a
+// masked -inf is still -inf behind it, and a sum of 0 still 0. (A sum is below
+// 2^27: what the lower bound holds back is a score below 2^-99. Beyond the upper
+// one products of the largest q and k pass 2^146.)
+__device__ static inline float pair_score(float sc, int e) {
+    return __builtin_amdgcn_fmed3f(ldexpf(sc, e - 7), 0x1p-126f, 0x1.fffffep127f);
+}
 
 // Of a page's scales, for the f16 pairs below: 16 bytes, the exponents of each
 // group's largest V scale, of the largest K scale at PAIR_K, and at PAIR_BAD
@@ -1016,7 +1024,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const int last = ok ? my_last[ct] : -1;
-            const float scp = ldexpf(sc[ct], ke - 7);
+            const float scp = pair_score(sc[ct], ke);
             if (edge) {
 #pragma unroll
                 for (int tt = 0; tt < TT; tt++)
@@ -1242,7 +1250,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
 #pragma unroll
             for (int i = 0; i < NQ; i++) qs[b][256 * i + tid] = qn[i];
             const float2 t = tn;
-            const float sc = ldexpf(scn, e - 7);
+            const float sc = pair_score(scn, e);
             __syncthreads();   // (a piece's place is written again two pieces on, past the next barrier)
             if (t16 + 1 < to) load(t16 + 1);
             if (t16 < my_from) continue;
