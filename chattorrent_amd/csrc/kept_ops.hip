@@ -16,7 +16,12 @@
 // most 2^14, for the f16 pairs that enter the P.V product.
 typedef float4_t float4_a4 __attribute__((aligned(4)));
 constexpr float P_SHIFT = 6.0f, P_ROOM = 8.0f, P_UNSHIFT = 1.0f / 64.0f;
-constexpr float M_LARGE = 1048576.0f;   // beyond: the score is rounded before M is taken off, or the largest may miss it
+// From this M on a score is rounded before M is taken off, in k_weigh_many, which
+// sums up l, and in k_weigh_sums alike: the largest score then does not miss M,
+// and a column's p / l add up to 1. (Below it one fma does both. A column may be
+// past it in one and not yet in the other, by its M so far or by its neighbours':
+// the two p are then 2^-24 * 2^10 apart.)
+constexpr float M_LARGE = 1024.0f;
 
 // The largest of a lane's value and those of the lanes 16, 32 and 48 away.
 __device__ static inline float rows_max(float x) {
@@ -979,7 +984,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
     };
 
     float M[CT], lsum[CT], base[CT];
-    bool large = false;   // an M so large that a score is rounded before M is taken off
+    bool large = false;   // an M of M_LARGE or more
     int ev[NG];   // O of a group's channels is relative to 2^(ev - 7)
     float4_t o[CT][DT];
 #pragma unroll
@@ -1284,8 +1289,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_sums(CacheDev c, WeighJobs job
             for (int tt = 0; tt < TT; tt++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    float a = __builtin_fmaf(acc[tt][r], sc, base);
-                    if (large && a > P_ROOM) a = P_ROOM;   // its rounding alone can be above that
+                    const float a = large ? acc[tt][r] * sc + base : __builtin_fmaf(acc[tt][r], sc, base);
                     const bool sees = r0 + 16 * tt + 4 * j4 + r <= last;
                     const float x = __builtin_amdgcn_exp2f(a);
                     got[tt][r] = __builtin_fmaf(sees ? x : 0.0f, sees ? t.y : 0.0f, got[tt][r]);

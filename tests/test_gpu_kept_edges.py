@@ -4,7 +4,9 @@ implementation in 64 bits."""
 import numpy as np
 import pytest
 
-from test_gpu_kept import Kept, check_weigh, ctx, filled  # noqa: F401
+import test_gpu_kept as base
+from test_gpu_kept import Kept, check_weigh, ctx, dev, filled, scale_index  # noqa: F401
+from test_gpu_operators import code_index, quantise
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +53,52 @@ def test_weigh_large_queries_across_large_keys(ctx, D, n):
     q = np.zeros((n, 2 * D), np.float32)
     q[:, [5, D + 5]] = 1e38
     check_weigh(ctx, c, [(0, 70, n)], 2, q=q)
+
+
+# ------------------------------------------------- scores that f32 rounds to whole numbers ---
+
+def one_hot_values(c, pages, T):
+    """v of row t: 1 in channel t % D. So an output's channel is the probability of the rows t % D."""
+    v = np.zeros((T, c.nkv, c.D), np.float32)
+    v[np.arange(T), :, np.arange(T) % c.D] = 1
+    code, scale = quantise(v)
+    for t in range(T):
+        page = pages[t // 64]
+        for h in range(c.nkv):
+            c.v[page, h, code_index(1, c.D)[t % 64]] = (code[t, h] + 128).astype(np.uint8)
+            c.v.view(np.float32)[page, h, 16 * c.D + scale_index(1, c.D)[t % 64]] = scale[t, h]
+
+
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("size", [300.0, 3e3, 2e5, 1e6, 3e7, 1e10, 1e15])
+@pytest.mark.parametrize("n", [1, 8, 40, 300])
+def test_weigh_adds_up_what_attention_gives(ctx, n, size, mixed):
+    """However large the scores: what a row's weight gains is what the outputs took of it, also where rows of small and of
+    large scores stand beside each other (`mixed`). An output's p is a sum of pairs, 2^-20 of the largest value (1), so n * 2 of
+    them are off by no more than n * 2^-19; a weight's p is formed from the same score, once the fused and once the rounded
+    product where the scores of a column pass 2^10 within the call: 2^-14 of it. l's two roundings and the sums of n * 2 terms
+    are below another 2^-14."""
+    rng = np.random.default_rng(int(np.log10(size)) + n)
+    nkv, D, past, heads = 2, 128, 130, 4
+    T = past + n
+    c = filled(rng, nkv, D, D, [T])
+    one_hot_values(c, c.table[0], T)
+    q = (size * rng.standard_normal((n, heads * D))).astype(np.float32)
+    if mixed:
+        q *= np.repeat(2.0 ** rng.integers(-9, 5, (n, heads)), D, 1).astype(np.float32)
+    cache, marks = c.device()
+    out = ctx.attend_weigh(cache, [(0, past, n)], dev(q), marks=marks, fade=0.0).numpy().reshape(n, nkv, 2, D)
+    got = c.m[0].numpy()[c.table[0]].transpose(1, 0, 2).reshape(nkv, -1)[:, :T].astype(np.float64)
+    took = out.astype(np.float64).sum((0, 2))
+    gained = np.zeros((nkv, D))
+    for t in range(T):
+        gained[:, t % D] += got[:, t]
+    off = np.abs(gained - took)
+    assert (off <= gained * 2.0 ** -13 + n * 2.0 ** -19).all(), (off.max(), gained[np.unravel_index(off.argmax(), off.shape)])
+    assert (np.abs(got.sum(1) - 2 * n) <= 2 * n * 2.0 ** -13).all(), got.sum(1)
+    assert (got <= 2 * n * (1 + 2.0 ** -13)).all()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-4, 300.0, 1e6, 1e12])
+def test_weigh_scores_of_any_magnitude_in_many_columns(ctx, size):
+    base.test_weigh_scores_of_any_magnitude(ctx, 40, size)
