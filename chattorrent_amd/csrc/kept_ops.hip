@@ -13,7 +13,9 @@
 // brings sums from one M to another is a power of two, exactly, and it stays as
 // it is while no score passes it by more than P_ROOM; then it is the largest
 // score rounded up. p is formed 2^P_SHIFT times as large, in one rounding, at
-// most 2^14, for the f16 pairs that enter the P.V product.
+// most 2^14, for the f16 pairs that enter the P.V product. (Whether a score is
+// that far above M is asked of their difference, which is exact where they are
+// near: from 2^27 on f32 rounds M + P_ROOM.)
 typedef float4_t float4_a4 __attribute__((aligned(4)));
 constexpr float P_SHIFT = 6.0f, P_ROOM = 8.0f, P_UNSHIFT = 1.0f / 64.0f;
 // From this M on a score is rounded before M is taken off, in k_weigh_many, which
@@ -457,7 +459,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const float m = fmaxf(fmaxf(tops[b][0][ct][l16], tops[b][1][ct][l16]), fmaxf(tops[b][2][ct][l16], tops[b][3][ct][l16]));
-            const bool mine = M[ct] == -INFINITY ? m > -INFINITY : m > M[ct] + P_ROOM;
+            const bool mine = m - M[ct] > P_ROOM;
             Mn[ct] = mine ? ceilf(m) : M[ct];
             over = over || mine;
         }
@@ -1042,9 +1044,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
             for (int tt = 0; tt < TT; tt++)
                 top = fmaxf(fmaxf(top, fmaxf(acc[ct][tt][0], acc[ct][tt][1])), fmaxf(acc[ct][tt][2], acc[ct][tt][3]));
             top *= scp;
-            if (__any(top > M[ct] + P_ROOM)) {   // (M -inf: the first score of a column)
+            if (__any(top - M[ct] > P_ROOM)) {   // (M -inf: the first score of a column)
                 top = rows_max(top);
-                const float Mn = top > M[ct] + P_ROOM ? ceilf(top) : M[ct];
+                const float Mn = top - M[ct] > P_ROOM ? ceilf(top) : M[ct];
                 const float alpha = pow2_diff(M[ct], Mn);
                 M[ct] = Mn;
                 lsum[ct] *= alpha;

@@ -102,3 +102,44 @@ def test_weigh_adds_up_what_attention_gives(ctx, n, size, mixed):
 @pytest.mark.parametrize("size", [1e-30, 1e-4, 300.0, 1e6, 1e12])
 def test_weigh_scores_of_any_magnitude_in_many_columns(ctx, size):
     base.test_weigh_scores_of_any_magnitude(ctx, 40, size)
+
+
+@pytest.mark.parametrize("D,first,n", [(64, 64, 1), (256, 64, 1), (64, 64, 40), (256, 64, 12), (256, 32, 80)])
+def test_weigh_a_score_one_step_of_f32_above(ctx, D, first, n):
+    """Scores of 1.44 * 2^27, whole multiples of 16 in f32: an odd one in the first rows, the next in those behind, which then
+    take all but 2^-16 of the attention or less. (f32 has nothing between the two: the first plus 8 is rounded to the second.)"""
+    # q . k / sqrt(D) is 2^27 + 16 c, with codes 64 and c in channels of different groups; the score's 24 bits are those of
+    # log2(e) * (1 + c * 2^-23)
+    log2e = np.float32(1.4426950408889634)
+    bits = [int((log2e * np.float32(1 + c * 2.0 ** -23)).view(np.uint32)) for c in range(12)]
+    c0, c1 = next((a, b) for a in range(12) for b in range(12) if bits[a] % 2 and bits[b] == bits[a] + 1)
+    rng = np.random.default_rng(D + n)
+    past = 128
+    c = filled(rng, 1, D, 2, [past + n])
+    k = np.zeros((past + n, D), np.float32)
+    cache_pages = c.table[0]
+    for t in range(past):      # codes as they are, scales of 1
+        page, at = cache_pages[t // 64], t % 64
+        c.k[page, 0, code_index(0, D)[at]] = 128
+        c.k[page, 0, code_index(0, D)[at, 4]] = 128 + 64
+        c.k[page, 0, code_index(0, D)[at, 36]] = 128 + (c0 if t < first else c1)
+        c.k.view(np.float32)[page, 0, 16 * D + scale_index(0, D)[at]] = 1.0
+    for t in range(past, past + n):
+        page, at = cache_pages[t // 64], t % 64
+        c.k[page, 0, code_index(0, D)[at]] = 128
+        c.k.view(np.float32)[page, 0, 16 * D + scale_index(0, D)[at]] = 1.0
+    root = {64: 8, 256: 16}[D]
+    q = np.zeros((n, D), np.float32)
+    q[:, 4] = root * 2.0 ** 21            # times 64 / root: 2^27
+    q[:, 36] = root * 2.0 ** 4            # times c / root: c * 2^4, a step of 2^27 in f32 for each c
+    cache, marks = c.device()
+    out = ctx.attend_weigh(cache, [(0, past, n)], dev(q), marks=marks, fade=0.0).numpy()
+    values = np.concatenate([c.exact_rows(1, p, 0) for p in cache_pages])
+    want = values[first:past].mean(0)
+    # p of the first rows: 2^-16 of the others', 1/3 .. 1 times as many; f16 pairs and f32 sums of 128 rows: 2^-16 more
+    lim = np.abs(values[:past]).max() * 2.0 ** -14
+    assert np.isfinite(out).all()
+    assert (np.abs(out - want) <= lim).all()
+    got = c.m[0].numpy()[cache_pages, 0].reshape(-1)
+    assert (np.abs(got[first:past] - n / (past - first)) <= n / (past - first) * 2.0 ** -14).all()
+    assert (got[:first] <= n * 2.0 ** -14 / first).all() and not got[past:past + n].any()
