@@ -743,9 +743,11 @@ __global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs
     for (int i = 0; i < WP; i++) {
         if (!wt[i]) continue;
         float got = 0.0f;
+        const int sees = (64 * (p0 + wave + 4 * i) + lane - jb.past) * p.group;   // the first column that sees the lane's row
         auto add = [&](float x1, int col) {
             const float2 t = total[min(col, cols - 1)];
-            if (col < cols) got = __builtin_fmaf(__builtin_amdgcn_exp2f(x1 - t.x), t.y, got);
+            // (p of one that does not is 0, but its 1/l may be NaN)
+            if (col < cols) got = __builtin_fmaf(__builtin_amdgcn_exp2f(x1 - t.x), col >= sees ? t.y : 0.0f, got);
         };
 #pragma unroll
         for (int e = 0; e < 8; e++) add(x[i][e], c0 + e);

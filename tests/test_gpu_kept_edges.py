@@ -143,3 +143,28 @@ def test_weigh_a_score_one_step_of_f32_above(ctx, D, first, n):
     got = c.m[0].numpy()[cache_pages, 0].reshape(-1)
     assert (np.abs(got[first:past] - n / (past - first)) <= n / (past - first) * 2.0 ** -14).all()
     assert (got[:first] <= n * 2.0 ** -14 / first).all() and not got[past:past + n].any()
+
+
+# ------------------------------------------------------------ what is no number ---
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("past,n", [(70, 2), (60, 8), (70, 30), (70, 40), (1500, 8), (1500, 40)])
+def test_weigh_a_query_that_is_no_number_counts_for_what_it_sees(ctx, D, past, n):
+    """A NaN in the first row's query: the weights of the rows that it sees, of its kv head, are NaN, those of the rows behind it
+    are the others' sums."""
+    rng = np.random.default_rng(D + n)
+    c = filled(rng, 2, D, D, [past + n], rope_rows=2000)
+    q = rng.standard_normal((n, 4 * D)).astype(np.float32)
+    q[0, D + 5] = np.nan                       # head 1, of kv head 0
+    cache, marks = c.device()
+    out = ctx.attend_weigh(cache, [(0, past, n)], dev(q), marks=marks, fade=0.0).numpy().reshape(n, 4, D)
+    q[0, D + 5] = 0
+    want, bound, weight, wbound = c.weigh([(0, past, n)], q, 4, fade=0.0)
+    bad = np.zeros((n, 4), bool)
+    bad[0, 1] = True
+    assert np.isnan(out[bad]).all()
+    assert (np.abs(out - want.reshape(out.shape))[~bad] <= np.broadcast_to(bound[:, None, None], out.shape)[~bad]).all()
+    got, weight, wbound = (a[c.table[0]].transpose(1, 0, 2).reshape(2, -1)[:, :past + n] for a in (c.m[0].numpy(), weight, wbound))
+    assert np.isnan(got[0, :past + 1]).all()
+    got[0, :past + 1] = weight[0, :past + 1]
+    assert (np.abs(got - weight) <= wbound).all()
