@@ -25,6 +25,14 @@ constexpr float P_SHIFT = 6.0f, P_ROOM = 8.0f, P_UNSHIFT = 1.0f / 64.0f;
 // the two p are then 2^-24 * 2^10 apart.)
 constexpr float M_LARGE = 1024.0f;
 
+// Between what a wave's lanes write to LDS and what other lanes of it read or
+// write there: the wave's LDS instructions run in their order, and the compiler
+// keeps it.
+__device__ static inline void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // The largest of a lane's value and those of the lanes 16, 32 and 48 away.
 __device__ static inline float rows_max(float x) {
     auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
@@ -398,6 +406,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
         for (int ct = 0; ct < CT; ct++) s[ct] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < SK; i++) ksl[wave][(ke0 + i) % NG][(ke0 + i) / NG] = u2f(ksr[i]);
+        wave_lds();
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             const float4_t ks = *(const float4_t*)&ksl[wave][g][4 * j4];
@@ -505,6 +514,7 @@ __global__ __launch_bounds__(256, 2) void k_weigh_page(CacheDev c, WeighJobs job
         const float down = pair_down(GW > 1 && lane >= 32 ? ev[GW - 1] : ev[0]) * (PS ? 1.0f / 128.0f : 1.0f);
 #pragma unroll
         for (int i = 0; i < SK; i++) vsl[wave][(ve0 + i) >> 6][(ve0 + i) & 63] = u2f(vsr[i]) * down;
+        wave_lds();
         auto scales8 = [&](int g, int ks, float (&s8)[8]) {   // of the lane's rows 16 * (2 ks + i / 4) + 4 * j4 + i % 4
             const float4_t sa = *(const float4_t*)&vsl[wave][g][16 * j4 + 8 * ks], sb = *(const float4_t*)&vsl[wave][g][16 * j4 + 8 * ks + 4];
 #pragma unroll
@@ -1641,7 +1651,8 @@ __global__ __launch_bounds__(256) void k_evict_move(CacheDev c, EvictJobs jobs, 
     const uint32_t* pt = c.page_table + (size_t)jb.slot * c.max_pages;
     if (tid < 64) {
         move_to[tid] = -1;
-        if (tid < n) {   // (the 64 lanes of a wave)
+        wave_lds();      // (the 64 lanes of a wave)
+        if (tid < n) {
             const int2 m = *(const int2*)(pairs + 2 * (first + tid));
             moves[tid] = move_at(c, pt, head, m.x, m.y);
             if (moves[tid].of_row >= 0) move_to[m.y & 63] = tid;
