@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import test_gpu_kept as base
-from test_gpu_kept import Kept, check_weigh, ctx, dev, filled, scale_index  # noqa: F401
+from test_gpu_kept import Kept, check_weigh, ctx, dev, filled, same_bits, scale_index  # noqa: F401
 from test_gpu_operators import code_index, quantise
 
 pytestmark = pytest.mark.gpu
@@ -168,3 +168,54 @@ def test_weigh_a_query_that_is_no_number_counts_for_what_it_sees(ctx, D, past, n
     assert np.isnan(got[0, :past + 1]).all()
     got[0, :past + 1] = weight[0, :past + 1]
     assert (np.abs(got - weight) <= wbound).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_weigh_a_key_that_is_no_number_among_many_columns(ctx, D):
+    """A NaN scale of the last row's key: the row that sees it is NaN, and with it every weight; the others are as without it."""
+    rng = np.random.default_rng(D)
+    n = 40
+    c = filled(rng, 1, D, D, [70 + n])
+    at = c.table[0, (69 + n) // 64], 0, 16 * D + scale_index(0, D)[(69 + n) % 64, 1]
+    q = rng.standard_normal((n, 2 * D)).astype(np.float32)
+    want, bound, weight, wbound = c.weigh([(0, 70, n)], q, 2)
+    c.k.view(np.float32)[at] = np.nan
+    cache, marks = c.device()
+    out = ctx.attend_weigh(cache, [(0, 70, n)], dev(q), marks=marks).numpy()
+    assert np.isnan(out[-1]).all()
+    assert (np.abs(out - want)[:-1] <= bound[:-1, None]).all()
+    assert np.isnan(c.m[0].numpy()[c.table[0], 0].reshape(-1)[:70 + n]).all()
+
+
+# ------------------------------------- what test_gpu_kept.py asks of up to 64 columns ---
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_weigh_what_many_columns_do_not_see(ctx, D):
+    base.test_weigh_what_rows_do_not_see(ctx, D, 40)
+
+
+def test_weigh_a_nan_query_among_many_columns(ctx):
+    base.test_weigh_keys_and_queries_that_are_no_numbers(ctx, 40)
+
+
+@pytest.mark.parametrize("observe", [1000, 7])
+def test_weigh_many_columns_past_4_gib(ctx, observe):
+    """80 rows of two heads over blocks past 2^31 and 2^32 bytes of the pools, as over a small cache's."""
+    from chattorrent_amd.ccdecode import DeviceArray, KVCache, Marks
+    rng = np.random.default_rng(18)
+    nkv, D, n = 8, 256, 30000
+    small = Kept(rng, nkv, D, D, 6, 1, 6)
+    small.table[0] = np.arange(6)
+    near, near_marks = small.device()
+    pools = [DeviceArray((n, nkv, small.k.shape[2]), np.uint8) for _ in range(2)]
+    marks = [DeviceArray((n, nkv, 64), t) for t in (np.float32, np.int32)]
+    table = np.array([[29999, 3, 14800, 29400, 14650, 29250]], np.int32)
+    far = KVCache(*pools, dev(table), small.d[3], D)
+    k, v = (dev(rng.standard_normal((380, nkv * D)).astype(np.float32)) for _ in range(2))
+    q = dev(rng.standard_normal((80, 2 * nkv * D)).astype(np.float32))
+    got = []
+    for cache, m in ((near, near_marks), (far, Marks(*marks))):
+        ctx.kv_append_at(cache, [(0, 0, 380)], k, v, marks=m)
+        got.append(ctx.attend_weigh(cache, [(0, 300, 80)], q, marks=m, observe=observe).numpy())
+    assert np.isfinite(got[0]).all() and same_bits(*got)
+    assert same_bits(marks[0].numpy()[table[0]].reshape(6, -1)[:5], small.m[0].numpy().reshape(6, -1)[:5])
