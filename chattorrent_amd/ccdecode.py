@@ -364,7 +364,8 @@ class KVCache(_Buffers):
 
     @classmethod
     def of_context(cls, ctx, layer, bounds=None):
-        """The context's own cache of block `layer`; `bounds`: key bounds of the caller's."""
+        """The context's own cache of block `layer`; `bounds`: key bounds of the caller's. A slot whose rows kv_append_at placed
+        or kv_evict moved is no longer one that the context's own passes can go on with."""
         self = cls.__new__(cls)
         _Buffers.__init__(self)
         self.c = CCache()
@@ -910,7 +911,9 @@ class Context:
     def kv_evict(self, cache, marks, jobs, sink=0, recent=0, stream=None):
         """cc_kv_evict: of each job's (slot, rows, keep, seen) rows every kv head
         keeps `keep`: those of the chat's first `sink` and latest `recent` of
-        its `seen` tokens, then those with the largest weight."""
+        its `seen` tokens, then those with the largest weight. Only
+        kv_append_at and attend_weigh go on with such a slot: the others, the
+        context's own passes among them, take a row's index for its position."""
         like = marks.kept[0]
         given, stream = stream, self._on(stream, cache, like)
         self._beside(stream, cache, like, marks)

@@ -344,7 +344,11 @@ typedef struct cc_cache {
 } cc_cache;
 /* The context's own cache of block `layer` (bounds NULL: the caller may set
  * its own). Its pages are the context's to give: cc_step, cc_fill_random_kv
- * and cc_release change the page table on the context's stream. */
+ * and cc_release change the page table on the context's stream. The context's
+ * own passes (cc_step, cc_decode_steps, cc_mtp_draft) and cc_op_attend take a
+ * row's index for its position. Once a slot's rows were placed otherwise
+ * (cc_kv_append_at) or given up (cc_kv_evict) they compute wrong attention for
+ * it, with no error: go on with the operators, or release the slot. */
 cc_status cc_cache_of(cc_ctx* ctx, int32_t layer, cc_cache* out);
 /* Bytes of key bounds a page takes; 0 for a head_dim that is not supported. */
 size_t cc_bounds_bytes(const cc_cache* cache);
@@ -440,7 +444,10 @@ cc_status cc_kv_append_at(cc_ctx* ctx, const cc_cache* cache, const cc_positions
  * row that sees no row (its pages are outside the cache) gives 0 and adds
  * nothing. An output value's error is relative to the largest finite |v| of its
  * 32 channels among the rows that the job sees; a row that sees one that is no
- * finite number has NaN in these 32 channels. `workspace`: cc_weigh_workspace
+ * finite number has NaN in these 32 channels. A query row and head with a value
+ * that is no number, or that sees such a key, has NaN in its output and, if it
+ * counts, in the weights of the rows that it sees, and in no others. Keys and
+ * values of the cache are below 2^96. `workspace`: cc_weigh_workspace
  * bytes for the same jobs (0: the call would be refused), 16-byte aligned, of
  * any contents; two calls that may overlap need two. */
 size_t cc_weigh_workspace(cc_ctx* ctx, const cc_cache* cache, const cc_rows* jobs, int32_t njobs, int32_t n_heads,
@@ -465,8 +472,9 @@ typedef struct cc_keep {
  * moves to the i-th row below `keep` that goes, with its codes, scales and
  * marks, and rows from `keep` on are left as they were. So a slot's kv heads
  * hold different tokens in its rows 0 .. keep - 1, in no order; the pages
- * behind them are the caller's again, and cc_kv_append and cc_attend_pages,
- * which take a row's index for its position, no longer fit the slot. Key bounds
+ * behind them are the caller's again, and cc_kv_append, cc_attend_pages and a
+ * context's own passes (see cc_cache_of), which take a row's index for its
+ * position, no longer fit the slot. Key bounds
  * are not touched (cc_kv_bounds makes them anew). 1 <= keep, sink >= 0, recent
  * >= 0; one job a slot, and no page that another slot reads (its rows are
  * written over). `workspace`: cc_evict_workspace bytes (may be 0 even for a
