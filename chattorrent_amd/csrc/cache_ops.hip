@@ -16,7 +16,8 @@
 // so the codes and scales are its bits. 4000 rows of 8 heads of 128 (42 MB)
 // take 15.5-16 us, 2.7 TB/s: half the rate of a copy. A wave of a whole page
 // walks its strides of rows one after another, and loads the next when the one
-// before is stored: a chain of four latencies. 32 rows take 4.4 us. Bounds
+// before is stored: a chain of four latencies. (Not what bounds it: see AT
+// below.) 32 rows take 4.4 us. Bounds
 // alone, of 16 chats of 16384 tokens (311 MB): 160 us, 1.9 TB/s, the same walk.
 //
 // Key bounds (a page's, made when its 64th row is stored): per channel the
@@ -39,8 +40,9 @@ __device__ static inline void bound_code(float mx, float mn, float B, int8_t& hi
 // channels turning by its own axis's (AxesDev), and each row gets its mark: no
 // weight yet, and its token's number. The walk is the same, and so is its time:
 // 4000 rows of 8 x 128 beside 3 chats' 15.6 us, 2 x 1024 rows of 4 x 256 beside
-// 30 chats' 15.0, one row 3.8. (Five workgroups for a page's K and V, a quarter
-// of K's rows each: 17.3 for the first.)
+// 30 chats' 15.0, one row 3.8. Five workgroups for a page's K and V, a quarter
+// of K's rows each, took 17.3 for the first: the chain of strides is not what
+// bounds it. K alone takes 12 of it and V alone 9; what does is not found.
 template <int D, bool VEC, bool AT>
 __device__ static inline void append_rows(const CacheDev& c, const OpJobs& jobs, const float* __restrict__ k, int64_t ldk,
                                           const float* __restrict__ v, int64_t ldv, int only, const AppendAt* at) {

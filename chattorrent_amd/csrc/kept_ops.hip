@@ -286,7 +286,7 @@ __global__ __launch_bounds__(256) void k_weigh_query(CacheDev c, WeighJobs jobs,
 // f32, for k_weigh_finish: 4 bytes a column and token beside the 2 * (D + D/8)
 // that a token's K and V take.
 //
-// 32 chats of 2048 .. 16384 tokens, 5 heads of 128 a kv head: 127 us, 0.5 TB of
+// 32 chats of 2048 .. 16384 tokens, 5 heads of 128 a kv head: 127 us, 0.57 GB of
 // K, V and scores at 4.5 TB/s (a copy: 5.0). One chat of 9000: 12, a chain of
 // the query's loads and five pages a workgroup. 16 chats x 8 verify rows
 // (48 columns), heads of 256: 69 us, 2.6 TB/s: vector instructions (codes to
@@ -666,9 +666,10 @@ __device__ static inline float2 column_total(const float2* __restrict__ at, int 
 // WEIGH_JOIN floats of a 16-column piece each, its splits dealt to four waves)
 // and, from the stored scores, adds up the weights of FINISH_PAGES pages of a
 // (job, kv head) a workgroup, a row a lane. Loads in sequence (the columns' M and
-// l; scores, ahead of these) and one exp2 a score: 4.5 us for one chat, 21 for 32
-// chats (37 MB of scores, still in the last-level cache), 22 for verify rows. 4
-// and 16 pages a workgroup were slower.
+// l; scores, ahead of these, 4 bytes a lane) and one exp2 a score: 4.5 us for one
+// chat; 21 for 32 chats, the joins alone 10 (37 MB of scores, still in the
+// last-level cache: 1.8 TB/s over the whole); 21 for verify rows (61 MB, 2.9
+// TB/s). 4 and 16 pages a workgroup were slower.
 template <int NG>
 __global__ __launch_bounds__(256) void k_weigh_finish(CacheDev c, WeighJobs jobs, WeighPlan p, MarksDev marks,
                                                       float* __restrict__ out, int64_t ldo, const uint8_t* __restrict__ ws) {
@@ -1201,7 +1202,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_weigh_many(CacheDev c, WeighJobs 
 // l, and 16 lanes meet at the end, in a fixed order. With one chunk the result
 // goes to the marks, else to the chunk's line in the workspace (k_weigh_add).
 // Three products as above: all 512 rows of 40 heads at 8192 counting 138 us
-// (0.96 PFLOP/s), the last 64 of 512 rows of 32 heads at 4000 17. (Scores kept
+// (0.96 PFLOP/s), the last 64 of 512 rows of 32 heads at 4000 16. (Scores kept
 // from the attention would be 0.7 GB of the former, written and read: 275 us.)
 __device__ static inline void weigh_add(float* at, const WeighPlan& p, bool fades, float got) {
     const float before = fades && p.fade == 0.0f ? 0.0f : *at;
