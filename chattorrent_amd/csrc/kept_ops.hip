@@ -22,7 +22,9 @@ constexpr float P_SHIFT = 6.0f, P_ROOM = 8.0f, P_UNSHIFT = 1.0f / 64.0f;
 // sums up l, and in k_weigh_sums alike: the largest score then does not miss M,
 // and a column's p / l add up to 1. (Below it one fma does both. A column may be
 // past it in one and not yet in the other, by its M so far or by its neighbours':
-// the two p are then 2^-24 * 2^10 apart.)
+// the two p are then 2^-24 * 2^10 apart. Scores of this size, some 700 before
+// log2(e), cost a call of many rows 5-7%: 2^20 in its place would be faster for
+// them, and p 4% apart.)
 constexpr float M_LARGE = 1024.0f;
 
 // Between what a wave's lanes write to LDS and what other lanes of it read or
